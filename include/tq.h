@@ -439,6 +439,107 @@ int tq_attention_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, c
                      int64_t heads, int64_t head_dim, float* out, int64_t ldo, tq_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Serving state of a decoder layer: rotary positions, an 8-bit key/value cache and
+ * attention over it.  The reference has none of these (its MultiheadAttention,
+ * crates/theano-nn/src/transformer.rs:9-162, knows neither a cache nor positions);
+ * the formats are the row formats above, applied to each token's head.
+ *
+ * Rows of q, k and v: `n` tokens of `heads` heads of head_dim elements, element type
+ * `dtype` (TQ_DT_F32, TQ_DT_BF16 or TQ_DT_F16), token i's head h at
+ * x + i * token_stride + h * head_stride (in elements; the head's own elements are
+ * adjacent), so that a fused projection's output is read in place.  Outputs are
+ * dense [n, heads, head_dim] and do not overlap inputs.  1 <= head_dim <= 128.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+    const void* data;
+    int64_t heads, token_stride, head_stride;
+} tq_heads;
+
+/* Rotary positions: the first rotary_dim (even, <= head_dim) elements of a head turn in
+ * planes i < rotary_dim / 2 by pos * frequencies[i]; the others pass.
+ *   interleaved 0: plane i is elements i and i + rotary_dim / 2; 1: 2 i and 2 i + 1
+ *   y0 = scale (x0 cos a - x1 sin a), y1 = scale (x1 cos a + x0 sin a)
+ * inverse: the transpose (angles negated), which is also the gradient.  The angle is
+ * formed and reduced in f64, cosine and sine are f32, one rounding to dtype. */
+typedef struct {
+    const double* frequencies; /* device, rotary_dim / 2 */
+    int64_t rotary_dim;
+    int32_t interleaved, inverse;
+    float scale;
+} tq_rotary;
+
+/* positions: int64, device, n (any values below 2^53).  q or k may be absent (heads 0). */
+int tq_rotary_apply(const tq_rotary* rotary, const int64_t* positions, int64_t n, const tq_heads* q,
+                    const tq_heads* k, int dtype, int64_t head_dim, void* q_out, void* k_out,
+                    tq_stream_t stream);
+
+/* A paged cache: `pages` pages of `page` tokens (a multiple of 16).  Codes (int8, or
+ * e4m3 bit patterns) [pages, heads, page, row], row = head_dim rounded up to 32, zeros
+ * past head_dim; scales f32 [pages, heads, page] (>= 0; a write leaves at least 1e-10,
+ * and tq_kv_attention takes value scales under 1e-25 for that).  Codes and scales 16-byte
+ * aligned.  A token's head is coded as a row of tq_quantize_i8_rowwise or
+ * tq_quantize_fp8_rowwise.  codes: TQ_QINT8 or TQ_QFP8. */
+typedef struct {
+    void* k;
+    float* k_scale;
+    void* v;
+    float* v_scale;
+    int64_t pages, heads, page, head_dim;
+    int32_t codes;
+} tq_kv_cache;
+
+/* Which tokens a call is about: sequence b < batch has lengths[b] tokens (those of this
+ * call among them, the last ones) on the pages table[b * table_stride + i], position p on
+ * page p / page.  The call's `tokens` rows are sequence after sequence: rows offsets[b]
+ * .. offsets[b + 1] - 1 are the last of sequence b.  offsets NULL: max_tokens rows each
+ * (tokens = batch * max_tokens).  No sequence has more than max_tokens rows.
+ * Everything the device arrays say is checked where it is used: a row with no place
+ * (before position 0, past the table, on a page outside the cache, behind the last
+ * sequence) is not written, reads as zeros or, behind the last sequence, is left as it
+ * was; lengths past the table are cut.  A page that one call writes for two places holds
+ * either: positions being written need a page of their own. */
+typedef struct {
+    const int32_t* table;
+    int64_t table_stride, table_pages;
+    const int32_t* lengths;
+    const int32_t* offsets;
+    int64_t batch, max_tokens, tokens;
+} tq_kv_batch;
+
+/* Codes k and v [tokens, heads, head_dim] into the cache. */
+int tq_kv_write(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_heads* k, const tq_heads* v,
+                int dtype, tq_stream_t stream);
+/* The same with q and k turned first, in one launch: q_out is q turned (dtype); k is coded
+ * from its f32 turned values.  positions: int64, device, one for each row, or NULL for the
+ * places in the sequences (drafted trees have positions of their own). */
+int tq_kv_write_rotary(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
+                       const int64_t* positions, const tq_heads* q, const tq_heads* k, const tq_heads* v, int dtype,
+                       void* q_out, tq_stream_t stream);
+/* The batch's rows back as f32(code * scale), rounded to dtype: k_out and v_out
+ * [tokens, heads, head_dim] (max_tokens or offsets say how many of each sequence). */
+int tq_kv_read(const tq_kv_cache* cache, const tq_kv_batch* batch, int dtype, void* k_out, void* v_out,
+               tq_stream_t stream);
+
+/* Attention of the batch's rows over the cache:
+ *   out[row, h] = softmax_keys(scale q[row, h] . k[key, h / group]) v[key, h / group]
+ * with q_heads = group * heads.  Row t of a sequence's T new tokens sees every key
+ * before the new tokens and, of these, its own and earlier ones (tree NULL), or those
+ * whose bit is set: bit j & 31 of tree[row * tree_words + j / 32] is new token j
+ * (tree_words >= ceil(T / 32); a drafted token sees its ancestors and itself).  A key
+ * with no place (see tq_kv_batch) is seen by nobody.  Softmax, sums and outputs are f32, q is
+ * taken as f16 planes (two for f32) and the codes are exact, so the result is as near as
+ * f32 gets for f32 and one rounding to dtype otherwise.  A row that sees no key, or
+ * whose scores are all -inf, gives zeros (the idle slots of a serving batch); what a
+ * row does not see cannot reach it, NaN and infinities included.  Rows behind the last
+ * sequence are left as they were.  out: dtype, dense [tokens, q_heads, head_dim].
+ * workspace: device memory of tq_kv_attention_workspace_bytes(...) bytes (which depend on
+ * the descriptors' sizes alone), 256-byte aligned, contents need not be initialised. */
+int64_t tq_kv_attention_workspace_bytes(const tq_kv_cache* cache, const tq_kv_batch* batch, int64_t q_heads);
+int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_heads* q, int dtype,
+                    const int32_t* tree, int64_t tree_words, float scale, void* workspace, int64_t workspace_bytes,
+                    void* out, tq_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Element type conversion of device buffers: the device half of Tensor::to
  * (crates/theano-core/src/tensor.rs:277-299) and of RocmStorage::from_host_f64
  * / to_host_f64 (crates/theano-rocm/src/storage.rs:54-99), whose tensors hold

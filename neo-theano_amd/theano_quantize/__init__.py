@@ -10,6 +10,7 @@ QuantizedLinear, QuantizedMLP; quantized checkpoints (save_quantized /
 load_quantized over the safetensors container of crates/theano-serialize).
 """
 from ._tensor import convert
+from .cache import KVBatch, KVCache, Rotary, tree_mask
 from .checkpoint import load_quantized, load_safetensors, save_quantized, save_safetensors
 from .errors import InvalidArgument, KernelError, OutOfMemory, TheanoError
 from .formats import (
@@ -38,4 +39,5 @@ __all__ = [
     "quantize_per_channel_fp8", "dequantize_per_channel_fp8", "fake_quantize_per_channel_fp8",
     "quantize_i4_g128", "dequantize_i4_g128", "repack_i4_g128_tiled", "repack_i4_g128_gate_up_tiled", "tile_rows_for", "Module", "QuantizedLinear", "QuantizedMLP", "QuantizedMultiheadAttention",
     "save_safetensors", "load_safetensors", "save_quantized", "load_quantized", "convert",
+    "Rotary", "KVBatch", "KVCache", "tree_mask",
 ]

@@ -20,6 +20,31 @@ _int = ctypes.c_int
 _dbl = ctypes.c_double
 _p = ctypes.c_void_p
 
+
+
+class Heads(ctypes.Structure):
+    """tq_heads"""
+    _fields_ = [("data", _p), ("heads", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """tq_rotary"""
+    _fields_ = [("frequencies", _p), ("rotary_dim", _i64), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class KVCacheDesc(ctypes.Structure):
+    """tq_kv_cache"""
+    _fields_ = [("k", _p), ("k_scale", _p), ("v", _p), ("v_scale", _p), ("pages", _i64), ("heads", _i64), ("page", _i64),
+                ("head_dim", _i64), ("codes", ctypes.c_int32)]
+
+
+class KVBatchDesc(ctypes.Structure):
+    """tq_kv_batch"""
+    _fields_ = [("table", _p), ("table_stride", _i64), ("table_pages", _i64), ("lengths", _p), ("offsets", _p),
+                ("batch", _i64), ("max_tokens", _i64), ("tokens", _i64)]
+
+
 # name -> argtypes (all return int status unless listed in _RESTYPE)
 SIGNATURES = {
     "tq_version": [],
@@ -86,6 +111,13 @@ SIGNATURES = {
     "tq_repack_w4g128_gate_up_tiled": [_p, _p, _p, _p, _i64, _i64, _p, _p, _p],
     "tq_mlp_w4g128_decode": [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p],
     "tq_mlp_w4g128_decode_noalloc": [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p],
+    # descriptors are passed as the address of their ctypes structure
+    "tq_rotary_apply": [_p, _p, _i64, _p, _p, _int, _i64, _p, _p, _p],
+    "tq_kv_write": [_p, _p, _p, _p, _int, _p],
+    "tq_kv_write_rotary": [_p, _p, _p, _p, _p, _p, _p, _int, _p, _p],
+    "tq_kv_read": [_p, _p, _int, _p, _p, _p],
+    "tq_kv_attention_workspace_bytes": [_p, _p, _i64],
+    "tq_kv_attention": [_p, _p, _p, _int, _p, _i64, ctypes.c_float, _p, _i64, _p, _p],
 }
 _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_p,
             "tq_w4g128_tile_rows": ctypes.c_int64, "tq_mlp_w4g128_workspace_bytes": ctypes.c_int64,
@@ -95,6 +127,7 @@ _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_
             "tq_mlp_w4g128_split_workspace_bytes": ctypes.c_int64,
             "tq_linear_w8a8_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w8a8_workspace_bytes": ctypes.c_int64, "tq_gemm_fp8_workspace_bytes": ctypes.c_int64,
+            "tq_kv_attention_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w4g128_bf16_workspace_bytes": ctypes.c_int64, "tq_dtype_size": ctypes.c_int64}
 
 _lib = None
