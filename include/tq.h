@@ -439,6 +439,34 @@ int tq_attention_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, c
                      int64_t heads, int64_t head_dim, float* out, int64_t ldo, tq_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * FP8 (e4m3) with a scale for each block of 128: weights [N, K] in blocks of 128 x 128
+ * (the last ones of ragged N and K smaller), activations in rows of 128 columns.
+ *   s     = f32(max(absmax of the block / 448, 1e-10)), code = e4m3(f32(x / s)) as in
+ *           tq_quantize_fp8_rowwise (NaN ignored by the maximum, 0x7F as a code)
+ *   y[m,n] = sum_b sa[b, m] sw[n / 128, b] sum_{k in block b} qa[m,k] qw[n,k]  (+ bias[n])
+ * Products of codes are exact and summed in f32 (on the f16 matrix cores: the FP8 ones
+ * drop bits inside their sums, 1.3e-5 of y), as are the scaled blocks.  y is f32.  Any M, N, K.
+ * ------------------------------------------------------------------------ */
+int tq_quantize_fp8_block(const float* w, int64_t n, int64_t k, uint8_t* q, float* s, tq_stream_t stream);
+/* w_hat = f32(e4m3(q) * s of its block). */
+int tq_dequantize_fp8_block(const uint8_t* q, const float* s, int64_t n, int64_t k, float* w_hat, tq_stream_t stream);
+/* Activations x [M, K] (dtype f32, bf16 or f16): codes [M, K rounded up to 128] with zeros
+ * past K, scales [K / 128 rounded up, M]; codes 16-byte aligned. */
+int tq_quantize_fp8_g128(const void* x, int dtype, int64_t m, int64_t k, uint8_t* q, float* s, tq_stream_t stream);
+/* The product of such codes.  qa 16-byte aligned, the f32 pointers 4-byte, qw any.
+ * `workspace`: at least tq_gemm_fp8_block_workspace_bytes(M, N, K) bytes (may be 0),
+ * 256-byte aligned, contents need not be initialised. */
+int64_t tq_gemm_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int tq_gemm_fp8_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const float* sw, const float* bias,
+                      int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, float* y,
+                      tq_stream_t stream);
+/* Both in one call: the codes, their scales and partial sums live in `workspace` (at
+ * least tq_linear_fp8_block_workspace_bytes(M, N, K) bytes, 256-byte aligned). */
+int64_t tq_linear_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int tq_linear_fp8_block(const void* x, int dtype, int64_t m, const uint8_t* qw, const float* sw, const float* bias,
+                        int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, float* y, tq_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Serving state of a decoder layer: rotary positions, an 8-bit key/value cache and
  * attention over it.  The reference has none of these (its MultiheadAttention,
  * crates/theano-nn/src/transformer.rs:9-162, knows neither a cache nor positions);

@@ -16,6 +16,9 @@
 //    is scaled by its f16 scale as it is added to the total.  GemmW4GateUp runs two
 //    weight matrices side by side and stores h = SiLU(gate) * up.
 //
+//  * GemmF8Block: e4m3 codes of both operands widened to f16 (exact products, f32 sums),
+//    every 128-long sum scaled by A's and W's block scales as it is added to the total.
+//
 // The 8-bit bf16 forms add their running sums into a second set of accumulators every
 // kFlushStages stages (in f64 for GemmF8b), so that a sum's rounding grows with
 // the square root of a run's length and not of K: relative errors at K = 14336 are
@@ -173,6 +176,22 @@ struct SrcBf16 {
     }
 };
 
+// 8 e4m3 codes per chunk as f16 (exact: 2^-9 to 448), two to an instruction.
+struct SrcFp8F16 {
+    typedef uint8_t elem_t;
+    static constexpr int kElems = 8, kPlanes = 1, kPer = 1;
+    typedef SrcBf16<ValFp8>::Raw Raw;
+    __device__ static Raw load(const elem_t* p) { return SrcBf16<ValFp8>::load(p); }
+    __device__ static Raw load_tail(const elem_t* p, int n, int k) { return SrcBf16<ValFp8>::load_tail(p, n, k); }
+    __device__ static void planes(const Raw& r, u32x4 (&out)[1]) {
+        const int a = static_cast<int>(r.v.x), b = static_cast<int>(r.v.y);
+        out[0] = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true))};
+    }
+};
+
 // 16 byte codes per chunk, as they are.
 template <class T>
 struct SrcBytes {
@@ -246,7 +265,7 @@ struct SrcW4 {
 // many chunks of a row (one share per lane half).
 struct OpBf16 {
     typedef f32x16 Acc;
-    static constexpr bool kFlush = true, kGroups = false, kGateUp = false;
+    static constexpr bool kFlush = true, kGroups = false, kGateUp = false, kBlocks = false;
     static constexpr int kFragChunks = 1;
     typedef u32x4 Frag;
     __device__ static Frag frag(const u32x4 (&c)[1]) { return c[0]; }
@@ -285,12 +304,28 @@ struct GemmW4GateUp : GemmW4 {
 struct GemmW4H : GemmW4 {
     typedef SrcF32HiLo A;
 };
+typedef _Float16 tile_f16x8 __attribute__((ext_vector_type(8)));
+struct GemmF8Block {
+    typedef SrcFp8F16 A;
+    typedef SrcFp8F16 W;
+    typedef f32x16 Acc;
+    typedef float part_t;
+    static constexpr bool kRowScale = false, kFlush = true, kGroups = true, kGateUp = false, kBlocks = true;
+    static constexpr int kFlushStages = 2;  // one block
+    static constexpr int kFragChunks = 1;
+    typedef u32x4 Frag;
+    __device__ static Frag frag(const u32x4 (&c)[1]) { return c[0]; }
+    __device__ static Acc mfma(Frag a, Frag b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(tile_f16x8, a), __builtin_bit_cast(tile_f16x8, b),
+                                                      c, 0, 0, 0);
+    }
+};
 struct GemmI8 {
     typedef SrcBytes<int8_t> A;
     typedef SrcBytes<int8_t> W;
     typedef i32x16 Acc;
     typedef int32_t part_t;
-    static constexpr bool kRowScale = true, kFlush = false, kGroups = false, kGateUp = false;
+    static constexpr bool kRowScale = true, kFlush = false, kGroups = false, kGateUp = false, kBlocks = false;
     static constexpr int kFragChunks = 1;
     typedef i32x4 Frag;
     __device__ static Frag frag(const u32x4 (&c)[1]) { return __builtin_bit_cast(i32x4, c[0]); }
@@ -303,7 +338,7 @@ struct GemmF8 {
     typedef SrcBytes<uint8_t> W;
     typedef f32x16 Acc;
     typedef float part_t;
-    static constexpr bool kRowScale = true, kFlush = false, kGroups = false, kGateUp = false;
+    static constexpr bool kRowScale = true, kFlush = false, kGroups = false, kGateUp = false, kBlocks = false;
     static constexpr int kFragChunks = 2;
     typedef i32x8 Frag;
     __device__ static Frag frag(const u32x4 (&c)[2]) {
@@ -320,13 +355,14 @@ struct GemmF8 {
 struct TileArgs {
     const void* a;      // A [m, k]
     const void* w;      // W [n, k]
-    const float* sa;    // row scales [m] (kRowScale)
-    const float* sw;    // column scales [n]
+    const float* sa;    // row scales [m] (kRowScale); A's block scales [blocks of K, m] (kBlocks)
+    const float* sw;    // column scales [n]; W's block scales [n / 128, blocks of K] (kBlocks)
     const float* bias;  // [n] or null
     const uint16_t* sg;   // f16 group scales [n, k / 128] (kGroups)
     const void* w2;       // kGateUp: w and sg are gate's, w2 and sg2 up's, n both rows' count
     const uint16_t* sg2;  // (n = 2 F: partial sums hold gate's F columns, then up's)
     int m, n, k;
+    int lda;            // kBlocks: A's rows in codes, k rounded up to 128 (zeros past k)
     int tiles_m, tiles_n, split;
     int32_t* acc;  // int32 sums [m, n] or null (GemmI8)
     float* y;      // [m, n]
@@ -393,8 +429,9 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
     static_assert(!T::kGateUp || TN == 2, "a wave holds 32 gate and the same 32 up columns");
     const int stages = (p.k + BK - 1) / BK;
     constexpr int kUnit = T::kGroups ? 2 : 1;  // whole groups per split (two stages each)
-    const int s_begin = static_cast<int>(static_cast<int64_t>(ks) * (stages / kUnit) / p.split) * kUnit;
-    const int s_end = static_cast<int>(static_cast<int64_t>(ks + 1) * (stages / kUnit) / p.split) * kUnit;
+    const int units = (stages + kUnit - 1) / kUnit;
+    const int s_begin = static_cast<int>(static_cast<int64_t>(ks) * units / p.split) * kUnit;
+    const int s_end = min(static_cast<int>(static_cast<int64_t>(ks + 1) * units / p.split) * kUnit, stages);
 
     // item i: row (tid + 256 i) / 8, chunk tid % 8
     const int chunk = tid & 7;
@@ -404,7 +441,7 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
 #pragma unroll
     for (int i = 0; i < kAItems; ++i) {
         const int r = (tid >> 3) + 32 * i;
-        asrc[i] = static_cast<const typename SA::elem_t*>(p.a) + static_cast<int64_t>(min(m0 + r, p.m - 1)) * p.k;
+        asrc[i] = static_cast<const typename SA::elem_t*>(p.a) + static_cast<int64_t>(min(m0 + r, p.m - 1)) * (T::kBlocks ? p.lda : p.k);
         adst[i] = r * kTileRow + ((chunk ^ tile_swz(r)) << 4);
     }
 #pragma unroll
@@ -441,13 +478,30 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
     auto load_w = [&](Regs& r, int i, int s) { r.w[i] = SW::load(wsrc[i] + (s * BK + chunk * SW::kElems) / SW::kPer); };
     // output column of the lane in its j-th tile (kGateUp: of gate and of up alike)
     auto column = [&](int j) { return T::kGateUp ? n0 / 2 + wn * 32 + l32 : n0 + (wn * TN + j) * 32 + l32; };
-    // the f16 scales of group g of the lane's columns
+    // the f16 scales of group g of the lane's columns; kBlocks: the scale of the lane's columns and
+    // those of its rows 8 q + 4 lh .. + 3 of each tile
     uint16_t sc[TN];
+    float sb[TN];
+    f32x4 sr[T::kBlocks ? TM : 1][4];
     auto load_scales = [&](int g) {
+        if constexpr (T::kBlocks) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const uint16_t* sg = T::kGateUp && j == 1 ? p.sg2 : p.sg;
-            sc[j] = sg[static_cast<int64_t>(min(column(j), rows_w - 1)) * (p.k / 128) + g];
+            for (int j = 0; j < TN; ++j)
+                sb[j] = p.sw[static_cast<int64_t>(min(n0 + (wn * TN + j) * 32, p.n - 1) >> 7) * ((p.k + 127) >> 7) + g];
+            const float* row = p.sa + static_cast<int64_t>(g) * p.m;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sr[i][q][e] = row[min(m0 + (wm * TM + i) * 32 + 8 * q + 4 * lh + e, p.m - 1)];
+        } else {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint16_t* sg = T::kGateUp && j == 1 ? p.sg2 : p.sg;
+                sc[j] = sg[static_cast<int64_t>(min(column(j), rows_w - 1)) * (p.k / 128) + g];
+            }
         }
     };
     // fragment of row r (of a plane at `base`) for step `step`
@@ -526,7 +580,11 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     if constexpr (kSets == 2) acc[0][i][j] += acc[1][i][j];
-                    if constexpr (T::kGroups) {
+                    if constexpr (T::kBlocks) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            tot[i][j][e] = fmaf(acc[0][i][j][e], sr[i][e >> 2][e & 3] * sb[j], tot[i][j][e]);
+                    } else if constexpr (T::kGroups) {
                         const float sj = 16.0f * __half2float(__ushort_as_half(sc[j]));
 #pragma unroll
                         for (int e = 0; e < 16; ++e) tot[i][j][e] = fmaf(acc[0][i][j][e], sj, tot[i][j][e]);
@@ -574,9 +632,12 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
             if constexpr (T::kFlush)
                 if (((s + 2 - s_begin) & (T::kFlushStages - 1)) == 0) flush();
         }
+        if constexpr (T::kBlocks)
+            if (s < s_full) load_scales(s / kUnit);
         if (s < s_full) stage(lds, lds + kStage, rg[1], s_last);
     }
     if (s_full < s_end) {  // the partial last stage (zeros past K)
+        if constexpr (T::kBlocks) load_scales(s_full / kUnit);
         const int k0 = s_full * BK + chunk * SA::kElems;
 #pragma unroll
         for (int i = 0; i < kAItems; ++i) {
@@ -592,7 +653,11 @@ __global__ __launch_bounds__(256, kOcc) void k_gemm_tile(TileArgs p) {
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) step_mfma(lds, step);
     }
-    if constexpr (!T::kGroups) flush();
+    if constexpr (T::kBlocks) {
+        if (p.k % (kUnit * BK) != 0 && s_end == stages && s_begin < s_end) flush();  // the partial last block
+    } else if constexpr (!T::kGroups) {
+        flush();
+    }
 
     auto sum = [&](int i, int j, int e) {
         if constexpr (T::kFlush)
@@ -698,6 +763,12 @@ template <class Val>
 struct TileCosts<GemmF32<Val>> {
     static constexpr TileShape shape[kTileShapes] = {{128, 128, 0, 0, 0, 0}, {64, 64, 785, 575, 5300, 2200}, {32, 128, 820, 535, 4650, 3150}, {64, 128, 1055, 840, 7200, 2770}};
     static constexpr int split = 3000;
+};
+
+template <>
+struct TileCosts<GemmF8Block> {
+    static constexpr TileShape shape[kTileShapes] = {{128, 128, 820, 1060, 8300, 8300}, {64, 64, 390, 260, 4770, 1190}, {32, 128, 550, 330, 4610, 1140}, {64, 128, 640, 500, 6430, 1450}};
+    static constexpr int split = 2600;
 };
 
 template <>

@@ -14,11 +14,15 @@ from .cache import KVBatch, KVCache, Rotary, tree_mask
 from .checkpoint import load_quantized, load_safetensors, save_quantized, save_safetensors
 from .errors import InvalidArgument, KernelError, OutOfMemory, TheanoError
 from .formats import (
+    dequantize_fp8_block,
     dequantize_i4_g128,
     dequantize_per_channel_fp8,
     dequantize_per_channel_i8,
     fake_quantize_per_channel_fp8,
     fake_quantize_per_channel_i8,
+    gemm_fp8_block,
+    quantize_fp8_block,
+    quantize_fp8_g128,
     quantize_i4_g128,
     quantize_per_channel_fp8,
     quantize_per_channel_i8,
@@ -39,5 +43,6 @@ __all__ = [
     "quantize_per_channel_fp8", "dequantize_per_channel_fp8", "fake_quantize_per_channel_fp8",
     "quantize_i4_g128", "dequantize_i4_g128", "repack_i4_g128_tiled", "repack_i4_g128_gate_up_tiled", "tile_rows_for", "Module", "QuantizedLinear", "QuantizedMLP", "QuantizedMultiheadAttention",
     "save_safetensors", "load_safetensors", "save_quantized", "load_quantized", "convert",
+    "quantize_fp8_block", "dequantize_fp8_block", "quantize_fp8_g128", "gemm_fp8_block",
     "Rotary", "KVBatch", "KVCache", "tree_mask",
 ]

@@ -111,6 +111,13 @@ SIGNATURES = {
     "tq_repack_w4g128_gate_up_tiled": [_p, _p, _p, _p, _i64, _i64, _p, _p, _p],
     "tq_mlp_w4g128_decode": [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p],
     "tq_mlp_w4g128_decode_noalloc": [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p, _p],
+    "tq_quantize_fp8_block": [_p, _i64, _i64, _p, _p, _p],
+    "tq_dequantize_fp8_block": [_p, _p, _i64, _i64, _p, _p],
+    "tq_quantize_fp8_g128": [_p, _int, _i64, _i64, _p, _p, _p],
+    "tq_gemm_fp8_block_workspace_bytes": [_i64, _i64, _i64],
+    "tq_gemm_fp8_block": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p],
+    "tq_linear_fp8_block_workspace_bytes": [_i64, _i64, _i64],
+    "tq_linear_fp8_block": [_p, _int, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p, _p],
     # descriptors are passed as the address of their ctypes structure
     "tq_rotary_apply": [_p, _p, _i64, _p, _p, _int, _i64, _p, _p, _p],
     "tq_kv_write": [_p, _p, _p, _p, _int, _p],
@@ -128,6 +135,7 @@ _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_
             "tq_linear_w8a8_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w8a8_workspace_bytes": ctypes.c_int64, "tq_gemm_fp8_workspace_bytes": ctypes.c_int64,
             "tq_kv_attention_workspace_bytes": ctypes.c_int64,
+            "tq_gemm_fp8_block_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_block_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w4g128_bf16_workspace_bytes": ctypes.c_int64, "tq_dtype_size": ctypes.c_int64}
 
 _lib = None

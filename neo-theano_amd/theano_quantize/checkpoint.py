@@ -28,7 +28,8 @@ becomes
     <name>.bias          F32 [N]      (when present)
 with ``__metadata__`` entries ``<name>.quant`` ("int8_per_channel",
 "int8_per_channel_a8" for W8A8, "int4_g128", "fp8_e4m3_per_channel" (FP8
-weight-only) or "fp8_e4m3_per_channel_a8" (FP8 weights and activations)),
+weight-only), "fp8_e4m3_per_channel_a8" (FP8 weights and activations) or
+"fp8_e4m3_block128" (FP8 with a scale F32 [ceil(N/128), ceil(K/128)] for each block)),
 ``<name>.group_size`` ("128",
 INT4), ``<name>.in_features`` and
 ``<name>.out_features``; a ``QuantizedMLP`` ``<name>`` is the three INT4
@@ -166,13 +167,15 @@ def _linear_entries(name, lin, tensors, meta):
         meta[f"{name}.quant"] = "int8_per_channel" if lin.mode == "w8" else "int8_per_channel_a8"
     elif lin.mode in ("fp8", "fp8_weight"):
         meta[f"{name}.quant"] = "fp8_e4m3_per_channel_a8" if lin.mode == "fp8" else "fp8_e4m3_per_channel"
+    elif lin.mode == "fp8_block":
+        meta[f"{name}.quant"] = "fp8_e4m3_block128"
     else:
         raise InvalidArgument(f"save_quantized: '{name}' has mode {lin.mode!r}")
     meta[f"{name}.in_features"] = str(lin.in_features)
     meta[f"{name}.out_features"] = str(lin.out_features)
     import torch
 
-    fp8 = lin.mode in ("fp8", "fp8_weight")
+    fp8 = lin.mode in ("fp8", "fp8_weight", "fp8_block")
     tensors[f"{name}.weight"] = lin.qweight.view(torch.float8_e4m3fn) if fp8 else lin.qweight
     tensors[f"{name}.weight_scale"] = lin.scales
     if lin.bias is not None:
@@ -257,12 +260,14 @@ def _load(tensors, meta, dtypes, device):
             s = dev(_need(tensors, f"{name}.weight_scale", np.float16, (n, k // 128)).view(np.int16))
             s = s.view(torch.float16)
             mode = "w4"
-        elif kind in ("fp8_e4m3_per_channel", "fp8_e4m3_per_channel_a8"):
+        elif kind in ("fp8_e4m3_per_channel", "fp8_e4m3_per_channel_a8", "fp8_e4m3_block128"):
             if dtypes.get(f"{name}.weight") != "F8_E4M3":
                 raise InvalidArgument(f"load_quantized: '{name}.weight' is not F8_E4M3")
+            block = kind == "fp8_e4m3_block128"
             q = dev(_need(tensors, f"{name}.weight", np.uint8, (n, k)))
-            s = dev(_need(tensors, f"{name}.weight_scale", np.float32, (n,)))
-            mode = "fp8" if kind.endswith("_a8") else "fp8_weight"
+            s = dev(_need(tensors, f"{name}.weight_scale", np.float32,
+                          ((n + 127) // 128, (k + 127) // 128) if block else (n,)))
+            mode = "fp8_block" if block else "fp8" if kind.endswith("_a8") else "fp8_weight"
         elif kind in ("int8_per_channel", "int8_per_channel_a8"):
             q = dev(_need(tensors, f"{name}.weight", np.int8, (n, k)))
             s = dev(_need(tensors, f"{name}.weight_scale", np.float32, (n,)))

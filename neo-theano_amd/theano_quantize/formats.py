@@ -8,6 +8,8 @@
   its [-448, 448] range, qconfig.rs:29,38): s_r = f32(max(absmax_r/448, 1e-10)),
   q = e4m3_rne(clamp(f32(x/s_r), -448, 448)), NaN -> 0x7F.  Codes are kept as
   uint8 bit patterns (``q.view(torch.float8_e4m3fn)`` reads them as floats).
+* FP8 with a scale for each block of 128 x 128 of a weight, and for each 128 columns of
+  an activation row: the same codes, absmax over the block.
 """
 from __future__ import annotations
 
@@ -87,6 +89,70 @@ def fake_quantize_per_channel_fp8(weight):
     out = torch.empty((n, k), dtype=torch.float32, device=w.device)
     _abi.call("tq_fake_quantize_fp8_rowwise", ptr(w), n, k, ptr(q), ptr(s), ptr(out), stream())
     return q, s, out
+
+
+def quantize_fp8_block(weight):
+    """FP8 e4m3 in blocks of 128 x 128 -> (codes uint8 [N, K], scales f32 [ceil(N/128), ceil(K/128)])."""
+    w = _as_2d(weight, "quantize_fp8_block")
+    n, k = w.shape
+    q = torch.empty((n, k), dtype=torch.uint8, device=w.device)
+    s = torch.empty(((n + GROUP - 1) // GROUP, (k + GROUP - 1) // GROUP), dtype=torch.float32, device=w.device)
+    _abi.call("tq_quantize_fp8_block", ptr(w), n, k, ptr(q), ptr(s), stream())
+    return q, s
+
+
+def _block_scales(q, s, name):
+    s = on_device(s, torch.float32, name)
+    if q.dim() != 2 or tuple(s.shape) != tuple((d + GROUP - 1) // GROUP for d in q.shape):
+        raise InvalidArgument(f"{name}: codes {tuple(q.shape)} with scales {tuple(s.shape)}")
+    return s
+
+
+def dequantize_fp8_block(q, s):
+    """w_hat = f32(e4m3(q) * s[row // 128, column // 128])."""
+    q = on_device(q, torch.uint8, "dequantize_fp8_block")
+    s = _block_scales(q, s, "dequantize_fp8_block")
+    out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    _abi.call("tq_dequantize_fp8_block", ptr(q), ptr(s), q.shape[0], q.shape[1], ptr(out), stream())
+    return out
+
+
+_ACT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # tq_dtype
+
+
+def quantize_fp8_g128(x):
+    """Activations [M, K] (f32, bf16 or f16) in rows of 128 columns -> (codes uint8 [M, K rounded up to
+    128], zeros past K, scales f32 [ceil(K/128), M])."""
+    code = _ACT_TYPES.get(x.dtype)
+    if code is None or x.dim() != 2:
+        raise InvalidArgument(f"quantize_fp8_g128: expected a float32, bfloat16 or float16 [M, K] tensor, got {x.dtype} "
+                              f"{tuple(x.shape)}")
+    x = on_device(x, x.dtype, "quantize_fp8_g128")
+    m, k = x.shape
+    kb = (k + GROUP - 1) // GROUP
+    q = torch.empty((m, kb * GROUP), dtype=torch.uint8, device=x.device)
+    s = torch.empty((kb, m), dtype=torch.float32, device=x.device)
+    _abi.call("tq_quantize_fp8_g128", ptr(x), code, m, k, ptr(q), ptr(s), stream())
+    return q, s
+
+
+def gemm_fp8_block(qa, sa, qw, sw, bias=None):
+    """y [M, N] = sum_b sa[b, m] sw[n // 128, b] (qa qw^T over block b) (+ bias) of the codes and scales of
+    quantize_fp8_g128 and quantize_fp8_block; sums and y in f32."""
+    qa, qw = on_device(qa, torch.uint8, "gemm_fp8_block"), on_device(qw, torch.uint8, "gemm_fp8_block")
+    sw, sa = _block_scales(qw, sw, "gemm_fp8_block"), on_device(sa, torch.float32, "gemm_fp8_block")
+    (m, kp), (n, k) = qa.shape, qw.shape
+    if kp != (k + GROUP - 1) // GROUP * GROUP or tuple(sa.shape) != (kp // GROUP, m):
+        raise InvalidArgument(f"gemm_fp8_block: activations {tuple(qa.shape)}, scales {tuple(sa.shape)} for weights {tuple(qw.shape)}")
+    if bias is not None:
+        bias = on_device(bias, torch.float32, "gemm_fp8_block: bias")
+        if tuple(bias.shape) != (n,):
+            raise InvalidArgument(f"gemm_fp8_block: bias {tuple(bias.shape)} for {n} outputs")
+    y = torch.empty((m, n), dtype=torch.float32, device=qa.device)
+    nb = _abi.entry("tq_gemm_fp8_block_workspace_bytes")(m, n, k)
+    ws = torch.empty(nb, dtype=torch.uint8, device=qa.device) if nb > 0 else None
+    _abi.call("tq_gemm_fp8_block", ptr(qa), ptr(sa), ptr(qw), ptr(sw), ptr(bias), m, n, k, ptr(ws), max(nb, 0), ptr(y), stream())
+    return y
 
 
 def quantize_i4_g128(weight):

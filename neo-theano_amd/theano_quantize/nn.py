@@ -15,6 +15,9 @@ Modes (chosen from the QConfig):
            (QConfig.default_int4());
   * "fp8"  FP8 e4m3 weights per output channel and per-row dynamic FP8
            activations (QConfig with weight_dtype and activation_dtype FP8);
+  * "fp8_block"  FP8 e4m3 weights with a scale for each 128 x 128 block and
+           activations (f32, bf16 or f16) coded with one for each 128 columns of a row
+           (QConfig.fp8_block(), or codes and scales of a checkpoint);
   * "fp8_weight"  FP8 e4m3 weight-only, f32 activations (weight_dtype FP8,
            activations not FP8).
 Decode shapes (a few tokens) run the dequant-GEMV kernels; in "w8a8" and "fp8"
@@ -32,8 +35,8 @@ import torch
 from . import _abi
 from ._tensor import on_device, ptr, stream
 from .errors import InvalidArgument
-from .formats import (quantize_i4_g128, quantize_per_channel_fp8, quantize_per_channel_i8, repack_i4_g128_gate_up_tiled,
-                      repack_i4_g128_tiled)
+from .formats import (_ACT_TYPES, quantize_fp8_block, quantize_i4_g128, quantize_per_channel_fp8, quantize_per_channel_i8,
+                      repack_i4_g128_gate_up_tiled, repack_i4_g128_tiled)
 from .qconfig import QConfig, QuantDType
 
 DECODE_MAX_M = 16
@@ -81,6 +84,10 @@ class Module:
 
 
 def _mode_of(qconfig: QConfig) -> str:
+    if qconfig.block:
+        if qconfig.weight_dtype != QuantDType.FP8 or qconfig.activation_dtype != QuantDType.FP8:
+            raise InvalidArgument("QuantizedLinear: block scales are for FP8 weights and activations")
+        return "fp8_block"
     if qconfig.weight_dtype == QuantDType.Int4:
         return "w4"
     if qconfig.weight_dtype == QuantDType.Int8:
@@ -106,6 +113,14 @@ class QuantizedLinear(Module):
         self.scales = scales
         self.bias = bias
         self.tiled = None
+        if mode == "fp8_block":
+            shape = (self.out_features + 127) // 128, (self.in_features + 127) // 128
+            if qweight.dtype != torch.uint8 or tuple(qweight.shape) != (self.out_features, self.in_features) or \
+                    scales.dtype != torch.float32 or tuple(scales.shape) != shape or not qweight.is_contiguous() or \
+                    not scales.is_contiguous() or (bias is not None and (bias.dtype != torch.float32 or
+                                                                         tuple(bias.shape) != (self.out_features,))):
+                raise InvalidArgument(f"QuantizedLinear: fp8_block takes contiguous uint8 [{self.out_features}, "
+                                      f"{self.in_features}] codes, float32 {shape} scales and a float32 bias")
         if tiled and mode == "w4" and self.in_features <= 16384:
             # row-tiled copy (a permutation of qweight) for the decode GEMV (passes
             # of 16 tokens up to M = 32)
@@ -122,6 +137,8 @@ class QuantizedLinear(Module):
         out_f, in_f = w.shape
         if mode == "w4":
             q, s = quantize_i4_g128(w)
+        elif mode == "fp8_block":
+            q, s = quantize_fp8_block(w)
         elif mode in ("fp8", "fp8_weight"):
             q, s = quantize_per_channel_fp8(w)
         else:
@@ -150,7 +167,10 @@ class QuantizedLinear(Module):
                   y.data_ptr(), st)
 
     def forward(self, x):
-        x = on_device(x, self._act_dtype(), "QuantizedLinear.forward")
+        act = self._act_dtype()
+        if self.mode == "fp8_block" and isinstance(x, torch.Tensor) and x.dtype in _ACT_TYPES:
+            act = x.dtype
+        x = on_device(x, act, "QuantizedLinear.forward")
         squeeze = x.dim() == 1
         if squeeze:
             x = x.unsqueeze(0)
@@ -162,7 +182,14 @@ class QuantizedLinear(Module):
         m = x.shape[0]
         y = x.new_empty((m, n), dtype=torch.float32)
         mode, st = self.mode, stream()
-        if mode == "w4":
+        if mode == "fp8_block":
+            if x.device != self.qweight.device or x.device.index != torch._C._cuda_getDevice():
+                raise InvalidArgument("QuantizedLinear.forward: input, weight and current device differ")
+            nb = _abi.entry("tq_linear_fp8_block_workspace_bytes")(m, n, k)
+            ws = x.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
+            _abi.call("tq_linear_fp8_block", x.data_ptr(), _ACT_TYPES[act], m, self.qweight.data_ptr(),
+                      self.scales.data_ptr(), ptr(self.bias), n, k, ptr(ws), max(nb, 0), y.data_ptr(), st)
+        elif mode == "w4":
             bias = ptr(self.bias)
             if m <= TILED_PASSES_MAX_M and self.tiled is not None:
                 pt, ts, t = self.tiled
@@ -293,9 +320,13 @@ class QuantizedMultiheadAttention(Module):
         self.embed_dim, self.num_heads, self.head_dim = e, int(num_heads), e // int(num_heads)
         self.qkv, self.out_proj = qkv, out_proj
         self._parts = []
+        block = qkv.mode == "fp8_block"
+        if block and e % 128:
+            raise InvalidArgument("QuantizedMultiheadAttention: fp8_block needs embed_dim % 128 == 0 (blocks of q, k and v apart)")
         for i in range(3):  # row slices (views) of the fused weight
             rows = slice(i * e, (i + 1) * e)
-            self._parts.append(QuantizedLinear(qkv.mode, e, e, qkv.qweight[rows], qkv.scales[rows],
+            srows = slice(i * e // 128, (i + 1) * e // 128) if block else rows
+            self._parts.append(QuantizedLinear(qkv.mode, e, e, qkv.qweight[rows], qkv.scales[srows],
                                                None if qkv.bias is None else qkv.bias[rows], tiled=False))
 
     @staticmethod
@@ -362,6 +393,24 @@ class QuantizedMultiheadAttention(Module):
             q, k, v = (part(self._act(x)) for part, x in zip(self._parts, flat))
             o = self._attend(q, k, v, e, e, e, batch, seq, mask)
         return self.out_proj(self._act(o)).reshape(batch, seq, e)
+
+    def forward_cached(self, x, cache, new, rotary=None, positions=None, tree=None):
+        """The layer over a KVCache, for the rows of a KVBatch: x [rows, embed_dim] (f32) is projected, q and k
+        are turned (where a Rotary is given), k and v stored, and the rows attend to what the cache holds
+        of their sequences (causally, or as `tree` says).  Returns [rows, embed_dim]."""
+        x = on_device(x, torch.float32, "QuantizedMultiheadAttention.forward_cached")
+        e, h, d = self.embed_dim, self.num_heads, self.head_dim
+        if tuple(x.shape) != (new.rows, e) or cache.heads != h or cache.head_dim != d:
+            raise InvalidArgument(f"QuantizedMultiheadAttention.forward_cached: x {tuple(x.shape)} for {new.rows} rows of {e}, "
+                                  f"a cache of {cache.heads} heads of {cache.head_dim} for {h} of {d}")
+        qkv = self.qkv(self._act(x))
+        q, k, v = (qkv[:, i * e:(i + 1) * e].view(new.rows, h, d) for i in range(3))
+        if rotary is None:
+            cache.write(k, v, new)
+        else:
+            q = cache.write_rotary(q, k, v, rotary, new, positions)
+        o = cache.attention(q, new, tree=tree).view(new.rows, e)
+        return self.out_proj(self._act(o))
 
     def forward_qkv(self, query, key, value):
         return self.forward_with_mask(query, key, value, None)

@@ -42,12 +42,19 @@ class QConfig:
 
     As in the reference, `symmetric` and `per_channel` are recorded; the
     quantized Linear here always uses symmetric per-output-channel INT8 or
-    symmetric group-128 INT4 weights, selected by `weight_dtype`."""
+    symmetric group-128 INT4 weights, selected by `weight_dtype`.  `block` (not in
+    the reference; FP8 weights and activations) takes a scale for each block of 128
+    instead of one per output channel and token."""
 
     weight_dtype: QuantDType
     activation_dtype: QuantDType
     symmetric: bool
     per_channel: bool
+    block: bool = False
+
+    @staticmethod
+    def fp8_block() -> "QConfig":
+        return QConfig(QuantDType.FP8, QuantDType.FP8, True, False, True)
 
     @staticmethod
     def default_int8() -> "QConfig":  # qconfig.rs:53-60
