@@ -22,6 +22,7 @@
 // Work is split along the keys by units of 128: the units of all sequences, heads and row
 // tiles in one line, cut into equal shares for a grid that fits the chip at once, whatever the lengths.  A share that
 // is not a whole (sequence, head, tile) leaves maximum, sum and O in the workspace, and a second launch joins them in order.
+#include <algorithm>
 #include <cmath>
 
 #include "tq_kv.h"
@@ -180,6 +181,13 @@ __device__ __forceinline__ f32x4 mfma_f16(h8 a, h8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// x, as a value the compiler knows nothing of: what is computed from it is computed here, not
+// before a loop and kept in registers that the loop needs
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // max over the lanes l, l ^ 16, l ^ 32, l ^ 48 (the four that hold a row)
@@ -313,6 +321,24 @@ __device__ __forceinline__ void load_8(const void* p, int64_t i, int dtype, floa
             x[2 * e + 1] = static_cast<float>(h.y);
         }
     }
+}
+
+// 8 adjacent elements, 16-byte aligned
+__device__ __forceinline__ void store_8(void* p, int64_t i, int dtype, const float (&x)[8]) {
+    if (dtype == TQ_DT_F32) {
+        f32x4* o = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);
+        o[0] = f32x4{x[0], x[1], x[2], x[3]};
+        o[1] = f32x4{x[4], x[5], x[6], x[7]};
+        return;
+    }
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        w[e] = dtype == TQ_DT_BF16
+                   ? __builtin_bit_cast(uint32_t, (b2{static_cast<__bf16>(x[2 * e]), static_cast<__bf16>(x[2 * e + 1])}))
+                   : __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(x[2 * e]), static_cast<_Float16>(x[2 * e + 1])}));
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = u32x4{w[0], w[1], w[2], w[3]};
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -579,7 +605,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
                         for (int w = 0; w < VBytes<kDP>::kWords; ++w) {
                             const uint32_t x = vb[j].w[w];
                             const uint32_t top_bits = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                            vb[j].w[w] = x & ~((top_bits >> 7) * 0xFFu);
+                            vb[j].w[w] = x & ~((top_bits << 1) - (top_bits >> 7));
                         }
                 }
             }
@@ -672,38 +698,62 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
     }
 }
 
-// Joins the shares of the items that several blocks worked on: a wave for each row, 2 kDP / 128
-// elements of it in each lane.
-template <int kDP, int kNQ>
+// Joins the shares of the items that several blocks worked on: kW waves for each row (of 4 in
+// a block), which take the item's shares in turn; kDP / 64 elements of the row in each lane.  64 shares'
+// maxima and sums lie in the lanes at a time, so the loads of their O rows depend on nothing
+// (a loop over the shares that waited for each one's maximum took 23.5 us for 64 shares of 32 rows, this one 4.9).
+template <int kDP, int kTile, int kW>
 __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
-    constexpr int kTile = 16 * kNQ, kE = (kDP + 63) / 64;
-    const int lane = threadIdx.x & 63;
-    const int row = blockIdx.y * kAttWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kE = (kDP + 63) / 64;
+    __shared__ float x_lds[kAttWaves][kE * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = blockIdx.y * (kAttWaves / kW) + wave / kW, part = wave % kW;
     const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
     const Item it = find_item<kTile, false>(a, s0, blockIdx.x, lane);
-    if (!it.ok || it.tile * kTile + row >= it.rows * a.group) return;
+    if (!it.ok) return;  // (kW > 1: row is the block's, so whole blocks leave)
+    if (it.tile * kTile + row >= it.rows * a.group) return;
     const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
     const Shares sh(units, a.blocks);
     const int b0 = sh.of(it.unit0), b1 = sh.of(it.unit0 + it.units - 1);
     if (b0 == b1) return;  // one block had it all
-    const float* ml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP);
-    const int64_t skip = sh.begin(b0) == it.unit0 ? 0 : 1;
-    auto slot = [&](int b) { return 2 * static_cast<int64_t>(b) + (b == b0 ? skip : 0); };
+    const float* ml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP) + 2 * row;
+    const int skip = sh.begin(b0) == it.unit0 ? 0 : 1;
+    auto slot = [&](int b) { return static_cast<int64_t>(2 * b + (b == b0 ? skip : 0)) * kTile; };
     float top = -INFINITY;
-    for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, ml[(slot(b) * kTile + row) * 2]);
+    for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, ml[2 * slot(b)]);
     top = wave_max(top);
     float sum = 0.f, x[kE] = {};
-    for (int b = b0; b <= b1; ++b) {
-        const int64_t s = slot(b);
-        const float mb = ml[(s * kTile + row) * 2], lb = ml[(s * kTile + row) * 2 + 1];
-        const float f = mb == -INFINITY ? 0.f : exp2_hw(mb - top);
-        sum = fmaf(lb, f, sum);
-        const float* po = a.part + (s * kTile + row) * kDP;
+    for (int c = b0; c <= b1; c += 64) {
+        const int b = min(c + lane, b1);
+        const float mb = ml[2 * slot(b)], lb = ml[2 * slot(b) + 1];
+        const float f = mb == -INFINITY || c + lane > b1 ? 0.f : exp2_hw(mb - top);
+        sum += wave_sum(lb * f);
+        const int n = min(64, b1 - c + 1);
+        for (int i = part; i < n; i += 8 * kW) {  // eight shares' rows in flight
+            float v[8][kE], fi[8];
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-            const int d = lane + 64 * e;
-            if (d < kDP) x[e] = fmaf(po[d], f, x[e]);
+            for (int u = 0; u < 8; ++u) {
+                const int j = min(i + u * kW, n - 1);
+                fi[u] = i + u * kW < n ? readlane(f, j) : 0.f;
+                const float* po = a.part + (slot(c + j) + row) * kDP;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) v[u][e] = po[min(lane + 64 * e, kDP - 1)];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < kE; ++e) x[e] = i + u * kW < n ? fmaf(v[u][e], fi[u], x[e]) : x[e];
         }
+    }
+    if constexpr (kW > 1) {
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x_lds[wave][lane + 64 * e] = x[e];
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int w = 1; w < kW; ++w)
+#pragma unroll
+            for (int e = 0; e < kE; ++e) x[e] += x_lds[wave + w][lane + 64 * e];
     }
     const int rr = it.tile * kTile + row, t = static_cast<int>(a.by_group.div(rr));
     const int64_t dst = ((it.first + static_cast<int64_t>(t)) * (static_cast<int64_t>(a.heads) * a.group) +
@@ -715,23 +765,444 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
     }
 }
 
+// ------------------------------------------------------------------ many rows
+// More than 32 rows of a sequence's head: converting the codes for each 16 of them would cost more than
+// the products, so four waves share the keys, 64 at a time, converted once into LDS as the very fragments
+// that the matrix cores take (16 bytes a lane, read without conflicts).  Wave (wq, wk) has rows 32 wq ..
+// of the tile and, with two row groups, the wk-th 32 of the 64 keys; v_mfma_f32_32x32x16_f16:
+//  * S^T = K Q^T: lane (r, h) = (l % 32, l / 32) gives key r's elements 16 s + 8 h .. + 7 in step s and
+//    gets the scores of keys 8 (e / 4) + 4 h + e % 4 for row r;
+//  * which are, 8 at a time, the k-slots of P^T in O^T += V^T P^T; V's fragment holds the same keys at
+//    element d = 32 c + 4 (r % 8) + r / 8, so that a thread that loaded 4 adjacent elements of 8 keys
+//    writes them where its neighbours write the next ones, and lane (r, h) ends up with the 16
+//    adjacent elements 32 c + 16 h .. of row r.
+// One power of two scales q in the whole tile (rows up to 2^17 times smaller than the largest keep
+// their 22 bits), so a score is one fma: t = S (sk scale 2^e) + log2 sv.  Keys with no place become
+// zero codes with log2 sv = -inf, and only tiles that some row sees in part pay for a mask.
+template <int kDP, int kWQ, class Codes, int kPlanes>
+__global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
+    constexpr int kTile = 32 * kWQ, kWK = kAttWaves / kWQ;
+    constexpr int kKeys = 64, kSub = 2 / kWK;      // keys of a turn; 32-key halves of a wave
+    constexpr int kSteps = kDP / 16, kCols = kDP / 32;
+    constexpr int kKF = 2 * kSteps * 64, kVF = 4 * kCols * 64;  // 16-byte fragments of a turn
+    constexpr int kRun = kDP / 4, kQuads = kDP / 4;
+    constexpr int kORow = kDP + 4;
+    struct Buf {
+        h8 k[kKF], v[kVF];
+        float ck[kKeys], lsv[kKeys], rsv[kKeys];
+        uint8_t bad[Codes::kNan ? kKeys * kQuads : 4];
+        int any_bad[kAttWaves];
+    };
+    // the tile's rows as f32, q before the keys and o after them, in the buffers' place
+    constexpr size_t kRowBytes = sizeof(float) * kTile * kORow;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * sizeof(Buf) > kRowBytes ? 2 * sizeof(Buf) : kRowBytes];
+    __shared__ float m_lds[kAttWaves][32], l_lds[kTile];
+    Buf* buf = reinterpret_cast<Buf*>(lds);
+    float* rows = reinterpret_cast<float*>(lds);
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wq = wave % kWQ, wk = wave / kWQ;
+
+    int at, end;
+    if (a.part) {
+        const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
+        const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
+        const Shares sh(units, a.blocks);
+        at = sh.begin(blockIdx.x);
+        end = sh.begin(blockIdx.x + 1);
+    } else {
+        at = 0;
+        end = 1;
+    }
+    bool first_share = true;
+    while (at < end) {
+        const SeqLane s0 = seq_lane<kTile>(a, 0, here(lane));  // (again for each item: it would hold ten registers)
+        const Item it = a.part ? find_item<kTile, true>(a, s0, at, lane) : find_item<kTile, false>(a, s0, blockIdx.x, lane);
+        if (!it.ok) return;
+        const int u_first = a.part ? at - it.unit0 : 0;
+        const int u_count = a.part ? min(it.units - u_first, end - at) : it.units;
+        const int n_rows = it.rows * a.group, row0 = it.tile * kTile;
+
+        // what the block's and the wave's rows see: every key before `all`, none from `lim` on
+        auto sees = [&](int row_a, int row_b, int& all, int& lim) {
+            const int ta = static_cast<int>(a.by_group.div(min(row_a, n_rows - 1)));
+            const int tb = static_cast<int>(a.by_group.div(min(row_b, n_rows - 1)));
+            lim = a.tree ? it.len : min(it.base + tb + 1, it.len);
+            all = a.tree ? it.base : it.base + ta + 1;
+        };
+        int all_b, lim_b, all_w, lim_w;
+        sees(row0, row0 + kTile - 1, all_b, lim_b);
+        sees(row0 + 32 * wq, row0 + 32 * wq + 31, all_w, lim_w);
+        const bool idle = row0 + 32 * wq >= n_rows;  // a wave without rows
+
+        // where row `row` of the tile lies in q (token and head strides) or in the output
+        auto row_at = [&](int row, int64_t token, int64_t head) {
+            const int rr = row0 + row, t = static_cast<int>(a.by_group.div(rr));
+            return (it.first + static_cast<int64_t>(t)) * token + (static_cast<int64_t>(it.head) * a.group + (rr - t * a.group)) * head;
+        };
+        const int valid = min(kTile, n_rows - row0);
+#pragma unroll 1
+        for (int i = here(tid); i < kTile * (kDP / 8); i += kAttBlock) {
+            const int row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
+            float x[8] = {};
+            if (row < valid && d0 < a.d) {
+                const int64_t at_q = row_at(row, a.q_token, a.q_head) + d0;
+                if (a.q_vec) {
+                    load_8(a.q, at_q, a.dtype, x);
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < 8 && d0 + j < a.d; ++j) rows[row * kORow + d0 + j] = load_elem(a.q, at_q + j, a.dtype);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.d ? rows[row * kORow + d0 + j] : 0.f;
+                }
+            }
+            f32x4* o = reinterpret_cast<f32x4*>(&rows[row * kORow + d0]);
+            o[0] = f32x4{x[0], x[1], x[2], x[3]};
+            o[1] = f32x4{x[4], x[5], x[6], x[7]};
+        }
+        __syncthreads();
+
+        // q: row r of the wave's 32, elements 16 s + 8 h + j
+        const int row = 32 * wq + r;
+        const int t_row = static_cast<int>(a.by_group.div(min(row0 + row, n_rows - 1)));
+        h8 q[kPlanes][kSteps];
+        float rq;
+        {
+            const float* mine = &rows[here(row) * kORow + 8 * h];
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const f32x4 u = *reinterpret_cast<const f32x4*>(mine + 16 * s), v = *reinterpret_cast<const f32x4*>(mine + 16 * s + 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(u[j]), fabsf(v[j])));
+            }
+            // the row's largest (its two lanes), 0 where it is not finite: such a row is NaN by itself
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+            top = wave_max(top < INFINITY ? top : 0.f);
+            if (lane == 0) m_lds[wave][0] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(m_lds[0][0], m_lds[1][0]), fmaxf(m_lds[2][0], m_lds[3][0]));
+            const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+            rq = a.scale2 * ldexpf(1.0f, e);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    _Float16 hi, lo;
+                    to_planes<kPlanes>(ldexpf(mine[16 * s + j], -e), hi, lo);
+                    q[0][s][j] = hi;
+                    if constexpr (kPlanes == 2) q[1][s][j] = lo;
+                }
+                if (s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            __syncthreads();  // the rows are read: the buffers may be filled
+        }
+
+        f32x16 o[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] = f32x16{};
+        float m = -INFINITY, l = 0.f;
+
+        const int k_begin = u_first * kUnit;
+        const int k_end = min((u_first + u_count) * kUnit, lim_b);
+        const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
+
+        // ---- staging: raw codes of a turn in registers, then fragments in LDS
+        // K: key `lane`, bytes kRun wave ..; V: keys 16 vt + 4 vh + {0..3, 8..11}, elements 4 vd ..
+        const int vd = tid % kQuads, vth = tid / kQuads, vt = vth >> 1, vh = vth & 1;
+        const bool v_on = vth < 8;
+        uint32_t kw[kRun / 4], vw[8];
+        float sk = 0.f, sv = 0.f;
+        bool k_ok = false, v_ok = false;
+        auto place = [&](int key, bool& ok) -> int64_t {
+            ok = key < it.len;
+            const int kk = ok ? key : 0, i = static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(kk)));
+            int page = table[i];
+            if (page < 0 || page >= a.b.pages) {
+                page = 0;
+                ok = false;
+            }
+            return (static_cast<int64_t>(page) * a.heads + it.head) * a.b.page + (kk - i * a.b.page);
+        };
+        auto load = [&](int key) {
+            const int64_t rk = place(key + lane, k_ok);
+            KBytes<kDP> kb;
+            kb.load(a.k + rk * kDP + kRun * wave);
+#pragma unroll
+            for (int i = 0; i < kRun / 4; ++i) kw[i] = kb.w[i];
+            if (wave == 0) {
+                sk = a.k_scale[rk];
+                sv = a.v_scale[rk];
+            }
+            if (v_on) {
+                // the first of the sixteen keys decides: a page holds whole sixteens, and keys past the length read
+                // what lies there and are dropped by their scale
+                const int64_t rv = place(key + 16 * vt, v_ok);
+                const uint8_t* p = a.v + (rv + 4 * vh) * kDP + 4 * vd;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    vw[j] = *reinterpret_cast<const uint32_t*>(p + ((j & 3) + 8 * (j >> 2)) * kDP);
+            }
+        };
+        auto store = [&](Buf& b, int key) {
+#pragma unroll
+            for (int i = 0; i < kRun / 8; ++i) {
+                const int gi = wave * (kRun / 8) + i;  // elements 8 gi ..: step gi / 2, half gi % 2
+                const uint32_t w0 = Codes::ready(k_ok ? kw[2 * i] : 0u), w1 = Codes::ready(k_ok ? kw[2 * i + 1] : 0u);
+                b.k[((lane >> 5) * kSteps + (gi >> 1)) * 64 + (gi & 1) * 32 + (lane & 31)] =
+                    join(Codes::template pair<false>(w0), Codes::template pair<true>(w0),
+                         Codes::template pair<false>(w1), Codes::template pair<true>(w1));
+            }
+            if (wave == 0) {
+                const float c = fmaxf(sv, 1e-25f);
+                b.ck[lane] = k_ok ? sk * rq : 0.f;
+                b.lsv[lane] = k_ok ? __builtin_amdgcn_logf(sv != sv ? sv : c) : -INFINITY;
+                b.rsv[lane] = k_ok ? __builtin_amdgcn_rcpf(c) : 0.f;
+            }
+            uint32_t bad_here = 0;
+            if (v_on) {
+                const int to = Codes::kNan && kPlanes == 2 ? here(tid) : tid;  // (one form is short of registers)
+                const int vd = to % kQuads, vth = to / kQuads, vt = vth >> 1, vh = vth & 1;
+                const int k16 = key + 16 * vt + 4 * vh;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool ok = v_ok && k16 + (j & 3) + 8 * (j >> 2) < it.len;
+                    vw[j] = ok ? vw[j] : 0u;
+                }
+                if (Codes::kNan && key + kKeys > all_b) {  // rows that do not see a key must not meet its NaN
+                    const int t3 = here(tid);
+                    uint8_t* bad = &b.bad[(16 * (t3 / kQuads >> 1) + 4 * (t3 / kQuads & 1)) * kQuads + t3 % kQuads];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t x = vw[j], top = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                        vw[j] = x & ~((top << 1) - (top >> 7));
+                        const uint32_t bits = (top >> 7 & 1) | (top >> 14 & 2) | (top >> 21 & 4) | (top >> 28 & 8);
+                        bad[((j & 3) + 8 * (j >> 2)) * kQuads] = static_cast<uint8_t>(bits);
+                        bad_here |= bits;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) vw[j] = Codes::ready(vw[j]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    h2 lo[4], hi[4];
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const uint32_t w = __builtin_amdgcn_perm(vw[j + 1], vw[j], half ? 0x07030602u : 0x05010400u);
+                        lo[j >> 1] = Codes::template pair<false>(w);
+                        hi[j >> 1] = Codes::template pair<true>(w);
+                    }
+                    // element 4 vd + i at row 8 i + vd % 8 of column block vd / 8
+                    h8* f = &b.v[(vt * kCols + (vd >> 3)) * 64 + vh * 32 + (vd & 7)];
+                    f[8 * (2 * half)] = join(lo[0], lo[1], lo[2], lo[3]);
+                    f[8 * (2 * half + 1)] = join(hi[0], hi[1], hi[2], hi[3]);
+                }
+            }
+            if (Codes::kNan) b.any_bad[wave] = __ballot(bad_here != 0) != 0;
+        };
+        auto row_sees = [&](int key) {
+            if (!a.tree) return key < min(it.base + t_row + 1, it.len);
+            const int j = key - it.base;
+            if (key >= it.len || j >= it.rows) return false;
+            if (j < 0) return true;
+            return ((a.tree[(it.first + static_cast<int64_t>(t_row)) * a.tree_words + (j >> 5)] >> (j & 31)) & 1) != 0;
+        };
+
+        if (k_begin < k_end) {
+            load(k_begin);
+            store(buf[0], k_begin);
+            __builtin_amdgcn_sched_barrier(0);
+            load(k_begin + kKeys < k_end ? k_begin + kKeys : k_begin);
+        }
+        __syncthreads();
+        int bi = 0;
+        for (int key = k_begin; key < k_end; key += kKeys, bi ^= 1) {
+            const Buf& b = buf[bi];
+            if (!idle) {
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {
+                    const int sub = kWK == 2 ? wk : u, k32 = key + 32 * sub;
+                    if (k32 >= lim_w) continue;  // uniform: nothing that the wave's rows see
+                    f32x16 st = f32x16{};
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s) {
+                        const h8 kf = b.k[(sub * kSteps + s) * 64 + lane];
+#pragma unroll
+                        for (int p = 0; p < kPlanes; ++p)
+                            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[p][s], st, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    float t[16];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int k4 = 32 * sub + 8 * c + 4 * h;
+                        const f32x4 ck = *reinterpret_cast<const f32x4*>(&b.ck[k4]);
+                        const f32x4 ls = *reinterpret_cast<const f32x4*>(&b.lsv[k4]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t[4 * c + e] = fmaf(st[4 * c + e], ck[e], ls[e]);
+                    }
+                    const bool slow = k32 + 32 > all_w;  // uniform
+                    if (slow) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            t[e] = row_sees(k32 + 8 * (e >> 2) + 4 * h + (e & 3)) ? t[e] : -INFINITY;
+                            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    float top = t[0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) top = fmaxf(top, t[e]);
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                    top = fmaxf(m, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kPShift);
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    if (__ballot(top != m)) {
+                        const float alpha = exp2_hw(m - ref);
+                        l *= alpha;
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) o[c] *= alpha;
+                        m = top;
+                    }
+                    h8 pf[2][kPlanes];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const f32x4 rv = *reinterpret_cast<const f32x4*>(&b.rsv[32 * sub + 8 * c + 4 * h]);
+#pragma unroll
+                        for (int e = 4 * c; e < 4 * c + 4; ++e) {
+                            const float p = exp2_hw(t[e] - ref);
+                            l = fmaf(p, rv[e & 3], l);
+                            _Float16 hi, lo;
+                            to_planes<kPlanes>(p, hi, lo);
+                            pf[e >> 3][0][e & 7] = hi;
+                            if constexpr (kPlanes == 2) pf[e >> 3][1][e & 7] = lo;
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) {
+                            const h8 vf = b.v[((2 * sub + t2) * kCols + c) * 64 + lane];
+#pragma unroll
+                            for (int p = 0; p < kPlanes; ++p)
+                                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t2][p], o[c], 0, 0, 0);
+                        }
+                    if (Codes::kNan && key + kKeys > all_b &&
+                        (b.any_bad[0] | b.any_bad[1] | b.any_bad[2] | b.any_bad[3])) {
+                        const int half = here(h);
+                        for (int k2 = 0; k2 < 32; ++k2) {
+                            if (k32 + k2 >= it.len || !row_sees(k32 + k2)) continue;
+#pragma unroll
+                            for (int c = 0; c < kCols; ++c) {
+                                const uint32_t w = *reinterpret_cast<const uint32_t*>(
+                                    &b.bad[(32 * sub + k2) * kQuads + 8 * c + 4 * half]);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e)  // element 16 h + 4 (e % 4) + e / 4
+                                    o[c][e] = w >> (8 * (e & 3) + (e >> 2)) & 1 ? NAN : o[c][e];
+                            }
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (key + kKeys < k_end) {
+                store(buf[bi ^ 1], key + kKeys);
+                load(key + 2 * kKeys < k_end ? key + 2 * kKeys : key);  // past the end: this turn again, never used
+            }
+            __syncthreads();
+        }
+
+        // the row's two lanes, then the two key groups
+        {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+            l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        }
+        const int tid2 = here(tid), row2 = 32 * wq + (tid2 & 31), h2 = (tid2 >> 5) & 1;
+        float f = 1.0f;
+        if constexpr (kWK == 2) {
+            if (h2 == 0) m_lds[wave][tid2 & 31] = m;
+            __syncthreads();
+            const float top = fmaxf(m, m_lds[wave ^ kWQ][tid2 & 31]);
+            f = m == -INFINITY ? 0.f : exp2_hw(m - top);
+            l *= f;
+            m = top;
+            if (wk == 1 && h2 == 0) l_lds[row2] = l;
+        }
+#pragma unroll
+        for (int w = kWK - 1; w >= 0; --w) {  // (the buffers are free since the loop's last barrier)
+            if (w == wk) {
+#pragma unroll
+                for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {  // elements 32 c + 16 h + 4 b + e / 4 ..
+                        f32x4* p = reinterpret_cast<f32x4*>(&rows[row2 * kORow + 32 * c + 16 * h2 + 4 * b]);
+                        f32x4 x = f32x4{o[c][b], o[c][4 + b], o[c][8 + b], o[c][12 + b]} * f;
+                        if (w != kWK - 1) x += *p;
+                        *p = x;
+                    }
+            }
+            __syncthreads();
+        }
+        const bool whole = u_count == it.units;
+        const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (first_share ? 0 : 1)) * kTile;
+        if (kWK == 2 && wk == 0) l += l_lds[row2];
+        if (wk == 0 && h2 == 0 && row2 < valid) {
+            if (whole) {
+                l_lds[row2] = l;
+            } else {
+                float* pml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP) + 2 * (slot + row2);
+                pml[0] = m;
+                pml[1] = l;
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid2; i < valid * (kDP / 8); i += kAttBlock) {
+            const int row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
+            const f32x4* p = reinterpret_cast<const f32x4*>(&rows[row * kORow + d0]);
+            if (!whole) {
+                f32x4* po = reinterpret_cast<f32x4*>(a.part + (slot + row) * kDP + d0);
+                po[0] = p[0];
+                po[1] = p[1];
+            } else if (d0 < a.d) {
+                const float sum = l_lds[row];
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = sum == 0.f ? 0.f : p[j >> 2][j & 3] / sum;
+                const int64_t dst = row_at(row, static_cast<int64_t>(a.heads) * a.group * a.d, a.d) + d0;
+                if (a.out_vec) {
+                    store_8(a.out, dst, a.dtype, x);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (d0 + j < a.d) store_elem(a.out, dst + j, a.dtype, x[j]);
+                }
+            }
+        }
+        __syncthreads();
+        first_share = false;
+        at += u_count;
+    }
+}
+
 // ------------------------------------------------------------------ host
 struct AttPlan {
-    int nq, blocks;
-    int64_t items;  // at most
+    int tile, blocks;  // rows of a tile
+    int64_t items;     // at most
     bool split;
     int64_t bytes;
 };
 
-// 16 rows per tile where no sequence has more, 32 beyond (a tile's keys are read and
-// converted once for all of its rows).  Split wherever a sequence can have more than a unit
-// of keys, over the blocks that the chip holds at once (two per CU, one of the 32-row tiles).
+// Rows of a tile by the most that a sequence's head can have: 16 and 32 on the kernel whose waves take
+// their keys straight from memory, 64 and 128 on the one that shares converted keys (see there).
+// Split wherever a sequence can have more than a unit of keys, over the blocks that the chip
+// holds at once (two per CU, one of the 32-row tiles).
 int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64_t group, AttPlan* p) {
     TQ_REQUIRE(b->max_tokens * group <= kKvMaxRows, "%s: %lld rows of a sequence's head", what,
                (long long)(b->max_tokens * group));
     const int64_t rows = b->max_tokens * group;
-    p->nq = rows <= 16 ? 1 : 2;
-    const int64_t tile = 16 * p->nq;
+    p->tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const int64_t tile = p->tile;
     int64_t tiles = b->batch * ((rows + tile - 1) / tile);
     if (b->offsets) tiles = tiles < b->tokens * group / tile + b->batch ? tiles : b->tokens * group / tile + b->batch;
     p->items = tiles * c->heads;
@@ -739,30 +1210,49 @@ int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64
     TQ_REQUIRE(p->items * (units > 0 ? units : 1) < (int64_t(1) << 31), "%s: %lld heads and tiles of %lld keys", what,
                (long long)p->items, (long long)(b->table_pages * c->page));
     p->split = units > 1;
-    const int64_t fit = static_cast<int64_t>(device_cu_count()) * (p->nq == 2 ? 1 : 2);
+    const int64_t fit = static_cast<int64_t>(device_cu_count()) * (tile == 32 ? 1 : 2);
     p->blocks = static_cast<int>(!p->split || fit < p->items * units ? (p->split ? fit : p->items) : p->items * units);
     p->bytes = p->split ? 2 * static_cast<int64_t>(p->blocks) * tile * (kv_row(c->head_dim) + 2) * 4 : 0;
     return TQ_OK;
 }
 
-template <int kDP, int kNQ, class Codes>
+template <int kDP, int kTile, class Codes, int kPlanes>
 int launch_attention(const AttArg& a, const AttPlan& p, hipStream_t st) {
     clear_error();
-    if (a.dtype == TQ_DT_F32)
-        k_kv_attention<kDP, kNQ, Codes, 2><<<p.blocks, kAttBlock, 0, st>>>(a);
+    if constexpr (kTile <= 32)
+        k_kv_attention<kDP, kTile / 16, Codes, kPlanes><<<p.blocks, kAttBlock, 0, st>>>(a);
     else
-        k_kv_attention<kDP, kNQ, Codes, 1><<<p.blocks, kAttBlock, 0, st>>>(a);
-    const int rc = check_launch("tq_kv_attention");
-    if (rc != TQ_OK || !p.split) return rc;
-    const int64_t rows = static_cast<int64_t>(a.b.max_tokens) * a.group;
-    const dim3 grid(static_cast<unsigned>(p.items), static_cast<unsigned>(((rows < 16 * kNQ ? rows : 16 * kNQ) + kAttWaves - 1) / kAttWaves));
-    k_kv_attention_join<kDP, kNQ><<<grid, kAttBlock, 0, st>>>(a);
+        k_kv_attention_rows<kDP, kTile / 32, Codes, kPlanes><<<p.blocks, kAttBlock, 0, st>>>(a);
     return check_launch("tq_kv_attention");
+}
+
+// four waves for each row where an item has many shares
+template <int kDP, int kTile>
+int launch_join(const AttArg& a, const AttPlan& p, hipStream_t st) {
+    const int64_t rows = std::min<int64_t>(static_cast<int64_t>(a.b.max_tokens) * a.group, kTile);
+    const unsigned items = static_cast<unsigned>(p.items);
+    if (p.blocks >= 8 * p.items)
+        k_kv_attention_join<kDP, kTile, 4><<<dim3(items, static_cast<unsigned>(rows)), kAttBlock, 0, st>>>(a);
+    else
+        k_kv_attention_join<kDP, kTile, 1><<<dim3(items, static_cast<unsigned>((rows + 3) / 4)), kAttBlock, 0, st>>>(a);
+    return check_launch("tq_kv_attention");
+}
+
+template <int kDP, int kTile, class Codes>
+int launch_attention_tile(const AttArg& a, const AttPlan& p, hipStream_t st) {
+    const int rc = a.dtype == TQ_DT_F32 ? launch_attention<kDP, kTile, Codes, 2>(a, p, st)
+                                        : launch_attention<kDP, kTile, Codes, 1>(a, p, st);
+    return rc != TQ_OK || !p.split ? rc : launch_join<kDP, kTile>(a, p, st);
 }
 
 template <int kDP, class Codes>
 int launch_attention_rows(const AttArg& a, const AttPlan& p, hipStream_t st) {
-    return p.nq == 1 ? launch_attention<kDP, 1, Codes>(a, p, st) : launch_attention<kDP, 2, Codes>(a, p, st);
+    switch (p.tile) {
+    case 16: return launch_attention_tile<kDP, 16, Codes>(a, p, st);
+    case 32: return launch_attention_tile<kDP, 32, Codes>(a, p, st);
+    case 64: return launch_attention_tile<kDP, 64, Codes>(a, p, st);
+    default: return launch_attention_tile<kDP, 128, Codes>(a, p, st);
+    }
 }
 
 template <class Codes>
@@ -832,6 +1322,7 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
     a.blocks = p.blocks;
     a.q_vec = aligned(q->data, 16) && cache->head_dim % 8 == 0 && q->token_stride * size % 16 == 0 &&
               q->head_stride * size % 16 == 0;
+    a.out_vec = aligned(out, 16) && cache->head_dim % 8 == 0;
     a.scale2 = scale * 1.4426950408889634f;
     a.by_group = FastDiv(static_cast<uint32_t>(group));
     return cache->codes == TQ_QINT8 ? launch_attention_dim<CodesI8>(a, p, as_hip(stream))
