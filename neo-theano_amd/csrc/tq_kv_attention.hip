@@ -14,7 +14,7 @@
 //  * bytes become f16 pairs by byte permutes: INT8 as 1024 + (code + 128) (the bytes of an f16
 //    with exponent 2^10) minus 1152, e4m3 by v_cvt_scalef32_pk_f16_fp8, both exact.
 // The value scale sv_j goes into the exponent: with t_j = s_j + log2 sv_j and the running
-// maximum of t, P_j = 2^(t_j - max + 14) = p_j sv_j needs no normalising to fit f16's
+// maximum of t, P_j = 2^(t_j - max) = p_j sv_j needs no normalising to fit f16's
 // range whatever the scales, and the sum takes P_j / sv_j.  f32 rows use two f16 planes of
 // q (scaled by a power of two for each row) and P, 22 bits; 16-bit rows one (11 bits: an
 // eighth of a bf16 output's rounding).
@@ -36,7 +36,10 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 constexpr int kAttBlock = 256, kAttWaves = kAttBlock / kWave;
 constexpr int kStep = 32;                    // keys of a wave's step
 constexpr int kUnit = kAttWaves * kStep;     // keys of a unit
-constexpr float kPShift = 14.0f;             // P in [0, 2^14]: small probabilities stay normal f16 numbers
+// P = 2^(t - m): m is the running maximum less kPShift, and it and O move only once the maximum
+// has passed it by more than kPShift + kPSlack, so that P stays in [0, 2^15] of f16's 2^16 (at 32 rows some
+// row's maximum moves in nearly every step: rescaling O each time took as long as the softmax)
+constexpr float kPShift = 8.0f, kPSlack = 7.0f;
 
 struct AttArg {
     KvBatch b;
@@ -174,6 +177,19 @@ __device__ __forceinline__ Item find_item(const AttArg& a, const SeqLane& s0, in
         units += nu;
     }
     return Item{};
+}
+
+// Which of the 32 keys from `key` row t of the item's new tokens sees, a bit each (keys past the
+// length may be among them): one comparison, or two words of the tree, for all of them.
+__device__ __forceinline__ uint32_t seen_from(const AttArg& a, const Item& it, int t, int key) {
+    auto first = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+    const int j = key - it.base;  // place among the new tokens, negative before them
+    if (!a.tree) return first(t + 1 - j);
+    const int32_t* row = a.tree + (it.first + static_cast<int64_t>(t)) * a.tree_words;
+    const int w = j >> 5;
+    const uint32_t lo = w < 0 ? ~0u : w < a.tree_words ? static_cast<uint32_t>(row[w]) : 0u;
+    const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < a.tree_words ? static_cast<uint32_t>(row[w + 1]) : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, j & 31) & first(it.rows - j);
 }
 
 // ------------------------------------------------------------------ arithmetic
@@ -428,7 +444,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
         }
 
         f32x4 o[kNQ][kVT];
-        float m[kNQ], l[kNQ];  // m: the running maximum less kPShift; l: of this lane's keys
+        float m[kNQ], l[kNQ];  // l: of this lane's keys
 #pragma unroll
         for (int n = 0; n < kNQ; ++n) {
             m[n] = -INFINITY;
@@ -520,23 +536,12 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
 #pragma unroll
                 for (int j = 0; j < 8; ++j) t[j] = fmaf(st[j >> 2][n][j & 3] * rq[n], ck[j >> 2][j & 3], lsv[j]);
                 if (slow) {
+                    const uint32_t window = seen_from(a, it, t_row[n], key);
                     uint32_t bits = 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int kk = key + 16 * (j >> 2) + 4 * g + (j & 3);
-                        bool see;
-                        if (a.tree) {
-                            const int jj = kk - it.base;
-                            see = kk < it.len && jj < it.rows;
-                            if (see && jj >= 0 && jj < 32 * a.tree_words)
-                                see = (a.tree[(it.first + static_cast<int64_t>(t_row[n])) * a.tree_words + (jj >> 5)] >>
-                                       (jj & 31)) & 1;
-                            else if (jj >= 0)
-                                see = false;
-                        } else {
-                            see = kk < min(it.base + t_row[n] + 1, it.len);
-                        }
-                        see = see && (j < 4 ? seen0 : seen1);
+                        const int i = 16 * (j >> 2) + 4 * g + (j & 3);
+                        const bool see = (window >> i & 1) != 0 && key + i < it.len && (j < 4 ? seen0 : seen1);
                         t[j] = see ? t[j] : -INFINITY;
                         bits |= see ? 1u << j : 0u;
                     }
@@ -545,15 +550,17 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j]);
-                top = fmaxf(m[n], over_groups(top, OpMax{}) - kPShift);
-                const float ref = top == -INFINITY ? 0.f : top;
-                if (__ballot(top != m[n])) {
+                top = over_groups(top, OpMax{}) - kPShift;
+                if (__ballot(top > m[n] + kPSlack)) {
+                    top = fmaxf(m[n], top);
+                    const float ref = top == -INFINITY ? 0.f : top;
                     const float alpha = exp2_hw(m[n] - ref);
                     l[n] *= alpha;
 #pragma unroll
                     for (int v = 0; v < kVT; ++v) o[n][v] *= alpha;
                     m[n] = top;
                 }
+                const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float p = exp2_hw(t[j] - ref);
@@ -1001,14 +1008,6 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
             }
             if (Codes::kNan) b.any_bad[wave] = __ballot(bad_here != 0) != 0;
         };
-        auto row_sees = [&](int key) {
-            if (!a.tree) return key < min(it.base + t_row + 1, it.len);
-            const int j = key - it.base;
-            if (key >= it.len || j >= it.rows) return false;
-            if (j < 0) return true;
-            return ((a.tree[(it.first + static_cast<int64_t>(t_row)) * a.tree_words + (j >> 5)] >> (j & 31)) & 1) != 0;
-        };
-
         if (k_begin < k_end) {
             load(k_begin);
             store(buf[0], k_begin);
@@ -1044,25 +1043,25 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                     }
                     const bool slow = k32 + 32 > all_w;  // uniform
                     if (slow) {
+                        const uint32_t window = seen_from(a, it, t_row, k32) >> (4 * h);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            t[e] = row_sees(k32 + 8 * (e >> 2) + 4 * h + (e & 3)) ? t[e] : -INFINITY;
-                            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                        }
+                        for (int e = 0; e < 16; ++e) t[e] = window >> (8 * (e >> 2) + (e & 3)) & 1 ? t[e] : -INFINITY;
                     }
                     float top = t[0];
 #pragma unroll
                     for (int e = 1; e < 16; ++e) top = fmaxf(top, t[e]);
                     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                    top = fmaxf(m, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kPShift);
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    if (__ballot(top != m)) {
+                    top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kPShift;
+                    if (__ballot(top > m + kPSlack)) {
+                        top = fmaxf(m, top);
+                        const float ref = top == -INFINITY ? 0.f : top;
                         const float alpha = exp2_hw(m - ref);
                         l *= alpha;
 #pragma unroll
                         for (int c = 0; c < kCols; ++c) o[c] *= alpha;
                         m = top;
                     }
+                    const float ref = m == -INFINITY ? 0.f : m;
                     h8 pf[2][kPlanes];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -1090,8 +1089,9 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                     if (Codes::kNan && key + kKeys > all_b &&
                         (b.any_bad[0] | b.any_bad[1] | b.any_bad[2] | b.any_bad[3])) {
                         const int half = here(h);
+                        const uint32_t window = seen_from(a, it, t_row, k32);
                         for (int k2 = 0; k2 < 32; ++k2) {
-                            if (k32 + k2 >= it.len || !row_sees(k32 + k2)) continue;
+                            if (!(window >> k2 & 1)) continue;  // (keys past the length hold no codes here)
 #pragma unroll
                             for (int c = 0; c < kCols; ++c) {
                                 const uint32_t w = *reinterpret_cast<const uint32_t*>(

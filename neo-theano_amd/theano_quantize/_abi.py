@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 from .errors import raise_for_status
 
@@ -22,27 +23,13 @@ _p = ctypes.c_void_p
 
 
 
-class Heads(ctypes.Structure):
-    """tq_heads"""
-    _fields_ = [("data", _p), ("heads", _i64), ("token_stride", _i64), ("head_stride", _i64)]
-
-
-class RotaryDesc(ctypes.Structure):
-    """tq_rotary"""
-    _fields_ = [("frequencies", _p), ("rotary_dim", _i64), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
-                ("scale", ctypes.c_float)]
-
-
-class KVCacheDesc(ctypes.Structure):
-    """tq_kv_cache"""
-    _fields_ = [("k", _p), ("k_scale", _p), ("v", _p), ("v_scale", _p), ("pages", _i64), ("heads", _i64), ("page", _i64),
-                ("head_dim", _i64), ("codes", ctypes.c_int32)]
-
-
-class KVBatchDesc(ctypes.Structure):
-    """tq_kv_batch"""
-    _fields_ = [("table", _p), ("table_stride", _i64), ("table_pages", _i64), ("lengths", _p), ("offsets", _p),
-                ("batch", _i64), ("max_tokens", _i64), ("tokens", _i64)]
+# The descriptor structures, packed to bytes (whose address ctypes passes for a pointer): building a
+# ctypes.Structure for each call took longer than the smallest kernels run.
+heads_desc = struct.Struct("@Pqqq").pack                 # tq_heads: data, heads, token_stride, head_stride
+rotary_desc = struct.Struct("@Pqiif4x").pack             # tq_rotary: frequencies, rotary_dim, interleaved, inverse, scale
+kv_cache_desc = struct.Struct("@PPPPqqqqi4x").pack       # tq_kv_cache: k, k_scale, v, v_scale, pages, heads, page, head_dim, codes
+kv_batch_desc = struct.Struct("@PqqPPqqq").pack          # tq_kv_batch: table, table_stride, table_pages, lengths, offsets, batch,
+#                                                          max_tokens, tokens
 
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
@@ -118,7 +105,7 @@ SIGNATURES = {
     "tq_gemm_fp8_block": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p],
     "tq_linear_fp8_block_workspace_bytes": [_i64, _i64, _i64],
     "tq_linear_fp8_block": [_p, _int, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p, _p],
-    # descriptors are passed as the address of their ctypes structure
+    # descriptors are passed as their packed bytes
     "tq_rotary_apply": [_p, _p, _i64, _p, _p, _int, _i64, _p, _p, _p],
     "tq_kv_write": [_p, _p, _p, _p, _int, _p],
     "tq_kv_write_rotary": [_p, _p, _p, _p, _p, _p, _p, _int, _p, _p],

@@ -19,12 +19,12 @@ what it says is checked on the device, see ``KVBatch``.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from . import _abi
+from ._abi import heads_desc as _heads_desc
 from ._tensor import stream
 from .errors import InvalidArgument
 from .qconfig import QuantDType
@@ -34,34 +34,40 @@ _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # tq_dtype
 _CODES = {torch.int8: 0, torch.uint8: 3}  # tq_qdtype
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _device(t, name):
     """`t` lies on the current device: the call goes to that device's current stream."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != torch._C._cuda_getDevice():
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != _current_device():
         raise InvalidArgument(f"{name}: expected a tensor on the current GPU")
     return t
 
 
 def _indices(t, dtype, dim, name):
-    _device(t, name)
-    if t.dtype != dtype or t.dim() != dim or (dim and t.shape[-1] > 1 and t.stride(-1) != 1):
+    """`t` as a tensor of `dtype` with `dim` dimensions on the current device, its last one dense."""
+    if _device(t, name).dtype != dtype or t.dim() != dim or (not t.is_contiguous() and t.stride(-1) != 1 and t.shape[-1] > 1):
         raise InvalidArgument(f"{name}: expected a dense {dim}-D {dtype} tensor, got {t.dtype} {tuple(t.shape)}")
     return t
 
 
 def _heads(t, name, dtype=None, tokens=None, heads=None, dim=None):
-    """(descriptor, dtype code) of a [tokens, heads, head_dim] tensor."""
+    """(tensor, descriptor, dtype code) of a [tokens, heads, head_dim] tensor."""
     _device(t, name)
     code = _TYPES.get(t.dtype)
     if code is None or (dtype is not None and t.dtype != dtype):
         raise InvalidArgument(f"{name}: expected {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[2] < 1 or (tokens is not None and t.shape[0] != tokens) or \
-            (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+    shape = t.shape
+    if len(shape) != 3 or shape[2] < 1 or (tokens is not None and shape[0] != tokens) or \
+            (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
         raise InvalidArgument(f"{name}: expected [{'tokens' if tokens is None else tokens}, "
                               f"{'heads' if heads is None else heads}, {'head_dim' if dim is None else dim}], "
-                              f"got {tuple(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+                              f"got {tuple(shape)}")
+    token, head, last = t.stride()
+    if last != 1 and shape[2] > 1:
         t = t.contiguous()
-    return t, _abi.Heads(t.data_ptr(), t.shape[1], t.stride(0), t.stride(1)), code
+        token, head, _ = t.stride()
+    return t, _heads_desc(t.data_ptr(), shape[1], token, head), code
 
 
 class Rotary:
@@ -75,8 +81,7 @@ class Rotary:
         _indices(frequencies, torch.float64, 1, "Rotary: frequencies")
         self.frequencies, self.interleaved, self.scale = frequencies, bool(interleaved), float(scale)
         self.rotary_dim = 2 * frequencies.shape[0]
-        self._desc = _abi.RotaryDesc(frequencies.data_ptr(), self.rotary_dim, self.interleaved, False, self.scale)
-        self._inverse = None
+        self._desc = _abi.rotary_desc(frequencies.data_ptr(), self.rotary_dim, self.interleaved, False, self.scale)
 
     @staticmethod
     def from_base(rotary_dim, base=10000.0, interleaved=False, scaling=None, factor=1.0, original_length=None,
@@ -113,14 +118,6 @@ class Rotary:
         return Rotary(f.to(torch.device("cuda", torch.cuda.current_device())), interleaved,
                       1.0 if scale is None else scale)
 
-    def _of(self, inverse):
-        if not inverse:
-            return self._desc
-        if self._inverse is None:
-            d = self._desc
-            self._inverse = _abi.RotaryDesc(d.frequencies, d.rotary_dim, d.interleaved, True, d.scale)
-        return self._inverse
-
     def apply(self, q, k, positions, inverse=False):
         """(q, k) [tokens, heads, head_dim] turned to int64 `positions` [tokens]; k may be None.
         inverse: turned back (the transpose, which is the gradient's rotation)."""
@@ -130,14 +127,16 @@ class Rotary:
         _indices(positions, torch.int64, 1, "Rotary.apply: positions")
         if positions.shape[0] != n:
             raise InvalidArgument(f"Rotary.apply: {positions.shape[0]} positions for {n} tokens")
-        qo = q.new_empty(q.shape)
-        ko = dk = None
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = dk = ko_ptr = None
         if k is not None:
             k, dk, _ = _heads(k, "Rotary.apply: k", q.dtype, n, None, d)
-            ko = k.new_empty(k.shape)
-        _abi.call("tq_rotary_apply", ctypes.addressof(self._of(inverse)), positions.data_ptr(), n, ctypes.addressof(dq),
-                  None if dk is None else ctypes.addressof(dk), code, d, qo.data_ptr(),
-                  None if ko is None else ko.data_ptr(), stream())
+            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+            ko_ptr = ko.data_ptr()
+        desc = self._desc
+        if inverse:
+            desc = _abi.rotary_desc(self.frequencies.data_ptr(), self.rotary_dim, self.interleaved, True, self.scale)
+        _abi.call("tq_rotary_apply", desc, positions.data_ptr(), n, dq, dk, code, d, qo.data_ptr(), ko_ptr, stream())
         return qo, ko
 
 
@@ -170,8 +169,9 @@ class KVBatch:
                 raise InvalidArgument("KVBatch: offsets are [batch + 1], with `rows` rows in all")
         self.table, self.lengths, self.offsets = table, lengths, offsets
         self.batch, self.tokens, self.rows = batch, int(tokens), int(rows)
-        self._desc = _abi.KVBatchDesc(table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-                                      None if offsets is None else offsets.data_ptr(), batch, self.tokens, self.rows)
+        self.device_index = table.get_device()
+        self._desc = _abi.kv_batch_desc(table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+                                        0 if offsets is None else offsets.data_ptr(), batch, self.tokens, self.rows)
 
 
 class KVCache:
@@ -198,9 +198,9 @@ class KVCache:
         self.pages, self.heads, self.page = shape[0], shape[1], shape[2]
         self.head_dim = int(head_dim)
         self.device = k.device
-        self._desc = _abi.KVCacheDesc(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), shape[0],
-                                      shape[1], shape[2], self.head_dim, code)
-        self._ref = ctypes.addressof(self._desc)
+        self.device_index = k.get_device()
+        self._ref = _abi.kv_cache_desc(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), shape[0],
+                                       shape[1], shape[2], self.head_dim, code)
 
     @staticmethod
     def allocate(pages, page, heads, head_dim, dtype=QuantDType.Int8):
@@ -216,17 +216,16 @@ class KVCache:
 
     def _here(self, new):
         """Cache, batch and current device are one."""
-        dev = torch._C._cuda_getDevice()
-        if self.device.index != dev or new.table.device.index != dev:
+        if self.device_index != new.device_index or self.device_index != _current_device():
             raise InvalidArgument("KVCache: the cache, the batch and the current device differ")
-        return ctypes.addressof(new._desc)
+        return new._desc
 
     def write(self, k, v, new):
         """Quantizes k and v [rows, heads, head_dim] into the places of the batch's rows."""
         b = self._here(new)
         k, dk, code = _heads(k, "KVCache.write: k", None, new.rows, self.heads, self.head_dim)
         v, dv, _ = _heads(v, "KVCache.write: v", k.dtype, new.rows, self.heads, self.head_dim)
-        _abi.call("tq_kv_write", self._ref, b, ctypes.addressof(dk), ctypes.addressof(dv), code, stream())
+        _abi.call("tq_kv_write", self._ref, b, dk, dv, code, stream())
 
     def write_rotary(self, q, k, v, rotary, new, positions=None):
         """The same with q [rows, query heads, head_dim] and k turned first; returns q turned.
@@ -240,10 +239,10 @@ class KVCache:
             _indices(positions, torch.int64, 1, "KVCache.write_rotary: positions")
             if positions.shape[0] != new.rows:
                 raise InvalidArgument(f"KVCache.write_rotary: {positions.shape[0]} positions for {new.rows} rows")
-        out = q.new_empty(q.shape)
-        _abi.call("tq_kv_write_rotary", self._ref, b, ctypes.addressof(rotary._desc),
-                  None if positions is None else positions.data_ptr(), ctypes.addressof(dq), ctypes.addressof(dk),
-                  ctypes.addressof(dv), code, out.data_ptr(), stream())
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _abi.call("tq_kv_write_rotary", self._ref, b, rotary._desc,
+                  None if positions is None else positions.data_ptr(), dq, dk,
+                  dv, code, out.data_ptr(), stream())
         return out
 
     def read(self, new, dtype=torch.float32, out=None):
@@ -282,12 +281,12 @@ class KVCache:
                                       f"got {tuple(tree.shape)}")
             words, tp = tree.shape[1], tree.data_ptr()
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif _device(out, "KVCache.attention: out").shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise InvalidArgument(f"KVCache.attention: out must be contiguous {q.dtype} {tuple(q.shape)}")
         nb = _abi.entry("tq_kv_attention_workspace_bytes")(self._ref, b, q.shape[1])
         ws = q.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
-        _abi.call("tq_kv_attention", self._ref, b, ctypes.addressof(dq), code, tp, words,
+        _abi.call("tq_kv_attention", self._ref, b, dq, code, tp, words,
                   1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), None if ws is None else ws.data_ptr(),
                   nb, out.data_ptr(), stream())
         return out

@@ -12,32 +12,55 @@ def abi():
     return _abi
 
 
+I64, PTR, I32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32
+
+
+def structure(*fields):
+    """A descriptor of include/tq.h, laid out by ctypes apart from the package's own packing."""
+    return type("Desc", (ctypes.Structure,), {"_fields_": list(fields)})
+
+
+Heads = structure(("data", PTR), ("heads", I64), ("token_stride", I64), ("head_stride", I64))
+RotaryDesc = structure(("frequencies", PTR), ("rotary_dim", I64), ("interleaved", I32), ("inverse", I32), ("scale", ctypes.c_float))
+KVCacheDesc = structure(("k", PTR), ("k_scale", PTR), ("v", PTR), ("v_scale", PTR), ("pages", I64), ("heads", I64), ("page", I64),
+                        ("head_dim", I64), ("codes", I32))
+KVBatchDesc = structure(("table", PTR), ("table_stride", I64), ("table_pages", I64), ("lengths", PTR), ("offsets", PTR),
+                        ("batch", I64), ("max_tokens", I64), ("tokens", I64))
+
+
 def at(x):
     return None if x is None else ctypes.addressof(x)
+
+
+def test_packed_descriptors_are_the_structures(abi):
+    assert abi.heads_desc(1, 2, 3, 4) == bytes(Heads(1, 2, 3, 4))
+    assert abi.rotary_desc(1, 2, 1, 0, 1.5) == bytes(RotaryDesc(1, 2, 1, 0, 1.5))
+    assert abi.kv_cache_desc(1, 2, 3, 4, 5, 6, 7, 8, 3) == bytes(KVCacheDesc(1, 2, 3, 4, 5, 6, 7, 8, 3))
+    assert abi.kv_batch_desc(1, 2, 3, 4, 5, 6, 7, 8) == bytes(KVBatchDesc(1, 2, 3, 4, 5, 6, 7, 8))
 
 
 def cache(abi, **kw):
     d = dict(k=256, k_scale=256, v=256, v_scale=256, pages=4, heads=2, page=16, head_dim=64, codes=0)
     d.update(kw)
-    return abi.KVCacheDesc(**d)
+    return KVCacheDesc(**d)
 
 
 def batch(abi, **kw):
     d = dict(table=256, table_stride=2, table_pages=2, lengths=256, offsets=None, batch=3, max_tokens=1, tokens=3)
     d.update(kw)
-    return abi.KVBatchDesc(**d)
+    return KVBatchDesc(**d)
 
 
 def heads(abi, **kw):
     d = dict(data=256, heads=2, token_stride=128, head_stride=64)
     d.update(kw)
-    return abi.Heads(**d)
+    return Heads(**d)
 
 
 def rotary(abi, **kw):
     d = dict(frequencies=256, rotary_dim=64, interleaved=0, inverse=0, scale=1.0)
     d.update(kw)
-    return abi.RotaryDesc(**d)
+    return RotaryDesc(**d)
 
 
 def refuse(abi, name, *args):
