@@ -115,43 +115,53 @@ struct RotaryArg {
     float scale;
 };
 
-// Turns one head whose own elements are in x; p is the head in memory, for the elements of
-// the other halves.
+// The elements that the head at p turns against its own: the other half's, or the neighbours (which
+// whole vectors hold already).
 template <int kType, bool kVec>
-__device__ __forceinline__ void turn_head(const typename Elem<kType>::type* p, int l, int d, const RotaryArg& r,
-                                          const float* cs, const float* sn, float (&x)[kPer]) {
-    float y[kPer];
-    if (r.pairs) {
-        if constexpr (kVec) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) y[i] = x[i ^ 1];
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int e = elem<false>(l, i);
-                y[i] = e < 2 * r.half ? Elem<kType>::to(p[e ^ 1]) : 0.f;
-            }
-        }
-    } else if constexpr (kVec) {  // half % 8 == 0: a lane's elements share their side
+__device__ __forceinline__ void load_others(const typename Elem<kType>::type* p, int l, int d, const RotaryArg& r,
+                                            float (&y)[kPer]) {
+    if constexpr (kVec) {  // half % 8 == 0: a lane's elements share their side
         const int e = kPer * l;
         load_head<kType, true>(p, l, e < r.half ? e + r.half : e < 2 * r.half ? e - r.half : d, d, y);
     } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int e = elem<false>(l, i);
-            y[i] = e < 2 * r.half ? Elem<kType>::to(p[e < r.half ? e + r.half : e - r.half]) : 0.f;
+            y[i] = e >= 2 * r.half ? 0.f : Elem<kType>::to(p[r.pairs ? e ^ 1 : e < r.half ? e + r.half : e - r.half]);
         }
     }
+}
+
+// Cosine and signed sine of the lane's own elements (the same in all of the token's heads); elements
+// that pass have plane -1.
+template <bool kVec>
+struct LaneAngles {
+    float c[kPer], s[kPer];
+    bool on[kPer];
+    __device__ LaneAngles(int l, const RotaryArg& r, const float* cs, const float* sn) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = elem<kVec>(l, i);
-        if (e < 2 * r.half) {
-            const int plane = r.pairs ? e >> 1 : e < r.half ? e : e - r.half;
+        for (int i = 0; i < kPer; ++i) {
+            const int e = elem<kVec>(l, i);
+            on[i] = e < 2 * r.half;
+            const int plane = !on[i] ? 0 : r.pairs ? e >> 1 : e < r.half ? e : e - r.half;
             const bool second = r.pairs ? (e & 1) != 0 : e >= r.half;
-            const float s = sn[plane];
-            x[i] = fmaf(x[i], cs[plane], y[i] * (second ? s : -s));
+            c[i] = cs[plane];
+            s[i] = second ? sn[plane] : -sn[plane];
         }
     }
+    // x cos + (its partner) sin, elements that pass as they are
+    __device__ void turn(float (&x)[kPer], const float (&y)[kPer]) const {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = on[i] ? fmaf(x[i], c[i], y[i] * s[i]) : x[i];
+    }
+};
+
+// row_scale in f32: the f64 quotient of two f32 values rounds to f32 as the f32 division does (53 >= 2 24 + 2
+// bits), and rounding keeps the order, so the floor may be applied after it.  A f64 division for each head cost
+// more than coding it.
+template <class Fmt>
+__device__ __forceinline__ float head_scale(float absmax) {
+    return fmaxf(absmax / static_cast<float>(Fmt::kQmax), static_cast<float>(1e-10));
 }
 
 struct RowsArg {
@@ -168,13 +178,47 @@ struct RowsArg {
     float* v_scale;
 };
 
-// Block (token, share of its heads).  Rows of a token: q's heads, then k's, then v's; the 16
-// groups of 16 lanes take one each, 16 at a time.
-template <int kType, bool kVec, class Fmt>
+// Block (token, share of its heads).  The heads of q, k and v are taken one kind after the other, 16 kU at
+// a time (a group of 16 lanes has kU heads, whose loads are issued together, the first ones before the
+// token's place and angles are known).  blockIdx.y counts such shares, or, where the grid has one block
+// for a token, it takes them all.
+template <int kType, bool kVec, int kU, class Fmt>
 __global__ __launch_bounds__(kRowBlock) void k_token_rows(RowsArg a) {
     typedef typename Elem<kType>::type T;
+    typedef typename Fmt::code_t C;
+    constexpr int kShare = kU * kHeadsAtOnce;
     __shared__ float cs[kKvMaxHeadDim / 2], sn[kKvMaxHeadDim / 2];
-    const int n = blockIdx.x, tid = threadIdx.x, l = tid % kGroup;
+    const int n = blockIdx.x, tid = threadIdx.x, l = tid % kGroup, j = tid / kGroup;
+
+    // the share: kind 0 q, 1 k, 2 v, and its first head; uniform
+    auto heads_of = [&](int kind) { return kind == 0 ? a.q.heads : kind == 1 ? a.k.heads : a.v.heads; };
+    int kind = 0, h0 = 0;
+    auto skip_empty = [&]() {
+        while (kind < 3 && h0 >= heads_of(kind)) {
+            ++kind;
+            h0 = 0;
+        }
+    };
+    skip_empty();
+    for (int i = 0; i < static_cast<int>(blockIdx.y); ++i) {
+        h0 += kShare;
+        skip_empty();
+    }
+    if (kind == 3) return;
+
+    float x[kU][kPer], y[kU][kPer];
+    auto load = [&]() {
+        const HeadsArg& src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+        const T* base = static_cast<const T*>(src.data) + n * src.token;
+        const bool others = a.rot.half && kind < 2 && !(kVec && a.rot.pairs);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {  // past the last head: the last one again, not stored
+            const T* p = base + min(h0 + u * kHeadsAtOnce + j, src.heads - 1) * src.head;
+            load_head<kType, kVec>(p, l, kPer * l, a.d, x[u]);
+            if (others) load_others<kType, kVec>(p, l, a.d, a.rot, y[u]);
+        }
+    };
+    load();
     KvPlace place{-1, -1, false};
     if (a.b.lengths) {
         place = kv_place(a.b, n, kv_sequence(a.b, n, tid & 63));
@@ -190,41 +234,60 @@ __global__ __launch_bounds__(kRowBlock) void k_token_rows(RowsArg a) {
         }
         __syncthreads();
     }
-    const int heads = a.q.heads + a.k.heads + a.v.heads;
-    for (int h = blockIdx.y * kHeadsAtOnce + tid / kGroup; h < heads; h += gridDim.y * kHeadsAtOnce) {
-        const bool is_q = h < a.q.heads, is_k = !is_q && h < a.q.heads + a.k.heads;
-        const HeadsArg& src = is_q ? a.q : is_k ? a.k : a.v;
-        const int hh = is_q ? h : is_k ? h - a.q.heads : h - a.q.heads - a.k.heads;
-        const T* p = static_cast<const T*>(src.data) + n * src.token + hh * src.head;
-        float x[kPer];
-        load_head<kType, kVec>(p, l, kPer * l, a.d, x);
-        if (a.rot.half && (is_q || is_k)) turn_head<kType, kVec>(p, l, a.d, a.rot, cs, sn, x);
-        void* out = is_q ? a.q_out : a.k_out;
-        if (is_q || (is_k && out)) {
-            store_head<kType, kVec>(static_cast<T*>(out) + (static_cast<int64_t>(n) * src.heads + hh) * a.d, l, a.d, x);
-            continue;
-        }
-        if (place.slot < 0) continue;
-        float m = -INFINITY;
+    const LaneAngles<kVec> angles(l, a.rot, cs, sn);
+    const int64_t page = place.slot < 0 ? 0 : place.slot / a.b.page, off = place.slot - page * a.b.page;
+    while (true) {
+        const int of = heads_of(kind);
+        if (a.rot.half && kind < 2) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (elem<kVec>(l, i) < a.d) m = fmaxf(m, fabsf(x[i]));
-        const float sc = row_scale<Fmt>(absmax_finish(group_max<kGroup>(m)));
-        const typename Fmt::Row coder(sc);
-        const int64_t page = place.slot / a.b.page, off = place.slot - page * a.b.page;
-        const int64_t at = (page * src.heads + hh) * a.b.page + off;
-        typedef typename Fmt::code_t C;
-        C* codes = static_cast<C*>(is_k ? a.k_codes : a.v_codes) + at * a.row;
-        if (l == 0) (is_k ? a.k_scale : a.v_scale)[at] = sc;
-        if constexpr (kVec) {
-            if (kPer * l < a.row)  // zeros past the head
-                *reinterpret_cast<uint2*>(codes + kPer * l) = make_uint2(
-                    coder.code4(f32x4{x[0], x[1], x[2], x[3]}), coder.code4(f32x4{x[4], x[5], x[6], x[7]}));
-        } else {
+            for (int u = 0; u < kU; ++u) {
+                if (kVec && a.rot.pairs) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (elem<false>(l, i) < a.row) codes[elem<false>(l, i)] = coder.code1(x[i]);
+                    for (int i = 0; i < kPer; ++i) y[u][i] = x[u][i ^ 1];
+                }
+                angles.turn(x[u], y[u]);
+            }
         }
+        T* out = static_cast<T*>(kind == 0 ? a.q_out : kind == 1 ? a.k_out : nullptr);
+        if (out) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int h = h0 + u * kHeadsAtOnce + j;
+                if (h < of) store_head<kType, kVec>(out + (static_cast<int64_t>(n) * of + h) * a.d, l, a.d, x[u]);
+            }
+        } else if (place.slot >= 0) {
+            C* codes0 = static_cast<C*>(kind == 1 ? a.k_codes : a.v_codes);
+            float* scale = kind == 1 ? a.k_scale : a.v_scale;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int h = h0 + u * kHeadsAtOnce + j;
+                if (h >= of) continue;
+                float m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (elem<kVec>(l, i) < a.d) m = fmaxf(m, fabsf(x[u][i]));
+                const float sc = head_scale<Fmt>(absmax_finish(group_max<kGroup>(m)));
+                const typename Fmt::Row coder(sc);
+                const int64_t at = (page * of + h) * a.b.page + off;
+                C* codes = codes0 + at * a.row;
+                if (l == 0) scale[at] = sc;
+                if constexpr (kVec) {
+                    if (kPer * l < a.row)  // zeros past the head
+                        *reinterpret_cast<uint2*>(codes + kPer * l) =
+                            make_uint2(coder.code4(f32x4{x[u][0], x[u][1], x[u][2], x[u][3]}),
+                                       coder.code4(f32x4{x[u][4], x[u][5], x[u][6], x[u][7]}));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        if (elem<false>(l, i) < a.row) codes[elem<false>(l, i)] = coder.code1(x[u][i]);
+                }
+            }
+        }
+        if (gridDim.y > 1) return;
+        h0 += kShare;
+        skip_empty();
+        if (kind == 3) return;
+        load();
     }
 }
 
@@ -240,20 +303,32 @@ struct ReadArg {
 };
 
 // Block: 16 adjacent tokens, a group of lanes each (so that a page's codes and scales are
-// read in runs), over the heads of its share.
+// read in runs), over the heads of its share, four at a time.
 template <int kType, bool kVec, class Fmt>
 __global__ __launch_bounds__(kRowBlock) void k_read_rows(ReadArg a) {
     typedef typename Elem<kType>::type T;
     typedef typename Fmt::code_t C;
+    constexpr int kU = 4;
     __shared__ int64_t slots[kHeadsAtOnce];
     const int tid = threadIdx.x, l = tid % kGroup, j = tid / kGroup, n0 = blockIdx.x * kHeadsAtOnce;
     if (tid < 64) {
-        for (int t = 0; t < kHeadsAtOnce && n0 + t < a.n; ++t) {
-            const int seq = kv_sequence(a.b, n0 + t, tid);
-            if (tid == t) {
-                const KvPlace p = kv_place(a.b, n0 + t, seq);
-                slots[t] = p.behind ? -2 : p.slot;
+        // lane t: the sequence of row n0 + t, all sixteen by the same loads
+        int seq = 0;
+        if (!a.b.offsets) {
+            seq = static_cast<int>(a.b.by_tokens.div(static_cast<uint32_t>(min(n0 + tid, a.n - 1))));
+        } else {
+            for (int i = 0; i < a.b.batch; i += 64) {
+                const int ends = i + tid < a.b.batch ? a.b.offsets[i + tid + 1] : INT32_MAX;
+#pragma unroll
+                for (int t = 0; t < kHeadsAtOnce; ++t) {
+                    const int ended = __popcll(__ballot(ends <= n0 + t));
+                    seq += tid == t ? ended : 0;
+                }
             }
+        }
+        if (tid < kHeadsAtOnce && n0 + tid < a.n) {
+            const KvPlace p = kv_place(a.b, n0 + tid, seq);
+            slots[tid] = p.behind ? -2 : p.slot;
         }
     }
     __syncthreads();
@@ -262,32 +337,50 @@ __global__ __launch_bounds__(kRowBlock) void k_read_rows(ReadArg a) {
     const int64_t slot = slots[j];
     if (slot == -2) return;  // left as it was
     const int64_t page = slot < 0 ? 0 : slot / a.b.page, off = slot < 0 ? 0 : slot - page * a.b.page;
-    for (int h = blockIdx.y; h < 2 * a.heads; h += gridDim.y) {
-        const bool is_k = h < a.heads;
-        const int hh = is_k ? h : h - a.heads;
-        const int64_t at = (page * a.heads + hh) * a.b.page + off;
-        const C* codes = static_cast<const C*>(is_k ? a.k : a.v) + at * a.row;
-        float x[kPer] = {};
-        if (slot >= 0) {
-            const float sc = (is_k ? a.k_scale : a.v_scale)[at];
-            if constexpr (kVec) {
-                if (kPer * l < a.d) {
-                    const uint2 c = *reinterpret_cast<const uint2*>(codes + kPer * l);
-                    const f32x4 u = Fmt::value4(c.x, sc), w = Fmt::value4(c.y, sc);
+    const float zero = slot < 0 ? 0.f : 1.f;
+    for (int h0 = blockIdx.y * kU; h0 < 2 * a.heads; h0 += gridDim.y * kU) {
+        uint32_t c[kU][kPer / 4];
+        C one[kU][kPer];
+        float sc[kU];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = u[i];
-                        x[4 + i] = w[i];
-                    }
+        for (int u = 0; u < kU; ++u) {
+            const int h = min(h0 + u, 2 * a.heads - 1);
+            const bool is_k = h < a.heads;
+            const int64_t at = (page * a.heads + (is_k ? h : h - a.heads)) * a.b.page + off;
+            const C* codes = static_cast<const C*>(is_k ? a.k : a.v) + at * a.row;
+            sc[u] = (is_k ? a.k_scale : a.v_scale)[at];
+            if constexpr (kVec) {
+                const uint2 w = *reinterpret_cast<const uint2*>(codes + min(kPer * l, a.row - kPer));
+                c[u][0] = w.x;
+                c[u][1] = w.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) one[u][i] = codes[min(elem<false>(l, i), a.row - 1)];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int h = h0 + u;
+            if (h >= 2 * a.heads) continue;
+            const bool is_k = h < a.heads;
+            float x[kPer];
+            if constexpr (kVec) {
+                const f32x4 v = Fmt::value4(c[u][0], sc[u]), w = Fmt::value4(c[u][1], sc[u]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = v[i];
+                    x[4 + i] = w[i];
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kPer; ++i)
-                    if (elem<false>(l, i) < a.d) x[i] = Fmt::value1(codes[elem<false>(l, i)], sc);
+                for (int i = 0; i < kPer; ++i) x[i] = Fmt::value1(one[u][i], sc[u]);
             }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) x[i] = zero != 0.f ? x[i] : 0.f;
+            store_head<kType, kVec>(static_cast<T*>(is_k ? a.k_out : a.v_out) +
+                                        (static_cast<int64_t>(n) * a.heads + (is_k ? h : h - a.heads)) * a.d,
+                                    l, a.d, x);
         }
-        store_head<kType, kVec>(static_cast<T*>(is_k ? a.k_out : a.v_out) + (static_cast<int64_t>(n) * a.heads + hh) * a.d, l,
-                                a.d, x);
     }
 }
 
@@ -315,18 +408,25 @@ RotaryArg rotary_arg(const tq_rotary* r) {
     return RotaryArg{r->frequencies, static_cast<int>(r->rotary_dim / 2), r->interleaved != 0, r->inverse != 0, r->scale};
 }
 
-// Blocks for each token: one that goes through all of its heads where there are tokens
-// enough to fill the chip, else one for every 16 heads.
+// One block for a token where there are tokens enough to fill the chip, else one for every 16 heads of
+// a kind.
+template <int kType, bool kVec, class Fmt>
+void launch_rows_vec(const RowsArg& a, hipStream_t st) {
+    auto shares = [](int heads) { return (heads + kHeadsAtOnce - 1) / kHeadsAtOnce; };
+    if (a.n >= 4 * device_cu_count())
+        k_token_rows<kType, kVec, 2, Fmt><<<dim3(a.n, 1), kRowBlock, 0, st>>>(a);
+    else
+        k_token_rows<kType, kVec, 1, Fmt>
+            <<<dim3(a.n, shares(a.q.heads) + shares(a.k.heads) + shares(a.v.heads)), kRowBlock, 0, st>>>(a);
+}
+
 template <int kType, class Fmt>
 int launch_rows(const RowsArg& a, bool vec, hipStream_t st, const char* what) {
-    const int heads = a.q.heads + a.k.heads + a.v.heads;
-    const int shares = a.n >= 4 * device_cu_count() ? 1 : (heads + kHeadsAtOnce - 1) / kHeadsAtOnce;
-    const dim3 grid(a.n, shares);
     clear_error();
     if (vec)
-        k_token_rows<kType, true, Fmt><<<grid, kRowBlock, 0, st>>>(a);
+        launch_rows_vec<kType, true, Fmt>(a, st);
     else
-        k_token_rows<kType, false, Fmt><<<grid, kRowBlock, 0, st>>>(a);
+        launch_rows_vec<kType, false, Fmt>(a, st);
     return check_launch(what);
 }
 
@@ -382,7 +482,8 @@ int write_rows(const char* what, const tq_kv_cache* cache, const tq_kv_batch* ba
 template <int kType, class Fmt>
 int launch_read(const ReadArg& a, bool vec, hipStream_t st, const char* what) {
     const int blocks = (a.n + kHeadsAtOnce - 1) / kHeadsAtOnce;
-    const dim3 grid(blocks, blocks >= 4 * device_cu_count() ? 1 : 2 * a.heads);
+    // all heads in a block where there are blocks enough, else four to a block
+    const dim3 grid(blocks, blocks >= 4 * device_cu_count() ? 1 : (2 * a.heads + 3) / 4);
     clear_error();
     if (vec)
         k_read_rows<kType, true, Fmt><<<grid, kRowBlock, 0, st>>>(a);
