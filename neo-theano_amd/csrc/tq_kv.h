@@ -54,6 +54,21 @@ __device__ __forceinline__ int kv_sequence(const KvBatch& b, int n, int lane) {
     return seq;
 }
 
+// Lane t < 16: the sequence of row n0 + t (of n), all sixteen by the same loads.  Called by one whole wave.
+__device__ __forceinline__ int kv_sequences16(const KvBatch& b, int n0, int n, int lane) {
+    if (!b.offsets) return static_cast<int>(b.by_tokens.div(static_cast<uint32_t>(min(n0 + lane, n - 1))));
+    int seq = 0;
+    for (int i = 0; i < b.batch; i += 64) {
+        const int ends = i + lane < b.batch ? b.offsets[i + lane + 1] : INT32_MAX;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int ended = __popcll(__ballot(ends <= n0 + t));
+            seq += lane == t ? ended : 0;
+        }
+    }
+    return seq;
+}
+
 __device__ __forceinline__ KvPlace kv_place(const KvBatch& b, int n, int seq) {
     KvPlace p{-1, -1, seq >= b.batch};
     if (p.behind) return p;
