@@ -128,6 +128,28 @@ def test_product(tq, m, n, k, bias):
         assert torch.equal(lin(h), tq.gemm_fp8_block(*tq.quantize_fp8_g128(h), qw, sw, b))
 
 
+@pytest.mark.parametrize("m,n,k,shift", [
+    (1, 9001, 144, 0), (7, 16400, 257, 0), (16, 4100, 1050, 0), (16, 4097, 130, 1),  # rows after rows in a block
+    (4, 48, 4096, 0), (5, 48, 4096, 0), (6, 64, 4096, 5), (2, 33, 8192, 0), (12, 20, 2176, 3),  # codes made or copied or read
+    (17, 4096, 4096, 0), (32, 300, 4096, 0), (32, 4112, 512, 0), (24, 40, 4224, 0), (29, 77, 128, 7), (32, 16, 127, 0),
+    (63, 500, 528, 0), (64, 130, 528, 0), (64, 130, 528, 8), (100, 260, 2048, 3), (128, 128, 4096, 0),
+    (140, 260, 4112, 0), (1200, 8000, 144, 0), (2000, 4500, 784, 0)])  # shares of K, with and without whole rounds before
+def test_product_at_its_turns(tq, m, n, k, shift):
+    """Sizes beside each choice of kernel, and weights off their boundary: the bound of `test_product`."""
+    import torch
+
+    x, w, b = rand(m, m, k, dtype=torch.bfloat16), rand(n, n, k, std=0.02), rand(4, n)
+    qa, sa = tq.quantize_fp8_g128(x)
+    qw, sw = tq.quantize_fp8_block(w)
+    if shift:
+        qw = torch.full((n * k + 64,), 0x7F, dtype=torch.uint8, device="cuda")[shift:shift + n * k].view(n, k).copy_(qw)
+    ref, size = product(qa, sa, qw, sw, b)
+    got = tq.gemm_fp8_block(qa, sa, qw, sw, b)
+    off = (got.double() - ref).abs()
+    assert (off <= (min(k, 128) + 3 + (k + 127) // 128) * 2.0 ** -24 * size).all(), float((off / size).max())
+    assert torch.equal(tq.QuantizedLinear("fp8_block", k, n, qw, sw, b)(x), got)
+
+
 def test_weights_at_any_address(tq):
     """Weight rows that start off every boundary, and a guard behind the last row that stays unread in
     the result."""
