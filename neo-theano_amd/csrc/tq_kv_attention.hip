@@ -68,12 +68,15 @@ struct SeqLane {
     int items_end, units_end;    // inclusive totals within the 64
 };
 
-__device__ __forceinline__ int scan64(int v, int lane) {
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-        const int u = __shfl_up(v, s);
-        v += lane >= s ? u : 0;
-    }
+// inclusive sums over the lanes: within rows of 16 by shifts, then lane 15's total into the next row and lane 31's
+// into the upper half
+__device__ __forceinline__ int scan64(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
 }
 
@@ -98,8 +101,8 @@ __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane)
         s.items_end = readlane(s.items, 0);
         s.units_end = readlane(s.items * s.units, 0);
     } else {
-        s.items_end = scan64(s.items, lane);
-        s.units_end = scan64(s.items * s.units, lane);
+        s.items_end = scan64(s.items);
+        s.units_end = scan64(s.items * s.units);
     }
     return s;
 }
@@ -312,23 +315,15 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, int dtype, float 
     else
         static_cast<_Float16*>(p)[i] = static_cast<_Float16>(x);
 }
-// 8 adjacent elements, 16-byte aligned
-__device__ __forceinline__ void load_8(const void* p, int64_t i, int dtype, float* x) {
-    if (dtype == TQ_DT_F32) {
-        const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-        const f32x4 a = s[0], b = s[1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] = a[e];
-            x[4 + e] = b[e];
-        }
-        return;
-    }
-    const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
+// 8 adjacent elements as they lie in memory (f32: both words, else the first)
+__device__ __forceinline__ void widen_8(const u32x4 (&raw)[2], int dtype, float* x) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t u = w[e];  // (a bit cast of the vector's element itself takes element 0)
-        if (dtype == TQ_DT_BF16) {
+        const uint32_t u = raw[0][e], u1 = raw[1][e];  // (a bit cast of the vector's element itself takes element 0)
+        if (dtype == TQ_DT_F32) {
+            x[e] = __uint_as_float(u);
+            x[4 + e] = __uint_as_float(u1);
+        } else if (dtype == TQ_DT_BF16) {
             x[2 * e] = __uint_as_float(u << 16);
             x[2 * e + 1] = __uint_as_float(u & 0xFFFF0000u);
         } else {
@@ -337,6 +332,18 @@ __device__ __forceinline__ void load_8(const void* p, int64_t i, int dtype, floa
             x[2 * e + 1] = static_cast<float>(h.y);
         }
     }
+}
+// 8 adjacent elements, 16-byte aligned
+__device__ __forceinline__ void load_8(const void* p, int64_t i, int dtype, float* x) {
+    u32x4 raw[2];
+    if (dtype == TQ_DT_F32) {
+        const u32x4* s = reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + i);
+        raw[0] = s[0];
+        raw[1] = s[1];
+    } else {
+        raw[0] = raw[1] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
+    }
+    widen_8(raw, dtype, x);
 }
 
 // 8 adjacent elements, 16-byte aligned
@@ -355,6 +362,22 @@ __device__ __forceinline__ void store_8(void* p, int64_t i, int dtype, const flo
                    ? __builtin_bit_cast(uint32_t, (b2{static_cast<__bf16>(x[2 * e]), static_cast<__bf16>(x[2 * e + 1])}))
                    : __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(x[2 * e]), static_cast<_Float16>(x[2 * e + 1])}));
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// 4 adjacent elements, aligned to their size
+__device__ __forceinline__ void store_4(void* p, int64_t i, int dtype, const float (&x)[4]) {
+    if (dtype == TQ_DT_F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = f32x4{x[0], x[1], x[2], x[3]};
+        return;
+    }
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    uint32_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        w[e] = dtype == TQ_DT_BF16
+                   ? __builtin_bit_cast(uint32_t, (b2{static_cast<__bf16>(x[2 * e]), static_cast<__bf16>(x[2 * e + 1])}))
+                   : __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(x[2 * e]), static_cast<_Float16>(x[2 * e + 1])}));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(w[0], w[1]);
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -395,6 +418,50 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
         const int lim = a.tree ? it.len : min(it.base + t_last + 1, it.len);
         const int all = a.tree ? min(it.base, it.len) : min(it.base + t_first + 1, it.len);
 
+        const int k_end = min((u_first + u_count) * kUnit, lim);
+        const int k_begin = u_first * kUnit + wave * kStep;
+        const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
+
+        // Pages of the 16 keys each (a page holds whole sixteens) of the step to be loaded next: read a step before
+        // they are needed, as a wave that waited for its pages had nothing under way.
+        int pages[2];
+        auto load_pages = [&](int key) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int kk = key + 16 * i < it.len ? key + 16 * i : 0;
+                pages[i] = table[a.b.by_page.div(static_cast<uint32_t>(kk))];
+            }
+        };
+        // Where the 16 keys from `key`, the step's i-th, lie: row of the cache's [pages, heads, page], and whether they
+        // lie anywhere.
+        auto place16 = [&](int key, int i, bool& ok) -> int64_t {
+            ok = key < it.len && pages[i] >= 0 && pages[i] < a.b.pages;
+            const int kk = ok ? key : 0, in = kk - static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(kk))) * a.b.page;
+            return (static_cast<int64_t>(ok ? pages[i] : 0) * a.heads + it.head) * a.b.page + in;
+        };
+
+        KBytes<kDP> kb[2];
+        VBytes<kDP> vb[8];
+        f32x4 ks[2], vs[2];
+        bool ok_k[2], ok_v[2];
+        auto load_k = [&](int key) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t row = place16(key + 16 * i, i, ok_k[i]);
+                kb[i].load(a.k + row * kDP + (r * kDP + kRun * g));
+                ks[i] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * g);
+            }
+        };
+        auto load_v = [&](int key) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t row = place16(key + 16 * i, i, ok_v[i]);
+                const uint8_t* p = a.v + row * kDP + 4 * g * kDP;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) vb[4 * i + j].load(p + j * kDP, r);
+                vs[i] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
+            }
+        };
         // q: row r of each 16, elements kRun g + 8 s + j
         h8 q[kNQ][kPlanes][kSteps];
         float rq[kNQ];
@@ -453,48 +520,11 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
             for (int t = 0; t < kVT; ++t) o[n][t] = f32x4{};
         }
 
-        const int k_end = min((u_first + u_count) * kUnit, lim);
-        const int k_begin = u_first * kUnit + wave * kStep;
-        const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
-
-        // Where the 16 keys from `key` lie (a page holds whole sixteens): row of the cache's
-        // [pages, heads, page], and whether they lie anywhere.
-        auto place16 = [&](int key, bool& ok) -> int64_t {
-            ok = key < it.len;
-            const int i = static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(ok ? key : 0)));
-            int page = it.len > 0 ? table[i] : 0;
-            if (page < 0 || page >= a.b.pages) {
-                page = 0;
-                ok = false;
-            }
-            return (static_cast<int64_t>(page) * a.heads + it.head) * a.b.page + (ok ? key - i * a.b.page : 0);
-        };
-
-        KBytes<kDP> kb[2];
-        VBytes<kDP> vb[8];
-        f32x4 ks[2], vs[2];
-        bool ok_k[2], ok_v[2];
-        auto load_k = [&](int key) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t row = place16(key + 16 * i, ok_k[i]);
-                kb[i].load(a.k + row * kDP + (r * kDP + kRun * g));
-                ks[i] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * g);
-            }
-        };
-        auto load_v = [&](int key) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t row = place16(key + 16 * i, ok_v[i]);
-                const uint8_t* p = a.v + row * kDP + 4 * g * kDP;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) vb[4 * i + j].load(p + j * kDP, r);
-                vs[i] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
-            }
-        };
         if (k_begin < k_end) {
+            load_pages(k_begin);
             load_k(k_begin);
             load_v(k_begin);
+            load_pages(k_begin + kUnit);
         }
         for (int key = k_begin; key < k_end; key += kUnit) {
             const int next = key + kUnit < k_end ? key + kUnit : key;  // the last step again: never used
@@ -637,6 +667,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
                     }
             }
             load_v(next);
+            load_pages(next + kUnit);
         }
 
         // the four waves' shares of the keys meet in LDS, in the order of the waves
@@ -705,70 +736,97 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
     }
 }
 
-// Joins the shares of the items that several blocks worked on: kW waves for each row (of 4 in
-// a block), which take the item's shares in turn; kDP / 64 elements of the row in each lane.  64 shares'
-// maxima and sums lie in the lanes at a time, so the loads of their O rows depend on nothing
-// (a loop over the shares that waited for each one's maximum took 23.5 us for 64 shares of 32 rows, this one 4.9).
-template <int kDP, int kTile, int kW>
+// Joins the shares of the items that several blocks worked on, in their order: kDP / 4 lanes (of a group of kG) for a
+// row, four elements each.  A row has one group, or (kAll) those of the whole block, which take its shares by turns, eight
+// at a time: maxima, sums and rows of O are all on their way before the first is needed (2000 rows of 8 heads in four
+// shares: 13.7 us when the maxima came first).
+template <int kDP, int kTile, bool kAll>
 __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
-    constexpr int kE = (kDP + 63) / 64;
-    __shared__ float x_lds[kAttWaves][kE * 64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = blockIdx.y * (kAttWaves / kW) + wave / kW, part = wave % kW;
+    constexpr int kG = kDP <= 32 ? 8 : kDP <= 64 ? 16 : 32, kGroups = kAttBlock / kG, kParts = kAll ? kGroups : 1;
+    __shared__ f32x4 x_lds[kAll ? kGroups : 1][kG];
+    __shared__ float m_lds[kGroups], l_lds[kGroups];
+    const int lane = threadIdx.x & 63, group = threadIdx.x / kG, d = 4 * (threadIdx.x % kG);
+    const int row = kAll ? blockIdx.y : blockIdx.y * kGroups + group, part = kAll ? group : 0;
     const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
     const Item it = find_item<kTile, false>(a, s0, blockIdx.x, lane);
-    if (!it.ok) return;  // (kW > 1: row is the block's, so whole blocks leave)
-    if (it.tile * kTile + row >= it.rows * a.group) return;
+    if (!it.ok) return;
+    const bool mine = it.tile * kTile + row < it.rows * a.group;
+    if (kAll && !mine) return;  // (the whole block)
     const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
     const Shares sh(units, a.blocks);
     const int b0 = sh.of(it.unit0), b1 = sh.of(it.unit0 + it.units - 1);
     if (b0 == b1) return;  // one block had it all
-    const float* ml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP) + 2 * row;
-    const int skip = sh.begin(b0) == it.unit0 ? 0 : 1;
-    auto slot = [&](int b) { return static_cast<int64_t>(2 * b + (b == b0 ? skip : 0)) * kTile; };
-    float top = -INFINITY;
-    for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, ml[2 * slot(b)]);
-    top = wave_max(top);
-    float sum = 0.f, x[kE] = {};
-    for (int c = b0; c <= b1; c += 64) {
-        const int b = min(c + lane, b1);
-        const float mb = ml[2 * slot(b)], lb = ml[2 * slot(b) + 1];
-        const float f = mb == -INFINITY || c + lane > b1 ? 0.f : exp2_hw(mb - top);
-        sum += wave_sum(lb * f);
-        const int n = min(64, b1 - c + 1);
-        for (int i = part; i < n; i += 8 * kW) {  // eight shares' rows in flight
-            float v[8][kE], fi[8];
+    const float* ml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP);
+    const int skip = sh.begin(b0) == it.unit0 ? 0 : 1, at_row = mine ? row : 0, at_d = min(d, kDP - 4);
+    float top = -INFINITY, sum = 0.f;
+    f32x4 x{};
+    for (int b = b0 + part; b <= b1; b += 8 * kParts) {
+        float m[8], l[8];
+        f32x4 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int j = min(i + u * kW, n - 1);
-                fi[u] = i + u * kW < n ? readlane(f, j) : 0.f;
-                const float* po = a.part + (slot(c + j) + row) * kDP;
-#pragma unroll
-                for (int e = 0; e < kE; ++e) v[u][e] = po[min(lane + 64 * e, kDP - 1)];
+        for (int u = 0; u < 8; ++u) {
+            if (u >= 4 && b + 4 * kParts > b1) {  // uniform without kAll; four cost less than eight
+                m[u] = -INFINITY;
+                l[u] = 0.f;
+                v[u] = f32x4{};
+                continue;
             }
+            const int c = min(b + u * kParts, b1);
+            const int64_t slot = static_cast<int64_t>(2 * c + (c == b0 ? skip : 0)) * kTile + at_row;
+            m[u] = b + u * kParts <= b1 ? ml[2 * slot] : -INFINITY;
+            l[u] = ml[2 * slot + 1];
+            v[u] = *reinterpret_cast<const f32x4*>(a.part + slot * kDP + at_d);
+        }
+        float next = top;
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 8; ++u) next = fmaxf(next, m[u]);
+        const float ref = next == -INFINITY ? 0.f : next, f0 = exp2_hw(top - ref);
+        sum *= f0;
+        x *= f0;
+        top = next;
 #pragma unroll
-                for (int e = 0; e < kE; ++e) x[e] = i + u * kW < n ? fmaf(v[u][e], fi[u], x[e]) : x[e];
+        for (int u = 0; u < 8; ++u) {
+            const float f = exp2_hw(m[u] - ref);
+            sum = m[u] == -INFINITY ? sum : fmaf(l[u], f, sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = m[u] == -INFINITY ? x[e] : fmaf(v[u][e], f, x[e]);
         }
     }
-    if constexpr (kW > 1) {
-#pragma unroll
-        for (int e = 0; e < kE; ++e) x_lds[wave][lane + 64 * e] = x[e];
+    if constexpr (kAll) {
+        x_lds[group][d / 4] = x;
+        if (d == 0) {
+            m_lds[group] = top;
+            l_lds[group] = sum;
+        }
         __syncthreads();
-        if (part) return;
+        if (group) return;
+        const float mine_top = top;
 #pragma unroll
-        for (int w = 1; w < kW; ++w)
+        for (int w = 1; w < kGroups; ++w) top = fmaxf(top, m_lds[w]);
+        const float f0 = mine_top == -INFINITY ? 0.f : exp2_hw(mine_top - top);
+        sum *= f0;
+        x *= f0;
 #pragma unroll
-            for (int e = 0; e < kE; ++e) x[e] += x_lds[wave + w][lane + 64 * e];
+        for (int w = 1; w < kGroups; ++w) {
+            const float mw = m_lds[w], f = mw == -INFINITY ? 0.f : exp2_hw(mw - top);
+            if (mw == -INFINITY) continue;
+            sum = fmaf(l_lds[w], f, sum);
+            x += x_lds[w][d / 4] * f;
+        }
     }
+    if (!mine || d >= a.d) return;
     const int rr = it.tile * kTile + row, t = static_cast<int>(a.by_group.div(rr));
     const int64_t dst = ((it.first + static_cast<int64_t>(t)) * (static_cast<int64_t>(a.heads) * a.group) +
-                         static_cast<int64_t>(it.head) * a.group + (rr - t * a.group)) * a.d;
+                         static_cast<int64_t>(it.head) * a.group + (rr - t * a.group)) * a.d + d;
+    float y[4];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-        const int d = lane + 64 * e;
-        if (d < a.d) store_elem(a.out, dst + d, a.dtype, sum == 0.f ? 0.f : x[e] / sum);
+    for (int e = 0; e < 4; ++e) y[e] = sum == 0.f ? 0.f : x[e] / sum;
+    if (a.out_vec) {
+        store_4(a.out, dst, a.dtype, y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.d) store_elem(a.out, dst + e, a.dtype, y[e]);
     }
 }
 
@@ -842,30 +900,106 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
         sees(row0 + 32 * wq, row0 + 32 * wq + 31, all_w, lim_w);
         const bool idle = row0 + 32 * wq >= n_rows;  // a wave without rows
 
+        const int k_begin = u_first * kUnit;
+        const int k_end = min((u_first + u_count) * kUnit, lim_b);
+        const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
+
+        // ---- staging: raw codes of a turn in registers, then fragments in LDS
+        // K: key `lane`, bytes kRun wave ..; V: keys 16 vt + 4 vh + {0..3, 8..11}, elements 4 vd ..
+        const bool v_on = tid / kQuads < 8;
+        constexpr bool kShort = kPlanes == 2 && kDP == 128;  // of registers: places are worked out again in each turn
+        uint32_t kw[kRun / 4], vw[8];
+        float sk = 0.f, sv = 0.f;
+        bool k_ok = false, v_ok = false;
+        // page of key `lane` of the turn to be loaded next, read a turn before it is needed (a wait for it is a wait
+        // for all loads before it)
+        int page = 0;
+        auto load_page = [&](int key) {
+            const int lane = (kShort ? here(tid) : tid) & 63;
+            const int kk = key + lane < it.len ? key + lane : 0;
+            page = table[a.b.by_page.div(static_cast<uint32_t>(kk))];
+        };
+        auto place = [&](int key, int pg, bool& ok) -> int64_t {
+            ok = key < it.len && pg >= 0 && pg < a.b.pages;
+            const int kk = ok ? key : 0, in = kk - static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(kk))) * a.b.page;
+            return (static_cast<int64_t>(ok ? pg : 0) * a.heads + it.head) * a.b.page + in;
+        };
+        // loads a turn's codes, and the page of the one after it
+        auto load = [&](int key) {
+            const int tl = kShort ? here(tid) : tid, lane = tl & 63;
+            const int vd = tl % kQuads, vth = tl / kQuads, vt = vth >> 1, vh = vth & 1;
+            const int v_page = __shfl(page, 16 * (vt & 3));
+            const int64_t rk = place(key + lane, page, k_ok);
+            KBytes<kDP> kb;
+            kb.load(a.k + rk * kDP + kRun * wave);
+#pragma unroll
+            for (int i = 0; i < kRun / 4; ++i) kw[i] = kb.w[i];
+            if (wave == 0) {
+                sk = a.k_scale[rk];
+                sv = a.v_scale[rk];
+            }
+            if (v_on) {
+                // the first of the sixteen keys decides: a page holds whole sixteens, and keys past the length read
+                // what lies there and are dropped by their scale
+                const int64_t rv = place(key + 16 * vt, v_page, v_ok);
+                const uint8_t* p = a.v + (rv + 4 * vh) * kDP + 4 * vd;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    vw[j] = *reinterpret_cast<const uint32_t*>(p + ((j & 3) + 8 * (j >> 2)) * kDP);
+            }
+            load_page(key + kKeys);
+        };
+        if (k_begin < k_end) {  // on its way while q is worked out
+            load_page(k_begin);
+            load(k_begin);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
         // where row `row` of the tile lies in q (token and head strides) or in the output
         auto row_at = [&](int row, int64_t token, int64_t head) {
             const int rr = row0 + row, t = static_cast<int>(a.by_group.div(rr));
             return (it.first + static_cast<int64_t>(t)) * token + (static_cast<int64_t>(it.head) * a.group + (rr - t * a.group)) * head;
         };
         const int valid = min(kTile, n_rows - row0);
+        constexpr int kAtOnce = kShort ? 2 : 4;  // 16-byte loads in flight (f32: two each)
 #pragma unroll 1
-        for (int i = here(tid); i < kTile * (kDP / 8); i += kAttBlock) {
-            const int row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
-            float x[8] = {};
-            if (row < valid && d0 < a.d) {
-                const int64_t at_q = row_at(row, a.q_token, a.q_head) + d0;
-                if (a.q_vec) {
-                    load_8(a.q, at_q, a.dtype, x);
-                } else {
-#pragma unroll 1
-                    for (int j = 0; j < 8 && d0 + j < a.d; ++j) rows[row * kORow + d0 + j] = load_elem(a.q, at_q + j, a.dtype);
+        for (int i0 = here(tid); i0 < kTile * (kDP / 8); i0 += kAtOnce * kAttBlock) {
+            u32x4 raw[kAtOnce][2];
+            if (a.q_vec) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.d ? rows[row * kORow + d0 + j] : 0.f;
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int i = i0 + u * kAttBlock, row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
+                    const int64_t at_q = row_at(min(row, valid - 1), a.q_token, a.q_head) + (d0 < a.d ? d0 : 0);
+                    if (a.dtype == TQ_DT_F32) {
+                        const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at_q);
+                        raw[u][0] = src[0];
+                        raw[u][1] = src[1];
+                    } else {
+                        raw[u][0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at_q);
+                    }
                 }
             }
-            f32x4* o = reinterpret_cast<f32x4*>(&rows[row * kORow + d0]);
-            o[0] = f32x4{x[0], x[1], x[2], x[3]};
-            o[1] = f32x4{x[4], x[5], x[6], x[7]};
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int i = i0 + u * kAttBlock, row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
+                if (row >= kTile) continue;
+                float x[8] = {};
+                if (row < valid && d0 < a.d) {
+                    if (a.q_vec) {
+                        widen_8(raw[u], a.dtype, x);
+                    } else {
+                        const int64_t at_q = row_at(row, a.q_token, a.q_head) + d0;
+#pragma unroll 1
+                        for (int j = 0; j < 8 && d0 + j < a.d; ++j)
+                            rows[row * kORow + d0 + j] = load_elem(a.q, at_q + j, a.dtype);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] = d0 + j < a.d ? rows[row * kORow + d0 + j] : 0.f;
+                    }
+                }
+                f32x4* o = reinterpret_cast<f32x4*>(&rows[row * kORow + d0]);
+                o[0] = f32x4{x[0], x[1], x[2], x[3]};
+                o[1] = f32x4{x[4], x[5], x[6], x[7]};
+            }
         }
         __syncthreads();
 
@@ -911,48 +1045,8 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
         for (int c = 0; c < kCols; ++c) o[c] = f32x16{};
         float m = -INFINITY, l = 0.f;
 
-        const int k_begin = u_first * kUnit;
-        const int k_end = min((u_first + u_count) * kUnit, lim_b);
-        const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
-
-        // ---- staging: raw codes of a turn in registers, then fragments in LDS
-        // K: key `lane`, bytes kRun wave ..; V: keys 16 vt + 4 vh + {0..3, 8..11}, elements 4 vd ..
-        const int vd = tid % kQuads, vth = tid / kQuads, vt = vth >> 1, vh = vth & 1;
-        const bool v_on = vth < 8;
-        uint32_t kw[kRun / 4], vw[8];
-        float sk = 0.f, sv = 0.f;
-        bool k_ok = false, v_ok = false;
-        auto place = [&](int key, bool& ok) -> int64_t {
-            ok = key < it.len;
-            const int kk = ok ? key : 0, i = static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(kk)));
-            int page = table[i];
-            if (page < 0 || page >= a.b.pages) {
-                page = 0;
-                ok = false;
-            }
-            return (static_cast<int64_t>(page) * a.heads + it.head) * a.b.page + (kk - i * a.b.page);
-        };
-        auto load = [&](int key) {
-            const int64_t rk = place(key + lane, k_ok);
-            KBytes<kDP> kb;
-            kb.load(a.k + rk * kDP + kRun * wave);
-#pragma unroll
-            for (int i = 0; i < kRun / 4; ++i) kw[i] = kb.w[i];
-            if (wave == 0) {
-                sk = a.k_scale[rk];
-                sv = a.v_scale[rk];
-            }
-            if (v_on) {
-                // the first of the sixteen keys decides: a page holds whole sixteens, and keys past the length read
-                // what lies there and are dropped by their scale
-                const int64_t rv = place(key + 16 * vt, v_ok);
-                const uint8_t* p = a.v + (rv + 4 * vh) * kDP + 4 * vd;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    vw[j] = *reinterpret_cast<const uint32_t*>(p + ((j & 3) + 8 * (j >> 2)) * kDP);
-            }
-        };
         auto store = [&](Buf& b, int key) {
+            const int lane = (kShort ? here(tid) : tid) & 63;
 #pragma unroll
             for (int i = 0; i < kRun / 8; ++i) {
                 const int gi = wave * (kRun / 8) + i;  // elements 8 gi ..: step gi / 2, half gi % 2
@@ -969,13 +1063,14 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
             }
             uint32_t bad_here = 0;
             if (v_on) {
-                const int to = Codes::kNan && kPlanes == 2 ? here(tid) : tid;  // (one form is short of registers)
+                const int to = kShort ? here(tid) : tid;
                 const int vd = to % kQuads, vth = to / kQuads, vt = vth >> 1, vh = vth & 1;
                 const int k16 = key + 16 * vt + 4 * vh;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool ok = v_ok && k16 + (j & 3) + 8 * (j >> 2) < it.len;
-                    vw[j] = ok ? vw[j] : 0u;
+                for (int j = 0; j < 8; ++j) vw[j] = v_ok ? vw[j] : 0u;
+                if (key + kKeys > it.len) {  // uniform
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) vw[j] = k16 + (j & 3) + 8 * (j >> 2) < it.len ? vw[j] : 0u;
                 }
                 if (Codes::kNan && key + kKeys > all_b) {  // rows that do not see a key must not meet its NaN
                     const int t3 = here(tid);
@@ -1009,7 +1104,6 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
             if (Codes::kNan) b.any_bad[wave] = __ballot(bad_here != 0) != 0;
         };
         if (k_begin < k_end) {
-            load(k_begin);
             store(buf[0], k_begin);
             __builtin_amdgcn_sched_barrier(0);
             load(k_begin + kKeys < k_end ? k_begin + kKeys : k_begin);
@@ -1023,6 +1117,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                 for (int u = 0; u < kSub; ++u) {
                     const int sub = kWK == 2 ? wk : u, k32 = key + 32 * sub;
                     if (k32 >= lim_w) continue;  // uniform: nothing that the wave's rows see
+                    const int lane = (kShort ? here(tid) : tid) & 63, h = lane >> 5;
                     f32x16 st = f32x16{};
 #pragma unroll
                     for (int s = 0; s < kSteps; ++s) {
@@ -1226,15 +1321,17 @@ int launch_attention(const AttArg& a, const AttPlan& p, hipStream_t st) {
     return check_launch("tq_kv_attention");
 }
 
-// four waves for each row where an item has many shares
+// a block for each row where an item has many shares
 template <int kDP, int kTile>
 int launch_join(const AttArg& a, const AttPlan& p, hipStream_t st) {
+    constexpr int kG = kDP <= 32 ? 8 : kDP <= 64 ? 16 : 32, kRows = kAttBlock / kG;
     const int64_t rows = std::min<int64_t>(static_cast<int64_t>(a.b.max_tokens) * a.group, kTile);
     const unsigned items = static_cast<unsigned>(p.items);
-    if (p.blocks >= 8 * p.items)
-        k_kv_attention_join<kDP, kTile, 4><<<dim3(items, static_cast<unsigned>(rows)), kAttBlock, 0, st>>>(a);
+    if (p.blocks >= 16 * p.items)
+        k_kv_attention_join<kDP, kTile, true><<<dim3(items, static_cast<unsigned>(rows)), kAttBlock, 0, st>>>(a);
     else
-        k_kv_attention_join<kDP, kTile, 1><<<dim3(items, static_cast<unsigned>((rows + 3) / 4)), kAttBlock, 0, st>>>(a);
+        k_kv_attention_join<kDP, kTile, false>
+            <<<dim3(items, static_cast<unsigned>((rows + kRows - 1) / kRows)), kAttBlock, 0, st>>>(a);
     return check_launch("tq_kv_attention");
 }
 
