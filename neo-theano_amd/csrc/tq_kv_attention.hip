@@ -911,25 +911,32 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
         uint32_t kw[kRun / 4], vw[8];
         float sk = 0.f, sv = 0.f;
         bool k_ok = false, v_ok = false;
-        // page of key `lane` of the turn to be loaded next, read a turn before it is needed (a wait for it is a wait
-        // for all loads before it)
+        // page of key `lane` of the turn to be loaded next and the key's place there, read a turn before they are
+        // needed (a wait for the page is a wait for all loads before it)
+        const uint32_t page_rows = static_cast<uint32_t>(a.heads) * static_cast<uint32_t>(a.b.page);  // below 2^32
+        const uint32_t head_row = static_cast<uint32_t>(it.head) * static_cast<uint32_t>(a.b.page);
         int page = 0;
+        uint32_t in = 0;
         auto load_page = [&](int key) {
             const int lane = (kShort ? here(tid) : tid) & 63;
-            const int kk = key + lane < it.len ? key + lane : 0;
-            page = table[a.b.by_page.div(static_cast<uint32_t>(kk))];
+            const uint32_t kk = key + lane < it.len ? key + lane : 0, i = a.b.by_page.div(kk);
+            in = kk - i * a.b.page + head_row;
+            page = table[i];
         };
-        auto place = [&](int key, int pg, bool& ok) -> int64_t {
-            ok = key < it.len && pg >= 0 && pg < a.b.pages;
-            const int kk = ok ? key : 0, in = kk - static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(kk))) * a.b.page;
-            return (static_cast<int64_t>(ok ? pg : 0) * a.heads + it.head) * a.b.page + in;
+        auto place = [&](int pg, uint32_t in, bool& ok) -> int64_t {
+            ok = ok && pg >= 0 && pg < a.b.pages;
+            return static_cast<int64_t>(static_cast<uint64_t>(ok ? static_cast<uint32_t>(pg) : 0u) * page_rows + in);
         };
         // loads a turn's codes, and the page of the one after it
         auto load = [&](int key) {
             const int tl = kShort ? here(tid) : tid, lane = tl & 63;
             const int vd = tl % kQuads, vth = tl / kQuads, vt = vth >> 1, vh = vth & 1;
+            // the first of the sixteen keys decides: a page holds whole sixteens, and keys past the length read
+            // what lies there and are dropped by their scale
             const int v_page = __shfl(page, 16 * (vt & 3));
-            const int64_t rk = place(key + lane, page, k_ok);
+            const uint32_t v_in = __shfl(in, 16 * (vt & 3));
+            k_ok = key + lane < it.len;
+            const int64_t rk = place(page, in, k_ok);
             KBytes<kDP> kb;
             kb.load(a.k + rk * kDP + kRun * wave);
 #pragma unroll
@@ -939,9 +946,8 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                 sv = a.v_scale[rk];
             }
             if (v_on) {
-                // the first of the sixteen keys decides: a page holds whole sixteens, and keys past the length read
-                // what lies there and are dropped by their scale
-                const int64_t rv = place(key + 16 * vt, v_page, v_ok);
+                v_ok = key + 16 * vt < it.len;
+                const int64_t rv = place(v_page, v_in, v_ok);
                 const uint8_t* p = a.v + (rv + 4 * vh) * kDP + 4 * vd;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -949,36 +955,39 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
             }
             load_page(key + kKeys);
         };
-        if (k_begin < k_end) {  // on its way while q is worked out
-            load_page(k_begin);
-            load(k_begin);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-
         // where row `row` of the tile lies in q (token and head strides) or in the output
         auto row_at = [&](int row, int64_t token, int64_t head) {
             const int rr = row0 + row, t = static_cast<int>(a.by_group.div(rr));
             return (it.first + static_cast<int64_t>(t)) * token + (static_cast<int64_t>(it.head) * a.group + (rr - t * a.group)) * head;
         };
         const int valid = min(kTile, n_rows - row0);
-        constexpr int kAtOnce = kShort ? 2 : 4;  // 16-byte loads in flight (f32: two each)
-#pragma unroll 1
-        for (int i0 = here(tid); i0 < kTile * (kDP / 8); i0 += kAtOnce * kAttBlock) {
-            u32x4 raw[kAtOnce][2];
-            if (a.q_vec) {
+        // loads in flight of a thread, of 8 elements each (f32, which is what takes two planes: two of 16 bytes)
+        constexpr int kAll = (kTile * (kDP / 8) + kAttBlock - 1) / kAttBlock;
+        constexpr int kAtOnce = kPlanes == 1 ? std::min(kAll, 8) : kShort ? 2 : std::min(kAll, 4);
+        u32x4 raw[kAtOnce][2];
+        auto q_load = [&](int i0) {
 #pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    const int i = i0 + u * kAttBlock, row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
-                    const int64_t at_q = row_at(min(row, valid - 1), a.q_token, a.q_head) + (d0 < a.d ? d0 : 0);
-                    if (a.dtype == TQ_DT_F32) {
-                        const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at_q);
-                        raw[u][0] = src[0];
-                        raw[u][1] = src[1];
-                    } else {
-                        raw[u][0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at_q);
-                    }
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int i = i0 + u * kAttBlock, row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
+                const int64_t at_q = row_at(min(row, valid - 1), a.q_token, a.q_head) + (d0 < a.d ? d0 : 0);
+                if (kPlanes == 2) {
+                    const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + at_q);
+                    raw[u][0] = src[0];
+                    raw[u][1] = src[1];
+                } else {
+                    raw[u][0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at_q);
                 }
             }
+        };
+        if (a.q_vec) q_load(here(tid));
+        if (k_begin < k_end) {  // and the first turn's codes
+            load_page(k_begin);
+            load(k_begin);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+        for (int i0 = here(tid); i0 < kTile * (kDP / 8); i0 += kAtOnce * kAttBlock) {
+            if (a.q_vec && i0 >= kAttBlock) q_load(i0);
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const int i = i0 + u * kAttBlock, row = i / (kDP / 8), d0 = 8 * (i % (kDP / 8));
