@@ -550,3 +550,145 @@ def test_no_tokens(tq):
     assert c.cache.read(none)[0].shape == (0, 2, 64)
     rot = tq.Rotary.from_base(64)
     assert rot.apply(x, x, torch.empty(0, dtype=torch.int64, device="cuda"))[0].shape == (0, 2, 64)
+
+
+# ------------------------------------------------------------------ many rows, and calls beside each other
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,r,pairs,h,hk", [(128, 128, False, 4, 2), (80, 40, True, 3, 3), (64, 64, True, 2, 1), (33, 0, False, 1, 1)])
+def test_many_rows_are_one_row_at_a_time(tq, codes, dtype, d, r, pairs, h, hk):
+    """Ragged batches of some hundred rows, with rows that have no place and rows behind the last sequence: codes,
+    turned q and what is read back are those of calls with one row, bit for bit."""
+    import torch
+
+    dt = dtype_of(dtype)
+    lengths, new, extra, page = [150, 3, 70, 40, 12], [97, 3, 0, 40, 9], 6, 16
+    a, b = (Case(tq, lengths, new, page, hk, d, codes, ragged=True, extra=extra) for _ in range(2))
+    a.table[0, 4] = b.table[0, 4] = 10000  # positions 64..79 of the first sequence lie nowhere
+    n = a.rows
+    assert n >= 150
+    q, k, v = rand(1, n, h, d, dtype=dt), rand(2, n, hk, d, dtype=dt), rand(3, n, hk, d, dtype=dt)
+    rot = tq.Rotary.from_base(r, 500.0, pairs, scale=1.5)
+    got = a.cache.write_rotary(q, k, v, rot, a.batch)
+    row = 0
+    for s, (length, t) in enumerate(zip(lengths, new)):
+        for i in range(t):
+            one = tq.KVBatch(b.table[s:s + 1], torch.tensor([length - t + i + 1], dtype=torch.int32).cuda(), 1)
+            part = slice(row, row + 1)
+            assert torch.equal(b.cache.write_rotary(q[part], k[part], v[part], rot, one), got[part]), row
+            row += 1
+    for name in ("k", "k_scale", "v", "v_scale"):
+        assert torch.equal(getattr(a.cache, name), getattr(b.cache, name)), name
+    out = tuple(torch.full((n, hk, d), 5.0, device="cuda", dtype=dt) for _ in range(2))
+    a.cache.read(a.batch, dt, out)
+    row = 0
+    for s, (length, t) in enumerate(zip(lengths, new)):
+        for i in range(t):
+            one = tq.KVBatch(b.table[s:s + 1], torch.tensor([length - t + i + 1], dtype=torch.int32).cuda(), 1)
+            for x, y in zip(out, b.cache.read(one, dt)):
+                assert torch.equal(x[row:row + 1], y), row
+                if 64 <= length - t + i < 80 and s == 0:
+                    assert (y == 0).all()
+            row += 1
+    assert all((x[row:] == 5.0).all() for x in out)
+    # a plain write leaves the same as a write that turns nothing
+    c = Case(tq, lengths, new, page, hk, d, codes, ragged=True, extra=extra)
+    e = Case(tq, lengths, new, page, hk, d, codes, ragged=True, extra=extra)
+    c.cache.write(k, v, c.batch)
+    e.cache.write_rotary(q, k, v, tq.Rotary.from_base(0), e.batch)
+    for name in ("k", "k_scale", "v", "v_scale"):
+        assert torch.equal(getattr(c.cache, name), getattr(e.cache, name)), name
+
+
+def test_rotary_of_one_tensor_twice(tq):
+    import torch
+
+    x, pos = rand(1, 40, 3, 64), torch.arange(40, device="cuda") * 37
+    rot = tq.Rotary.from_base(64)
+    a, b = rot.apply(x, x, pos)
+    assert torch.equal(a, b) and torch.equal(a, rot.apply(x, None, pos)[0]) and a.data_ptr() != b.data_ptr()
+
+
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,new,page,heads,group,d", [
+    ([1500], [100], 64, 1, 2, 128), ([700, 90], [70, 48], 32, 2, 1, 64), ([1000, 20, 400], [33, 20, 5], 16, 1, 2, 96),
+    ([400], [129], 16, 1, 1, 33), ([600], [300], 48, 1, 1, 128), ([2000, 1], [9, 1], 16, 1, 5, 80)])
+def test_attention_of_many_rows_and_keys(tq, codes, dtype, lengths, new, page, heads, group, d):
+    """Tiles of 64 and 128 rows whose keys lie in several shares, behind each other and masked by trees of several
+    words (one more than they need)."""
+    import torch
+
+    dt = dtype_of(dtype)
+    c = Case(tq, lengths, new, page, heads, d, codes, seed=d)
+    for t in (c.cache.k, c.cache.v):
+        t.fill_(127)
+    c.fill(13)
+    q = rand(14, c.rows, heads * group, d, dtype=dt, std=1.5)
+    seen = torch.rand(c.rows, (max(new) + 31) // 32 * 32 + 32, generator=torch.Generator().manual_seed(d)) < 0.3
+    check.v_abs = float(c.cache.v_scale.max()) * (127 if codes == "i8" else 448)
+    for tree in (None, seen):
+        ref, tol = reference(c, q, tree)
+        got = c.cache.attention(q, c.batch, tree=None if tree is None else tq.tree_mask(tree).cuda())
+        check(got, ref, tol, f"{lengths} {new} tree={tree is not None}")
+
+
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("new,group", [(1, 4), (9, 3), (40, 1), (150, 1)])
+def test_attention_skips_keys_without_a_page(tq, codes, new, group):
+    """Keys on pages outside the cache are seen by nobody: the rest attended to alone, on other pages, gives the
+    same up to the order of the sums."""
+    import torch
+
+    page, d, length = 16, 64, 500
+    c = Case(tq, [length], [new], page, 2, d, codes)
+    k, v = c.fill(17)
+    lost = [0, 3, 4, 19]  # pages of the table, before the new tokens
+    keep = [p for p in range(length) if p // page not in lost]
+    e = Case(tq, [len(keep)], [new], page, 2, d, codes)
+    e.cache.write(k[keep], v[keep], e.all_tokens())
+    for i, p in enumerate(lost):
+        c.table[0, p] = (-1, 1 << 30, c.cache.pages, -(1 << 31))[i]
+    q = rand(18, new, 2 * group, d)
+    ref, tol = reference(e, q)
+    check(c.cache.attention(q, c.batch), ref, tol)
+    check(e.cache.attention(q, e.batch), ref, tol)
+
+
+def test_two_streams_and_two_graphs_beside_each_other(tq):
+    """Calls on two streams at once, and two captured calls replayed by turns, each with the results of its own."""
+    import torch
+
+    jobs = []
+    for i, (new, group, d) in enumerate([(1, 4, 128), (3, 2, 64), (60, 2, 128), (200, 1, 96)]):
+        c = Case(tq, [900 + 7 * i, 300], [new, new], 32, 2, d, "i8")
+        c.fill(90 + i)
+        q = rand(95 + i, c.rows, 2 * group, d, dtype=torch.bfloat16)
+        jobs.append((c, q, c.cache.attention(q, c.batch)))
+    x, w = rand(99, 100, 512), tq.QuantizedLinear.from_tensors(rand(98, 300, 512), None, tq.QConfig.fp8_block())
+    want = w(x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for i, (c, q, _) in enumerate(jobs):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, c.cache.attention(q, c.batch), w(x)))
+    torch.cuda.synchronize()
+    for i, o, y in got:
+        assert torch.equal(o, jobs[i][2]) and torch.equal(y, want)
+    graphs, outs = [], []
+    for c, q, _ in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append((c.cache.attention(q, c.batch), w(x)))
+        graphs.append(g)
+    for order in ([0, 1, 2, 3], [3, 1, 2, 0], [2, 2, 0, 3, 1]):
+        for o, y in outs:
+            o.zero_()
+            y.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for (o, y), (_, _, ref) in zip(outs, jobs):
+            assert torch.equal(o, ref) and torch.equal(y, want)
