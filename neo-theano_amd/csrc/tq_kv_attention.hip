@@ -80,8 +80,9 @@ __device__ __forceinline__ int scan64(int v) {
     return v;
 }
 
+// kUnit * per keys are a unit of the line.
 template <int kTile>
-__device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane) {
+__device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane, int per) {
     SeqLane s{};
     const int seq = seq0 + lane;
     if (seq < a.b.batch) {
@@ -95,6 +96,7 @@ __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane)
         s.base = length - s.rows;
         s.tiles = (s.rows * a.group + kTile - 1) / kTile;
         s.units = max((s.len + kUnit - 1) / kUnit, 1);
+        if (per > 1) s.units = (s.units + per - 1) / per;
         s.items = s.tiles * a.heads;
     }
     if (a.b.batch == 1) {  // every lane past the first holds nothing
@@ -107,19 +109,36 @@ __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane)
     return s;
 }
 
-struct Totals {
-    int items, units;
+// The line as the blocks share it: `units` of kUnit * per keys over `blocks`.  Where items are few, `per` is the least
+// for which each unit can have a block of its own, so that no block works on two items, whose rows would be read, set up
+// and written twice (trees of 48 drafts, 128 items of 4 to 16 units: 26 us with equal shares of the line, 22 so); where
+// they are many, such units would leave blocks idle, and the line is cut into equal shares of single units.
+struct Line {
+    int per, units, blocks;
 };
 
 template <int kTile>
-__device__ __forceinline__ Totals all_work(const AttArg& a, int lane) {
-    Totals t{0, 0};
-    for (int s0 = 0; s0 < a.b.batch; s0 += 64) {
-        const SeqLane s = seq_lane<kTile>(a, s0, lane);
-        t.items += readlane(s.items_end, 63);
-        t.units += readlane(s.units_end, 63);
+__device__ __forceinline__ Line share_line(const AttArg& a, SeqLane& s, int lane) {
+    Line w{1, 0, a.blocks};
+    s = seq_lane<kTile>(a, 0, lane, 1);
+    if (!a.part) return w;
+    w.units = readlane(s.units_end, 63);
+    if (a.b.batch > 64) {
+        for (int s0 = 64; s0 < a.b.batch; s0 += 64) w.units += readlane(seq_lane<kTile>(a, s0, lane, 1).units_end, 63);
+        return w;
     }
-    return t;
+    if (w.units <= a.blocks || readlane(s.items_end, 63) > a.blocks / 2) return w;
+    // ends: with `per` at the longest item's units there are as many units as items
+    for (w.per = (w.units + a.blocks - 1) / a.blocks;; w.per += 1 + w.per / 16) {
+        const int mine = (s.units + w.per - 1) / w.per, v = s.items * mine;
+        const int end = a.b.batch == 1 ? readlane(v, 0) : scan64(v), units = readlane(end, 63);
+        if (units <= a.blocks) {
+            s.units = mine;
+            s.units_end = end;
+            w.units = w.blocks = units;
+            return w;
+        }
+    }
 }
 
 // Share i of u units over n blocks: u / n each, one more for the first u % n.
@@ -173,7 +192,7 @@ __device__ __forceinline__ Item find_item(const AttArg& a, const SeqLane& s0, in
     }
     int items = 0, units = 0;
     for (int seq = 0; seq < a.b.batch; seq += 64) {
-        const SeqLane s = seq_lane<kTile>(a, seq, lane);
+        const SeqLane s = seq_lane<kTile>(a, seq, lane, 1);
         const int ni = readlane(s.items_end, 63), nu = readlane(s.units_end, 63);
         if (at < (kByUnit ? units + nu : items + ni)) return pick<kByUnit>(s, seq, items, units, at, 0);
         items += ni;
@@ -393,16 +412,14 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
-    int at, end;
+    SeqLane s0;
+    const Line line = share_line<kTile>(a, s0, lane);
+    int at = 0, end = 1;
     if (a.part) {
-        const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
-        const Shares sh(units, a.blocks);
+        if (static_cast<int>(blockIdx.x) >= line.blocks) return;
+        const Shares sh(line.units, line.blocks);
         at = sh.begin(blockIdx.x);
         end = sh.begin(blockIdx.x + 1);
-    } else {
-        at = 0;
-        end = 1;
     }
     bool first_share = true;
     while (at < end) {
@@ -418,8 +435,8 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
         const int lim = a.tree ? it.len : min(it.base + t_last + 1, it.len);
         const int all = a.tree ? min(it.base, it.len) : min(it.base + t_first + 1, it.len);
 
-        const int k_end = min((u_first + u_count) * kUnit, lim);
-        const int k_begin = u_first * kUnit + wave * kStep;
+        const int k_end = min((u_first + u_count) * line.per * kUnit, lim);
+        const int k_begin = u_first * line.per * kUnit + wave * kStep;
         const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
 
         // Pages of the 16 keys each (a page holds whole sixteens) of the step to be loaded next: read a step before
@@ -747,13 +764,13 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
     __shared__ float m_lds[kGroups], l_lds[kGroups];
     const int lane = threadIdx.x & 63, group = threadIdx.x / kG, d = 4 * (threadIdx.x % kG);
     const int row = kAll ? blockIdx.y : blockIdx.y * kGroups + group, part = kAll ? group : 0;
-    const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
+    SeqLane s0;
+    const Line line = share_line<kTile>(a, s0, lane);
     const Item it = find_item<kTile, false>(a, s0, blockIdx.x, lane);
     if (!it.ok) return;
     const bool mine = it.tile * kTile + row < it.rows * a.group;
     if (kAll && !mine) return;  // (the whole block)
-    const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
-    const Shares sh(units, a.blocks);
+    const Shares sh(line.units, line.blocks);
     const int b0 = sh.of(it.unit0), b1 = sh.of(it.unit0 + it.units - 1);
     if (b0 == b1) return;  // one block had it all
     const float* ml = a.part + 2 * static_cast<int64_t>(a.blocks) * (kTile * kDP);
@@ -852,6 +869,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     constexpr int kKF = 2 * kSteps * 64, kVF = 4 * kCols * 64;  // 16-byte fragments of a turn
     constexpr int kRun = kDP / 4, kQuads = kDP / 4;
     constexpr int kORow = kDP + 4;
+    constexpr bool kShort = kPlanes == 2 && kDP == 128;  // of registers: places are worked out again in each turn
     struct Buf {
         h8 k[kKF], v[kVF];
         float ck[kKeys], lsv[kKeys], rsv[kKeys];
@@ -868,20 +886,18 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wq = wave % kWQ, wk = wave / kWQ;
 
-    int at, end;
+    SeqLane s0;
+    const Line line = share_line<kTile>(a, s0, lane);
+    int at = 0, end = 1;
     if (a.part) {
-        const SeqLane s0 = seq_lane<kTile>(a, 0, lane);
-        const int units = a.b.batch <= 64 ? readlane(s0.units_end, 63) : all_work<kTile>(a, lane).units;
-        const Shares sh(units, a.blocks);
+        if (static_cast<int>(blockIdx.x) >= line.blocks) return;
+        const Shares sh(line.units, line.blocks);
         at = sh.begin(blockIdx.x);
         end = sh.begin(blockIdx.x + 1);
-    } else {
-        at = 0;
-        end = 1;
     }
     bool first_share = true;
     while (at < end) {
-        const SeqLane s0 = seq_lane<kTile>(a, 0, here(lane));  // (again for each item: it would hold ten registers)
+        if (!first_share || kShort) s0 = seq_lane<kTile>(a, 0, here(lane), line.per);  // (kept, it would hold ten registers)
         const Item it = a.part ? find_item<kTile, true>(a, s0, at, lane) : find_item<kTile, false>(a, s0, blockIdx.x, lane);
         if (!it.ok) return;
         const int u_first = a.part ? at - it.unit0 : 0;
@@ -900,14 +916,13 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
         sees(row0 + 32 * wq, row0 + 32 * wq + 31, all_w, lim_w);
         const bool idle = row0 + 32 * wq >= n_rows;  // a wave without rows
 
-        const int k_begin = u_first * kUnit;
-        const int k_end = min((u_first + u_count) * kUnit, lim_b);
+        const int k_begin = u_first * line.per * kUnit;
+        const int k_end = min((u_first + u_count) * line.per * kUnit, lim_b);
         const int32_t* table = a.b.table + static_cast<int64_t>(it.seq) * a.b.table_stride;
 
         // ---- staging: raw codes of a turn in registers, then fragments in LDS
         // K: key `lane`, bytes kRun wave ..; V: keys 16 vt + 4 vh + {0..3, 8..11}, elements 4 vd ..
         const bool v_on = tid / kQuads < 8;
-        constexpr bool kShort = kPlanes == 2 && kDP == 128;  // of registers: places are worked out again in each turn
         uint32_t kw[kRun / 4], vw[8];
         float sk = 0.f, sv = 0.f;
         bool k_ok = false, v_ok = false;

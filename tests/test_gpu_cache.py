@@ -692,3 +692,36 @@ def test_two_streams_and_two_graphs_beside_each_other(tq):
         torch.cuda.synchronize()
         for (o, y), (_, _, ref) in zip(outs, jobs):
             assert torch.equal(o, ref) and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("lengths,new,heads,group,d", [
+    ([20000, 12345, 300], [40, 33, 40], 4, 1, 64), ([9000, 30000], [3, 1], 4, 4, 128), ([17000], [200], 8, 1, 128),
+    ([4000] * 40 + [5], [1] * 41, 4, 2, 32)])
+def test_attention_of_a_few_long_sequences(tq, dtype, lengths, new, heads, group, d):
+    """Sequences of many more units than blocks, unequal ones: in units of several hundred keys, and (164 heads) in
+    equal shares of the line; against 64 bits on the GPU, the bound of `reference`."""
+    import torch
+
+    dt = dtype_of(dtype)
+    c = Case(tq, lengths, new, 64, heads, d, "i8", ragged=True)
+    c.fill(33)
+    q = rand(34, c.rows, heads * group, d, dtype=dt, std=1.5)
+    got = c.cache.attention(q, c.batch)
+    check.v_abs = float(c.cache.v_scale.max()) * 127
+    for b, (length, t) in enumerate(zip(lengths, new)):
+        pos = torch.arange(length, device="cuda")
+        pages = c.table[b, pos // 64].long()
+        k, v = ((x[pages, :, pos % 64, :d].double() * s[pages, :, pos % 64].double()[..., None]).transpose(0, 1).contiguous()
+                for x, s in ((c.cache.k, c.cache.k_scale), (c.cache.v, c.cache.v_scale)))
+        rows = slice(int(c.offsets[b]), int(c.offsets[b + 1]))
+        qq = q[rows].double().view(t, heads, group, d).transpose(0, 1).reshape(heads, t * group, d)
+        s = torch.matmul(qq, k.transpose(1, 2).contiguous()) / math.sqrt(d)
+        seen = pos[None] <= (length - t + torch.arange(t, device="cuda"))[:, None]
+        s = s.masked_fill(~seen.repeat_interleave(group, 0)[None], -math.inf)
+        size = (torch.matmul(qq.abs(), k.abs().transpose(1, 2).contiguous()) / math.sqrt(d)).amax(-1, keepdim=True)
+        p = torch.softmax(s, -1)
+        off = 2.0 ** -24 * ((d + 16) * size + 8 * (torch.where(s.isinf(), 0.0, s).abs().amax(-1, keepdim=True) + 64))
+        ref, tol = (x.view(heads, t, group, d).transpose(0, 1).reshape(t, heads * group, d).cpu()
+                    for x in (torch.matmul(p, v), 2 * off * torch.matmul(p, v.abs())))
+        check(got[rows], ref, tol, f"sequence {b}")
