@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kQuantBlock) void k_dequant_block(const uint8_t* __
 // sums start from zero and join the totals times sa sw: W is the matrix cores' row operand, so a lane's sums share
 // one token, and the factor is one number for each 32 tokens.
 // The activations' codes are padded to whole stages with zeros; weight chunks past K re-read their row's first one,
-// which meets those zeros.  Needs K % 16 == 0 and 16-byte aligned weights.
+// which meets those zeros.  Direct loads take K % 16 == 0 and 16-byte aligned weights.
 // M=2047, N=4104, K=4000: 72 us and 5 for the joins, 0.93 PFLOP/s; 128 x 256 tiles, a block a CU, take 158.  A stage's 8
 // conversions and 16 matrix instructions a wave fill the SIMD's issue; the two blocks of a CU cover each other's barriers.
 constexpr int kTN = 2, kBM = 128, kBN = 64 * kTN, kBK = 128;
@@ -146,6 +146,25 @@ __device__ __forceinline__ void block_tile(const BlockArgs& p, int L, int& tm, i
     tn = in / rows;
 }
 
+// Bytes k0 .. k0 + 15 of a row of k >= 16, zeros past it: 16 bytes that end where the row does, shifted into place.
+__device__ __forceinline__ u32x4 row_tail(const uint8_t* row, int k0, int k) {
+    const int back = min(max(k0 + 16 - k, 0), 16);
+    const u32x4 v = *reinterpret_cast<const u32x4_a1*>(row + k0 - max(k0 + 16 - k, 0));
+    const int s = 8 * (back & 7);
+    uint64_t lo = v.x | static_cast<uint64_t>(v.y) << 32, hi = v.z | static_cast<uint64_t>(v.w) << 32;
+    lo = back >= 8 ? hi : lo;
+    hi = back >= 8 ? 0 : hi;
+    const uint64_t carry = s ? hi << (64 - s) : 0;
+    lo = (lo >> s) | carry;
+    hi >>= s;
+    if (back == 16) lo = hi = 0;
+    return u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                 static_cast<uint32_t>(hi >> 32)};
+}
+
+// kAligned: as above; else the weights come through registers, 16 bytes at any address, and go to LDS behind the stage's
+// products (M=2047, N=4104, the call of three launches: 88 us at K=4000, 102 at K=4001, 204 on the smaller tiles).
+template <bool kAligned>
 __global__ __launch_bounds__(256, 2) void k_gemm_block_dma(BlockArgs p) {
     constexpr int kWBytes = kBN * kBK, kStage = kWBytes + kBM * kBK;
     constexpr int kWDma = kBN / 32, kADma = kBM / 32;  // 16-byte loads of a lane for each stage (8 rows a wave and load)
@@ -185,9 +204,20 @@ __global__ __launch_bounds__(256, 2) void k_gemm_block_dma(BlockArgs p) {
         dst[t] = lds_addr(lds) + (isw ? 0 : kWBytes) + slot * 1024;
     }
     static_assert(kWDma % 2 == 0, "swizzles alternate between even and odd slots");
+    u32x4 held[kAligned ? 1 : kWDma];
     auto load_stage = [&](int k0, int buf) {
         const uint32_t to = buf * kStage;
-        if (k0 + kBK <= p.k) {
+        if constexpr (!kAligned) {
+#pragma unroll
+            for (int t = 0; t < kWDma; ++t) {
+                if (k0 + kBK <= p.k)
+                    held[t] = *reinterpret_cast<const u32x4_a1*>(src[t] + k0);
+                else
+                    held[t] = row_tail(reinterpret_cast<const uint8_t*>(src[t]) - chunk[t & 1], k0 + chunk[t & 1], p.k);
+            }
+#pragma unroll
+            for (int t = kWDma; t < kWDma + kADma; ++t) lds_dma16(src[t] + k0, dst[t] + to);
+        } else if (k0 + kBK <= p.k) {
 #pragma unroll
             for (int t = 0; t < kWDma + kADma; ++t) lds_dma16(src[t] + k0, dst[t] + to);
         } else {
@@ -196,6 +226,14 @@ __global__ __launch_bounds__(256, 2) void k_gemm_block_dma(BlockArgs p) {
                 lds_dma16(src[t] + (k0 + chunk[t & 1] < p.k ? k0 : -chunk[t & 1]), dst[t] + to);
 #pragma unroll
             for (int t = kWDma; t < kWDma + kADma; ++t) lds_dma16(src[t] + k0, dst[t] + to);
+        }
+    };
+
+    auto store_stage = [&](int buf) {
+        if constexpr (!kAligned) {
+#pragma unroll
+            for (int t = 0; t < kWDma; ++t)
+                *reinterpret_cast<u32x4*>(lds + buf * kStage + (kWDma * wave + t) * 1024 + 16 * lane) = held[t];
         }
     };
 
@@ -220,7 +258,8 @@ __global__ __launch_bounds__(256, 2) void k_gemm_block_dma(BlockArgs p) {
     };
     load_scales(s_begin);
     load_stage(s_begin * kBK, s_begin & 1);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    store_stage(s_begin & 1);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // fragments: the next 32 codes' are read while these run, a stage's first ones while the sums of the one
     // before join the totals
     i32x4 w[2][kTN], x[2][2];
@@ -266,6 +305,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_block_dma(BlockArgs p) {
                 }
             }
         }
+        if (s + 1 < s_end) store_stage((s + 1) & 1);
         // the next stage has landed and every wave is past its reads of this one
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         read(lds + ((s + 1) & 1) * kStage, 0);  // (after the last stage: read and not used)
@@ -349,22 +389,6 @@ struct SkinnyArgs {
     int m, n, k, lda;
     float* y;
 };
-
-// Bytes k0 .. k0 + 15 of a row of k >= 16, zeros past it: 16 bytes that end where the row does, shifted into place.
-__device__ __forceinline__ u32x4 row_tail(const uint8_t* row, int k0, int k) {
-    const int back = min(max(k0 + 16 - k, 0), 16);
-    const u32x4 v = *reinterpret_cast<const u32x4_a1*>(row + k0 - max(k0 + 16 - k, 0));
-    const int s = 8 * (back & 7);
-    uint64_t lo = v.x | static_cast<uint64_t>(v.y) << 32, hi = v.z | static_cast<uint64_t>(v.w) << 32;
-    lo = back >= 8 ? hi : lo;
-    hi = back >= 8 ? 0 : hi;
-    const uint64_t carry = s ? hi << (64 - s) : 0;
-    lo = (lo >> s) | carry;
-    hi >>= s;
-    if (back == 16) lo = hi = 0;
-    return u32x4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
-                 static_cast<uint32_t>(hi >> 32)};
-}
 
 template <int kType, int kFrom, int kNT>
 __global__ __launch_bounds__(kSkinnyThreads, 4) void k_gemm_block_skinny(SkinnyArgs p) {
@@ -555,9 +579,9 @@ BlockPlan block_plan(int64_t m, int64_t n, int64_t k) {
     b.part_bytes = b.split > 1 ? static_cast<int64_t>(b.left) * b.split * (kBM * 128 * 4) : 0;
     return b;
 }
-// From 64 tokens on (N=14336, K=4096: 31.5 us against the smaller tiles' 32.3, with 96 tokens 33.8 against 45); rows of
-// whole 16-byte pieces, as its loads into LDS take them.
-bool block_dma(int64_t m, int64_t k) { return k >= 16 && k % 16 == 0 && m >= 64; }
+// From 64 tokens on (N=14336, K=4096: 31.5 us against the smaller tiles' 32.3, with 96 tokens 33.8 against 45); a stage
+// of K at least.
+bool block_dma(int64_t m, int64_t k) { return k >= kBK && m >= 64; }
 
 bool block_fits(int64_t m, int64_t n, int64_t k) { return tile_fits(m, n, k); }
 
@@ -630,7 +654,7 @@ int gemm_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const floa
         return m * p.lda <= kSkinnyCodes ? launch_skinny<TQ_DT_F32, kFromCodes>(p, st, what)
                                          : launch_skinny<TQ_DT_F32, kFromMemory>(p, st, what);
     }
-    if (block_dma(m, k) && aligned(qw, 16)) {
+    if (block_dma(m, k)) {
         const BlockPlan plan = block_plan(m, n, k);
         TQ_REQUIRE(plan.part_bytes == 0 || (ws && aligned(ws, 256) && ws_bytes >= plan.part_bytes),
                    "%s: workspace of %lld bytes (256-byte aligned), %lld needed", what, (long long)ws_bytes,
@@ -653,7 +677,11 @@ int gemm_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const floa
         b.y = y;
         b.part = static_cast<float*>(ws);
         clear_error();
-        k_gemm_block_dma<<<plan.full + plan.left * plan.split, 256, 0, st>>>(b);
+        const unsigned grid = static_cast<unsigned>(plan.full + plan.left * plan.split);
+        if (k % 16 == 0 && aligned(qw, 16))
+            k_gemm_block_dma<true><<<grid, 256, 0, st>>>(b);
+        else
+            k_gemm_block_dma<false><<<grid, 256, 0, st>>>(b);
         rc = check_launch(what);
         if (rc != TQ_OK || plan.split == 1) return rc;
         k_gemm_block_join<<<plan.left * (kBM * kBN / 4 / 256), 256, 0, st>>>(b);
@@ -751,8 +779,7 @@ int tq_quantize_fp8_g128(const void* x, int dtype, int64_t m, int64_t k, uint8_t
 int64_t tq_gemm_fp8_block_workspace_bytes(int64_t m, int64_t n, int64_t k) {
     if (m < 0 || n < 0 || k < 0 || !block_fits(m, n, k)) return -1;
     if (m == 0 || n == 0) return 0;
-    const int64_t tile = tile_plan<GemmF8Block>(m, n, k, nullptr, true).part_bytes;  // (weights at any address)
-    return block_dma(m, k) ? std::max(tile, block_plan(m, n, k).part_bytes) : tile;
+    return block_dma(m, k) ? block_plan(m, n, k).part_bytes : tile_plan<GemmF8Block>(m, n, k, nullptr, true).part_bytes;
 }
 
 int tq_gemm_fp8_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const float* sw, const float* bias,

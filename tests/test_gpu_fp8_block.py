@@ -133,7 +133,8 @@ def test_product(tq, m, n, k, bias):
     (4, 48, 4096, 0), (5, 48, 4096, 0), (6, 64, 4096, 5), (2, 33, 8192, 0), (12, 20, 2176, 3),  # codes made or copied or read
     (17, 4096, 4096, 0), (32, 300, 4096, 0), (32, 4112, 512, 0), (24, 40, 4224, 0), (29, 77, 128, 7), (32, 16, 127, 0),
     (63, 500, 528, 0), (64, 130, 528, 0), (64, 130, 528, 8), (100, 260, 2048, 3), (128, 128, 4096, 0),
-    (140, 260, 4112, 0), (1200, 8000, 144, 0), (2000, 4500, 784, 0)])  # shares of K, with and without whole rounds before
+    (140, 260, 4112, 0), (1200, 8000, 144, 0), (2000, 4500, 784, 0),  # shares of K, with and without whole rounds before
+    (100, 260, 2047, 0), (300, 500, 129, 0), (64, 128, 143, 1), (2000, 4500, 777, 5), (65, 3, 128, 9), (129, 257, 4090, 0)])
 def test_product_at_its_turns(tq, m, n, k, shift):
     """Sizes beside each choice of kernel, and weights off their boundary: the bound of `test_product`."""
     import torch
@@ -184,6 +185,25 @@ def test_nan_and_infinite_rows_stay_in_their_rows(tq, m):
     if m > 2:
         assert torch.isnan(y[1]).all()
         assert torch.equal(y[2:], clean[2:])
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 40, 100])
+@pytest.mark.parametrize("k", [128, 200, 1000, 2047, 4096])
+def test_nan_weights_stay_in_their_rows(tq, m, k):
+    """A NaN code reaches its own output column: not the ones before and behind it, whose bytes its row's ends touch."""
+    import torch
+
+    n = 160
+    x = rand(7, m, k)
+    qa, sa = tq.quantize_fp8_g128(x)
+    qw, sw = tq.quantize_fp8_block(rand(8, n, k))
+    clean = tq.gemm_fp8_block(qa, sa, qw, sw)
+    bad = qw.clone()
+    bad[5, 0], bad[9, k - 1], bad[n - 1, k - 1] = 0x7F, 0xFF, 0x7F
+    y = tq.gemm_fp8_block(qa, sa, bad, sw)
+    hit = torch.zeros(n, dtype=torch.bool, device="cuda")
+    hit[[5, 9, n - 1]] = True
+    assert torch.isnan(y[:, hit]).all() and torch.equal(y[:, ~hit], clean[:, ~hit])
 
 
 def test_refusals(tq):
