@@ -599,7 +599,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j]);
                 top = over_groups(top, OpMax{}) - kPShift;
                 if (__ballot(top > m[n] + kPSlack)) {
-                    top = fmaxf(m[n], top);
+                    top = top > m[n] + kPSlack ? top : m[n];  // (a row's result depends on no other row)
                     const float ref = top == -INFINITY ? 0.f : top;
                     const float alpha = exp2_hw(m[n] - ref);
                     l[n] *= alpha;
@@ -858,9 +858,8 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
 //    element d = 32 c + 4 (r % 8) + r / 8, so that a thread that loaded 4 adjacent elements of 8 keys
 //    writes them where its neighbours write the next ones, and lane (r, h) ends up with the 16
 //    adjacent elements 32 c + 16 h .. of row r.
-// One power of two scales q in the whole tile (rows up to 2^17 times smaller than the largest keep
-// their 22 bits), so a score is one fma: t = S (sk scale 2^e) + log2 sv.  Keys with no place become
-// zero codes with log2 sv = -inf, and only tiles that some row sees in part pay for a mask.
+// A power of two scales each row of q, as above.  Keys with no place become zero codes with log2 sv = -inf, and only
+// tiles that some row sees in part pay for a mask.
 template <int kDP, int kWQ, class Codes, int kPlanes>
 __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     constexpr int kTile = 32 * kWQ, kWK = kAttWaves / kWQ;
@@ -1041,14 +1040,10 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(u[j]), fabsf(v[j])));
             }
-            // the row's largest (its two lanes), 0 where it is not finite: such a row is NaN by itself
+            // the row's largest (its two lanes)
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-            top = wave_max(top < INFINITY ? top : 0.f);
-            if (lane == 0) m_lds[wave][0] = top;
-            __syncthreads();
-            top = fmaxf(fmaxf(m_lds[0][0], m_lds[1][0]), fmaxf(m_lds[2][0], m_lds[3][0]));
-            const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+            const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
             rq = a.scale2 * ldexpf(1.0f, e);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
@@ -1081,7 +1076,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
             }
             if (wave == 0) {
                 const float c = fmaxf(sv, 1e-25f);
-                b.ck[lane] = k_ok ? sk * rq : 0.f;
+                b.ck[lane] = k_ok ? sk : 0.f;
                 b.lsv[lane] = k_ok ? __builtin_amdgcn_logf(sv != sv ? sv : c) : -INFINITY;
                 b.rsv[lane] = k_ok ? __builtin_amdgcn_rcpf(c) : 0.f;
             }
@@ -1158,7 +1153,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                         const f32x4 ck = *reinterpret_cast<const f32x4*>(&b.ck[k4]);
                         const f32x4 ls = *reinterpret_cast<const f32x4*>(&b.lsv[k4]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) t[4 * c + e] = fmaf(st[4 * c + e], ck[e], ls[e]);
+                        for (int e = 0; e < 4; ++e) t[4 * c + e] = fmaf(st[4 * c + e] * rq, ck[e], ls[e]);
                     }
                     const bool slow = k32 + 32 > all_w;  // uniform
                     if (slow) {
@@ -1172,7 +1167,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                     top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kPShift;
                     if (__ballot(top > m + kPSlack)) {
-                        top = fmaxf(m, top);
+                        top = top > m + kPSlack ? top : m;
                         const float ref = top == -INFINITY ? 0.f : top;
                         const float alpha = exp2_hw(m - ref);
                         l *= alpha;

@@ -725,3 +725,21 @@ def test_attention_of_a_few_long_sequences(tq, dtype, lengths, new, heads, group
         ref, tol = (x.view(heads, t, group, d).transpose(0, 1).reshape(t, heads * group, d).cpu()
                     for x in (torch.matmul(p, v), 2 * off * torch.matmul(p, v.abs())))
         check(got[rows], ref, tol, f"sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new", [3, 20, 50, 200])
+def test_rows_of_far_apart_sizes(tq, dtype, new):
+    """A row's result does not depend on how large the other rows of its tile are."""
+    import torch
+
+    dt = dtype_of(dtype)
+    c = Case(tq, [300], [new], 16, 2, 64, "i8")
+    c.fill(71)
+    q = rand(72, new, 2, 64, dtype=dt)
+    want = c.cache.attention(q, c.batch)
+    far = q.clone()
+    far[1::3] *= 2.0 ** 60
+    far[2::3] *= 2.0 ** -60
+    got = c.cache.attention(far, c.batch)
+    assert torch.equal(got[::3], want[::3]) and torch.isfinite(got).all()
