@@ -70,7 +70,16 @@ def _heads(t, name, dtype=None, tokens=None, heads=None, dim=None):
     return t, _heads_desc(t.data_ptr(), shape[1], token, head), code
 
 
-class Rotary:
+class _Fixed:
+    """Attributes are set once, where the descriptor of the C calls is packed from them (`x.lengths += 1`, which writes
+    into the tensor and sets the attribute to it again, is fine)."""
+
+    def __setattr__(self, name, value):
+        if value is not self.__dict__.get(name):
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: make another {type(self).__name__}")
+
+
+class Rotary(_Fixed):
     """Rotary positions: plane i of a head turns by position * frequencies[i].
 
     frequencies: float64 device tensor of rotary_dim / 2 angles per position; the first
@@ -79,9 +88,9 @@ class Rotary:
 
     def __init__(self, frequencies, interleaved=False, scale=1.0):
         _indices(frequencies, torch.float64, 1, "Rotary: frequencies")
-        self.frequencies, self.interleaved, self.scale = frequencies, bool(interleaved), float(scale)
-        self.rotary_dim = 2 * frequencies.shape[0]
-        self._desc = _abi.rotary_desc(frequencies.data_ptr(), self.rotary_dim, self.interleaved, False, self.scale)
+        r, interleaved, scale = 2 * frequencies.shape[0], bool(interleaved), float(scale)
+        self.__dict__.update(frequencies=frequencies, interleaved=interleaved, scale=scale, rotary_dim=r,
+                             _desc=_abi.rotary_desc(frequencies.data_ptr(), r, interleaved, False, scale))
 
     @staticmethod
     def from_base(rotary_dim, base=10000.0, interleaved=False, scaling=None, factor=1.0, original_length=None,
@@ -140,7 +149,7 @@ class Rotary:
         return qo, ko
 
 
-class KVBatch:
+class KVBatch(_Fixed):
     """Which tokens a call is about.
 
     table: int32 [batch, pages] pages of each sequence; lengths: int32 [batch] its tokens,
@@ -167,14 +176,15 @@ class KVBatch:
             _indices(offsets, torch.int32, 1, "KVBatch: offsets")
             if offsets.shape[0] != batch + 1 or rows is None:
                 raise InvalidArgument("KVBatch: offsets are [batch + 1], with `rows` rows in all")
-        self.table, self.lengths, self.offsets = table, lengths, offsets
-        self.batch, self.tokens, self.rows = batch, int(tokens), int(rows)
-        self.device_index = table.get_device()
-        self._desc = _abi.kv_batch_desc(table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-                                        0 if offsets is None else offsets.data_ptr(), batch, self.tokens, self.rows)
+        tokens, rows = int(tokens), int(rows)
+        self.__dict__.update(
+            table=table, lengths=lengths, offsets=offsets, batch=batch, tokens=tokens, rows=rows,
+            device_index=table.get_device(),
+            _desc=_abi.kv_batch_desc(table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+                                     0 if offsets is None else offsets.data_ptr(), batch, tokens, rows))
 
 
-class KVCache:
+class KVCache(_Fixed):
     """A paged 8-bit cache of keys and values.
 
     k, v: int8 (INT8) or uint8 (FP8 e4m3 bit patterns) [pages, heads, page, row], row =
@@ -194,13 +204,12 @@ class KVCache:
         for t in (k, k_scale, v, v_scale):
             if not _device(t, "KVCache").is_contiguous():
                 raise InvalidArgument("KVCache: buffers must be contiguous")
-        self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
-        self.pages, self.heads, self.page = shape[0], shape[1], shape[2]
-        self.head_dim = int(head_dim)
-        self.device = k.device
-        self.device_index = k.get_device()
-        self._ref = _abi.kv_cache_desc(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), shape[0],
-                                       shape[1], shape[2], self.head_dim, code)
+        head_dim = int(head_dim)
+        self.__dict__.update(
+            k=k, k_scale=k_scale, v=v, v_scale=v_scale, pages=shape[0], heads=shape[1], page=shape[2], head_dim=head_dim,
+            device=k.device, device_index=k.get_device(),
+            _ref=_abi.kv_cache_desc(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), shape[0], shape[1],
+                                    shape[2], head_dim, code))
 
     @staticmethod
     def allocate(pages, page, heads, head_dim, dtype=QuantDType.Int8):

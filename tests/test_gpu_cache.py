@@ -743,3 +743,40 @@ def test_rows_of_far_apart_sizes(tq, dtype, new):
     far[2::3] *= 2.0 ** -60
     got = c.cache.attention(far, c.batch)
     assert torch.equal(got[::3], want[::3]) and torch.isfinite(got).all()
+
+
+def test_what_a_descriptor_names_is_fixed(tq):
+    """Replacing a tensor that the C calls were told of is refused (writing into it is not)."""
+    import torch
+
+    c = Case(tq, [10], [1], 16, 2, 64, "i8")
+    rot = tq.Rotary.from_base(64)
+    for x, name in ((c.cache, "k"), (c.cache, "v_scale"), (c.batch, "lengths"), (c.batch, "table"), (rot, "frequencies")):
+        with pytest.raises(AttributeError):
+            setattr(x, name, getattr(x, name) * 1)
+    c.fill(1)
+    q = rand(2, 1, 2, 64)
+    a = c.cache.attention(q, c.batch)
+    c.batch.lengths -= 3
+    c.lengths = [7]
+    ref, tol = reference(c, q)
+    check(c.cache.attention(q, c.batch), ref, tol)
+    assert not torch.equal(a, c.cache.attention(q, c.batch))
+
+
+def test_batches_of_nothing(tq):
+    """No sequences, a table without pages, and only rows behind the last sequence."""
+    import torch
+
+    c = Case(tq, [10], [1], 16, 2, 64, "i8")
+    none = tq.KVBatch(torch.empty(0, 1, dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), 1,
+                      torch.zeros(1, dtype=torch.int32, device="cuda"), 4)
+    x, out = rand(1, 4, 2, 64), torch.full((4, 2, 64), 2.0, device="cuda")
+    c.cache.write(x, x, none)
+    c.cache.attention(x, none, out=out)
+    c.cache.read(none, torch.float32, (out, out.clone()))
+    assert (out == 2.0).all()
+    empty = tq.KVBatch(torch.empty(2, 0, dtype=torch.int32, device="cuda"), torch.tensor([3, 0], dtype=torch.int32).cuda(), 2)
+    c.cache.write(x, x, empty)
+    assert (c.cache.attention(x, empty) == 0).all() and (c.cache.k == 0).all()
+    assert all((t == 0).all() for t in c.cache.read(empty))
