@@ -397,7 +397,8 @@ class QuantizedMultiheadAttention(Module):
     def forward_cached(self, x, cache, new, rotary=None, positions=None, tree=None):
         """The layer over a KVCache, for the rows of a KVBatch: x [rows, embed_dim] (f32) is projected, q and k
         are turned (where a Rotary is given), k and v stored, and the rows attend to what the cache holds
-        of their sequences (causally, or as `tree` says).  Returns [rows, embed_dim]."""
+        of their sequences (causally, or as `tree` says).  Returns [rows, embed_dim]; rows behind the last sequence
+        hold anything."""
         x = on_device(x, torch.float32, "QuantizedMultiheadAttention.forward_cached")
         e, h, d = self.embed_dim, self.num_heads, self.head_dim
         if tuple(x.shape) != (new.rows, e) or cache.heads != h or cache.head_dim != d:
