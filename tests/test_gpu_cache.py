@@ -780,3 +780,29 @@ def test_batches_of_nothing(tq):
     c.cache.write(x, x, empty)
     assert (c.cache.attention(x, empty) == 0).all() and (c.cache.k == 0).all()
     assert all((t == 0).all() for t in c.cache.read(empty))
+
+
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+def test_a_cache_past_32_bits(tq, codes):
+    """Pages whose rows and bytes lie past 2^31 and 2^32: what is written there is what is read and attended to, as
+    on low pages."""
+    import torch
+
+    heads, d, page, pages = 16, 128, 64, 40000  # 5.2e9 bytes of keys, 41e6 rows
+    big = tq.KVCache.allocate(pages, page, heads, d, tq.QuantDType.Int8 if codes == "i8" else tq.QuantDType.FP8)
+    small = tq.KVCache.allocate(8, page, heads, d, tq.QuantDType.Int8 if codes == "i8" else tq.QuantDType.FP8)
+    high = torch.tensor([[pages - 1, 20000, 33000, 16400]], dtype=torch.int32, device="cuda")
+    low = torch.tensor([[5, 1, 7, 2]], dtype=torch.int32, device="cuda")
+    n = 4 * page - 3
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    k, v = rand(1, n, heads, d), rand(2, n, heads, d)
+    for cache, table in ((big, high), (small, low)):
+        cache.write(k, v, tq.KVBatch(table, length, n))
+    for new in (1, 9, 200):
+        q = rand(3, new, heads, d)
+        a, b = (cache.attention(q, tq.KVBatch(table, length, new)) for cache, table in ((big, high), (small, low)))
+        assert torch.equal(a, b), new
+        for x, y in zip(big.read(tq.KVBatch(high, length, new)), small.read(tq.KVBatch(low, length, new))):
+            assert torch.equal(x, y) and float(x.abs().max()) > 1
+    for i in range(4):
+        assert torch.equal(big.k[int(high[0, i])], small.k[int(low[0, i])])

@@ -278,3 +278,19 @@ def test_graph_replays(tq):
         assert torch.equal(out, y)
         lin(xs[3])
         torch.cuda.synchronize()
+
+
+def test_weights_past_32_bits(tq):
+    """A weight of more than 2^31 codes: its last rows give what they give alone."""
+    import torch
+
+    n, k = 140032, 16400
+    g = torch.Generator(device="cuda").manual_seed(5)
+    qw = torch.randint(0, 0x70, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    sw = torch.rand((n + 127) // 128, (k + 127) // 128, generator=g, device="cuda") + 0.5
+    part = slice(n - 256, n)
+    for m in (1, 20, 70):
+        qa, sa = tq.quantize_fp8_g128(rand(6, m, k))
+        y = tq.gemm_fp8_block(qa, sa, qw, sw)[:, part]
+        ref, size = product(qa, sa, qw[part], sw[-2:], None)
+        assert ((y.double() - ref).abs() <= (131 + (k + 127) // 128) * 2.0 ** -24 * size).all()
