@@ -1309,8 +1309,12 @@ struct AttPlan {
 
 // Rows of a tile by the most that a sequence's head can have: 16 and 32 on the kernel whose waves take
 // their keys straight from memory, 64 and 128 on the one that shares converted keys (see there).
-// Split wherever a sequence can have more than a unit of keys, over the blocks that the chip
-// holds at once (two per CU, one of the 32-row tiles).
+// A block for each item, and no join, where sequences are short: up to four units, of 16-row tiles (1 token, 32 on 8 heads
+// of 128: 12.3 us a call for 500 keys against 13.9, 10.8 for 240 against 14.2; 64 sequences 18.7 against 21.2; from seven
+// units on one sequence is slower so) or of enough items to fill the chip (16 sequences of 200 tokens, 8 heads: 34.5
+// against 41.7; one of them: 32.6 against 19.3); up to eight units of enough items for two rounds (64 such sequences of 1000
+// keys: 119 against 139), whose unequal lengths even out.  Else split along the keys over the blocks that the chip holds at once (two
+// per CU, one of the 32-row tiles).
 int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64_t group, AttPlan* p) {
     TQ_REQUIRE(b->max_tokens * group <= kKvMaxRows, "%s: %lld rows of a sequence's head", what,
                (long long)(b->max_tokens * group));
@@ -1323,8 +1327,8 @@ int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64
     const int64_t units = (b->table_pages * c->page + kUnit - 1) / kUnit;
     TQ_REQUIRE(p->items * (units > 0 ? units : 1) < (int64_t(1) << 31), "%s: %lld heads and tiles of %lld keys", what,
                (long long)p->items, (long long)(b->table_pages * c->page));
-    p->split = units > 1;
-    const int64_t fit = static_cast<int64_t>(device_cu_count()) * (tile == 32 ? 1 : 2);
+    const int64_t cus = device_cu_count(), fit = cus * (tile == 32 ? 1 : 2);
+    p->split = units > (p->items >= 2 * fit ? 8 : tile == 16 || p->items >= cus ? 4 : 1);
     p->blocks = static_cast<int>(!p->split || fit < p->items * units ? (p->split ? fit : p->items) : p->items * units);
     p->bytes = p->split ? 2 * static_cast<int64_t>(p->blocks) * tile * (kv_row(c->head_dim) + 2) * 4 : 0;
     return TQ_OK;

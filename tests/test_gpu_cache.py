@@ -806,3 +806,23 @@ def test_a_cache_past_32_bits(tq, codes):
             assert torch.equal(x, y) and float(x.abs().max()) > 1
     for i in range(4):
         assert torch.equal(big.k[int(high[0, i])], small.k[int(low[0, i])])
+
+
+@pytest.mark.parametrize("longest,most", [(900, 1), (900, 4), (1300, 30), (500, 40)])
+def test_attention_of_more_sequences_than_lanes(tq, longest, most):
+    """Ragged batches of 130 sequences whose shares begin and end within them, or that are not cut."""
+    import torch
+
+    rng = np.random.default_rng(longest + most)
+    lengths = [int(x) for x in rng.integers(0, longest + 1, 130)]
+    lengths[3], lengths[100] = longest, 0
+    new = [min(n, int(x)) for n, x in zip(lengths, rng.integers(0, most + 1, 130))]
+    new[3], new[64] = min(most, longest), 0
+    c = Case(tq, lengths, new, 16, 1, 64, "fp8", ragged=True, extra=3)
+    c.fill(25)
+    q = rand(26, c.rows, 2, 64)
+    out = torch.full_like(q, 3.0)
+    c.cache.attention(q, c.batch, out=out)
+    assert (out[-3:] == 3.0).all()
+    ref, tol = reference(c, q)
+    check(out[:-3], ref[:-3], tol[:-3])
