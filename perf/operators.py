@@ -352,21 +352,13 @@ def _plain_fp8(s):
 
 
 # ------------------------------------------------------------------ the framework's calls
-_tq = None
-
-
 def _framework():
-    """The package, imported once, as a program does."""
-    global _tq
-    if _tq is not None:
-        return _tq
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "neo-theano_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
     import theano_quantize
 
-    _tq = theano_quantize
-    return _tq
+    return theano_quantize
 
 
 def _own_run(s):
