@@ -756,7 +756,8 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
 // Joins the shares of the items that several blocks worked on, in their order: kDP / 4 lanes (of a group of kG) for a
 // row, four elements each.  A row has one group, or (kAll) those of the whole block, which take its shares by turns, eight
 // at a time: maxima, sums and rows of O are all on their way before the first is needed (2000 rows of 8 heads in four
-// shares: 13.7 us when the maxima came first).
+// shares: 13.7 us when the maxima came first).  A share whose maximum is -inf saw nothing (sum and O zero) or only NaN scores (both
+// NaN): either way it is added, at weight 2^-inf = 0, which keeps the NaN.
 template <int kDP, int kTile, bool kAll>
 __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
     constexpr int kG = kDP <= 32 ? 8 : kDP <= 64 ? 16 : 32, kGroups = kAttBlock / kG, kParts = kAll ? kGroups : 1;
@@ -804,9 +805,10 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const float f = exp2_hw(m[u] - ref);
-            sum = m[u] == -INFINITY ? sum : fmaf(l[u], f, sum);
+            const bool there = b + u * kParts <= b1;  // (past the last share: read again, not added)
+            sum = there ? fmaf(l[u], f, sum) : sum;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = m[u] == -INFINITY ? x[e] : fmaf(v[u][e], f, x[e]);
+            for (int e = 0; e < 4; ++e) x[e] = there ? fmaf(v[u][e], f, x[e]) : x[e];
         }
     }
     if constexpr (kAll) {
@@ -826,7 +828,6 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
 #pragma unroll
         for (int w = 1; w < kGroups; ++w) {
             const float mw = m_lds[w], f = mw == -INFINITY ? 0.f : exp2_hw(mw - top);
-            if (mw == -INFINITY) continue;
             sum = fmaf(l_lds[w], f, sum);
             x += x_lds[w][d / 4] * f;
         }
