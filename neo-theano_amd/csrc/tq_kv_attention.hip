@@ -15,9 +15,9 @@
 //    with exponent 2^10) minus 1152, e4m3 by v_cvt_scalef32_pk_f16_fp8, both exact.
 // The value scale sv_j goes into the exponent: with t_j = s_j + log2 sv_j and the running
 // maximum of t, P_j = 2^(t_j - max) = p_j sv_j needs no normalising to fit f16's
-// range whatever the scales, and the sum takes P_j / sv_j.  f32 rows use two f16 planes of
-// q (scaled by a power of two for each row) and P, 22 bits; 16-bit rows one (11 bits: an
-// eighth of a bf16 output's rounding).
+// range whatever the scales, and the sum takes P_j / sv_j.  P has two f16 planes, 22 bits, for every type (in one, 11
+// bits, 36 % of f16 outputs and 6 % of bf16 ones were not the nearest to the exact result); q, scaled by a power of
+// two for each row, has two for f32 and one for 16-bit rows, which it holds exactly.
 //
 // Work is split along the keys by units of 128: the units of all sequences, heads and row
 // tiles in one line, cut into equal shares for a grid that fits the chip at once, whatever the lengths.  A share that
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
             }
             const bool slow = !both || key + kStep > all;  // uniform
             uint32_t seen[kNQ];                            // bit j: key j of the lane is seen by row n
-            h8 pf[kNQ][kPlanes];
+            h8 pf[kNQ][2];
 #pragma unroll
             for (int n = 0; n < kNQ; ++n) {
                 float t[8];
@@ -613,9 +613,9 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
                     const float p = exp2_hw(t[j] - ref);
                     l[n] = fmaf(p, rsv[j], l[n]);
                     _Float16 hi, lo;
-                    to_planes<kPlanes>(p, hi, lo);
+                    to_planes<2>(p, hi, lo);
                     pf[n][0][j] = hi;
-                    if constexpr (kPlanes == 2) pf[n][1][j] = lo;
+                    pf[n][1][j] = lo;
                 }
             }
             // Rows that do not see a key must not meet its codes' NaNs (0 * NaN): codes nobody sees
@@ -678,7 +678,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
 #pragma unroll
                 for (int n = 0; n < kNQ; ++n)
 #pragma unroll
-                    for (int p = 0; p < kPlanes; ++p) {
+                    for (int p = 0; p < 2; ++p) {
                         o[n][v] = mfma_f16(f0, pf[n][p], o[n][v]);
                         o[n][v + 1] = mfma_f16(f1, pf[n][p], o[n][v + 1]);
                     }
@@ -1177,7 +1177,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                         m = top;
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
-                    h8 pf[2][kPlanes];
+                    h8 pf[2][2];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const f32x4 rv = *reinterpret_cast<const f32x4*>(&b.rsv[32 * sub + 8 * c + 4 * h]);
@@ -1186,9 +1186,9 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                             const float p = exp2_hw(t[e] - ref);
                             l = fmaf(p, rv[e & 3], l);
                             _Float16 hi, lo;
-                            to_planes<kPlanes>(p, hi, lo);
+                            to_planes<2>(p, hi, lo);
                             pf[e >> 3][0][e & 7] = hi;
-                            if constexpr (kPlanes == 2) pf[e >> 3][1][e & 7] = lo;
+                            pf[e >> 3][1][e & 7] = lo;
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -1198,7 +1198,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                         for (int c = 0; c < kCols; ++c) {
                             const h8 vf = b.v[((2 * sub + t2) * kCols + c) * 64 + lane];
 #pragma unroll
-                            for (int p = 0; p < kPlanes; ++p)
+                            for (int p = 0; p < 2; ++p)
                                 o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[t2][p], o[c], 0, 0, 0);
                         }
                     if (Codes::kNan && key + kKeys > all_b &&

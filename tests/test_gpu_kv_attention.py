@@ -5,7 +5,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_cache import Case, dtype_of, rand
+from test_gpu_cache import CASES, Case, dtype_of, eps_half, least, rand, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,99 @@ def test_a_nan_key_alone_in_its_share_reaches_the_rows(tq, codes, new, group, un
     got = c.cache.attention(q, c.batch)
     assert torch.isnan(got[-1]).all()
     assert torch.equal(got[:-1], want[:-1]) and torch.isfinite(want).all()
+
+
+# ------------------------------------------------------------------ the bits of 16-bit outputs
+def exact_rows(c, q, b=0):
+    """Sequence b's rows in 64 bits on the GPU: (o, sum p |v|, the largest |score| and sum |q k| of each row), [t, h, ...]."""
+    import torch
+
+    cache, page, d = c.cache, c.page, c.cache.head_dim
+    length, t, heads, group = c.lengths[b], c.new[b], cache.heads, q.shape[1] // cache.heads
+    pos = torch.arange(length, device="cuda")
+    pages = c.table[b, pos // page].long()
+
+    def floats(codes, scale):
+        x = codes[pages, :, pos % page, :d]
+        x = x.double() if x.dtype == torch.int8 else x.view(torch.float8_e4m3fn).float().double()
+        return (x * scale[pages, :, pos % page].double()[..., None]).transpose(0, 1).contiguous()
+
+    k, v = floats(cache.k, cache.k_scale), floats(cache.v, cache.v_scale)
+    rows = slice(int(c.offsets[b]), int(c.offsets[b + 1]))
+    qq = q[rows].double().view(t, heads, group, d).transpose(0, 1).reshape(heads, t * group, d)
+    s = torch.matmul(qq, k.transpose(1, 2).contiguous()) / math.sqrt(d)
+    size = (torch.matmul(qq.abs(), k.abs().transpose(1, 2).contiguous()) / math.sqrt(d)).amax(-1, keepdim=True)
+    seen = pos[None] <= (length - t + torch.arange(t, device="cuda"))[:, None]
+    s = s.masked_fill(~seen.repeat_interleave(group, 0)[None], -math.inf)
+    top = torch.where(s.isinf(), 0.0, s).abs().amax(-1, keepdim=True)
+    p = torch.softmax(s, -1)
+    back = [x.view(heads, t, group, -1).transpose(0, 1).reshape(t, heads * group, -1)
+            for x in (torch.matmul(p, v), torch.matmul(p, v.abs()), top, size)]
+    return back
+
+
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new,group", TILES)
+@pytest.mark.parametrize("length", [8, 200, 777, 4096])
+def test_16_bit_outputs_are_the_nearest_ones(tq, codes, dtype, new, group, length):
+    """An f32 evaluation gives the 16-bit number nearest to the exact result but where that lies within the evaluation's
+    error of a border.  Scores up to 16 with eight f32 roundings are off by 2^-17 relative, one step of the type is eps / 2 to
+    eps of the value, and elements smaller than the typical one (their steps are smaller, the errors not) make it
+    four times as many: a share of 4 * 2^-17 / eps (f16 3 %, bf16 0.4 %).  Probabilities of 11 bits, off by 2^-12.8 (rms),
+    would give 16 and 2 % before that factor."""
+    import torch
+
+    if length < new:
+        new = length
+    dt = dtype_of(dtype)
+    c = Case(tq, [length], [new], 64, 8, 128, codes)
+    c.fill(7)
+    q = rand(8, new, 8 * group, 128, dtype=dt, std=1.5)
+    ref = exact_rows(c, q)[0]
+    got = c.cache.attention(q, c.batch)
+    off = float((got != ref.to(dt)).double().mean())
+    assert off <= 4 * 2.0 ** -17 / torch.finfo(dt).eps + 8 / got.numel(), off
+
+
+def near(got, ref, tol, what=""):
+    """`tol` of `reference` (f32 evaluation, in sum p |v| of each element), and one rounding of the element to its type."""
+    err = (got.double().cpu() - ref).abs()
+    bound = tol + eps_half(got.dtype) * (ref.abs() + tol) + least(got.dtype) + 1e-30
+    bad = err > bound
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()}, worst {float((err - bound).max()):.3g} over"
+
+
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("lengths,new,page,heads,group,d", CASES + [
+    ([1500], [100], 64, 1, 2, 128), ([700, 90], [70, 48], 32, 2, 1, 64), ([1000, 20, 400], [33, 20, 5], 16, 1, 2, 96),
+    ([400], [129], 16, 1, 1, 33), ([600], [300], 48, 1, 1, 128), ([2000, 1], [9, 1], 16, 1, 5, 80)])
+def test_16_bit_attention_by_the_element(tq, codes, dtype, lengths, new, page, heads, group, d):
+    """Each element within the bound of its own terms, sum p |v|, not of the cache's largest value."""
+    import torch
+
+    c = Case(tq, lengths, new, page, heads, d, codes, seed=d)
+    c.fill(15)
+    q = rand(16, c.rows, heads * group, d, dtype=dtype_of(dtype), std=1.5)
+    seen = torch.rand(c.rows, max(new), generator=torch.Generator().manual_seed(d)) < 0.4
+    for tree in (None, seen):
+        ref, tol = reference(c, q, tree)
+        near(c.cache.attention(q, c.batch, tree=None if tree is None else tq.tree_mask(tree).cuda()), ref, tol,
+             f"{lengths} {new} tree={tree is not None}")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("lengths,new,heads,group,d", [
+    ([20000, 12345, 300], [40, 33, 40], 4, 1, 64), ([9000, 30000], [3, 1], 4, 4, 128), ([17000], [200], 8, 1, 128),
+    ([4000] * 40 + [5], [1] * 41, 4, 2, 32)])
+def test_16_bit_attention_of_long_sequences_by_the_element(tq, dtype, lengths, new, heads, group, d):
+    """Long sequences, whose outputs are small beside the values: a unit of keys left out would show."""
+    c = Case(tq, lengths, new, 64, heads, d, "i8", ragged=True)
+    c.fill(33)
+    q = rand(34, c.rows, heads * group, d, dtype=dtype_of(dtype), std=1.5)
+    got = c.cache.attention(q, c.batch)
+    for b in range(len(lengths)):
+        ref, pv, top, size = exact_rows(c, q, b)
+        tol = 2 * 2.0 ** -24 * ((d + 16) * size + 8 * (top + 64)) * pv
+        near(got[int(c.offsets[b]):int(c.offsets[b + 1])], ref.cpu(), tol.cpu(), f"sequence {b}")
