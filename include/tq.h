@@ -520,11 +520,13 @@ typedef struct {
  * call among them, the last ones) on the pages table[b * table_stride + i], position p on
  * page p / page.  The call's `tokens` rows are sequence after sequence: rows offsets[b]
  * .. offsets[b + 1] - 1 are the last of sequence b.  offsets NULL: max_tokens rows each
- * (tokens = batch * max_tokens).  No sequence has more than max_tokens rows.
+ * (tokens = batch * max_tokens).  Offsets do not decrease.
  * Everything the device arrays say is checked where it is used: a row with no place
- * (before position 0, past the table, on a page outside the cache, behind the last
+ * (before position 0, past the table, on a page outside the cache, before the first
+ * sequence, of one with more than max_tokens rows or past `tokens`, behind the last
  * sequence) is not written, reads as zeros or, behind the last sequence, is left as it
- * was; lengths past the table are cut.  A page that one call writes for two places holds
+ * was; lengths past the table are cut.  A row before the first sequence or of one that
+ * does not fit gets zeros from attention.  A page that one call writes for two places holds
  * either: positions being written need a page of their own. */
 typedef struct {
     const int32_t* table;

@@ -42,6 +42,12 @@ struct KvPlace {
     bool behind;
 };
 
+// Whether rows first .. last - 1 are a sequence's: some, inside the call's and no more than max_tokens.  Those of others have
+// no place.
+__device__ __forceinline__ bool kv_rows_fit(const KvBatch& b, int first, int last) {
+    return first >= 0 && last <= b.tokens && last > first && last - first <= b.max_tokens;
+}
+
 // Sequence of row n: the number of sequences that end at or before it.  Called by whole waves
 // with a uniform n.
 __device__ __forceinline__ int kv_sequence(const KvBatch& b, int n, int lane) {
@@ -74,7 +80,7 @@ __device__ __forceinline__ KvPlace kv_place(const KvBatch& b, int n, int seq) {
     if (p.behind) return p;
     const int first = b.offsets ? b.offsets[seq] : seq * b.max_tokens;
     const int last = b.offsets ? b.offsets[seq + 1] : first + b.max_tokens;
-    if (n < first || last - first > b.max_tokens) return p;
+    if (n < first || !kv_rows_fit(b, first, last)) return p;
     const int64_t pos = static_cast<int64_t>(b.lengths[seq]) - (last - n);
     if (pos < 0 || pos >= b.cap) {
         p.pos = pos < 0 ? -1 : b.cap;

@@ -59,6 +59,8 @@ struct AttArg {
     FastDiv by_group;
 };
 
+__device__ __forceinline__ void store_elem(void* p, int64_t i, int dtype, float x);
+
 // ------------------------------------------------------------------ the line of work
 // 64 sequences at a time, one in each lane: rows, keys and units, with the running totals of
 // items ((head, tile) pairs) and units.
@@ -88,9 +90,8 @@ __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane,
     if (seq < a.b.batch) {
         int first = a.b.offsets ? a.b.offsets[seq] : seq * a.b.max_tokens;
         const int last = a.b.offsets ? a.b.offsets[seq + 1] : first + a.b.max_tokens;
-        const bool ok = first >= 0 && last <= a.b.tokens && last > first && last - first <= a.b.max_tokens;
         s.first = first;
-        s.rows = ok ? last - first : 0;
+        s.rows = kv_rows_fit(a.b, first, last) ? last - first : 0;
         const int length = min(max(a.b.lengths[seq], 0), 1 << 30);
         s.len = min(length, a.b.cap);
         s.base = length - s.rows;
@@ -199,6 +200,28 @@ __device__ __forceinline__ Item find_item(const AttArg& a, const SeqLane& s0, in
         units += nu;
     }
     return Item{};
+}
+
+// Zeros for the rows of no sequence: those before the first one, and those whose offsets do not fit the batch.  A block looks at 64
+// sequences, at its end (at the start, which the loop over the keys is scheduled with, a batch of 64 took 91 us for 79).
+__device__ __forceinline__ void zero_strays(const AttArg& a, int tid) {
+    if (!a.b.offsets) return;
+    const int lane = tid & 63;
+    const int64_t row = static_cast<int64_t>(a.heads) * a.group * a.d;
+    for (int g = blockIdx.x; g <= (a.b.batch - 1) / 64; g += gridDim.x) {
+        const int seq = 64 * g + lane;
+        int begin = 0, end = 0;
+        if (seq < a.b.batch) {
+            const int first = a.b.offsets[seq], last = a.b.offsets[seq + 1];
+            const bool fits = kv_rows_fit(a.b, first, last);
+            begin = seq == 0 ? 0 : max(first, 0);
+            end = fits ? (seq == 0 ? first : begin) : min(last, a.b.tokens);
+        }
+        for (uint64_t todo = __ballot(begin < end); todo; todo &= todo - 1) {  // as a rule none
+            const int j = __ffsll(static_cast<unsigned long long>(todo)) - 1, r0 = readlane(begin, j), r1 = readlane(end, j);
+            for (int64_t i = r0 * row + tid; i < r1 * row; i += kAttBlock) store_elem(a.out, i, a.dtype, 0.f);
+        }
+    }
 }
 
 // Which of the 32 keys from `key` row t of the item's new tokens sees, a bit each (keys past the
@@ -416,15 +439,14 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
     const Line line = share_line<kTile>(a, s0, lane);
     int at = 0, end = 1;
     if (a.part) {
-        if (static_cast<int>(blockIdx.x) >= line.blocks) return;
         const Shares sh(line.units, line.blocks);
         at = sh.begin(blockIdx.x);
-        end = sh.begin(blockIdx.x + 1);
+        end = static_cast<int>(blockIdx.x) < line.blocks ? sh.begin(blockIdx.x + 1) : at;
     }
     bool first_share = true;
     while (at < end) {
         const Item it = a.part ? find_item<kTile, true>(a, s0, at, lane) : find_item<kTile, false>(a, s0, blockIdx.x, lane);
-        if (!it.ok) return;
+        if (!it.ok) break;
         const int u_first = a.part ? at - it.unit0 : 0;
         const int u_count = a.part ? min(it.units - u_first, end - at) : it.units;
         const int n_rows = it.rows * a.group;
@@ -751,6 +773,7 @@ __global__ __launch_bounds__(kAttBlock, kNQ == 2 ? 1 : 2) void k_kv_attention(At
         first_share = false;
         at += u_count;
     }
+    zero_strays(a, threadIdx.x);
 }
 
 // Joins the shares of the items that several blocks worked on, in their order: kDP / 4 lanes (of a group of kG) for a
@@ -890,16 +913,15 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     const Line line = share_line<kTile>(a, s0, lane);
     int at = 0, end = 1;
     if (a.part) {
-        if (static_cast<int>(blockIdx.x) >= line.blocks) return;
         const Shares sh(line.units, line.blocks);
         at = sh.begin(blockIdx.x);
-        end = sh.begin(blockIdx.x + 1);
+        end = static_cast<int>(blockIdx.x) < line.blocks ? sh.begin(blockIdx.x + 1) : at;
     }
     bool first_share = true;
     while (at < end) {
         if (!first_share || kShort) s0 = seq_lane<kTile>(a, 0, here(lane), line.per);  // (kept, it would hold ten registers)
         const Item it = a.part ? find_item<kTile, true>(a, s0, at, lane) : find_item<kTile, false>(a, s0, blockIdx.x, lane);
-        if (!it.ok) return;
+        if (!it.ok) break;
         const int u_first = a.part ? at - it.unit0 : 0;
         const int u_count = a.part ? min(it.units - u_first, end - at) : it.units;
         const int n_rows = it.rows * a.group, row0 = it.tile * kTile;
@@ -1298,6 +1320,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
         first_share = false;
         at += u_count;
     }
+    zero_strays(a, threadIdx.x);
 }
 
 // ------------------------------------------------------------------ host

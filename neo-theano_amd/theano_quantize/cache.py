@@ -158,7 +158,8 @@ class KVBatch(_Fixed):
     offsets[b] .. offsets[b + 1] - 1 of `rows` in all, no sequence more than `tokens`.
 
     The device checks what it reads: a row with no place (before position 0, past the
-    table, on a page outside the cache) is not written and reads as zeros, a key with no place is
+    table, on a page outside the cache, before offsets[0], of a sequence with more than `tokens`
+    rows or past `rows`) is not written and reads as zeros, a key with no place is
     seen by nobody, rows behind the last sequence are left as they were.  Positions that one call
     writes must not share a page's place."""
 

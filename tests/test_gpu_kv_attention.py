@@ -149,3 +149,59 @@ def test_16_bit_attention_of_long_sequences_by_the_element(tq, dtype, lengths, n
         ref, pv, top, size = exact_rows(c, q, b)
         tol = 2 * 2.0 ** -24 * ((d + 16) * size + 8 * (top + 64)) * pv
         near(got[int(c.offsets[b]):int(c.offsets[b + 1])], ref.cpu(), tol.cpu(), f"sequence {b}")
+
+
+# ------------------------------------------------------------------ rows that belong to no sequence
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("most,sequences", [(1, 3), (8, 3), (60, 3), (8, 150)])
+@pytest.mark.parametrize("fault", ["long", "past", "before"])
+def test_rows_of_no_sequence_are_zeros(tq, dtype, most, sequences, fault):
+    """A sequence with more rows than max_tokens, one that reaches past the call's rows, and rows before the first
+    sequence: not written to the cache, read as zeros and attended to as zeros, wherever they lie in the batch; the other rows
+    as without them."""
+    import torch
+
+    dt = dtype_of(dtype)
+    new = [most] * sequences
+    bad = {"long": sequences // 2, "past": sequences - 1, "before": -1}[fault]
+    before = 3 if fault == "before" else 0
+    if fault == "long":
+        new[bad] = most + 5
+    lengths = [100 + i % 7 for i in range(sequences)]
+    off = before + np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    rows = int(off[-1]) - (1 if fault == "past" else 0)
+    stray = slice(0, before) if fault == "before" else slice(int(off[bad]), min(int(off[bad + 1]), rows))
+    c = Case(tq, lengths, new, 16, 2, 64, "i8")
+    c.fill(51)
+    kept = [x.clone() for x in (c.cache.k, c.cache.k_scale, c.cache.v, c.cache.v_scale)]
+    batch = tq.KVBatch(c.table, c.batch.lengths, most, torch.from_numpy(off.astype(np.int32)).cuda(), rows)
+    q, k, v = rand(52, rows, 4, 64, dtype=dt), rand(53, rows, 2, 64, dtype=dt), rand(54, rows, 2, 64, dtype=dt)
+    out = torch.full_like(q, 9.0)
+    c.cache.attention(q, batch, out=out)
+    assert (out[stray] == 0).all()
+    for b in {0, sequences // 3, sequences - 2, sequences - 1} - {bad}:
+        part = slice(int(off[b]), int(off[b + 1]))
+        one = tq.KVBatch(c.table[b:b + 1], c.batch.lengths[b:b + 1], new[b])
+        near(out[part], *reference_of(c, q[part], b), f"sequence {b}")
+        assert torch.equal(out[part], c.cache.attention(q[part], one)), b  # (one block has each: the same sums)
+    back = tuple(torch.full((rows, 2, 64), 5.0, device="cuda") for _ in range(2))
+    c.cache.read(batch, torch.float32, back)
+    assert all((x[stray] == 0).all() for x in back)
+    c.cache.write(k, v, batch)
+    if fault != "before":  # the stray sequence's places are as they were
+        pages = c.table[bad].long()
+        for x, y in zip((c.cache.k, c.cache.k_scale, c.cache.v, c.cache.v_scale), kept):
+            assert torch.equal(x[pages], y[pages])
+    if before:
+        assert torch.equal(c.cache.k[c.table[0].long()][0, :, :50], kept[0][c.table[0].long()][0, :, :50])
+
+
+def reference_of(c, q, b):
+    """Sequence b's rows q in 64 bits, and the bound of `reference`."""
+    import torch
+
+    one = Case.__new__(Case)
+    one.__dict__.update(c.__dict__)
+    one.lengths, one.new = [c.lengths[b]], [q.shape[0]]
+    one.table, one.offsets, one.rows = c.table[b:b + 1], np.array([0, q.shape[0]]), q.shape[0]
+    return reference(one, q)
