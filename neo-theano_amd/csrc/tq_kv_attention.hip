@@ -883,7 +883,7 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
 //    writes them where its neighbours write the next ones, and lane (r, h) ends up with the 16
 //    adjacent elements 32 c + 16 h .. of row r.
 // A power of two scales each row of q, as above.  Keys with no place become zero codes with log2 sv = -inf, and only
-// tiles that some row sees in part pay for a mask.
+// tiles that hold one, or that some row sees in part, pay for a mask.
 template <int kDP, int kWQ, class Codes, int kPlanes>
 __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     constexpr int kTile = 32 * kWQ, kWK = kAttWaves / kWQ;
@@ -896,6 +896,7 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
     struct Buf {
         h8 k[kKF], v[kVF];
         float ck[kKeys], lsv[kKeys], rsv[kKeys];
+        uint32_t lie[2];  // a bit for each key that has a place
         uint8_t bad[Codes::kNan ? kKeys * kQuads : 4];
         int any_bad[kAttWaves];
     };
@@ -1102,6 +1103,8 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
                 b.ck[lane] = k_ok ? sk : 0.f;
                 b.lsv[lane] = k_ok ? __builtin_amdgcn_logf(sv != sv ? sv : c) : -INFINITY;
                 b.rsv[lane] = k_ok ? __builtin_amdgcn_rcpf(c) : 0.f;
+                const uint64_t lie = __ballot(k_ok);
+                if (lane < 2) b.lie[lane] = static_cast<uint32_t>(lie >> (32 * lane));
             }
             uint32_t bad_here = 0;
             if (v_on) {
@@ -1178,9 +1181,11 @@ __global__ __launch_bounds__(kAttBlock, 2) void k_kv_attention_rows(AttArg a) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) t[4 * c + e] = fmaf(st[4 * c + e] * rq, ck[e], ls[e]);
                     }
-                    const bool slow = k32 + 32 > all_w;  // uniform
+                    // (log2 sv = -inf alone would not keep a key without a place from a row of NaN scores)
+                    const uint32_t lie = __builtin_amdgcn_readfirstlane(b.lie[sub]);
+                    const bool slow = k32 + 32 > all_w || lie != ~0u;  // uniform
                     if (slow) {
-                        const uint32_t window = seen_from(a, it, t_row, k32) >> (4 * h);
+                        const uint32_t window = (seen_from(a, it, t_row, k32) & lie) >> (4 * h);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) t[e] = window >> (8 * (e >> 2) + (e & 3)) & 1 ? t[e] : -INFINITY;
                     }

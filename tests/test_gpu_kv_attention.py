@@ -55,6 +55,28 @@ def test_a_nan_key_alone_in_its_share_reaches_the_rows(tq, codes, new, group, un
     assert torch.equal(got[:-1], want[:-1]) and torch.isfinite(want).all()
 
 
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+@pytest.mark.parametrize("new,group", TILES)
+@pytest.mark.parametrize("length", [250, 3000])
+def test_a_nan_row_that_sees_no_key_is_zeros(tq, codes, new, group, length):
+    """Keys without a page are seen by nobody, whatever the row: only such ones, zeros; some such ones among others, what the
+    others give (to the rounding of sums in another order), and NaN for the NaN rows."""
+    import torch
+
+    c = Case(tq, [length], [new], 16, 2, 64, codes)
+    c.fill(9)
+    q = rand(10, new, 2 * group, 64)
+    q[new // 2, 0, 7], q[new // 3, 1, 8] = math.nan, math.inf
+    whole = c.table.clone()
+    c.table.fill_(-1)
+    assert (c.cache.attention(q, c.batch) == 0).all()
+    c.table.copy_(whole)
+    c.table[:, :-2:3] = 1 << 20
+    got = c.cache.attention(q, c.batch)
+    bad = torch.isnan(q).any(-1) | torch.isinf(q).any(-1)
+    assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+
+
 # ------------------------------------------------------------------ the bits of 16-bit outputs
 def exact_rows(c, q, b=0):
     """Sequence b's rows in 64 bits on the GPU: (o, sum p |v|, the largest |score| and sum |q k| of each row), [t, h, ...]."""
