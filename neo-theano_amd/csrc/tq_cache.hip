@@ -522,13 +522,16 @@ void launch_many(const RowsArg& a, hipStream_t st) {
 // Tokens to a block from 128 tokens on: 1 where heads only turn (4093 tokens, 64 heads of 128, bf16: 24 us, 26 with 4
 // and 28 with 16), 16 where they are only coded, since a page's lines of codes and scales are then written by one
 // block (4096 tokens, 32 heads of 80, FP8: 31 us with 1, 29 with 4, 27 with 16), 4 for both.
-constexpr int kManyFrom = 128;
+constexpr int kManyFrom = 128, kTurnTokens = 1, kCodeTokens = 16, kBothTokens = 4;
+int tokens_to_a_block(const RowsArg& a) {
+    return a.n < kManyFrom ? 1 : a.rot.half == 0 ? kCodeTokens : a.k_codes ? kBothTokens : kTurnTokens;
+}
 template <int kType, bool kVec, bool kTurn, class Fmt>
 void launch_rows_vec(const RowsArg& a, hipStream_t st) {
     if (a.n >= kManyFrom) {
-        if constexpr (!kTurn) return launch_many<kType, kVec, false, 16, Fmt>(a, st);
-        if (a.k_codes) return launch_many<kType, kVec, true, 4, Fmt>(a, st);
-        return launch_many<kType, kVec, true, 1, FmtI8>(a, st);
+        if constexpr (!kTurn) return launch_many<kType, kVec, false, kCodeTokens, Fmt>(a, st);
+        if (a.k_codes) return launch_many<kType, kVec, true, kBothTokens, Fmt>(a, st);
+        return launch_many<kType, kVec, true, kTurnTokens, FmtI8>(a, st);
     }
     auto shares = [](int heads) { return (heads + kHeadsAtOnce - 1) / kHeadsAtOnce; };
     k_token_rows<kType, kVec, kTurn, Fmt>
@@ -552,6 +555,8 @@ int launch_rows(const RowsArg& a, bool vec, hipStream_t st, const char* what) {
 
 template <class Fmt>
 int launch_rows_typed(const RowsArg& a, int dtype, bool vec, hipStream_t st, const char* what) {
+    TQ_REQUIRE(a.n <= kMaxBlocks * tokens_to_a_block(a), "%s: %d tokens, %d to a block, are more than %lld blocks", what, a.n,
+               tokens_to_a_block(a), (long long)kMaxBlocks);
     if (dtype == TQ_DT_F32) return launch_rows<TQ_DT_F32, Fmt>(a, vec, st, what);
     if (dtype == TQ_DT_BF16) return launch_rows<TQ_DT_BF16, Fmt>(a, vec, st, what);
     return launch_rows<TQ_DT_F16, Fmt>(a, vec, st, what);
@@ -608,14 +613,15 @@ void launch_read_many(const ReadArg& a, hipStream_t st) {
     k_read_rows<kType, kVec, kTB, Fmt><<<dim3(groups, (all + per - 1) / per), kRowBlock, 0, st>>>(a, per);
 }
 
+// four tokens to a block (32767 tokens, 8 heads of 128 to f32: 115 us with 1, 62 with 4, 75 with 16)
+constexpr int kReadTokens = 4;
 template <int kType, class Fmt>
 int launch_read(const ReadArg& a, bool vec, hipStream_t st, const char* what) {
     clear_error();
-    // four tokens to a block (32767 tokens, 8 heads of 128 to f32: 115 us with 1, 62 with 4, 75 with 16)
     if (vec)
-        launch_read_many<kType, true, 4, Fmt>(a, st);
+        launch_read_many<kType, true, kReadTokens, Fmt>(a, st);
     else
-        launch_read_many<kType, false, 4, Fmt>(a, st);
+        launch_read_many<kType, false, kReadTokens, Fmt>(a, st);
     return check_launch(what);
 }
 
@@ -738,6 +744,8 @@ int tq_kv_read(const tq_kv_cache* cache, const tq_kv_batch* batch, int dtype, vo
     TQ_REQUIRE(dtype == TQ_DT_F32 || dtype == TQ_DT_BF16 || dtype == TQ_DT_F16, "%s: dtype %d is not f32, bf16 or f16", what,
                dtype);
     if (batch->tokens == 0 || batch->batch == 0) return TQ_OK;
+    TQ_REQUIRE(batch->tokens <= kMaxBlocks * kReadTokens, "%s: %lld tokens, %d to a block, are more than %lld blocks", what,
+               (long long)batch->tokens, kReadTokens, (long long)kMaxBlocks);
     TQ_REQUIRE(k_out && v_out && aligned(k_out, type_size(dtype)) && aligned(v_out, type_size(dtype)),
                "%s: null or unaligned output", what);
     a.k = cache->k;

@@ -95,10 +95,12 @@ __global__ __launch_bounds__(kQuantBlock) void k_quant_block(const float* __rest
 
 __global__ __launch_bounds__(kQuantBlock) void k_dequant_block(const uint8_t* __restrict__ q, const float* __restrict__ s,
                                                                int64_t total, int k, float* __restrict__ w) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kQuantBlock + threadIdx.x;
-    if (i >= total) return;
-    const int row = static_cast<int>(i / k), col = static_cast<int>(i - static_cast<int64_t>(row) * k);
-    w[i] = FmtFp8::value1(q[i], s[static_cast<int64_t>(row / kBlk) * ((k + kBlk - 1) / kBlk) + col / kBlk]);
+    // (as many turns as it takes: weights may have more codes than a launch has threads)
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQuantBlock + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * kQuantBlock) {
+        const int row = static_cast<int>(i / k), col = static_cast<int>(i - static_cast<int64_t>(row) * k);
+        w[i] = FmtFp8::value1(q[i], s[static_cast<int64_t>(row / kBlk) * ((k + kBlk - 1) / kBlk) + col / kBlk]);
+    }
 }
 
 // ------------------------------------------------------------------ many tokens
@@ -676,6 +678,8 @@ int gemm_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const floa
         b.vec = n % 4 == 0 && aligned(y, 16) && aligned(bias, 16);
         b.y = y;
         b.part = static_cast<float*>(ws);
+        TQ_REQUIRE(plan.full <= kMaxBlocks - plan.left * plan.split, "%s: M=%lld, N=%lld are more than %lld blocks", what, (long long)m,
+                   (long long)n, (long long)kMaxBlocks);
         clear_error();
         const unsigned grid = static_cast<unsigned>(plan.full + plan.left * plan.split);
         if (k % 16 == 0 && aligned(qw, 16))
@@ -691,6 +695,8 @@ int gemm_block(const uint8_t* qa, const float* sa, const uint8_t* qw, const floa
     TQ_REQUIRE(plan.part_bytes == 0 || (ws && aligned(ws, 256) && ws_bytes >= plan.part_bytes),
                "%s: workspace of %lld bytes (256-byte aligned), %lld needed", what, (long long)ws_bytes,
                (long long)plan.part_bytes);
+    TQ_REQUIRE(static_cast<int64_t>(plan.tiles_m) * plan.tiles_n * plan.split <= kMaxBlocks, "%s: M=%lld, N=%lld are more than %lld blocks",
+               what, (long long)m, (long long)n, (long long)kMaxBlocks);
     TileArgs p{};
     p.a = qa;
     p.w = qw;
@@ -717,7 +723,8 @@ int quantize_g128(const void* x, int dtype, int64_t m, int64_t k, uint8_t* q, fl
     TQ_REQUIRE(x && q && s, "%s: null pointer", what);
     TQ_REQUIRE(aligned(x, size) && aligned(q, 16) && aligned(s, 4), "%s: misaligned pointer", what);
     const int64_t groups = m * ((k + kBlk - 1) / kBlk);
-    TQ_REQUIRE((groups + 15) / 16 < (int64_t(1) << 31), "%s: M=%lld, K=%lld", what, (long long)m, (long long)k);
+    TQ_REQUIRE((groups + 15) / 16 <= kMaxBlocks, "%s: M=%lld, K=%lld are more than %lld blocks", what, (long long)m, (long long)k,
+               (long long)kMaxBlocks);
     const unsigned grid = static_cast<unsigned>((groups + 15) / 16);
     const bool vec = k % 8 == 0 && aligned(x, 16);
     const int mi = static_cast<int>(m), ki = static_cast<int>(k);
@@ -752,7 +759,8 @@ int tq_quantize_fp8_block(const float* w, int64_t n, int64_t k, uint8_t* q, floa
     TQ_REQUIRE(w && q && s, "%s: null pointer", what);
     TQ_REQUIRE(aligned(w, 4) && aligned(s, 4), "%s: misaligned pointer", what);
     const int64_t blocks = ((n + kBlk - 1) / kBlk) * ((k + kBlk - 1) / kBlk);
-    TQ_REQUIRE(blocks < (int64_t(1) << 31), "%s: N=%lld, K=%lld", what, (long long)n, (long long)k);
+    TQ_REQUIRE(blocks <= kMaxBlocks, "%s: N=%lld, K=%lld are more than %lld blocks", what, (long long)n, (long long)k,
+               (long long)kMaxBlocks);
     clear_error();
     k_quant_block<<<static_cast<unsigned>(blocks), kQuantBlock, 0, as_hip(stream)>>>(w, static_cast<int>(n),
                                                                                      static_cast<int>(k), q, s);
@@ -765,8 +773,7 @@ int tq_dequantize_fp8_block(const uint8_t* q, const float* s, int64_t n, int64_t
     if (rc != TQ_OK || n == 0 || k == 0) return rc;
     TQ_REQUIRE(q && s && w_hat, "%s: null pointer", what);
     TQ_REQUIRE(aligned(s, 4) && aligned(w_hat, 4), "%s: misaligned pointer", what);
-    const int64_t grid = (n * k + kQuantBlock - 1) / kQuantBlock;
-    TQ_REQUIRE(grid < (int64_t(1) << 31), "%s: N=%lld, K=%lld", what, (long long)n, (long long)k);
+    const int64_t grid = std::min((n * k + kQuantBlock - 1) / kQuantBlock, kMaxBlocks);
     clear_error();
     k_dequant_block<<<static_cast<unsigned>(grid), kQuantBlock, 0, as_hip(stream)>>>(q, s, n * k, static_cast<int>(k), w_hat);
     return check_launch(what);

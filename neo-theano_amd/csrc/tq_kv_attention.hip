@@ -1356,6 +1356,8 @@ int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64
     const int64_t units = (b->table_pages * c->page + kUnit - 1) / kUnit;
     TQ_REQUIRE(p->items * (units > 0 ? units : 1) < (int64_t(1) << 31), "%s: %lld heads and tiles of %lld keys", what,
                (long long)p->items, (long long)(b->table_pages * c->page));
+    TQ_REQUIRE(p->items <= kMaxBlocks, "%s: %lld heads and tiles are more than %lld blocks", what, (long long)p->items,
+               (long long)kMaxBlocks);
     const int64_t cus = device_cu_count(), fit = cus * (tile == 32 ? 1 : 2);
     p->split = units > (p->items >= 2 * fit ? 8 : tile == 16 || p->items >= cus ? 4 : 1);
     p->blocks = static_cast<int>(!p->split || fit < p->items * units ? (p->split ? fit : p->items) : p->items * units);
