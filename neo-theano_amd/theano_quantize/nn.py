@@ -115,12 +115,13 @@ class QuantizedLinear(Module):
         self.tiled = None
         if mode == "fp8_block":
             shape = (self.out_features + 127) // 128, (self.in_features + 127) // 128
+            given = [t for t in (qweight, scales, bias) if t is not None]
             if qweight.dtype != torch.uint8 or tuple(qweight.shape) != (self.out_features, self.in_features) or \
-                    scales.dtype != torch.float32 or tuple(scales.shape) != shape or not qweight.is_contiguous() or \
-                    not scales.is_contiguous() or (bias is not None and (bias.dtype != torch.float32 or
-                                                                         tuple(bias.shape) != (self.out_features,))):
+                    scales.dtype != torch.float32 or tuple(scales.shape) != shape or \
+                    (bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (self.out_features,))) or \
+                    not all(t.is_contiguous() and t.device == qweight.device for t in given):
                 raise InvalidArgument(f"QuantizedLinear: fp8_block takes contiguous uint8 [{self.out_features}, "
-                                      f"{self.in_features}] codes, float32 {shape} scales and a float32 bias")
+                                      f"{self.in_features}] codes, float32 {shape} scales and a float32 bias of one device")
         if tiled and mode == "w4" and self.in_features <= 16384:
             # row-tiled copy (a permutation of qweight) for the decode GEMV (passes
             # of 16 tokens up to M = 32)

@@ -73,3 +73,17 @@ def test_rotary_of_as_many_tokens_as_a_launch_holds(tq):
     y = rot.apply(x, None, pos)[0]
     for i in (0, 1 << 23, n - 3):
         assert torch.equal(y[i:i + 3], rot.apply(x[i:i + 3], None, pos[i:i + 3])[0])
+
+
+def test_fp8_block_layers_take_tensors_that_the_kernels_can_read():
+    """Codes, scales and bias of one device, dense: the kernels take their addresses as they are."""
+    import torch
+
+    import theano_quantize as tq
+
+    q, s, b = torch.zeros(300, 200, dtype=torch.uint8), torch.ones(3, 2), torch.zeros(300)
+    assert tq.QuantizedLinear("fp8_block", 200, 300, q, s, b).bias is b
+    for args in ((q, s.to("meta"), b), (q, s, b.to("meta")), (q.to("meta"), s, None), (q, s, torch.zeros(600)[::2]),
+                 (q, s, torch.zeros(1).expand(300))):
+        with pytest.raises(tq.InvalidArgument):
+            tq.QuantizedLinear("fp8_block", 200, 300, *args)
