@@ -558,8 +558,11 @@ int tq_kv_read(const tq_kv_cache* cache, const tq_kv_batch* batch, int dtype, vo
  * (tree_words >= ceil(T / 32); a drafted token sees its ancestors and itself).  A key
  * with no place (see tq_kv_batch) is seen by nobody.  Softmax, sums and outputs are f32, q is
  * taken as f16 planes (two for f32) and the codes are exact, so the result is as near as
- * f32 gets for f32 and one rounding to dtype otherwise (the value scales that a row sees
- * within 2^120 of each other: a probability is carried as its product with its key's).
+ * f32 gets for f32 and one rounding to dtype otherwise.  A probability p is carried as
+ * p s, s being its key's value scale, in 22 bits and no finer than 2^-33 of the row's
+ * largest p s: an element in which only keys of far smaller products hold codes is off by
+ * up to that times the sum of its |codes| (full precision within about 2^10), and the
+ * scales that a row sees have to lie within 2^120 of each other.
  * A row's result depends on no other row's.  A row that sees no key, or
  * whose scores are all -inf, gives zeros (the idle slots of a serving batch); what a
  * row does not see cannot reach it, NaN and infinities included.  Rows behind the last

@@ -173,6 +173,33 @@ def test_16_bit_attention_of_long_sequences_by_the_element(tq, dtype, lengths, n
         near(got[int(c.offsets[b]):int(c.offsets[b + 1])], ref.cpu(), tol.cpu(), f"sequence {b}")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,group", TILES)
+@pytest.mark.parametrize("far", [2, 10, 18, 26, 34])
+def test_elements_that_only_light_keys_hold(tq, dtype, new, group, far):
+    """One key's values are 2^far times the others' and zero in the last 32 elements: these are the other keys', carried in
+    two f16 planes P = hi + lo + e, |e| <= max(2^-22 P, 2^-25), with the row's largest P at 2^8 or more, so off by 2^-22 of
+    their terms and 2^-33 of the largest p s for each unit of the codes, next to the f32 evaluation's own bound."""
+    import torch
+
+    length, d = 400, 64
+    c = Case(tq, [length], [new], 16, 1, d, "i8")
+    k, v = rand(61, length, 1, d) * 0.2, rand(62, length, 1, d)
+    v[5, :, :32] *= 2.0 ** far
+    v[5, :, 32:] = 0.0
+    c.cache.write(k, v, c.all_tokens())
+    q = rand(63, new, group, d, dtype=dtype_of(dtype))
+    ref, pv, top, size = exact_rows(c, q)
+    tol = 2 * 2.0 ** -24 * ((d + 16) * size + 8 * (top + 64)) * pv + 2.0 ** -22 * pv
+    pos = torch.arange(length, device="cuda")
+    at = c.table[0, pos // 16].long()
+    codes = c.cache.v[at, 0, pos % 16, :d].double().abs().sum(0)  # of each element
+    largest = float(c.cache.v_scale.max())  # p <= 1
+    tol = tol + 2.0 ** -33 * largest * codes
+    near(c.cache.attention(q, c.batch), ref.cpu(), tol.cpu())
+    assert float(c.cache.v_scale.max()) > 2.0 ** (far - 2) * float(c.cache.v_scale[at[6], 0, 6])
+
+
 # ------------------------------------------------------------------ rows that belong to no sequence
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("most,sequences", [(1, 3), (8, 3), (60, 3), (8, 150)])
