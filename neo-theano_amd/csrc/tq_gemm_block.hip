@@ -382,7 +382,7 @@ constexpr int kSkinnyWaves = 16, kSkinnyThreads = 64 * kSkinnyWaves, kSkinnyU = 
 constexpr int kSkinnyCodes = 24576, kSkinnyFused = 16384;
 
 struct SkinnyArgs {
-    const void* x;     // activations (kFused)
+    const void* x;     // activations (kFromX)
     const uint8_t* a;  // codes [m, lda] and scales [lda / 128, m] (else)
     const float* sa;
     const uint8_t* w;

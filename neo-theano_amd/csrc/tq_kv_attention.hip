@@ -160,7 +160,7 @@ struct Item {
 };
 
 template <bool kByUnit>
-__device__ __forceinline__ Item pick(const SeqLane& s, int seq0, int items0, int units0, int at, int tiles_hint) {
+__device__ __forceinline__ Item pick(const SeqLane& s, int seq0, int items0, int units0, int at) {
     const int end = kByUnit ? units0 + s.units_end : items0 + s.items_end;
     const int j = __popcll(__ballot(end <= at));
     Item it;
@@ -189,13 +189,13 @@ template <int kTile, bool kByUnit>
 __device__ __forceinline__ Item find_item(const AttArg& a, const SeqLane& s0, int at, int lane) {
     if (a.b.batch <= 64) {
         if (at >= readlane(kByUnit ? s0.units_end : s0.items_end, 63)) return Item{};
-        return pick<kByUnit>(s0, 0, 0, 0, at, 0);
+        return pick<kByUnit>(s0, 0, 0, 0, at);
     }
     int items = 0, units = 0;
     for (int seq = 0; seq < a.b.batch; seq += 64) {
         const SeqLane s = seq_lane<kTile>(a, seq, lane, 1);
         const int ni = readlane(s.items_end, 63), nu = readlane(s.units_end, 63);
-        if (at < (kByUnit ? units + nu : items + ni)) return pick<kByUnit>(s, seq, items, units, at, 0);
+        if (at < (kByUnit ? units + nu : items + ni)) return pick<kByUnit>(s, seq, items, units, at);
         items += ni;
         units += nu;
     }
@@ -1339,11 +1339,11 @@ struct AttPlan {
 // Rows of a tile by the most that a sequence's head can have: 16 and 32 on the kernel whose waves take
 // their keys straight from memory, 64 and 128 on the one that shares converted keys (see there).
 // A block for each item, and no join, where sequences are short: up to four units, of 16-row tiles (1 token, 32 on 8 heads
-// of 128: 12.3 us a call for 500 keys against 13.9, 10.8 for 240 against 14.2; 64 sequences 18.7 against 21.2; from seven
-// units on one sequence is slower so) or of enough items to fill the chip (16 sequences of 200 tokens, 8 heads: 34.5
-// against 41.7; one of them: 32.6 against 19.3); up to eight units of enough items for two rounds (64 such sequences of 1000
-// keys: 119 against 139), whose unequal lengths even out.  Else split along the keys over the blocks that the chip holds at once (two
-// per CU, one of the 32-row tiles).
+// of 128, bf16: 13.4 us a call for 500 keys against 17.2, 13.7 for 240 against 16.9, 64 sequences of 500 19.5 against 22.0; of
+// six units 15.8 against 16.8, of eight 18.4 against 16.8) or of enough items to fill the chip (16 sequences of 200 tokens and 500
+// keys, 8 heads: 38 against 44.5; one of them: 36 against 20); up to eight units of enough items for two rounds (64 such
+// sequences of 1000 keys: 141 against 161), whose unequal lengths even out.  Else split along the keys over the blocks that
+// the chip holds at once (two per CU, one of the 32-row tiles).
 int att_plan(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, int64_t group, AttPlan* p) {
     TQ_REQUIRE(b->max_tokens * group <= kKvMaxRows, "%s: %lld rows of a sequence's head", what,
                (long long)(b->max_tokens * group));
