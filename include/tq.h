@@ -520,7 +520,8 @@ typedef struct {
  * call among them, the last ones) on the pages table[b * table_stride + i], position p on
  * page p / page.  The call's `tokens` rows are sequence after sequence: rows offsets[b]
  * .. offsets[b + 1] - 1 are the last of sequence b.  offsets NULL: max_tokens rows each
- * (tokens = batch * max_tokens).  Offsets do not decrease.
+ * (tokens = batch * max_tokens).  Offsets do not decrease (where they do, nothing outside
+ * of what the descriptors name is touched, and what rows hold is unspecified).
  * Everything the device arrays say is checked where it is used: a row with no place
  * (before position 0, past the table, on a page outside the cache, before the first
  * sequence, of one with more than max_tokens rows or past `tokens`, behind the last

@@ -87,6 +87,7 @@ template <int kTile>
 __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane, int per) {
     SeqLane s{};
     const int seq = seq0 + lane;
+    bool falls = false;
     if (seq < a.b.batch) {
         int first = a.b.offsets ? a.b.offsets[seq] : seq * a.b.max_tokens;
         const int last = a.b.offsets ? a.b.offsets[seq + 1] : first + a.b.max_tokens;
@@ -99,7 +100,10 @@ __device__ __forceinline__ SeqLane seq_lane(const AttArg& a, int seq0, int lane,
         s.units = max((s.len + kUnit - 1) / kUnit, 1);
         if (per > 1) s.units = (s.units + per - 1) / per;
         s.items = s.tiles * a.heads;
+        falls = last < first;
     }
+    // Offsets that decrease would count rows twice, past what the host's limit on units keeps in 32 bits: none of these 64.
+    if (__ballot(falls)) s.items = 0;
     if (a.b.batch == 1) {  // every lane past the first holds nothing
         s.items_end = readlane(s.items, 0);
         s.units_end = readlane(s.items * s.units, 0);
@@ -125,7 +129,9 @@ __device__ __forceinline__ Line share_line(const AttArg& a, SeqLane& s, int lane
     if (!a.part) return w;
     w.units = readlane(s.units_end, 63);
     if (a.b.batch > 64) {
-        for (int s0 = 64; s0 < a.b.batch; s0 += 64) w.units += readlane(seq_lane<kTile>(a, s0, lane, 1).units_end, 63);
+        int64_t units = w.units;
+        for (int s0 = 64; s0 < a.b.batch; s0 += 64) units += readlane(seq_lane<kTile>(a, s0, lane, 1).units_end, 63);
+        w.units = units <= INT32_MAX ? static_cast<int>(units) : 0;  // (more only where offsets decrease from one 64 to another: nothing)
         return w;
     }
     if (w.units <= a.blocks || readlane(s.items_end, 63) > a.blocks / 2) return w;
@@ -791,7 +797,7 @@ __global__ __launch_bounds__(kAttBlock) void k_kv_attention_join(AttArg a) {
     SeqLane s0;
     const Line line = share_line<kTile>(a, s0, lane);
     const Item it = find_item<kTile, false>(a, s0, blockIdx.x, lane);
-    if (!it.ok) return;
+    if (!it.ok || line.units == 0) return;
     const bool mine = it.tile * kTile + row < it.rows * a.group;
     if (kAll && !mine) return;  // (the whole block)
     const Shares sh(line.units, line.blocks);

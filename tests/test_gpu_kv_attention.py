@@ -254,3 +254,45 @@ def reference_of(c, q, b):
     one.lengths, one.new = [c.lengths[b]], [q.shape[0]]
     one.table, one.offsets, one.rows = c.table[b:b + 1], np.array([0, q.shape[0]]), q.shape[0]
     return reference(one, q)
+
+
+@pytest.mark.parametrize("length", [300, 3000])
+def test_offsets_that_decrease(tq, length):
+    """Nothing is counted twice: sequences of other 64s than that of the decrease are attended to as ever, and so many rows
+    counted again that 32 bits would not hold their units are not worked on."""
+    import torch
+
+    new = [2] * 200
+    c = Case(tq, [length] * 200, new, 16, 2, 64, "i8", ragged=True)
+    c.fill(71)
+    q = rand(72, 400, 2, 64)
+    off = torch.from_numpy(c.offsets).cuda()
+    off[70] = 137  # sequence 69 begins at 138
+    got = c.cache.attention(q, tq.KVBatch(c.table, c.batch.lengths, 2, off, 400))
+    for b in (0, 1, 62, 63, 128, 129, 199):  # (the line of work is another, and so are the shares: not the same bits)
+        ref, pv, top, size = exact_rows(c, q, b)
+        near(got[2 * b:2 * b + 2], ref.cpu(), (2 * 2.0 ** -24 * (80 * size + 8 * (top + 64)) * pv).cpu(), f"sequence {b}")
+
+
+def test_offsets_that_decrease_past_32_bits(tq):
+    import torch
+
+    rows, heads, page = 1 << 20, 64, 1 << 16
+    cache = tq.KVCache.allocate(4, page, heads, 32)
+    for sequences in (10, 200):  # five times the rows in one 64, and in several of which some do not decrease
+        off = torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
+        if sequences == 10:
+            off[1::2] = rows
+        else:
+            off[64:] = rows
+            off[128] = 0
+            off[129:] = rows
+        table = torch.arange(4, dtype=torch.int32, device="cuda").expand(sequences, 4).contiguous()
+        lengths = torch.full((sequences,), 8, dtype=torch.int32, device="cuda")
+        if sequences == 10:
+            lengths.fill_(4 * page)
+        batch = tq.KVBatch(table, lengths, rows, off, rows)
+        q = torch.zeros(rows, heads, 32, dtype=torch.float16, device="cuda")
+        out = cache.attention(q, batch)
+        torch.cuda.synchronize()
+        assert out.shape == q.shape
