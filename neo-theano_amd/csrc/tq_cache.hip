@@ -49,7 +49,10 @@ template <>
 struct Elem<TQ_DT_F16> {
     typedef _Float16 type;
     __device__ static float to(_Float16 v) { return static_cast<float>(v); }
-    __device__ static _Float16 from(float v) { return static_cast<_Float16>(v); }
+    __device__ static _Float16 from(float v) {
+        asm("" : "+v"(v));  // (a product and its rounding to f16 would become one instruction, which skips the f32 value)
+        return static_cast<_Float16>(v);
+    }
 };
 
 // Element i of lane l where whole vectors are moved: 16 bytes at a time, adjacent from lane to lane (8 of a

@@ -48,3 +48,36 @@ def test_frequencies(tq, r, base, kw):
     if kw.get("scaling") == "ntk":
         plain = planes(r, base)
         assert got[0] == plain[0] and abs(float(got[-1]) * kw["factor"] / plain[-1] - 1.0) < 1e-12
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("d,r,pairs", [(128, 128, False), (97, 56, False), (100, 50, True), (64, 64, True), (80, 36, False)])
+@pytest.mark.parametrize("far", [1 << 20, 1 << 40])
+def test_a_far_token_is_turned_alike_by_every_call(tq, dtype, d, r, pairs, far):
+    """A token's angles are the same numbers in calls of one token and of many, of q and k alone and with the cache, in
+    every element type and layout: the f32 values that are rounded or coded are bit for bit the same."""
+    import torch
+
+    from test_gpu_cache import Case, dtype_of, rand
+
+    n, h = 200, 3
+    x = rand(d, n, h, d, dtype=dtype_of(dtype))
+    rot = tq.Rotary.from_base(r, 1000.0, pairs, scale=1.25)
+    pos = torch.randint(0, far, (n,), generator=torch.Generator().manual_seed(r)).cuda()
+    want = rot.apply(x.float(), None, pos)[0]
+    odd = torch.empty(n * (h * d + 1) + 1, device="cuda")[1:].view(n, -1)[:, :h * d].view(n, h, d)
+    odd.copy_(x)
+    assert torch.equal(rot.apply(odd, None, pos)[0], want)  # the same values by elements
+    assert torch.equal(rot.apply(x, None, pos)[0], want.to(x.dtype))
+    for i in range(0, n, 17):
+        assert torch.equal(rot.apply(x[i:i + 1], None, pos[i:i + 1])[0], want[i:i + 1].to(x.dtype))
+    a, b, c = (Case(tq, [n], [n], 16, h, d, "fp8") for _ in range(3))
+    b.cache.write(want, x.float(), b.batch)
+    assert torch.equal(a.cache.write_rotary(x, x, x, rot, a.batch, pos), want.to(x.dtype))
+    for i in range(n):
+        one = tq.KVBatch(c.table, torch.tensor([i + 1], dtype=torch.int32).cuda(), 1)
+        part = slice(i, i + 1)
+        assert torch.equal(c.cache.write_rotary(x[part], x[part], x[part], rot, one, pos[part]), want[part].to(x.dtype))
+    for name in ("k", "k_scale", "v", "v_scale"):
+        assert torch.equal(getattr(a.cache, name), getattr(b.cache, name)), name
+        assert torch.equal(getattr(c.cache, name), getattr(b.cache, name)), name
