@@ -664,7 +664,7 @@ int kv_check(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, KvBat
                    b->max_tokens <= kKvMaxRows && b->tokens <= kKvMaxRows,
                "%s: batch of %lld sequences, %lld tokens, %lld pages each", what, (long long)b->batch, (long long)b->tokens,
                (long long)b->table_pages);
-    TQ_REQUIRE(b->table_pages * c->page <= kKvMaxRows, "%s: a table of %lld pages of %lld tokens is longer than 2^30 tokens",
+    TQ_REQUIRE(b->table_pages <= kKvMaxRows / c->page, "%s: a table of %lld pages of %lld tokens is longer than 2^30 tokens",
                what, (long long)b->table_pages, (long long)c->page);
     TQ_REQUIRE(b->table_stride >= b->table_pages || b->batch <= 1, "%s: table_stride=%lld under %lld pages", what,
                (long long)b->table_stride, (long long)b->table_pages);

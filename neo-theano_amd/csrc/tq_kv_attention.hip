@@ -1429,8 +1429,11 @@ extern "C" {
 
 int64_t tq_kv_attention_workspace_bytes(const tq_kv_cache* cache, const tq_kv_batch* batch, int64_t q_heads) {
     using namespace tq;
-    if (!cache || !batch || cache->heads < 1 || q_heads < 0 || q_heads % cache->heads || cache->page < 16 ||
-        batch->batch < 0 || batch->max_tokens < 0 || batch->tokens < 0 || batch->table_pages < 0)
+    if (!cache || !batch || cache->heads < 1 || cache->heads > 65535 || q_heads < 0 || q_heads > 65535 || q_heads % cache->heads ||
+        cache->head_dim < 1 || cache->head_dim > kKvMaxHeadDim || cache->page < 16 || cache->page % 16 || cache->page > kKvMaxPage ||
+        batch->batch < 0 || batch->batch > kKvMaxRows || batch->max_tokens < 0 || batch->max_tokens > kKvMaxRows ||
+        batch->tokens < 0 || batch->tokens > kKvMaxRows || batch->table_pages < 0 || batch->table_pages > kKvMaxRows / cache->page ||
+        (!batch->offsets && batch->tokens != batch->batch * batch->max_tokens))
         return -1;
     if (batch->batch == 0 || batch->tokens == 0 || batch->max_tokens == 0 || q_heads == 0) return 0;
     AttPlan p;

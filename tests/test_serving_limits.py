@@ -47,6 +47,28 @@ def test_fp8_blocks_past_a_launch(abi):
             assert abi.entry("tq_linear_fp8_block_workspace_bytes")(m, n, k) >= 0
 
 
+def test_descriptors_whose_products_do_not_fit(abi):
+    """2^60 pages of 16 tokens are 0 in 64 bits; sizes that every call refuses have no workspace."""
+    from theano_quantize import InvalidArgument
+
+    h = heads(abi)
+    ws = abi.entry("tq_kv_attention_workspace_bytes")
+    for c, b in ((cache(abi), batch(abi, table_pages=1 << 60, table_stride=1 << 60)),
+                 (cache(abi, page=1 << 16), batch(abi, table_pages=1 << 48, table_stride=1 << 48))):
+        for name, args in (("tq_kv_write", (at(h), at(h), 2, None)), ("tq_kv_read", (2, 256, 256, None)),
+                           ("tq_kv_attention", (at(h), 2, None, 0, 1.0, 256, 1 << 40, 256, None))):
+            with pytest.raises(InvalidArgument):
+                abi.call(name, at(c), at(b), *args)
+        assert ws(at(c), at(b), 2) == -1
+    big = dict(table_pages=64, table_stride=64)
+    for c, b in ((cache(abi), batch(abi, batch=1 << 31, tokens=1 << 31, **big)), (cache(abi), batch(abi, max_tokens=1 << 62, **big)),
+                 (cache(abi, head_dim=1000), batch(abi, **big)), (cache(abi, page=1 << 20), batch(abi, **big)),
+                 (cache(abi, head_dim=0), batch(abi, **big)), (cache(abi, page=24), batch(abi, **big))):
+        assert ws(at(c), at(b), 2) == -1
+    c, b = cache(abi), batch(abi, **big)
+    assert ws(at(c), at(b), 2 << 20) == -1 and ws(at(c), at(b), 2) > 0
+
+
 @pytest.mark.gpu
 def test_weights_of_2_to_the_32_codes_back(tq):
     """16 GB of floats: the first rows, those about each 2^31st code and the last ones."""
