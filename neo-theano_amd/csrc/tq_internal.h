@@ -30,10 +30,10 @@ void clear_error();
 
 inline hipStream_t as_hip(tq_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
-// Checks the launch that was just enqueued.
 // Blocks of 256 threads that a launch may have: HIP refuses 2^32 threads along x.
 constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 
+// Checks the launch that was just enqueued.
 int check_launch(const char* what);
 
 inline bool aligned(const void* p, uintptr_t a) {
