@@ -501,6 +501,18 @@ int tq_rotary_apply(const tq_rotary* rotary, const int64_t* positions, int64_t n
                     const tq_heads* k, int dtype, int64_t head_dim, void* q_out, void* k_out,
                     tq_stream_t stream);
 
+/* Positions of several axes (time, height, width, ...): plane i turns by
+ * positions[x * position_stride + row] * frequencies[i], x being its axis, bits 2 (i % 32) and
+ * up of planes[i / 32].  axes in 1..4, every plane's axis below it.  The calls are otherwise
+ * tq_rotary_apply and tq_kv_write_rotary (positions NULL: all axes at the rows' places). */
+typedef struct {
+    int64_t axes, position_stride;
+    uint64_t planes[2];
+} tq_rotary_axes;
+int tq_rotary_apply_axes(const tq_rotary* rotary, const tq_rotary_axes* axes, const int64_t* positions, int64_t n,
+                         const tq_heads* q, const tq_heads* k, int dtype, int64_t head_dim, void* q_out, void* k_out,
+                         tq_stream_t stream);
+
 /* A paged cache: `pages` pages of `page` tokens (a multiple of 16).  Codes (int8, or
  * e4m3 bit patterns) [pages, heads, page, row], row = head_dim rounded up to 32, zeros
  * past head_dim; scales f32 [pages, heads, page] (>= 0; a write leaves at least 1e-10,
@@ -546,6 +558,9 @@ int tq_kv_write(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_hea
 int tq_kv_write_rotary(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
                        const int64_t* positions, const tq_heads* q, const tq_heads* k, const tq_heads* v, int dtype,
                        void* q_out, tq_stream_t stream);
+int tq_kv_write_rotary_axes(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
+                            const tq_rotary_axes* axes, const int64_t* positions, const tq_heads* q, const tq_heads* k,
+                            const tq_heads* v, int dtype, void* q_out, tq_stream_t stream);
 /* The batch's rows back as f32(code * scale), rounded to dtype: k_out and v_out
  * [tokens, heads, head_dim] (max_tokens or offsets say how many of each sequence). */
 int tq_kv_read(const tq_kv_cache* cache, const tq_kv_batch* batch, int dtype, void* k_out, void* v_out,
@@ -574,6 +589,77 @@ int64_t tq_kv_attention_workspace_bytes(const tq_kv_cache* cache, const tq_kv_ba
 int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_heads* q, int dtype,
                     const int32_t* tree, int64_t tree_words, float scale, void* workspace, int64_t workspace_bytes,
                     void* out, tq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Drafted tokens: which of them the target's probabilities accept (speculative sampling),
+ * what stays of them in the cache, and pages as sequences fork, grow and end.
+ *
+ * Verification.  The batch (tq_kv_batch: offsets, batch, max_tokens and tokens are read) says
+ * which rows are a sequence's new tokens: the first is its root, already part of it, the
+ * others are drafted, row t a child of row parents[t] < t (counted within the sequence; a
+ * row whose parent is not before it is nobody's child; NULL: t - 1, a chain).  target and
+ * draft are probabilities [tokens, vocab] (dtype f32, bf16 or f16, rows target_stride and
+ * draft_stride elements apart): of the token after each row, and those that its children
+ * were drawn from (draft NULL: children are given, not drawn; each a point mass).
+ * accept [tokens] and final [batch] are uniform numbers in [0, 1).
+ *   From the root on, the children of the last accepted row c are tried in order.  After k
+ *   were turned down, left_k = max(p_c - a_k q_c, 0), a_0 = 0, W_0 = 1, a_{k+1} = a_k + W_k,
+ *   W_k = sum left_k; child x is accepted if accept * q_c(x) * W_k < p_c(x) - a_k q_c(x).
+ *   Without draft left_k is p_c without the tokens tried, W_k = 1 - their sum, and x is
+ *   accepted if accept * W_k < left_k(x).
+ *   next is the lowest token whose running sum of left exceeds final * sum left (nothing
+ *   left: of p_c; that empty too: -1).
+ * Compared and summed in f64; NaN and negative probabilities count as 0, a token outside
+ * the vocabulary is turned down.  path [batch, max_tokens]: the accepted rows (counted
+ * within the sequence, the root first), -1 behind them; kept [batch]: how many; next
+ * [batch].  A sequence without rows, or whose rows do not fit (see tq_kv_batch), has kept 0
+ * and next -1.  workspace: tq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned,
+ * contents need not be initialised. */
+int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab);
+int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void* target, int64_t target_stride,
+                     const void* draft, int64_t draft_stride, int dtype, int64_t vocab, const int32_t* parents,
+                     const float* accept, const float* final, void* workspace, int64_t workspace_bytes, int32_t* path,
+                     int32_t* kept, int64_t* next, tq_stream_t stream);
+
+/* What was verified stays: of a sequence's T new tokens, in the cache at its last T places,
+ * rows path[0] < path[1] < .. < path[kept - 1] move to the first `kept` of these places, in
+ * order and as they are coded.  path int32 [batch, path_width], rows path_stride apart; kept
+ * int32 [batch].  lengths_out (or NULL; not the batch's lengths): length - T + kept.  A
+ * sequence whose rows do not fit, whose kept is not in 0 .. min(T, path_width) or whose path does
+ * not ascend within its rows stays as it is, its length too.  Rows with no place do not
+ * move.  Pages that several sequences share are copied first: places are written. */
+int tq_kv_keep(const tq_kv_cache* cache, const tq_kv_batch* batch, const int32_t* path, int64_t path_stride, int64_t path_width,
+               const int32_t* kept, int32_t* lengths_out, tq_stream_t stream);
+
+/* Page target[j] becomes a copy of page source[j] (int32, device, n each), codes and scales.
+ * Pairs with a page outside the cache are skipped.  A target is named once and is no source. */
+int tq_kv_copy_pages(const tq_kv_cache* cache, const int32_t* source, const int32_t* target, int64_t n, tq_stream_t stream);
+
+/* Who holds a page: holders[p] (device, 16-byte aligned) counts the table entries that name
+ * page p; 0 is a free page.  Tables are int32 [batch, table_pages], rows table_stride apart,
+ * -1 where a sequence has no page, its pages first.  Pages that tables name are held;
+ * entries outside the pool are not counted.  Calls on one pool are ordered by one stream.
+ * grow:  gives a sequence pages from behind its last one up to ceil(lengths / page) (or the
+ *        table's end), the lowest free ones, sequence by sequence; entries for which none
+ *        is left stay -1.  At most 4096 sequences.
+ * fork:  child c becomes a copy of sequence parents[c] (outside 0 .. batch - 1: an empty one):
+ *        its whole pages (length / page) are shared, a page that it has begun is to be copied: target[c], the
+ *        lowest free one, from source[c] (-1, -1: nothing to copy, or no page left, then
+ *        the entry is -1 too).  children_table is dense [children, table_pages], -1 behind.
+ *        At most 4096 children.
+ * free:  the sequences (those whose byte is not 0; NULL: all) hold their pages no longer;
+ *        their entries become -1. */
+typedef struct {
+    int32_t* holders;
+    int64_t pages, page;
+} tq_page_pool;
+int tq_pages_grow(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                  int64_t batch, tq_stream_t stream);
+int tq_pages_fork(const tq_page_pool* pool, const int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                  int64_t batch, const int32_t* parents, int64_t children, int32_t* children_table, int32_t* source,
+                  int32_t* target, tq_stream_t stream);
+int tq_pages_free(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, int64_t batch,
+                  const uint8_t* sequences, tq_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Element type conversion of device buffers: the device half of Tensor::to

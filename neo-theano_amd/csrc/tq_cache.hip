@@ -24,6 +24,7 @@ constexpr int kGroup = 16;              // lanes of a head
 constexpr int kPer = 8;                 // elements of a lane
 constexpr int kRowBlock = 256;          // 16 heads at a time
 constexpr int kHeadsAtOnce = kRowBlock / kGroup;
+constexpr int kMaxAxes = 4;
 
 struct HeadsArg {
     const void* data;
@@ -220,9 +221,18 @@ struct OpMaxU {
     __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
 };
 
+// Which of the positions' rows turns a plane: two bits for each plane (all 0 where there is one axis).
+struct AxesArg {
+    uint64_t planes[2];
+    int64_t stride;
+    int count;
+    __device__ int of(int plane) const { return static_cast<int>((plane < 32 ? planes[0] : planes[1]) >> (2 * (plane & 31))) & 3; }
+};
+
 struct RowsArg {
     HeadsArg q, k, v;
     const int64_t* positions;
+    AxesArg axes;
     RotaryArg rot;
     KvBatch b;
     int d, row, n;
@@ -334,8 +344,9 @@ __global__ __launch_bounds__(kRowBlock) void k_token_rows(RowsArg a) {
         if (place.behind) return;  // the whole block: left as it was
     }
     if constexpr (kTurn) {
-        const double pos = static_cast<double>(a.positions ? a.positions[n] : place.pos);
-        if (tid < a.rot.half) plane_angle(a.rot, tid, pos, cs, sn);
+        if (tid < a.rot.half)
+            plane_angle(a.rot, tid, static_cast<double>(a.positions ? a.positions[a.axes.of(tid) * a.axes.stride + n] : place.pos), cs,
+                        sn);
         __syncthreads();
     }
     if (h >= of) return;  // (whole groups)
@@ -352,7 +363,7 @@ __global__ __launch_bounds__(kRowBlock) void k_rows(RowsArg a, int per_share) {
     constexpr int kHalf = kKvMaxHeadDim / 2, kHS = kHeadsAtOnce / kTB, kU = kTurn ? 2 : 4;
     __shared__ float cs[kTB][kHalf], sn[kTB][kHalf];
     __shared__ int64_t slots[kTB];
-    __shared__ double at[kTB];
+    __shared__ double at[kMaxAxes][kTB];
     const int tid = threadIdx.x, l = tid % kGroup, j = tid / kGroup, jt = j % kTB, jh = j / kTB, n0 = blockIdx.x * kTB;
     const int n = min(n0 + jt, a.n - 1);
     if (tid < 64) {
@@ -364,14 +375,15 @@ __global__ __launch_bounds__(kRowBlock) void k_rows(RowsArg a, int per_share) {
         }
         if (tid < kTB) {
             slots[tid] = n0 + tid >= a.n || p.behind ? -2 : p.slot;
-            at[tid] = static_cast<double>(a.positions ? a.positions[nn] : p.pos);
+            for (int x = 0; x < a.axes.count; ++x)
+                at[x][tid] = static_cast<double>(a.positions ? a.positions[x * a.axes.stride + nn] : p.pos);
         }
     }
     __syncthreads();
     if constexpr (kTurn) {
         for (int i = tid; i < kTB * a.rot.half; i += kRowBlock) {
-            const int t = i / a.rot.half;
-            plane_angle(a.rot, i - t * a.rot.half, at[t], cs[t], sn[t]);
+            const int t = i / a.rot.half, plane = i - t * a.rot.half;
+            plane_angle(a.rot, plane, at[a.axes.of(plane)][t], cs[t], sn[t]);
         }
         __syncthreads();
     }
@@ -508,6 +520,19 @@ int check_rotary(const char* what, const tq_rotary* r, int64_t d) {
     return TQ_OK;
 }
 
+// axes null: one axis.  Without positions every axis has the rows' places.
+int check_axes(const char* what, const tq_rotary_axes* x, const tq_rotary* r, AxesArg* out) {
+    *out = AxesArg{{0, 0}, 0, 1};
+    if (!x) return TQ_OK;
+    TQ_REQUIRE(x->axes >= 1 && x->axes <= kMaxAxes, "%s: axes=%lld is not in 1..4", what, (long long)x->axes);
+    TQ_REQUIRE(x->position_stride >= 0, "%s: position_stride=%lld", what, (long long)x->position_stride);
+    *out = AxesArg{{x->planes[0], x->planes[1]}, x->position_stride, static_cast<int>(x->axes)};
+    for (int64_t i = 0; i < r->rotary_dim / 2; ++i)
+        TQ_REQUIRE(static_cast<int64_t>(x->planes[i / 32] >> (2 * (i % 32)) & 3) < x->axes, "%s: plane %lld is of none of the %lld axes",
+                   what, (long long)i, (long long)x->axes);
+    return TQ_OK;
+}
+
 RotaryArg rotary_arg(const tq_rotary* r) {
     return RotaryArg{r->frequencies, static_cast<int>(r->rotary_dim / 2), r->interleaved != 0, r->inverse != 0, r->scale};
 }
@@ -569,8 +594,8 @@ int launch_rows_typed(const RowsArg& a, int dtype, bool vec, hipStream_t st, con
 bool vec_rotary(const RotaryArg& r, int dtype) { return r.pairs || r.half % run_of(dtype) == 0; }
 
 int write_rows(const char* what, const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
-               const int64_t* positions, const tq_heads* q, const tq_heads* k, const tq_heads* v, int dtype, void* q_out,
-               hipStream_t st) {
+               const tq_rotary_axes* axes, const int64_t* positions, const tq_heads* q, const tq_heads* k, const tq_heads* v,
+               int dtype, void* q_out, hipStream_t st) {
     RowsArg a{};
     int rc = kv_check(what, cache, batch, &a.b);
     if (rc != TQ_OK) return rc;
@@ -581,6 +606,7 @@ int write_rows(const char* what, const tq_kv_cache* cache, const tq_kv_batch* ba
     bool vec = vec_rows(k, d, dtype) && vec_rows(v, d, dtype);
     if (rotary) {
         if ((rc = check_rotary(what, rotary, d)) != TQ_OK) return rc;
+        if ((rc = check_axes(what, axes, rotary, &a.axes)) != TQ_OK) return rc;
         a.rot = rotary_arg(rotary);
         a.positions = positions;
         vec = vec && vec_rotary(a.rot, dtype);
@@ -692,16 +718,16 @@ int kv_check(const char* what, const tq_kv_cache* c, const tq_kv_batch* b, KvBat
 
 }  // namespace tq
 
-extern "C" {
+namespace tq {
+namespace {
 
-int tq_rotary_apply(const tq_rotary* rotary, const int64_t* positions, int64_t n, const tq_heads* q, const tq_heads* k,
-                    int dtype, int64_t head_dim, void* q_out, void* k_out, tq_stream_t stream) {
-    using namespace tq;
-    static const char* what = "tq_rotary_apply";
+int apply_rows(const char* what, const tq_rotary* rotary, const tq_rotary_axes* axes, const int64_t* positions, int64_t n,
+               const tq_heads* q, const tq_heads* k, int dtype, int64_t head_dim, void* q_out, void* k_out, tq_stream_t stream) {
     int rc = check_rotary(what, rotary, head_dim);
     if (rc != TQ_OK) return rc;
     TQ_REQUIRE(n >= 0 && n <= kKvMaxRows, "%s: n=%lld", what, (long long)n);
     RowsArg a{};
+    if ((rc = check_axes(what, axes, rotary, &a.axes)) != TQ_OK) return rc;
     bool vec = true;
     for (int i = 0; i < 2; ++i) {
         const tq_heads* x = i == 0 ? q : k;
@@ -724,9 +750,26 @@ int tq_rotary_apply(const tq_rotary* rotary, const int64_t* positions, int64_t n
     return launch_rows_typed<FmtI8>(a, dtype, vec && vec_rotary(a.rot, dtype), as_hip(stream), what);
 }
 
+}  // namespace
+}  // namespace tq
+
+extern "C" {
+
+int tq_rotary_apply(const tq_rotary* rotary, const int64_t* positions, int64_t n, const tq_heads* q, const tq_heads* k,
+                    int dtype, int64_t head_dim, void* q_out, void* k_out, tq_stream_t stream) {
+    return tq::apply_rows("tq_rotary_apply", rotary, nullptr, positions, n, q, k, dtype, head_dim, q_out, k_out, stream);
+}
+
+int tq_rotary_apply_axes(const tq_rotary* rotary, const tq_rotary_axes* axes, const int64_t* positions, int64_t n,
+                         const tq_heads* q, const tq_heads* k, int dtype, int64_t head_dim, void* q_out, void* k_out,
+                         tq_stream_t stream) {
+    TQ_REQUIRE(axes, "tq_rotary_apply_axes: null axes");
+    return tq::apply_rows("tq_rotary_apply_axes", rotary, axes, positions, n, q, k, dtype, head_dim, q_out, k_out, stream);
+}
+
 int tq_kv_write(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_heads* k, const tq_heads* v, int dtype,
                 tq_stream_t stream) {
-    return tq::write_rows("tq_kv_write", cache, batch, nullptr, nullptr, nullptr, k, v, dtype, nullptr, tq::as_hip(stream));
+    return tq::write_rows("tq_kv_write", cache, batch, nullptr, nullptr, nullptr, nullptr, k, v, dtype, nullptr, tq::as_hip(stream));
 }
 
 int tq_kv_write_rotary(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
@@ -734,7 +777,15 @@ int tq_kv_write_rotary(const tq_kv_cache* cache, const tq_kv_batch* batch, const
                        void* q_out, tq_stream_t stream) {
     TQ_REQUIRE(rotary, "tq_kv_write_rotary: null rotary");
     TQ_REQUIRE(tq::aligned(positions, 8), "tq_kv_write_rotary: unaligned positions");
-    return tq::write_rows("tq_kv_write_rotary", cache, batch, rotary, positions, q, k, v, dtype, q_out, tq::as_hip(stream));
+    return tq::write_rows("tq_kv_write_rotary", cache, batch, rotary, nullptr, positions, q, k, v, dtype, q_out, tq::as_hip(stream));
+}
+
+int tq_kv_write_rotary_axes(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq_rotary* rotary,
+                            const tq_rotary_axes* axes, const int64_t* positions, const tq_heads* q, const tq_heads* k,
+                            const tq_heads* v, int dtype, void* q_out, tq_stream_t stream) {
+    TQ_REQUIRE(rotary && axes, "tq_kv_write_rotary_axes: null rotary or axes");
+    TQ_REQUIRE(tq::aligned(positions, 8), "tq_kv_write_rotary_axes: unaligned positions");
+    return tq::write_rows("tq_kv_write_rotary_axes", cache, batch, rotary, axes, positions, q, k, v, dtype, q_out, tq::as_hip(stream));
 }
 
 int tq_kv_read(const tq_kv_cache* cache, const tq_kv_batch* batch, int dtype, void* k_out, void* v_out,

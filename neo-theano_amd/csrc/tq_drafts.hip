@@ -1,0 +1,527 @@
+// tq_drafts.hip -- which drafted tokens the target's probabilities accept, and the token that follows.
+//
+// Speculative sampling over trees.  At an accepted token c with target probabilities p and draft
+// probabilities q, its children are tried in order.  After k children were turned down
+//   left_k = max(p - a_k q, 0),   a_0 = 0, W_0 = 1,   a_{k+1} = a_k + W_k,   W_k = sum left_k,
+// and child x is accepted if u q(x) W_k < p(x) - a_k q(x): the residuals max(r - q, 0) / sum of repeated
+// rejection are left_k / W_k, since their clamps at zero nest.  Without q a child is a point mass: left_k is
+// p without the tokens tried, W_k = 1 - their sum.  The token that follows is drawn from left at the last
+// accepted token: the lowest i whose running sum exceeds final * sum left.
+//
+// Everything is compared and summed in f64 (the running sum is compared with a number next to a border).
+// The bytes are one row of p (and of q) for a sequence; what costs is the chain of dependent loads
+// (token -> its probability -> the row -> the sums -> the chosen share), so a row is cut into shares that
+// blocks sum side by side, and a second launch picks the share and looks into it again.
+#include <algorithm>
+
+#include "tq_kv.h"
+
+namespace tq {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWalkBlock = 1024;
+constexpr int kMaxShare = 8192;  // probabilities of a share
+
+template <int kType>
+struct Prob;
+template <>
+struct Prob<TQ_DT_F32> {
+    typedef float type;
+};
+template <>
+struct Prob<TQ_DT_BF16> {
+    typedef __bf16 type;
+};
+template <>
+struct Prob<TQ_DT_F16> {
+    typedef _Float16 type;
+};
+
+// Where the walk over a sequence's drafts ended.
+struct State {
+    double a;     // share of q that is gone
+    int node;     // last accepted row of the sequence; -1: the sequence has no rows
+    int kept;
+};
+
+struct DraftArg {
+    const int64_t* tokens;
+    const void* target;
+    const void* draft;
+    int64_t target_stride, draft_stride;
+    const int32_t* parents;
+    const float* accept;
+    const float* final;
+    const int32_t* offsets;
+    int batch, max_tokens, rows;
+    int vocab, share, shares;  // share: probabilities of a block, shares * share >= vocab
+    int32_t* path;
+    int32_t* kept;
+    int64_t* next;
+    State* state;   // [batch]
+    double* sums;   // [batch, shares]
+};
+
+struct Span {
+    int first, count;
+};
+__device__ __forceinline__ Span span_of(const DraftArg& a, int seq) {
+    const int first = a.offsets ? a.offsets[seq] : seq * a.max_tokens;
+    const int last = a.offsets ? a.offsets[seq + 1] : first + a.max_tokens;
+    const bool fits = first >= 0 && last <= a.rows && last > first && last - first <= a.max_tokens;
+    return Span{first, fits ? last - first : 0};
+}
+
+template <class T>
+__device__ __forceinline__ double at(const void* x, int64_t stride, int row, int64_t token) {
+    return static_cast<double>(static_cast<float>(static_cast<const T*>(x)[row * stride + token]));
+}
+
+// What is left of one token's probability (NaN: nothing).
+__device__ __forceinline__ double left_of(double p, double q, double a) {
+    const double v = p - a * q;
+    return v > 0.0 ? v : 0.0;
+}
+
+__device__ __forceinline__ double readlane_f64(double v, int l) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), l));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b >> 32), l));
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+
+// Walks the drafts of a sequence; whole waves, the result uniform.  path: where the accepted rows go, or null.
+// mass(node, a): the sum of what is left, called by all of the block's waves alike (only where q is there and a
+// node has another child after one that was turned down).
+template <class T, class Mass>
+__device__ __forceinline__ State walk(const DraftArg& a, Span s, int32_t* path, Mass mass) {
+    const int lane = threadIdx.x & 63;
+    State st{0.0, s.count > 0 ? 0 : -1, s.count > 0 ? 1 : 0};
+    if (path && lane == 0 && s.count > 0) path[0] = 0;
+    double w = 1.0;
+    bool pending = false;  // a child was turned down and w is not yet that of what is left
+    for (int t0 = 1; t0 < s.count; t0 += 64) {
+        const int t = t0 + lane;
+        const bool there = t < s.count;
+        const int row = s.first + (there ? t : 0);
+        int parent = there ? (a.parents ? a.parents[row] : t - 1) : -1;
+        if (parent >= t) parent = -1;
+        const int64_t x = there ? a.tokens[row] : -1;
+        const bool known = x >= 0 && x < a.vocab && parent >= 0;
+        const double u = there ? static_cast<double>(a.accept[row]) : 0.0;
+        const double p = known ? at<T>(a.target, a.target_stride, s.first + parent, x) : 0.0;
+        const double q = !known ? 0.0 : a.draft ? at<T>(a.draft, a.draft_stride, s.first + parent, x) : 1.0;
+        if (!a.parents) {  // a chain: all tests at once
+            const uint64_t turned_down = __ballot(there && !(u * q < p));
+            const int fine = turned_down ? __ffsll(static_cast<unsigned long long>(turned_down)) - 1 : min(64, s.count - t0);
+            if (path && lane < fine) path[t] = t;
+            st.kept += fine;
+            st.node += fine;
+            if (turned_down) {
+                st.a = 1.0;
+                return st;
+            }
+            continue;
+        }
+        for (int from = 0; from < 64;) {
+            const uint64_t children = __ballot(there && parent == st.node && lane >= from);
+            if (!children) break;
+            const int l = __ffsll(static_cast<unsigned long long>(children)) - 1;
+            from = l + 1;
+            double px = readlane_f64(p, l);
+            const double qx = readlane_f64(q, l), ux = readlane_f64(u, l);
+            const int tx = t0 + l;
+            bool yes;
+            if (a.draft) {
+                if (pending) w = mass(st.node, st.a);
+                pending = false;
+                yes = ux * qx * w < px - st.a * qx;
+            } else {
+                // a token that a sibling was turned down with has nothing left
+                const int xl = __builtin_amdgcn_readlane(static_cast<int>(x), l);  // (a known token is below 2^31)
+                bool again = there && parent == st.node && lane < l && known && static_cast<int>(x) == xl;
+                for (int e0 = 1; e0 < t0; e0 += 64) {
+                    const int e = s.first + e0 + lane;
+                    again |= a.parents[e] == st.node && e0 + lane > st.node && a.tokens[e] == xl;
+                }
+                if (__ballot(again)) px = 0.0;
+                yes = ux * w < px;
+            }
+            if (yes) {
+                st.node = tx;
+                if (path && lane == 0) path[st.kept] = tx;
+                ++st.kept;
+                st.a = 0.0;
+                w = 1.0;
+            } else if (a.draft) {
+                st.a += w;
+                pending = true;
+            } else {
+                w -= px;
+            }
+        }
+    }
+    return st;
+}
+
+// Sums of f64 over a block, the same in every thread (and in every call: a fixed order).
+template <int kThreads>
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) s += lds[w];
+    __syncthreads();
+    return s;
+}
+
+// Elements i .. i + 3 of a row as f64, zeros from `end` on.
+template <class T, bool kVec>
+__device__ __forceinline__ void load4(const T* row, int i, int end, double (&v)[4]) {
+    if constexpr (kVec) {  // rows 16-byte aligned (8 for 16-bit types), `end` a multiple of 4
+        typedef T V __attribute__((ext_vector_type(4)));
+        V x{};
+        if (i < end) x = *reinterpret_cast<const V*>(row + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<double>(static_cast<float>(x[e]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = i + e < end ? static_cast<double>(static_cast<float>(row[i + e])) : 0.0;
+    }
+}
+
+// What is left of elements i .. i + 3.  gone: bits of the tokens tried, from the share's start on, or null.
+template <class T, bool kVec>
+__device__ __forceinline__ void left4(const T* p, const T* q, double a, int i, int end, uint32_t gone, double (&v)[4]) {
+    double x[4], y[4] = {0, 0, 0, 0};
+    load4<T, kVec>(p, i, end, x);
+    if (q) load4<T, kVec>(q, i, end, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = gone >> e & 1 ? 0.0 : left_of(x[e], y[e], a);
+}
+
+// Sum of what is left over the whole row, by one block.
+template <class T, bool kVec, int kThreads>
+__device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int vocab, double* lds) {
+    double s = 0.0;
+    for (int i = 4 * static_cast<int>(threadIdx.x); i < vocab; i += 4 * kThreads) {
+        double v[4];
+        left4<T, kVec>(p, q, a, i, vocab, 0, v);
+        s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    return block_sum<kThreads>(s, lds);
+}
+
+template <class T>
+__device__ __forceinline__ const T* row_of(const void* x, int64_t stride, int row) {
+    return x ? static_cast<const T*>(x) + row * stride : nullptr;
+}
+
+// Trees with draft probabilities: the walk needs sums of its own.  A block for each sequence.
+template <class T, bool kVec>
+__global__ __launch_bounds__(kWalkBlock) void k_walk(DraftArg a) {
+    __shared__ double lds[kWalkBlock / 64];
+    const int seq = blockIdx.x;
+    const Span s = span_of(a, seq);
+    int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
+    const State st = walk<T>(a, s, threadIdx.x < 64 ? path : nullptr, [&](int node, double share) {
+        return row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node),
+                                             row_of<T>(a.draft, a.draft_stride, s.first + node), share, a.vocab, lds);
+    });
+    if (threadIdx.x == 0) a.state[seq] = st;
+}
+
+// Bits of the tokens that were tried at the node, from `begin` on, into gone (cleared by the caller).
+__device__ __forceinline__ void mark_tried(const DraftArg& a, Span s, int node, int begin, uint32_t* gone, int threads) {
+    for (int t = node + 1 + threadIdx.x; t < s.count; t += threads) {
+        if (a.parents ? a.parents[s.first + t] != node : t != node + 1) continue;
+        const int64_t x = a.tokens[s.first + t] - begin;
+        if (x >= 0 && x < a.share) atomicOr(gone + x / 32, 1u << (x & 31));
+    }
+}
+
+// Block (share, sequence): the sum of what is left of a share.  kWalked: k_walk was there; otherwise every block
+// walks (a few dependent loads) and the first share's block writes the path down.
+template <class T, bool kVec, bool kWalked>
+__global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
+    __shared__ double lds[kBlock / 64];
+    __shared__ State shared;
+    __shared__ uint32_t gone[kMaxShare / 32];
+    const int seq = blockIdx.x / a.shares, share = blockIdx.x - seq * a.shares, begin = share * a.share;
+    const Span s = span_of(a, seq);
+    if (!a.draft)
+        for (int i = threadIdx.x; i < a.share / 32; i += kBlock) gone[i] = 0;
+    if (threadIdx.x < 64) {
+        State st;
+        if constexpr (kWalked) {
+            st = a.state[seq];
+        } else {
+            st = walk<T>(a, s, share == 0 ? a.path + static_cast<int64_t>(seq) * a.max_tokens : nullptr,
+                         [](int, double) { return 0.0; });
+            if (share == 0 && threadIdx.x == 0) a.state[seq] = st;
+        }
+        if (threadIdx.x == 0) shared = st;
+    }
+    __syncthreads();
+    const State st = shared;
+    if (st.node < 0) return;
+    if (!a.draft) {
+        mark_tried(a, s, st.node, begin, gone, kBlock);
+        __syncthreads();
+    }
+    const T* p = row_of<T>(a.target, a.target_stride, s.first + st.node);
+    const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
+    const int end = min(begin + a.share, a.vocab);
+    double sum = 0.0;
+    for (int i = begin + 4 * static_cast<int>(threadIdx.x); i < end; i += 4 * kBlock) {
+        double v[4];
+        left4<T, kVec>(p, q, st.a, i, end, a.draft ? 0 : gone[(i - begin) / 32] >> ((i - begin) & 31), v);
+        sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    sum = block_sum<kBlock>(sum, lds);
+    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(seq) * a.shares + share] = sum;
+}
+
+// Running sums of v over a block's threads, this thread's own among them.
+template <int kThreads>
+__device__ __forceinline__ double block_running(double v, double* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double y = __shfl_up(v, d);
+        if (lane >= d) v += y;
+    }
+    if (lane == 63) lds[wave] = v;
+    __syncthreads();
+    double before = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) before += w < wave ? lds[w] : 0.0;
+    __syncthreads();
+    return before + v;
+}
+
+// A block for each sequence: the share where the running sum passes final * total, then the token in it.
+template <class T, bool kVec>
+__global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
+    __shared__ double lds[kBlock / 64];
+    __shared__ uint32_t gone[kMaxShare / 32];
+    __shared__ int first_over, last_some;
+    __shared__ double before_it;
+    const int seq = blockIdx.x, tid = threadIdx.x;
+    const Span s = span_of(a, seq);
+    const State st = a.state[seq];
+    int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
+    for (int i = st.kept + tid; i < a.max_tokens; i += kBlock) path[i] = -1;
+    if (tid == 0) a.kept[seq] = st.kept;
+    if (st.node < 0) {
+        if (tid == 0) a.next[seq] = -1;
+        return;
+    }
+    const double* sums = a.sums + static_cast<int64_t>(seq) * a.shares;
+    double share_of_q = st.a, total = 0.0;
+    bool tried = !a.draft;
+    for (int i = tid; i < a.shares; i += kBlock) total += sums[i];
+    total = block_sum<kBlock>(total, lds);
+    const T* p = row_of<T>(a.target, a.target_stride, s.first + st.node);
+    const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
+    // nothing left: the target's own probabilities, share by share (not on the way of any sound input)
+    const bool own = !(total > 0.0);
+    if (own) {
+        q = nullptr;
+        share_of_q = 0.0;
+        tried = false;
+        total = row_mass<T, kVec, kBlock>(p, q, 0.0, a.vocab, lds);
+    }
+    if (!(total > 0.0)) {
+        if (tid == 0) a.next[seq] = -1;
+        return;
+    }
+    const double goal = static_cast<double>(a.final[seq]) * total;
+    // (the share loop below reads sums of shares, or, in the rare case, sums the share itself)
+    double base = 0.0;
+    int chosen = -1, some = -1;
+    double chosen_before = 0.0, some_before = 0.0;
+    for (int c0 = 0; c0 < a.shares && chosen < 0; c0 += kBlock) {
+        double v = 0.0;
+        if (!own) {
+            v = c0 + tid < a.shares ? sums[c0 + tid] : 0.0;
+        } else if (c0 + tid < a.shares) {
+            const int b0 = (c0 + tid) * a.share, b1 = min(b0 + a.share, a.vocab);
+            for (int i = b0; i < b1; ++i) v += left_of(static_cast<double>(static_cast<float>(p[i])), 0.0, 0.0);
+        }
+        if (tid == 0) {
+            first_over = INT32_MAX;
+            last_some = -1;
+        }
+        const double run = block_running<kBlock>(v, lds) + base;
+        if (v > 0.0) {
+            if (run > goal) atomicMin(&first_over, tid);
+            atomicMax(&last_some, tid);
+        }
+        __syncthreads();
+        const int over = first_over, last = last_some;
+        if (tid == (over != INT32_MAX ? over : last)) before_it = run - v;
+        __syncthreads();
+        if (over != INT32_MAX) {
+            chosen = c0 + over;
+            chosen_before = before_it;
+        } else if (last >= 0) {
+            some = c0 + last;
+            some_before = before_it;
+        }
+        base += block_sum<kBlock>(v, lds);
+    }
+    if (chosen < 0) {  // (roundings, or sums that are not finite: the last share that has anything)
+        chosen = some;
+        chosen_before = some_before;
+    }
+    if (chosen < 0) {
+        if (tid == 0) a.next[seq] = -1;
+        return;
+    }
+    const int begin = chosen * a.share, end = min(begin + a.share, a.vocab);
+    for (int i = tid; i < a.share / 32; i += kBlock) gone[i] = 0;
+    __syncthreads();
+    if (tried) mark_tried(a, s, st.node, begin, gone, kBlock);
+    if (tid == 0) {
+        first_over = INT32_MAX;
+        last_some = -1;
+    }
+    __syncthreads();
+    base = chosen_before;
+    for (int i0 = begin; i0 < end; i0 += 4 * kBlock) {
+        const int i = i0 + 4 * tid;
+        double v[4] = {0, 0, 0, 0};
+        if (i < end) left4<T, kVec>(p, q, share_of_q, i, end, gone[(i - begin) / 32] >> ((i - begin) & 31), v);
+        const double mine = (v[0] + v[1]) + (v[2] + v[3]);
+        double run = block_running<kBlock>(mine, lds) - mine + base;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            run += v[e];
+            if (v[e] > 0.0) {
+                if (run > goal) atomicMin(&first_over, i + e);
+                atomicMax(&last_some, i + e);
+            }
+        }
+        __syncthreads();
+        if (first_over != INT32_MAX) break;
+        base += block_sum<kBlock>(mine, lds);
+    }
+    if (tid == 0) a.next[seq] = first_over != INT32_MAX ? first_over : last_some;
+}
+
+// Probabilities of a share: so that all shares are about two blocks for each CU, at least 1024 (a load for each
+// lane) and at most 8192.
+int share_of(int64_t vocab, int64_t batch) {
+    int share = 1024;
+    while (share < kMaxShare && batch * ((vocab + share - 1) / share) > 2 * device_cu_count()) share *= 2;
+    return share;
+}
+
+int64_t shares_of(int64_t vocab, int64_t batch) {
+    const int share = share_of(vocab, batch);
+    return (vocab + share - 1) / share;
+}
+
+int check_batch(const char* what, const tq_kv_batch* b, int64_t vocab) {
+    TQ_REQUIRE(b, "%s: null batch", what);
+    TQ_REQUIRE(b->batch >= 0 && b->max_tokens >= 0 && b->tokens >= 0 && b->batch <= kKvMaxRows && b->max_tokens <= kKvMaxRows &&
+                   b->tokens <= kKvMaxRows,
+               "%s: batch of %lld sequences, %lld tokens", what, (long long)b->batch, (long long)b->tokens);
+    TQ_REQUIRE(b->offsets || b->tokens == b->batch * b->max_tokens, "%s: without offsets tokens=%lld must be batch * max_tokens = %lld",
+               what, (long long)b->tokens, (long long)(b->batch * b->max_tokens));
+    TQ_REQUIRE(aligned(b->offsets, 4), "%s: unaligned offsets", what);
+    TQ_REQUIRE(vocab >= 1 && vocab <= kKvMaxRows, "%s: vocab=%lld is not in 1..2^30", what, (long long)vocab);
+    return TQ_OK;
+}
+
+template <class T, bool kVec>
+void launch_drafts(const DraftArg& a, hipStream_t st) {
+    const bool walk_first = a.draft && a.parents;
+    if (walk_first) {
+        k_walk<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
+        k_left<T, kVec, true><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+    } else {
+        k_left<T, kVec, false><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+    }
+    k_pick<T, kVec><<<a.batch, kBlock, 0, st>>>(a);
+}
+
+template <class T>
+int launch_typed(const DraftArg& a, hipStream_t st, const char* what) {
+    const int size = sizeof(T), align = 4 * size;
+    auto fits = [&](const void* x, int64_t stride) { return !x || (aligned(x, align) && stride * size % align == 0); };
+    clear_error();
+    if (a.vocab % 4 == 0 && fits(a.target, a.target_stride) && fits(a.draft, a.draft_stride))
+        launch_drafts<T, true>(a, st);
+    else
+        launch_drafts<T, false>(a, st);
+    return check_launch(what);
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" {
+
+int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab) {
+    using namespace tq;
+    if (check_batch("tq_verify_drafts", batch, vocab) != TQ_OK) return -1;
+    return (batch->batch * static_cast<int64_t>(sizeof(State)) + batch->batch * shares_of(vocab, batch->batch) * 8 + 15) / 16 * 16;
+}
+
+int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void* target, int64_t target_stride,
+                     const void* draft, int64_t draft_stride, int dtype, int64_t vocab, const int32_t* parents,
+                     const float* accept, const float* final, void* workspace, int64_t workspace_bytes, int32_t* path,
+                     int32_t* kept, int64_t* next, tq_stream_t stream) {
+    using namespace tq;
+    static const char* what = "tq_verify_drafts";
+    const int rc = check_batch(what, batch, vocab);
+    if (rc != TQ_OK) return rc;
+    TQ_REQUIRE(dtype == TQ_DT_F32 || dtype == TQ_DT_BF16 || dtype == TQ_DT_F16, "%s: dtype %d is not f32, bf16 or f16", what, dtype);
+    const int size = dtype == TQ_DT_F32 ? 4 : 2;
+    TQ_REQUIRE(target_stride >= 0 && (!draft || draft_stride >= 0), "%s: negative stride", what);
+    if (batch->batch == 0) return TQ_OK;
+    TQ_REQUIRE(kept && next && (path || batch->max_tokens == 0), "%s: null path, kept or next", what);
+    TQ_REQUIRE(batch->tokens == 0 || (tokens && target && accept && final), "%s: null tokens, target, accept or final", what);
+    TQ_REQUIRE(aligned(tokens, 8) && aligned(target, size) && aligned(draft, size) && aligned(parents, 4) && aligned(accept, 4) &&
+                   aligned(final, 4) && aligned(path, 4) && aligned(kept, 4) && aligned(next, 8),
+               "%s: a pointer is not aligned to its elements", what);
+    const int64_t shares = shares_of(vocab, batch->batch);
+    TQ_REQUIRE(batch->batch <= (int64_t(1) << 22) - 1 && batch->batch * shares <= kMaxBlocks,
+               "%s: %lld sequences with %lld shares of %lld tokens are more than %lld blocks", what, (long long)batch->batch,
+               (long long)shares, (long long)vocab, (long long)kMaxBlocks);
+    const int64_t need = tq_verify_drafts_workspace_bytes(batch, vocab);
+    TQ_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), "%s: workspace of %lld bytes, 16-byte aligned, needed",
+               what, (long long)need);
+    DraftArg a{};
+    a.tokens = tokens;
+    a.target = target;
+    a.draft = draft;
+    a.target_stride = target_stride;
+    a.draft_stride = draft_stride;
+    a.parents = parents;
+    a.accept = accept;
+    a.final = final;
+    a.offsets = batch->offsets;
+    a.batch = static_cast<int>(batch->batch);
+    a.max_tokens = static_cast<int>(batch->max_tokens);
+    a.rows = static_cast<int>(batch->tokens);
+    a.vocab = static_cast<int>(vocab);
+    a.share = share_of(vocab, batch->batch);
+    a.shares = static_cast<int>(shares);
+    a.path = path;
+    a.kept = kept;
+    a.next = next;
+    a.state = static_cast<State*>(workspace);
+    a.sums = reinterpret_cast<double*>(a.state + batch->batch);
+    if (dtype == TQ_DT_F32) return launch_typed<float>(a, as_hip(stream), what);
+    if (dtype == TQ_DT_BF16) return launch_typed<__bf16>(a, as_hip(stream), what);
+    return launch_typed<_Float16>(a, as_hip(stream), what);
+}
+
+}  // extern "C"

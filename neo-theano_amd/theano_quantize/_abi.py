@@ -30,6 +30,8 @@ rotary_desc = struct.Struct("@Pqiif4x").pack             # tq_rotary: frequencie
 kv_cache_desc = struct.Struct("@PPPPqqqqi4x").pack       # tq_kv_cache: k, k_scale, v, v_scale, pages, heads, page, head_dim, codes
 kv_batch_desc = struct.Struct("@PqqPPqqq").pack          # tq_kv_batch: table, table_stride, table_pages, lengths, offsets, batch,
 #                                                          max_tokens, tokens
+rotary_axes_desc = struct.Struct("@qqQQ").pack           # tq_rotary_axes: axes, position_stride, planes[2]
+page_pool_desc = struct.Struct("@Pqq").pack              # tq_page_pool: holders, pages, page
 
 
 # name -> argtypes (all return int status unless listed in _RESTYPE)
@@ -107,11 +109,20 @@ SIGNATURES = {
     "tq_linear_fp8_block": [_p, _int, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p, _p],
     # descriptors are passed as their packed bytes
     "tq_rotary_apply": [_p, _p, _i64, _p, _p, _int, _i64, _p, _p, _p],
+    "tq_rotary_apply_axes": [_p, _p, _p, _i64, _p, _p, _int, _i64, _p, _p, _p],
     "tq_kv_write": [_p, _p, _p, _p, _int, _p],
     "tq_kv_write_rotary": [_p, _p, _p, _p, _p, _p, _p, _int, _p, _p],
+    "tq_kv_write_rotary_axes": [_p, _p, _p, _p, _p, _p, _p, _p, _int, _p, _p],
     "tq_kv_read": [_p, _p, _int, _p, _p, _p],
     "tq_kv_attention_workspace_bytes": [_p, _p, _i64],
     "tq_kv_attention": [_p, _p, _p, _int, _p, _i64, ctypes.c_float, _p, _i64, _p, _p],
+    "tq_verify_drafts_workspace_bytes": [_p, _i64],
+    "tq_verify_drafts": [_p, _p, _p, _i64, _p, _i64, _int, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _p],
+    "tq_kv_keep": [_p, _p, _p, _i64, _i64, _p, _p, _p],
+    "tq_kv_copy_pages": [_p, _p, _p, _i64, _p],
+    "tq_pages_grow": [_p, _p, _i64, _i64, _p, _i64, _p],
+    "tq_pages_fork": [_p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p],
+    "tq_pages_free": [_p, _p, _i64, _i64, _i64, _p, _p],
 }
 _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_p,
             "tq_w4g128_tile_rows": ctypes.c_int64, "tq_mlp_w4g128_workspace_bytes": ctypes.c_int64,
@@ -121,7 +132,7 @@ _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_
             "tq_mlp_w4g128_split_workspace_bytes": ctypes.c_int64,
             "tq_linear_w8a8_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w8a8_workspace_bytes": ctypes.c_int64, "tq_gemm_fp8_workspace_bytes": ctypes.c_int64,
-            "tq_kv_attention_workspace_bytes": ctypes.c_int64,
+            "tq_kv_attention_workspace_bytes": ctypes.c_int64, "tq_verify_drafts_workspace_bytes": ctypes.c_int64,
             "tq_gemm_fp8_block_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_block_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w4g128_bf16_workspace_bytes": ctypes.c_int64, "tq_dtype_size": ctypes.c_int64}
 

@@ -84,17 +84,30 @@ class Rotary(_Fixed):
 
     frequencies: float64 device tensor of rotary_dim / 2 angles per position; the first
     rotary_dim elements of a head turn, the others pass.  Plane i is elements (i, i +
-    rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`.  Outputs are multiplied by `scale`."""
+    rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`.  Outputs are multiplied by `scale`.
 
-    def __init__(self, frequencies, interleaved=False, scale=1.0):
+    axes: for positions of several axes (time, height, width of an image's patches), the axis
+    (0 to 3) of each plane, see `axes_in_blocks` and `axes_in_turn`; positions are then int64
+    [axes, tokens], or [tokens] where all axes are the same (text)."""
+
+    def __init__(self, frequencies, interleaved=False, scale=1.0, axes=None):
         _indices(frequencies, torch.float64, 1, "Rotary: frequencies")
         r, interleaved, scale = 2 * frequencies.shape[0], bool(interleaved), float(scale)
-        self.__dict__.update(frequencies=frequencies, interleaved=interleaved, scale=scale, rotary_dim=r,
+        planes, count = [0] * 2, 0
+        if axes is not None:
+            axes = tuple(axes)
+            if len(axes) != r // 2 or r > MAX_HEAD_DIM or any(x not in (0, 1, 2, 3) for x in axes):
+                raise InvalidArgument(f"Rotary: axes are {r // 2} numbers from 0 to 3, one for each plane, got {axes}")
+            for i, x in enumerate(axes):
+                planes[i // 32] |= x << 2 * (i % 32)
+            count = max(axes, default=0) + 1
+        self.__dict__.update(frequencies=frequencies, interleaved=interleaved, scale=scale, rotary_dim=r, axes=axes,
+                             _planes=planes, _axes=count,
                              _desc=_abi.rotary_desc(frequencies.data_ptr(), r, interleaved, False, scale))
 
     @staticmethod
     def from_base(rotary_dim, base=10000.0, interleaved=False, scaling=None, factor=1.0, original_length=None,
-                  fast_turns=32.0, slow_turns=1.0, scale=None):
+                  fast_turns=32.0, slow_turns=1.0, scale=None, axes=None):
         """base^(-2 i / rotary_dim), for contexts `factor` times as long as trained on by
         `scaling`: "linear" (positions divided by factor), "ntk" (base * factor^(r / (r - 2)))
         or "yarn" (planes that turn fewer than `slow_turns` times over `original_length`
@@ -125,17 +138,37 @@ class Rotary(_Fixed):
             if scale is None:
                 scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
         return Rotary(f.to(torch.device("cuda", torch.cuda.current_device())), interleaved,
-                      1.0 if scale is None else scale)
+                      1.0 if scale is None else scale, axes)
+
+    @staticmethod
+    def axes_in_blocks(sizes):
+        """`axes` where the first sizes[0] planes turn by axis 0, the next sizes[1] by axis 1, and so on."""
+        return tuple(x for x, n in enumerate(sizes) for _ in range(n))
+
+    @staticmethod
+    def axes_in_turn(planes, axes):
+        """`axes` where plane i turns by axis i % axes."""
+        return tuple(i % axes for i in range(planes))
+
+    def _positions(self, positions, n, name):
+        """The descriptor of the axes for positions [axes, n]; None for [n] (one axis, or all alike)."""
+        if self.axes is None or not isinstance(positions, torch.Tensor) or positions.dim() != 2:
+            _indices(positions, torch.int64, 1, f"{name}: positions")
+            if positions.shape[0] != n:
+                raise InvalidArgument(f"{name}: {positions.shape[0]} positions for {n} rows")
+            return None
+        _indices(positions, torch.int64, 2, f"{name}: positions")
+        if positions.shape[0] < self._axes or positions.shape[1] != n:
+            raise InvalidArgument(f"{name}: positions are [{self._axes}, {n}], got {tuple(positions.shape)}")
+        return _abi.rotary_axes_desc(self._axes, positions.stride(0), *self._planes)
 
     def apply(self, q, k, positions, inverse=False):
-        """(q, k) [tokens, heads, head_dim] turned to int64 `positions` [tokens]; k may be None.
+        """(q, k) [tokens, heads, head_dim] turned to int64 `positions` [tokens] (or [axes, tokens]); k may be None.
         inverse: turned back (the transpose, which is the gradient's rotation)."""
         q, dq, code = _heads(q, "Rotary.apply: q")
         n, _, d = q.shape
         _device(self.frequencies, "Rotary: frequencies")
-        _indices(positions, torch.int64, 1, "Rotary.apply: positions")
-        if positions.shape[0] != n:
-            raise InvalidArgument(f"Rotary.apply: {positions.shape[0]} positions for {n} tokens")
+        axes = self._positions(positions, n, "Rotary.apply")
         qo = torch.empty_like(q, memory_format=torch.contiguous_format)
         ko = dk = ko_ptr = None
         if k is not None:
@@ -145,7 +178,11 @@ class Rotary(_Fixed):
         desc = self._desc
         if inverse:
             desc = _abi.rotary_desc(self.frequencies.data_ptr(), self.rotary_dim, self.interleaved, True, self.scale)
-        _abi.call("tq_rotary_apply", desc, positions.data_ptr(), n, dq, dk, code, d, qo.data_ptr(), ko_ptr, stream())
+        if axes is None:
+            _abi.call("tq_rotary_apply", desc, positions.data_ptr(), n, dq, dk, code, d, qo.data_ptr(), ko_ptr, stream())
+        else:
+            _abi.call("tq_rotary_apply_axes", desc, axes, positions.data_ptr(), n, dq, dk, code, d, qo.data_ptr(), ko_ptr,
+                      stream())
         return qo, ko
 
 
@@ -239,20 +276,21 @@ class KVCache(_Fixed):
 
     def write_rotary(self, q, k, v, rotary, new, positions=None):
         """The same with q [rows, query heads, head_dim] and k turned first; returns q turned.
-        positions: int64 [rows], or None for the rows' places in their sequences."""
+        positions: int64 [rows] (or [axes, rows]), or None for the rows' places in their sequences."""
         b = self._here(new)
         q, dq, code = _heads(q, "KVCache.write_rotary: q", None, new.rows, None, self.head_dim)
         k, dk, _ = _heads(k, "KVCache.write_rotary: k", q.dtype, new.rows, self.heads, self.head_dim)
         v, dv, _ = _heads(v, "KVCache.write_rotary: v", q.dtype, new.rows, self.heads, self.head_dim)
         _device(rotary.frequencies, "Rotary: frequencies")
-        if positions is not None:
-            _indices(positions, torch.int64, 1, "KVCache.write_rotary: positions")
-            if positions.shape[0] != new.rows:
-                raise InvalidArgument(f"KVCache.write_rotary: {positions.shape[0]} positions for {new.rows} rows")
+        axes = None if positions is None else rotary._positions(positions, new.rows, "KVCache.write_rotary")
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        _abi.call("tq_kv_write_rotary", self._ref, b, rotary._desc,
-                  None if positions is None else positions.data_ptr(), dq, dk,
-                  dv, code, out.data_ptr(), stream())
+        if axes is None:
+            _abi.call("tq_kv_write_rotary", self._ref, b, rotary._desc,
+                      None if positions is None else positions.data_ptr(), dq, dk,
+                      dv, code, out.data_ptr(), stream())
+        else:
+            _abi.call("tq_kv_write_rotary_axes", self._ref, b, rotary._desc, axes, positions.data_ptr(), dq, dk, dv, code,
+                      out.data_ptr(), stream())
         return out
 
     def read(self, new, dtype=torch.float32, out=None):
@@ -300,6 +338,30 @@ class KVCache(_Fixed):
                   1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), None if ws is None else ws.data_ptr(),
                   nb, out.data_ptr(), stream())
         return out
+
+    def keep(self, new, path, kept):
+        """What of the new tokens was verified (see `verify_drafts`) stays: row path[b, i] of sequence b moves to
+        the place of its i-th new token, for i < kept[b] (int32 [batch, n], ascending, and [batch]).  Returns the
+        lengths that the sequences then have (int32 [batch]).  A sequence whose path does not ascend inside its rows stays
+        as it is.  Pages that sequences share are copied first (PagePool.fork does)."""
+        b = self._here(new)
+        _indices(path, torch.int32, 2, "KVCache.keep: path")
+        _indices(kept, torch.int32, 1, "KVCache.keep: kept")
+        if path.shape[0] != new.batch or kept.shape[0] != new.batch:
+            raise InvalidArgument(f"KVCache.keep: paths {tuple(path.shape)} and kept {tuple(kept.shape)} of {new.batch} sequences")
+        lengths = torch.empty_like(kept)
+        _abi.call("tq_kv_keep", self._ref, b, path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(),
+                  lengths.data_ptr(), stream())
+        return lengths
+
+    def copy_pages(self, source, target):
+        """Page target[j] becomes a copy of page source[j] (int32 [n] each, as PagePool.fork gives them; pairs with a page
+        outside the cache are skipped).  A page is one pair's target and no pair's source."""
+        _indices(source, torch.int32, 1, "KVCache.copy_pages: source")
+        _indices(target, torch.int32, 1, "KVCache.copy_pages: target")
+        if source.shape != target.shape or self.device_index != source.get_device():
+            raise InvalidArgument(f"KVCache.copy_pages: {source.shape[0]} sources, {target.shape[0]} targets on the cache's device")
+        _abi.call("tq_kv_copy_pages", self._ref, source.data_ptr(), target.data_ptr(), source.shape[0], stream())
 
 
 def tree_mask(seen):
