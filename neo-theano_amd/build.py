@@ -36,7 +36,7 @@ HIP_FLAGS = [
 ]
 
 SOURCES = ["tq_api.hip", "tq_quant.hip", "tq_gemv.hip", "tq_decode_w4.hip", "tq_decode_tiled.hip", "tq_gemm.hip", "tq_gemm_w8.hip", "tq_mlp.hip", "tq_ffn.hip", "tq_generic.hip", "tq_convert.hip", "tq_attention.hip",
-           "tq_cache.hip", "tq_kv_attention.hip", "tq_gemm_block.hip", "tq_pages.hip", "tq_drafts.hip"]
+           "tq_cache.hip", "tq_kv_attention.hip", "tq_gemm_block.hip", "tq_pages.hip", "tq_drafts.hip", "tq_adapters.hip"]
 
 
 def _run(cmd):

@@ -10,6 +10,7 @@ QuantizedLinear, QuantizedMLP; quantized checkpoints (save_quantized /
 load_quantized over the safetensors container of crates/theano-serialize).
 """
 from ._tensor import convert
+from .adapters import Adapters
 from .cache import KVBatch, KVCache, Rotary, tree_mask
 from .checkpoint import load_quantized, load_safetensors, save_quantized, save_safetensors
 from .drafts import PagePool, verify_drafts
@@ -45,5 +46,5 @@ __all__ = [
     "quantize_i4_g128", "dequantize_i4_g128", "repack_i4_g128_tiled", "repack_i4_g128_gate_up_tiled", "tile_rows_for", "Module", "QuantizedLinear", "QuantizedMLP", "QuantizedMultiheadAttention",
     "save_safetensors", "load_safetensors", "save_quantized", "load_quantized", "convert",
     "quantize_fp8_block", "dequantize_fp8_block", "quantize_fp8_g128", "gemm_fp8_block",
-    "Rotary", "KVBatch", "KVCache", "tree_mask", "PagePool", "verify_drafts",
+    "Rotary", "KVBatch", "KVCache", "tree_mask", "PagePool", "verify_drafts", "Adapters",
 ]

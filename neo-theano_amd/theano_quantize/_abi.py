@@ -31,6 +31,7 @@ kv_cache_desc = struct.Struct("@PPPPqqqqi4x").pack       # tq_kv_cache: k, k_sca
 kv_batch_desc = struct.Struct("@PqqPPqqq").pack          # tq_kv_batch: table, table_stride, table_pages, lengths, offsets, batch,
 #                                                          max_tokens, tokens
 rotary_axes_desc = struct.Struct("@qqQQ").pack           # tq_rotary_axes: axes, position_stride, planes[2]
+adapters_desc = struct.Struct("@PPPqqqqqi4x").pack       # tq_adapters: a, b, scales, count, parts, rank, k, n, dtype
 page_pool_desc = struct.Struct("@Pqq").pack              # tq_page_pool: holders, pages, page
 
 
@@ -116,6 +117,8 @@ SIGNATURES = {
     "tq_kv_read": [_p, _p, _int, _p, _p, _p],
     "tq_kv_attention_workspace_bytes": [_p, _p, _i64],
     "tq_kv_attention": [_p, _p, _p, _int, _p, _i64, ctypes.c_float, _p, _i64, _p, _p],
+    "tq_adapters_workspace_bytes": [_p, _i64],
+    "tq_adapters_add": [_p, _p, _int, _i64, _p, _p, _p, _p, _i64, _p],
     "tq_verify_drafts_workspace_bytes": [_p, _i64],
     "tq_verify_drafts": [_p, _p, _p, _i64, _p, _i64, _int, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _p],
     "tq_kv_keep": [_p, _p, _p, _i64, _i64, _p, _p, _p],
@@ -133,6 +136,7 @@ _RESTYPE = {"tq_status_string": ctypes.c_char_p, "tq_last_error": ctypes.c_char_
             "tq_linear_w8a8_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w8a8_workspace_bytes": ctypes.c_int64, "tq_gemm_fp8_workspace_bytes": ctypes.c_int64,
             "tq_kv_attention_workspace_bytes": ctypes.c_int64, "tq_verify_drafts_workspace_bytes": ctypes.c_int64,
+            "tq_adapters_workspace_bytes": ctypes.c_int64,
             "tq_gemm_fp8_block_workspace_bytes": ctypes.c_int64, "tq_linear_fp8_block_workspace_bytes": ctypes.c_int64,
             "tq_gemm_w4g128_bf16_workspace_bytes": ctypes.c_int64, "tq_dtype_size": ctypes.c_int64}
 

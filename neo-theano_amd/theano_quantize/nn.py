@@ -67,8 +67,8 @@ class Module:
     def forward(self, x):
         raise NotImplementedError
 
-    def __call__(self, x):
-        return self.forward(x)
+    def __call__(self, *args, **kwargs):
+        return self.forward(*args, **kwargs)
 
     def parameters(self):
         return [t for _, t in self.named_parameters()]
@@ -167,7 +167,9 @@ class QuantizedLinear(Module):
         _abi.call(name, x.data_ptr(), m, self.qweight.data_ptr(), self.scales.data_ptr(), ptr(bias), n, k, ptr(ws), nb,
                   y.data_ptr(), st)
 
-    def forward(self, x):
+    def forward(self, x, adapters=None, index=None):
+        """y = x . dequant(W)^T + b for x [rows, in] or [in]; with Adapters and an index (int32 [rows]) each row's
+        adapter added, from the same x."""
         act = self._act_dtype()
         if self.mode == "fp8_block" and isinstance(x, torch.Tensor) and x.dtype in _ACT_TYPES:
             act = x.dtype
@@ -181,7 +183,10 @@ class QuantizedLinear(Module):
                 f"QuantizedLinear.forward: shape mismatch, expected [*, {self.in_features}], "
                 f"got {tuple(x.shape)}")
         m = x.shape[0]
-        y = x.new_empty((m, n), dtype=torch.float32)
+        if adapters is not None and (adapters.in_features != k or adapters.out_features != n or
+                                     not isinstance(index, torch.Tensor) or tuple(index.shape) != (m,)):
+            raise InvalidArgument(f"QuantizedLinear.forward: adapters of [{n}, {k}] take an index of {m} rows")
+        y, given = x.new_empty((m, n), dtype=torch.float32), x
         mode, st = self.mode, stream()
         if mode == "fp8_block":
             if x.device != self.qweight.device or x.device.index != torch._C._cuda_getDevice():
@@ -221,6 +226,8 @@ class QuantizedLinear(Module):
                 _abi.call("tq_fake_quantize_fp8_rowwise", ptr(x), m, k, ptr(qa), ptr(sa), ptr(xq), st)
                 x = xq
             self._run("tq_gemm_fp8_weight", x, m, y, st)
+        if adapters is not None:
+            adapters.add(given, index, y, out=y)
         return y.squeeze(0) if squeeze else y
 
 
@@ -395,24 +402,25 @@ class QuantizedMultiheadAttention(Module):
             o = self._attend(q, k, v, e, e, e, batch, seq, mask)
         return self.out_proj(self._act(o)).reshape(batch, seq, e)
 
-    def forward_cached(self, x, cache, new, rotary=None, positions=None, tree=None):
+    def forward_cached(self, x, cache, new, rotary=None, positions=None, tree=None, adapters=(None, None), index=None):
         """The layer over a KVCache, for the rows of a KVBatch: x [rows, embed_dim] (f32) is projected, q and k
         are turned (where a Rotary is given), k and v stored, and the rows attend to what the cache holds
-        of their sequences (causally, or as `tree` says).  Returns [rows, embed_dim]; rows behind the last sequence
+        of their sequences (causally, or as `tree` says).  adapters: those of the fused q, k and v projection (in 3 parts)
+        and those of the output's, either may be None, each row's given by `index`.  Returns [rows, embed_dim]; rows behind the last sequence
         hold anything."""
         x = on_device(x, torch.float32, "QuantizedMultiheadAttention.forward_cached")
         e, h, d = self.embed_dim, self.num_heads, self.head_dim
         if tuple(x.shape) != (new.rows, e) or cache.heads != h or cache.head_dim != d:
             raise InvalidArgument(f"QuantizedMultiheadAttention.forward_cached: x {tuple(x.shape)} for {new.rows} rows of {e}, "
                                   f"a cache of {cache.heads} heads of {cache.head_dim} for {h} of {d}")
-        qkv = self.qkv(self._act(x))
+        qkv = self.qkv(self._act(x), adapters[0], index)
         q, k, v = (qkv[:, i * e:(i + 1) * e].view(new.rows, h, d) for i in range(3))
         if rotary is None:
             cache.write(k, v, new)
         else:
             q = cache.write_rotary(q, k, v, rotary, new, positions)
         o = cache.attention(q, new, tree=tree).view(new.rows, e)
-        return self.out_proj(self._act(o))
+        return self.out_proj(self._act(o), adapters[1], index)
 
     def forward_qkv(self, query, key, value):
         return self.forward_with_mask(query, key, value, None)
