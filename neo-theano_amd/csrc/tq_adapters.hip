@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kBlock = 256, kWaves = 4;
 constexpr int kMaxRank = 256, kMaxParts = 16, kKUnit = 64;
+constexpr int kRowsOutputs = 64;  // of a wave's step where there are many rows
 constexpr int64_t kMaxRows = 1 << 30;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -248,25 +249,14 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
     }
 }
 
-// Wave (token tile, part, range of outputs): t of 16 kT tokens stays in registers as planes, outputs go by in tiles of 16;
-// up to kU distinct adapters' weights are loaded together.
-template <int kW, int kT, int kS, int kU, bool kVec>
-__global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
-    typedef Planes<TQ_DT_F32, kW> P;
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    int id = blockIdx.x * kWaves + (threadIdx.x >> 6);
-    const int tile = id % a.tiles;
-    id /= a.tiles;
-    const int p = id % a.parts, range = id / a.parts;
-    if (range >= a.ranges) return;
-    const int first = tile * 16 * kT, ranks = a.parts * a.rank, np = a.n / a.parts;
-    Distinct<kT> set(a.index, a.count, first, a.m, lane);
-    u32x4 tp[kT][kS][P::kOfX];
-    int64_t at[kT];
+// Planes of s_a t for the 16 kT tokens of a wave: the second operand of the second product, kept in registers.
+template <int kW, int kT, int kS>
+__device__ __forceinline__ void load_t(const AdaptArg& a, const Distinct<kT>& set, int first, int p,
+                                       u32x4 (&tp)[kT][kS][Planes<TQ_DT_F32, kW>::kOfX]) {
+    const int col = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4, ranks = a.parts * a.rank;
 #pragma unroll
     for (int s = 0; s < kT; ++s) {
         const int tok = min(first + 16 * s + col, a.m - 1);
-        at[s] = static_cast<int64_t>(tok) * a.n + static_cast<int64_t>(p) * np + 4 * quad;
         const float scale = set.mine[s] < 0 ? 0.f : a.scales ? a.scales[set.mine[s]] : 1.f;
 #pragma unroll
         for (int h = 0; h < kS; ++h) {
@@ -285,15 +275,67 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
                 v[i] = lo[i] * scale;
                 v[4 + i] = hi[i] * scale;
             }
-            cut8<P::kOfX>(v, tp[s][h]);
+            cut8(v, tp[s][h]);
         }
     }
-    const int end = min((range + 1) * a.per * 16, np);
-    for (int n0 = range * a.per * 16; n0 < end; n0 += 16) {
-        f32x4 y[kT], d[kT];
+}
+
+// What the wave's lanes wrote to LDS before is there for all of them (LDS serves a wave in order; the compiler has to
+// keep that order, too).
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Ranks of adapter `who` for output `row` of b: the first operand of the second product.
+template <int kS>
+__device__ __forceinline__ void load_b(const AdaptArg& a, int who, int64_t row, u32x4 (&raw)[kS]) {
+    const int quad = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int h = 0; h < kS; ++h) {
+        raw[h] = u32x4{0, 0, 0, 0};
+        if (who >= 0 && 32 * h + 8 * quad < a.rank)
+            raw[h] = *reinterpret_cast<const u32x4*>(a.b + (static_cast<int64_t>(who) * a.n + row) * a.rank + 32 * h + 8 * quad);
+    }
+}
+
+template <int kW, int kS>
+__device__ __forceinline__ f32x4 up_sums(const u32x4 (&raw)[kS], const u32x4 (&tp)[kS][Planes<TQ_DT_F32, kW>::kOfX]) {
+    typedef Planes<TQ_DT_F32, kW> P;
+    f32x4 v{0, 0, 0, 0};
+#pragma unroll
+    for (int h = 0; h < kS; ++h) {
+        u32x4 wp[P::kOfW];
+        planes_of_16(raw[h], wp);
+        v = products<false>(wp, tp[h], v);
+    }
+    return v;
+}
+
+// Few rows, and rows that no 16-byte access reaches.  Wave (token tile, part, range of outputs): outputs go by in tiles
+// of 16, 4 outputs of a token to a lane; up to kU distinct adapters' weights are loaded together, those of the
+// next tile before this one's sums.
+template <int kW, int kT, int kS, int kU, bool kVec>
+__global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    int id = blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int p = id % a.parts, range = id / a.parts;
+    if (range >= a.ranges) return;
+    const int first = tile * 16 * kT, np = a.n / a.parts, begin = range * a.per * 16, end = min(begin + a.per * 16, np);
+    Distinct<kT> set(a.index, a.count, first, a.m, lane);
+    int64_t at[kT];
+#pragma unroll
+    for (int s = 0; s < kT; ++s)
+        at[s] = static_cast<int64_t>(min(first + 16 * s + col, a.m - 1)) * a.n + static_cast<int64_t>(p) * np + 4 * quad;
+    auto row_of_b = [&](int n0) { return static_cast<int64_t>(p) * np + min(n0 + col, np - 1); };
+    f32x4 y[kT];
+    u32x4 raw[kU][kS];
+    int names[kU];
+    auto load = [&](int n0) {  // the tile's y, and its first kU adapters
 #pragma unroll
         for (int s = 0; s < kT; ++s) {
-            d[s] = f32x4{0, 0, 0, 0};
             if constexpr (kVec) {
                 y[s] = *reinterpret_cast<const f32x4*>(a.y + at[s] + min(n0, np - 4 - 4 * quad));
             } else {
@@ -301,64 +343,138 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
                 for (int i = 0; i < 4; ++i) y[s][i] = a.y[at[s] - 4 * quad + min(n0 + 4 * quad + i, np - 1)];
             }
         }
-        const int64_t brow = static_cast<int64_t>(p) * np + min(n0 + col, np - 1);
         set.restart();
-        for (int who; (who = set.next()) >= 0;) {
-            int names[kU];
-            names[0] = who;
 #pragma unroll
-            for (int i = 1; i < kU; ++i) names[i] = set.next();
-            u32x4 raw[kU][kS];
+        for (int i = 0; i < kU; ++i) {
+            names[i] = set.next();
+            load_b(a, names[i], row_of_b(n0), raw[i]);
+        }
+    };
+    load(begin);
+    u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
+    load_t<kW>(a, set, first, p, tp);
+    for (int n0 = begin; n0 < end; n0 += 16) {
+        f32x4 d[kT];
 #pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int h = 0; h < kS; ++h) {
-                    raw[i][h] = u32x4{0, 0, 0, 0};
-                    if (names[i] >= 0 && 32 * h + 8 * quad < a.rank)
-                        raw[i][h] = *reinterpret_cast<const u32x4*>(
-                            a.b + (static_cast<int64_t>(names[i]) * a.n + brow) * a.rank + 32 * h + 8 * quad);
-                }
+        for (int s = 0; s < kT; ++s) d[s] = f32x4{-0.f, -0.f, -0.f, -0.f};  // what leaves y as it is
+        while (true) {
 #pragma unroll
             for (int i = 0; i < kU; ++i) {
                 if (names[i] < 0) break;
-                u32x4 wp[kS][P::kOfW];
-#pragma unroll
-                for (int h = 0; h < kS; ++h) planes_of_16(raw[i][h], wp[h]);
 #pragma unroll
                 for (int s = 0; s < kT; ++s) {
                     const bool mine = set.mine[s] == names[i];
                     if (!__ballot(mine)) continue;
-                    f32x4 v{0, 0, 0, 0};
-#pragma unroll
-                    for (int h = 0; h < kS; ++h) v = products<false>(wp[h], tp[s][h], v);
+                    const f32x4 v = up_sums<kW>(raw[i], tp[s]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) d[s][e] = mine ? v[e] : d[s][e];
                 }
             }
+            names[0] = set.next();
+            if (names[0] < 0) break;
+#pragma unroll
+            for (int i = 1; i < kU; ++i) names[i] = set.next();
+#pragma unroll
+            for (int i = 0; i < kU; ++i) load_b(a, names[i], row_of_b(n0), raw[i]);
         }
+#pragma unroll
+        for (int s = 0; s < kT; ++s) d[s] += y[s];
+        if (n0 + 16 < end) load(n0 + 16);
 #pragma unroll
         for (int s = 0; s < kT; ++s) {
             if (first + 16 * s + col >= a.m) continue;
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = set.mine[s] < 0 ? y[s][e] : y[s][e] + d[s][e];
             if constexpr (kVec) {
-                if (n0 + 4 * quad < np) *reinterpret_cast<f32x4*>(a.out + at[s] + n0) = v;
+                if (n0 + 4 * quad < np) *reinterpret_cast<f32x4*>(a.out + at[s] + n0) = d[s];
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (n0 + 4 * quad + i < np) a.out[at[s] + n0 + i] = v[i];
+                    if (n0 + 4 * quad + i < np) a.out[at[s] + n0 + i] = d[s][i];
             }
         }
     }
 }
 
-// How a call is cut.  Few rows: tiles of 16 tokens, blocks of their own for a tile's distinct adapters.
+// Many rows.  Block (token tile, part, range of outputs), whose waves take 64 outputs each of 256 side by side: 16 kT tokens of a
+// wave.  The sums go through LDS (a wave's own part, no barrier) so that y is read and out written in runs of 256 bytes of a
+// row: the 64 bytes that a tile of the matrix instruction holds of one took 127 us where this takes 81 (4093 rows of 14336), with
+// stores that keep out of the caches (kStream: 106 us without), which then hold y and b.  y is on its way a step ahead.
+template <int kW, int kT, int kS, bool kStream>
+__global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
+    constexpr int kRows = 16 * kT, kY = kRows / 4, kStep = kRowsOutputs * kWaves;
+    __shared__ float sums[kWaves][kRows][kRowsOutputs + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    int id = blockIdx.x;
+    const int range = id % a.ranges;
+    id /= a.ranges;
+    const int p = id % a.parts, first = id / a.parts * kRows, np = a.n / a.parts;
+    const int begin = range * a.per * kStep, end = min(begin + a.per * kStep, np);
+    Distinct<kT> set(a.index, a.count, first, a.m, lane);
+    u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
+    load_t<kW>(a, set, first, p, tp);
+    // rows without an adapter: nothing is ever added
+#pragma unroll
+    for (int i = 0; i < kY; ++i) *reinterpret_cast<f32x4*>(&sums[wave][4 * i + quad][4 * col]) = f32x4{-0.f, -0.f, -0.f, -0.f};
+    auto place = [&](int i, int n) { return static_cast<int64_t>(min(first + 4 * i + quad, a.m - 1)) * a.n + static_cast<int64_t>(p) * np + n; };
+    auto load_y = [&](int n0, f32x4 (&y)[kY]) {
+        const int n = min(n0 + wave * kRowsOutputs + 4 * col, np - 4);
+#pragma unroll
+        for (int i = 0; i < kY; ++i) y[i] = *reinterpret_cast<const f32x4*>(a.y + place(i, n));
+    };
+    constexpr int kN = kRowsOutputs / 16;
+    u32x4 raw[kN][kS];
+    auto weights = [&](int who, int n0) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+            load_b(a, who, static_cast<int64_t>(p) * np + min(n0 + wave * kRowsOutputs + 16 * j + col, np - 1), raw[j]);
+    };
+    auto multiply = [&](int who) {
+#pragma unroll
+        for (int s = 0; s < kT; ++s) {
+            const bool mine = set.mine[s] == who;
+            if (!__ballot(mine)) continue;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const f32x4 v = up_sums<kW>(raw[j], tp[s]);
+                if (mine) *reinterpret_cast<f32x4*>(&sums[wave][16 * s + col][16 * j + 4 * quad]) = v;
+            }
+        }
+    };
+    auto step = [&](int n0, const f32x4 (&now)[kY], f32x4 (&next)[kY]) {
+        set.restart();
+        int who = set.next();
+        weights(who, n0);
+        load_y(n0 + kStep, next);
+        while (who >= 0) {
+            multiply(who);
+            if ((who = set.next()) >= 0) weights(who, n0);
+        }
+        wave_order();
+        const int n = n0 + wave * kRowsOutputs + 4 * col;
+#pragma unroll
+        for (int i = 0; i < kY; ++i) {
+            const f32x4 v = now[i] + *reinterpret_cast<const f32x4*>(&sums[wave][4 * i + quad][4 * col]);
+            if (first + 4 * i + quad >= a.m || n >= end) continue;
+            f32x4* to = reinterpret_cast<f32x4*>(a.out + place(i, n));
+            if constexpr (kStream) __builtin_nontemporal_store(v, to);
+            else *to = v;
+        }
+        wave_order();
+    };
+    f32x4 y[2][kY];
+    load_y(begin, y[0]);
+    for (int n0 = begin; n0 < end; n0 += 2 * kStep) {
+        step(n0, y[0], y[1]);
+        if (n0 + kStep < end) step(n0 + kStep, y[1], y[0]);
+    }
+}
+
+// How a call is cut.
 struct Cut {
     bool few;
     int low_tokens, low_ranks, slots, groups, splits, k_per;
-    int up_tokens;
 };
+
+// Up to this many rows tiles are of 16 tokens and a tile's distinct adapters have blocks of their own.
 constexpr int kFewRows = 256;
 
 Cut cut_of(const tq_adapters* a, int64_t m) {
@@ -371,11 +487,11 @@ Cut cut_of(const tq_adapters* a, int64_t m) {
     c.groups = static_cast<int>((rank_tiles + c.low_ranks - 1) / c.low_ranks);
     const int64_t units = (k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
     const int64_t blocks = (m + c.low_tokens - 1) / c.low_tokens * c.slots * c.groups;
-    const int64_t splits = std::max<int64_t>(1, std::min(units, 2 * device_cu_count() / std::max<int64_t>(1, blocks)));
+    // two blocks for each CU, four where there are many rows (4093 rows, rank 64: 38 us with one, 32 with two, 28 with four)
+    const int64_t splits = std::max<int64_t>(1, std::min(units, (c.few ? 2 : 4) * device_cu_count() / std::max<int64_t>(1, blocks)));
     const int64_t per = (units + splits - 1) / splits;
     c.k_per = static_cast<int>(per * kKUnit * kWaves);
     c.splits = static_cast<int>((units + per - 1) / per);
-    c.up_tokens = c.few || a->rank > 128 ? 16 : a->rank > 64 ? 32 : 64;
     return c;
 }
 
@@ -415,28 +531,72 @@ void launch_low_tokens(const AdaptArg& a, const Cut& c, bool vec, int64_t blocks
     else launch_low_ranks<kX, kW, 2>(a, c.low_ranks, vec, blocks, st);
 }
 
+int64_t blocks_of(const AdaptArg& a, int waves) {
+    return (static_cast<int64_t>(a.tiles) * a.parts * a.ranges + waves - 1) / waves;
+}
+
+// Tiles of 16 kT tokens, a wave each, ranges so that there are about sixteen waves for each CU.
 template <int kW, int kT, int kS, int kU>
-void launch_up(const AdaptArg& a, bool vec, int64_t blocks, hipStream_t st) {
+int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
+    const int64_t n_tiles = (a.n / a.parts + 15) / 16;
+    a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
+    const int64_t all = a.tiles * a.parts * n_tiles;
+    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(32, all / (16 * device_cu_count()))));
+    a.ranges = static_cast<int>((n_tiles + a.per - 1) / a.per);
+    const int64_t blocks = blocks_of(a, kWaves);
+    TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
     if (vec)
         k_adapt_up<kW, kT, kS, kU, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
     else
         k_adapt_up<kW, kT, kS, kU, false><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+    return check_launch(what);
+}
+
+// Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps of 16 output tiles, and about 9 tiles'
+// time for a block's start (4093 rows of 14336, rank 64: 80, 81 and 86 us with one, two and four blocks for each CU).
+template <int kW, int kT, int kS>
+int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
+    const int64_t np = a.n / a.parts, steps = (np + kRowsOutputs * kWaves - 1) / (kRowsOutputs * kWaves);
+    a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
+    const int64_t every = static_cast<int64_t>(a.tiles) * a.parts, cus = device_cu_count();
+    int64_t best = 0;
+    for (int64_t r = 1; r <= steps && r <= 64; ++r) {
+        const int64_t per = (steps + r - 1) / r, blocks = every * ((steps + per - 1) / per);
+        const int64_t cost = (blocks + cus - 1) / cus * (16 * per + 9);
+        if (best == 0 || cost < best) {
+            best = cost;
+            a.per = static_cast<int>(per);
+        }
+    }
+    a.ranges = static_cast<int>((steps + a.per - 1) / a.per);
+    const int64_t blocks = blocks_of(a, 1);
+    TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
+    // outputs that the L2 caches (4 MB for each XCD) would not hold anyway
+    if (static_cast<int64_t>(a.m) * a.n * 4 >= int64_t(32) << 20)
+        k_adapt_up_rows<kW, kT, kS, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+    else
+        k_adapt_up_rows<kW, kT, kS, false><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+    return check_launch(what);
 }
 
 template <int kW>
-int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool vec_y, int64_t low, int64_t up, hipStream_t st,
-                 const char* what) {
+int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool vec_y, int64_t low, hipStream_t st, const char* what) {
     clear_error();
     if (dtype == TQ_DT_F32) launch_low_tokens<TQ_DT_F32, kW>(a, c, vec_x, low, st);
     else if (dtype == TQ_DT_BF16) launch_low_tokens<TQ_DT_BF16, kW>(a, c, vec_x, low, st);
     else launch_low_tokens<TQ_DT_F16, kW>(a, c, vec_x, low, st);
     const int rc = check_launch(what);
     if (rc != TQ_OK) return rc;
-    if (a.rank > 128) launch_up<kW, 1, 8, 1>(a, vec_y, up, st);
-    else if (a.rank > 64) c.few ? launch_up<kW, 1, 4, 2>(a, vec_y, up, st) : launch_up<kW, 2, 4, 1>(a, vec_y, up, st);
-    else if (a.rank > 32) c.few ? launch_up<kW, 1, 2, 4>(a, vec_y, up, st) : launch_up<kW, 4, 2, 1>(a, vec_y, up, st);
-    else c.few ? launch_up<kW, 1, 1, 4>(a, vec_y, up, st) : launch_up<kW, 4, 1, 1>(a, vec_y, up, st);
-    return check_launch(what);
+    if (!c.few && vec_y) {
+        if (a.rank > 128) return launch_up_rows<kW, 1, 8>(a, st, what);
+        if (a.rank > 64) return launch_up_rows<kW, 1, 4>(a, st, what);
+        if (a.rank > 32) return launch_up_rows<kW, 2, 2>(a, st, what);
+        return launch_up_rows<kW, 2, 1>(a, st, what);
+    }
+    if (a.rank > 128) return launch_up<kW, 1, 8, 1>(a, vec_y, st, what);
+    if (a.rank > 64) return launch_up<kW, 1, 4, 2>(a, vec_y, st, what);
+    if (a.rank > 32) return launch_up<kW, 1, 2, 4>(a, vec_y, st, what);
+    return launch_up<kW, 1, 1, 4>(a, vec_y, st, what);
 }
 
 }  // namespace
@@ -487,19 +647,11 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.slots = c.slots;
     a.groups = c.groups;
     const int64_t low = (m + c.low_tokens - 1) / c.low_tokens * c.slots * c.groups * c.splits;
-    const int64_t np = adapters->n / adapters->parts, n_tiles = (np + 15) / 16;
-    a.tiles = static_cast<int>((m + c.up_tokens - 1) / c.up_tokens);
-    // about sixteen waves for each CU, of at most 32 tiles each
-    const int64_t waves = 16 * device_cu_count(), every = a.tiles * adapters->parts;
-    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(32, every * n_tiles / waves)));
-    a.ranges = static_cast<int>((n_tiles + a.per - 1) / a.per);
-    const int64_t up = (every * a.ranges + kWaves - 1) / kWaves;
-    TQ_REQUIRE(low <= kMaxBlocks && up <= kMaxBlocks, "%s: %lld tokens are more than %lld blocks", what, (long long)m,
-               (long long)kMaxBlocks);
+    TQ_REQUIRE(low <= kMaxBlocks, "%s: %lld tokens are more than %lld blocks", what, (long long)m, (long long)kMaxBlocks);
     const bool vec_x = aligned(x, 16) && adapters->k % 8 == 0;
-    const bool vec_y = aligned(y, 16) && aligned(out, 16) && adapters->n % 4 == 0 && np % 4 == 0;
-    return adapters->dtype == TQ_DT_F16 ? launch_typed<TQ_DT_F16>(a, c, dtype, vec_x, vec_y, low, up, as_hip(stream), what)
-                                        : launch_typed<TQ_DT_BF16>(a, c, dtype, vec_x, vec_y, low, up, as_hip(stream), what);
+    const bool vec_y = aligned(y, 16) && aligned(out, 16) && adapters->n / adapters->parts % 4 == 0;
+    return adapters->dtype == TQ_DT_F16 ? launch_typed<TQ_DT_F16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what)
+                                        : launch_typed<TQ_DT_BF16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what);
 }
 
 }  // extern "C"

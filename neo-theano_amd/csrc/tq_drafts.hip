@@ -10,8 +10,9 @@
 //
 // Everything is compared and summed in f64 (the running sum is compared with a number next to a border).
 // The bytes are one row of p (and of q) for a sequence; what costs is the chain of dependent loads
-// (token -> its probability -> the row -> the sums -> the chosen share), so a row is cut into shares that
-// blocks sum side by side, and a second launch picks the share and looks into it again.
+// (token -> its probability -> the row -> the sums -> the chosen ones), so a row is cut into shares that blocks
+// sum side by side, a sum for each 256 probabilities (a wave's load), and a second launch picks one of these sums and looks into
+// its 256 again.
 #include <algorithm>
 
 #include "tq_kv.h"
@@ -22,6 +23,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kWalkBlock = 1024;
 constexpr int kMaxShare = 8192;  // probabilities of a share
+constexpr int kSegment = 256;    // of a sum: four for each lane of a wave
 
 template <int kType>
 struct Prob;
@@ -60,7 +62,7 @@ struct DraftArg {
     int32_t* kept;
     int64_t* next;
     State* state;   // [batch]
-    double* sums;   // [batch, shares]
+    double* sums;   // [batch, segments], segments = shares * share / kSegment
 };
 
 struct Span {
@@ -165,11 +167,28 @@ __device__ __forceinline__ State walk(const DraftArg& a, Span s, int32_t* path, 
     return st;
 }
 
+// Sum over a wave, the same in every lane.
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Running sums over a wave, the lane's own among them.
+__device__ __forceinline__ double wave_running(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double y = __shfl_up(v, d);
+        if (lane >= d) v += y;
+    }
+    return v;
+}
+
 // Sums of f64 over a block, the same in every thread (and in every call: a fixed order).
 template <int kThreads>
 __device__ __forceinline__ double block_sum(double v, double* lds) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    v = wave_sum64(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0.0;
@@ -204,14 +223,24 @@ __device__ __forceinline__ void left4(const T* p, const T* q, double a, int i, i
     for (int e = 0; e < 4; ++e) v[e] = gone >> e & 1 ? 0.0 : left_of(x[e], y[e], a);
 }
 
-// Sum of what is left over the whole row, by one block.
+// Sum of what is left over the whole row, by one block; eight loads of a lane in flight (a block alone at work is bound
+// by their latency: 128256 f32 probabilities of two models took 12 us with two).
 template <class T, bool kVec, int kThreads>
 __device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int vocab, double* lds) {
+    constexpr int kU = 4;
     double s = 0.0;
-    for (int i = 4 * static_cast<int>(threadIdx.x); i < vocab; i += 4 * kThreads) {
-        double v[4];
-        left4<T, kVec>(p, q, a, i, vocab, 0, v);
-        s += (v[0] + v[1]) + (v[2] + v[3]);
+    for (int i0 = 4 * static_cast<int>(threadIdx.x); i0 < vocab; i0 += 4 * kThreads * kU) {
+        double x[kU][4], y[kU][4];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            load4<T, kVec>(p, i0 + 4 * kThreads * u, vocab, x[u]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[u][e] = 0.0;
+            if (q) load4<T, kVec>(q, i0 + 4 * kThreads * u, vocab, y[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+            s += (left_of(x[u][0], y[u][0], a) + left_of(x[u][1], y[u][1], a)) + (left_of(x[u][2], y[u][2], a) + left_of(x[u][3], y[u][3], a));
     }
     return block_sum<kThreads>(s, lds);
 }
@@ -244,11 +273,10 @@ __device__ __forceinline__ void mark_tried(const DraftArg& a, Span s, int node, 
     }
 }
 
-// Block (share, sequence): the sum of what is left of a share.  kWalked: k_walk was there; otherwise every block
+// Block (share, sequence): the sums of what is left of a share.  kWalked: k_walk was there; otherwise every block
 // walks (a few dependent loads) and the first share's block writes the path down.
 template <class T, bool kVec, bool kWalked>
 __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
-    __shared__ double lds[kBlock / 64];
     __shared__ State shared;
     __shared__ uint32_t gone[kMaxShare / 32];
     const int seq = blockIdx.x / a.shares, share = blockIdx.x - seq * a.shares, begin = share * a.share;
@@ -276,44 +304,34 @@ __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     const T* p = row_of<T>(a.target, a.target_stride, s.first + st.node);
     const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
     const int end = min(begin + a.share, a.vocab);
-    double sum = 0.0;
-    for (int i = begin + 4 * static_cast<int>(threadIdx.x); i < end; i += 4 * kBlock) {
+    double* sums = a.sums + (static_cast<int64_t>(seq) * a.shares + share) * (a.share / kSegment);
+    for (int i = begin + 4 * static_cast<int>(threadIdx.x); i < begin + a.share; i += 4 * kBlock) {
         double v[4];
         left4<T, kVec>(p, q, st.a, i, end, a.draft ? 0 : gone[(i - begin) / 32] >> ((i - begin) & 31), v);
-        sum += (v[0] + v[1]) + (v[2] + v[3]);
+        const double sum = wave_sum64((v[0] + v[1]) + (v[2] + v[3]));
+        if ((threadIdx.x & 63) == 0) sums[(i - begin) / kSegment] = sum;
     }
-    sum = block_sum<kBlock>(sum, lds);
-    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(seq) * a.shares + share] = sum;
 }
 
-// Running sums of v over a block's threads, this thread's own among them.
-template <int kThreads>
-__device__ __forceinline__ double block_running(double v, double* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double y = __shfl_up(v, d);
-        if (lane >= d) v += y;
-    }
-    if (lane == 63) lds[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) before += w < wave ? lds[w] : 0.0;
-    __syncthreads();
-    return before + v;
-}
+constexpr int kPickEach = 4;  // sums of a lane: 1024, of 262144 probabilities, in one round
 
-// A block for each sequence: the share where the running sum passes final * total, then the token in it.
+// A block for each sequence: the segment where the running sum passes final * total, then the token in it.
 template <class T, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
     __shared__ double lds[kBlock / 64];
-    __shared__ uint32_t gone[kMaxShare / 32];
-    __shared__ int first_over, last_some;
     __shared__ double before_it;
-    const int seq = blockIdx.x, tid = threadIdx.x;
+    __shared__ int chosen_one;
+    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Span s = span_of(a, seq);
     const State st = a.state[seq];
+    const int segments = a.shares * (a.share / kSegment);
+    const double* sums = a.sums + static_cast<int64_t>(seq) * segments;
+    double v[kPickEach];
+    auto load = [&](int c0) {
+#pragma unroll
+        for (int e = 0; e < kPickEach; ++e) v[e] = c0 + tid * kPickEach + e < segments ? sums[c0 + tid * kPickEach + e] : 0.0;
+    };
+    load(0);  // (where there are no rows what lies there is not used)
     int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
     for (int i = st.kept + tid; i < a.max_tokens; i += kBlock) path[i] = -1;
     if (tid == 0) a.kept[seq] = st.kept;
@@ -321,97 +339,135 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
         if (tid == 0) a.next[seq] = -1;
         return;
     }
-    const double* sums = a.sums + static_cast<int64_t>(seq) * a.shares;
-    double share_of_q = st.a, total = 0.0;
-    bool tried = !a.draft;
-    for (int i = tid; i < a.shares; i += kBlock) total += sums[i];
-    total = block_sum<kBlock>(total, lds);
     const T* p = row_of<T>(a.target, a.target_stride, s.first + st.node);
     const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
-    // nothing left: the target's own probabilities, share by share (not on the way of any sound input)
+    double share_of_q = st.a, total = 0.0;
+    bool tried = !a.draft;
+    for (int c0 = 0; c0 < segments; c0 += kBlock * kPickEach) {
+        if (c0) load(c0);
+        total += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    total = block_sum<kBlock>(total, lds);
+    // nothing left: the target's own probabilities, summed here segment by segment (on the way of no sound input)
     const bool own = !(total > 0.0);
     if (own) {
         q = nullptr;
         share_of_q = 0.0;
         tried = false;
-        total = row_mass<T, kVec, kBlock>(p, q, 0.0, a.vocab, lds);
-    }
-    if (!(total > 0.0)) {
-        if (tid == 0) a.next[seq] = -1;
-        return;
+        total = row_mass<T, kVec, kBlock>(p, nullptr, 0.0, a.vocab, lds);
+        if (!(total > 0.0)) {
+            if (tid == 0) a.next[seq] = -1;
+            return;
+        }
     }
     const double goal = static_cast<double>(a.final[seq]) * total;
-    // (the share loop below reads sums of shares, or, in the rare case, sums the share itself)
+    if (tid == 0) chosen_one = -1;
     double base = 0.0;
-    int chosen = -1, some = -1;
-    double chosen_before = 0.0, some_before = 0.0;
-    for (int c0 = 0; c0 < a.shares && chosen < 0; c0 += kBlock) {
-        double v = 0.0;
-        if (!own) {
-            v = c0 + tid < a.shares ? sums[c0 + tid] : 0.0;
-        } else if (c0 + tid < a.shares) {
-            const int b0 = (c0 + tid) * a.share, b1 = min(b0 + a.share, a.vocab);
-            for (int i = b0; i < b1; ++i) v += left_of(static_cast<double>(static_cast<float>(p[i])), 0.0, 0.0);
-        }
-        if (tid == 0) {
-            first_over = INT32_MAX;
-            last_some = -1;
-        }
-        const double run = block_running<kBlock>(v, lds) + base;
-        if (v > 0.0) {
-            if (run > goal) atomicMin(&first_over, tid);
-            atomicMax(&last_some, tid);
-        }
-        __syncthreads();
-        const int over = first_over, last = last_some;
-        if (tid == (over != INT32_MAX ? over : last)) before_it = run - v;
-        __syncthreads();
-        if (over != INT32_MAX) {
-            chosen = c0 + over;
-            chosen_before = before_it;
-        } else if (last >= 0) {
-            some = c0 + last;
-            some_before = before_it;
-        }
-        base += block_sum<kBlock>(v, lds);
-    }
-    if (chosen < 0) {  // (roundings, or sums that are not finite: the last share that has anything)
-        chosen = some;
-        chosen_before = some_before;
-    }
-    if (chosen < 0) {
-        if (tid == 0) a.next[seq] = -1;
-        return;
-    }
-    const int begin = chosen * a.share, end = min(begin + a.share, a.vocab);
-    for (int i = tid; i < a.share / 32; i += kBlock) gone[i] = 0;
-    __syncthreads();
-    if (tried) mark_tried(a, s, st.node, begin, gone, kBlock);
-    if (tid == 0) {
-        first_over = INT32_MAX;
-        last_some = -1;
-    }
-    __syncthreads();
-    base = chosen_before;
-    for (int i0 = begin; i0 < end; i0 += 4 * kBlock) {
-        const int i = i0 + 4 * tid;
-        double v[4] = {0, 0, 0, 0};
-        if (i < end) left4<T, kVec>(p, q, share_of_q, i, end, gone[(i - begin) / 32] >> ((i - begin) & 31), v);
-        const double mine = (v[0] + v[1]) + (v[2] + v[3]);
-        double run = block_running<kBlock>(mine, lds) - mine + base;
+    for (int c0 = 0; c0 < segments; c0 += kBlock * kPickEach) {
+        if (own) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            run += v[e];
+            for (int e = 0; e < kPickEach; ++e) {
+                const int b0 = (c0 + tid * kPickEach + e) * kSegment, b1 = min(b0 + kSegment, a.vocab);
+                v[e] = 0.0;
+                for (int i = b0; i < b1; ++i) v[e] += left_of(static_cast<double>(static_cast<float>(p[i])), 0.0, 0.0);
+            }
+        } else if (segments > kBlock * kPickEach) {
+            load(c0);
+        }
+        const double mine = (v[0] + v[1]) + (v[2] + v[3]), run = wave_running(mine);
+        if (lane == 63) lds[wave] = run;
+        __syncthreads();
+        double before = base + (run - mine);
+        for (int w = 0; w < wave; ++w) before += lds[w];
+        for (int w = 0; w < kBlock / 64; ++w) base += lds[w];
+        // the first segment that passes the goal, and the last that has anything (roundings, or sums that are not finite,
+        // may let none pass); a wave's first and last lane that have one put it down
+        int over = -1, some = -1;
+        double over_before = 0.0, some_before = 0.0;
+#pragma unroll
+        for (int e = 0; e < kPickEach; ++e) {
             if (v[e] > 0.0) {
-                if (run > goal) atomicMin(&first_over, i + e);
-                atomicMax(&last_some, i + e);
+                some = c0 + tid * kPickEach + e;
+                some_before = before;
+                if (over < 0 && before + v[e] > goal) {
+                    over = some;
+                    over_before = before;
+                }
+            }
+            before += v[e];
+        }
+        __shared__ int firsts[kBlock / 64], lasts[kBlock / 64];
+        __shared__ double first_before[kBlock / 64], last_before[kBlock / 64];
+        const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+        if (lane == 0) firsts[wave] = lasts[wave] = -1;
+        if (overs && lane == __ffsll(static_cast<unsigned long long>(overs)) - 1) {
+            firsts[wave] = over;
+            first_before[wave] = over_before;
+        }
+        if (somes && lane == 63 - __clzll(static_cast<long long>(somes))) {
+            lasts[wave] = some;
+            last_before[wave] = some_before;
+        }
+        __syncthreads();
+        bool passed = false;
+        int which = -1;
+        double at_it = 0.0;
+        for (int w = 0; w < kBlock / 64; ++w) {
+            if (lasts[w] >= 0 && !passed) {
+                which = lasts[w];
+                at_it = last_before[w];
+            }
+            if (firsts[w] >= 0 && !passed) {
+                passed = true;
+                which = firsts[w];
+                at_it = first_before[w];
             }
         }
+        if (tid == 0 && which >= 0) {
+            chosen_one = which;
+            before_it = at_it;
+        }
+        if (passed) break;
         __syncthreads();
-        if (first_over != INT32_MAX) break;
-        base += block_sum<kBlock>(mine, lds);
     }
-    if (tid == 0) a.next[seq] = first_over != INT32_MAX ? first_over : last_some;
+    __syncthreads();
+    if (wave != 0) return;
+    const int chosen = chosen_one;
+    if (chosen < 0) {
+        if (lane == 0) a.next[seq] = -1;
+        return;
+    }
+    const int i = chosen * kSegment + 4 * lane, end = min(chosen * kSegment + kSegment, a.vocab);
+    uint32_t gone = 0;
+    if (tried) {
+        for (int t0 = st.node + 1; t0 < s.count; t0 += 64) {
+            const int t = t0 + lane;
+            const bool child = t < s.count && (a.parents ? a.parents[s.first + t] == st.node : t == st.node + 1);
+            const int64_t x = child ? a.tokens[s.first + t] - chosen * static_cast<int64_t>(kSegment) : -1;
+            const int inside = x >= 0 && x < kSegment ? static_cast<int>(x) : -1;
+            for (uint64_t those = __ballot(inside >= 0); those; those &= those - 1) {
+                const int gone_one = readlane(inside, __ffsll(static_cast<unsigned long long>(those)) - 1);
+                if (gone_one >> 2 == lane) gone |= 1u << (gone_one & 3);
+            }
+        }
+    }
+    double left[4];
+    left4<T, kVec>(p, q, share_of_q, i, end, gone, left);
+    const double mine = (left[0] + left[1]) + (left[2] + left[3]);
+    double run = before_it + (wave_running(mine) - mine);
+    int over = -1, some = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        run += left[e];
+        if (left[e] > 0.0) {
+            some = i + e;
+            if (over < 0 && run > goal) over = i + e;
+        }
+    }
+    const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+    const int l = overs ? __ffsll(static_cast<unsigned long long>(overs)) - 1 : somes ? 63 - __clzll(static_cast<long long>(somes)) : 0;
+    const int token = overs ? over : some;
+    if (lane == l) a.next[seq] = token;
 }
 
 // Probabilities of a share: so that all shares are about two blocks for each CU, at least 1024 (a load for each
@@ -471,7 +527,8 @@ extern "C" {
 int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab) {
     using namespace tq;
     if (check_batch("tq_verify_drafts", batch, vocab) != TQ_OK) return -1;
-    return (batch->batch * static_cast<int64_t>(sizeof(State)) + batch->batch * shares_of(vocab, batch->batch) * 8 + 15) / 16 * 16;
+    return (batch->batch * static_cast<int64_t>(sizeof(State)) + batch->batch * shares_of(vocab, batch->batch) * (share_of(vocab, batch->batch) / kSegment) * 8 +
+            15) / 16 * 16;
 }
 
 int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void* target, int64_t target_stride,

@@ -160,10 +160,13 @@ __device__ __forceinline__ int scan_wants(int* prefix, int n, int pages, ScanLds
     return static_cast<int>(min(given, static_cast<int64_t>(pages)));
 }
 
-// Hands out the `total` lowest free pages: assign(rank, page), ranks ascending with pages.  One block.
+constexpr int kEach = 8;  // pages of a lane: 8192 holders looked at in one round of loads
+
+// Hands out the `total` lowest free pages: assign(rank, page), ranks ascending with pages, a lane for each of them
+// (a lane that handed out those that it finds would work through neighbours one by one: 12 against 7 us for 64 pages).
+// list: kPoolBlock * kEach places in LDS.  One block.
 template <class Assign>
-__device__ __forceinline__ void take_pages(const PoolArg& p, int total, ScanLds& lds, Assign assign) {
-    constexpr int kEach = 16;  // pages of a lane: 16384 holders looked at in one round of loads
+__device__ __forceinline__ void take_pages(const PoolArg& p, int total, ScanLds& lds, uint16_t* list, Assign assign) {
     int given = 0;
     for (int64_t base = 0; base < p.pages && given < total; base += kPoolBlock * kEach) {
         const int64_t mine = base + threadIdx.x * kEach;
@@ -179,13 +182,17 @@ __device__ __forceinline__ void take_pages(const PoolArg& p, int total, ScanLds&
                 if (mine + i < p.pages && p.holders[mine + i] <= 0) free |= 1u << i;
         }
         int64_t all;
-        int64_t rank = given + block_scan(__popc(free), lds, all);
-        for (; free && rank < total; free &= free - 1, ++rank) {
-            const int page = static_cast<int>(mine) + __ffs(free) - 1;
+        int place = static_cast<int>(block_scan(__popc(free), lds, all));
+        for (; free; free &= free - 1) list[place++] = static_cast<uint16_t>(threadIdx.x * kEach + __ffs(free) - 1);
+        __syncthreads();
+        const int count = min(static_cast<int>(all), total - given);
+        for (int i = threadIdx.x; i < count; i += kPoolBlock) {
+            const int page = static_cast<int>(base) + list[i];
             atomicAdd(p.holders + page, 1);
-            assign(static_cast<int>(rank), page);
+            assign(given + i, page);
         }
-        given += static_cast<int>(all);
+        given += count;
+        __syncthreads();
     }
 }
 
@@ -215,6 +222,7 @@ __device__ __forceinline__ int pages_of(int length, int page, int table_pages) {
 
 __global__ __launch_bounds__(kPoolBlock) void k_grow(GrowArg a) {
     __shared__ int want[kPoolSequences], have[kPoolSequences];
+    __shared__ uint16_t list[kPoolBlock * kEach];
     __shared__ ScanLds lds;
     const int lane = threadIdx.x & 63;
     for (int b = threadIdx.x >> 6; b < a.batch; b += kPoolBlock / 64) {
@@ -236,7 +244,7 @@ __global__ __launch_bounds__(kPoolBlock) void k_grow(GrowArg a) {
     }
     __syncthreads();
     const int total = scan_wants(want, a.batch, a.pool.pages, lds);
-    take_pages(a.pool, total, lds, [&](int rank, int page) {
+    take_pages(a.pool, total, lds, list, [&](int rank, int page) {
         const int b = owner(want, a.batch, rank);
         a.table[b * a.stride + have[b] + (rank - want[b])] = page;
     });
@@ -257,7 +265,8 @@ struct ForkArg {
 // Block 0 takes a page for each child whose parent has begun one; the others share the whole pages.  Sharing
 // only raises counts of pages that are held, so the free ones are the same for block 0 whenever it looks.
 __global__ __launch_bounds__(kPoolBlock) void k_fork(ForkArg a) {
-    __shared__ int want[kPoolSequences];
+    __shared__ int want[kPoolSequences], begins[kPoolSequences];
+    __shared__ uint16_t list[kPoolBlock * kEach];
     __shared__ ScanLds lds;
     auto begun = [&](int c, int& whole) {  // the page that child c's parent has begun, or -1
         const int p = a.parents[c];
@@ -274,19 +283,21 @@ __global__ __launch_bounds__(kPoolBlock) void k_fork(ForkArg a) {
             int whole;
             const int page = begun(c, whole);
             want[c] = page >= 0;
-            a.source[c] = -1;
+            begins[c] = whole;
+            a.source[c] = page;  // (where no page is left: -1 again below)
             a.target[c] = -1;
             if (whole < a.table_pages) a.out[static_cast<int64_t>(c) * a.table_pages + whole] = -1;
         }
         __syncthreads();  // (the writes above too: assign below writes the same places)
         const int total = scan_wants(want, a.children, a.pool.pages, lds);
-        take_pages(a.pool, total, lds, [&](int rank, int page) {
+        take_pages(a.pool, total, lds, list, [&](int rank, int page) {
             const int c = owner(want, a.children, rank);
-            int whole;
-            a.source[c] = begun(c, whole);
             a.target[c] = page;
-            a.out[static_cast<int64_t>(c) * a.table_pages + whole] = page;
+            a.out[static_cast<int64_t>(c) * a.table_pages + begins[c]] = page;
         });
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.children; c += kPoolBlock)
+            if (a.target[c] < 0) a.source[c] = -1;
         return;
     }
     const int64_t all = static_cast<int64_t>(a.children) * a.table_pages, step = static_cast<int64_t>(gridDim.x - 1) * kPoolBlock;
