@@ -22,7 +22,8 @@ namespace {
 
 constexpr int kBlock = 256, kWaves = 4;
 constexpr int kMaxRank = 256, kMaxParts = 16, kKUnit = 64;
-constexpr int kRowsOutputs = 64;  // of a wave's step where there are many rows
+constexpr int kMaxSplits = 8;  // shares of K that the second product adds
+constexpr int kStep = 256;  // outputs of a block's step where there are many rows
 constexpr int64_t kMaxRows = 1 << 30;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -77,40 +78,55 @@ __device__ __forceinline__ void planes_of_16(u32x4 raw, u32x4 (&out)[kN]) {
     }
 }
 
-// Elements k .. k + 7 of a row of x of `n`, zeros from n on (n is not 0).
-template <int kX, bool kVec, int kN>
-__device__ __forceinline__ void load_x(const void* row, int k, int n, u32x4 (&out)[kN]) {
+// Eight neighbours of a row of x as they are loaded: f32, or 16-bit values (in both words of `v`, the second unused).
+template <int kX>
+struct Raw8 {
+    f32x4 v[kX == TQ_DT_F32 ? 2 : 1];
+};
+
+// Elements k .. k + 7 of a row of n > 0; what lies past it is any element of the row, see planes_of.
+template <int kX, bool kVec>
+__device__ __forceinline__ Raw8<kX> fetch(const void* row, int k, int n) {
+    Raw8<kX> r;
     if constexpr (kX == TQ_DT_F32) {
         const float* p = static_cast<const float*>(row);
-        float v[8];
         if constexpr (kVec) {  // rows 16-byte aligned, n a multiple of 8
             const int at = min(k, n - 8);
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(p + at), hi = *reinterpret_cast<const f32x4*>(p + at + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = k < n ? lo[i] : 0.f;
-                v[4 + i] = k < n ? hi[i] : 0.f;
-            }
+            r.v[0] = *reinterpret_cast<const f32x4*>(p + at);
+            r.v[1] = *reinterpret_cast<const f32x4*>(p + at + 4);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = p[min(k + i, n - 1)];
-                v[i] = k + i < n ? x : 0.f;
-            }
+            for (int i = 0; i < 8; ++i) r.v[i / 4][i % 4] = p[min(k + i, n - 1)];
         }
-        cut8<kN>(v, out);
     } else {
         const uint16_t* p = static_cast<const uint16_t*>(row);
-        u32x4 raw;
         if constexpr (kVec) {
-            raw = *reinterpret_cast<const u32x4*>(p + min(k, n - 8));
-            if (k >= n) raw = u32x4{0, 0, 0, 0};
+            r.v[0] = *reinterpret_cast<const f32x4*>(p + min(k, n - 8));
         } else {
+            u32x4 raw;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t lo = p[min(k + 2 * i, n - 1)], hi = p[min(k + 2 * i + 1, n - 1)];
-                raw[i] = (k + 2 * i < n ? lo : 0) | (k + 2 * i + 1 < n ? hi << 16 : 0);
-            }
+            for (int i = 0; i < 4; ++i)
+                raw[i] = p[min(k + 2 * i, n - 1)] | static_cast<uint32_t>(p[min(k + 2 * i + 1, n - 1)]) << 16;
+            r.v[0] = __builtin_bit_cast(f32x4, raw);
+        }
+    }
+    return r;
+}
+
+// Their planes, zeros for elements from n on.
+template <int kX, bool kVec, int kN>
+__device__ __forceinline__ void planes_of(const Raw8<kX>& r, int k, int n, u32x4 (&out)[kN]) {
+    if constexpr (kX == TQ_DT_F32) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (kVec ? k : k + i) < n ? r.v[i / 4][i % 4] : 0.f;
+        cut8<kN>(v, out);
+    } else {
+        u32x4 raw = __builtin_bit_cast(u32x4, r.v[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kVec) raw[i] = k < n ? raw[i] : 0;
+            else raw[i] &= (k + 2 * i < n ? 0xFFFFu : 0) | (k + 2 * i + 1 < n ? 0xFFFF0000u : 0);
         }
         planes_of_16<kN>(raw, out);
     }
@@ -171,12 +187,12 @@ struct AdaptArg {
     int m, k, k_row, n, count, parts, rank;
     int splits, k_per;        // K of a block of the first product
     int slots, groups;        // first product: blocks for a tile's distinct adapters, and for its ranks
-    int ranges, per, tiles;   // second product: ranges of `per` 16-output tiles, and 16 kT-token tiles
+    int ranges, per, tiles;   // second product: ranges of `per` turns of a block's waves, and token tiles
 };
 
 // Block (token tile, rank group, slot, split): 16 kT tokens, 16 kR ranks, every slots-th distinct adapter.  The
-// waves take 64 of K in turn; a lane holds 16 neighbours of K (two steps of the matrix instruction, whose order of K is
-// free), so that a rank's 128 bytes and a token's 128 or 256 are read whole.
+// waves take 64 of K in turn, a rank's 64 and a token's 64 or 128 bytes side by side in each load; the next 64 are on
+// their way while these are multiplied.
 template <int kX, int kW, int kT, int kR, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
     typedef Planes<kX, kW> P;
@@ -205,32 +221,54 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
             const int rank = min((group * kR + r) * 16, ranks - 16) + col;
-            ws[r] = a.a + (static_cast<int64_t>(who) * ranks + rank) * a.k_row + 16 * quad;
+            ws[r] = a.a + (static_cast<int64_t>(who) * ranks + rank) * a.k_row + 8 * quad;
         }
         f32x4 acc[kT][kR];
 #pragma unroll
         for (int s = 0; s < kT; ++s)
 #pragma unroll
             for (int r = 0; r < kR; ++r) acc[s][r] = f32x4{0, 0, 0, 0};
-        for (int k = split * a.k_per + kKUnit * wave; k < end; k += kKUnit * kWaves) {
-            u32x4 raw[kR][2];
+        struct Loads {
+            Raw8<kX> x[kT][2];
+            u32x4 w[kR][2];
+        };
+        auto load = [&](int k) {
+            Loads l;
+            k = min(k, a.k_row - kKUnit);
 #pragma unroll
-            for (int r = 0; r < kR; ++r)
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) raw[r][h] = *reinterpret_cast<const u32x4*>(ws[r] + k + 8 * h);
+                for (int r = 0; r < kR; ++r) l.w[r][h] = *reinterpret_cast<const u32x4*>(ws[r] + k + 32 * h);
+#pragma unroll
+                for (int s = 0; s < kT; ++s) l.x[s][h] = fetch<kX, kVec>(xs[s], k + 32 * h + 8 * quad, a.k);
+            }
+            return l;
+        };
+        auto multiply = [&](int k, const Loads& l) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 u32x4 xp[kT][P::kOfX];
 #pragma unroll
-                for (int s = 0; s < kT; ++s) load_x<kX, kVec>(xs[s], k + 16 * quad + 8 * h, a.k, xp[s]);
+                for (int s = 0; s < kT; ++s) planes_of<kX, kVec>(l.x[s][h], k + 32 * h + 8 * quad, a.k, xp[s]);
 #pragma unroll
                 for (int r = 0; r < kR; ++r) {
                     u32x4 wp[P::kOfW];
-                    planes_of_16(raw[r][h], wp);
+                    planes_of_16(l.w[r][h], wp);
 #pragma unroll
                     for (int s = 0; s < kT; ++s) acc[s][r] = products<P::kF16>(wp, xp[s], acc[s][r]);
                 }
             }
+        };
+        constexpr int kAll = kKUnit * kWaves;
+        int k = split * a.k_per + kKUnit * wave;
+        if (k < end) {
+            Loads now = load(k);
+            for (; k + kAll < end; k += kAll) {
+                const Loads next = load(k + kAll);
+                multiply(k, now);
+                now = next;
+            }
+            multiply(k, now);
         }
 #pragma unroll
         for (int s = 0; s < kT; ++s)
@@ -249,54 +287,54 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
     }
 }
 
-// Planes of s_a t for the 16 kT tokens of a wave: the second operand of the second product, kept in registers.
-template <int kW, int kT, int kS>
-__device__ __forceinline__ void load_t(const AdaptArg& a, const Distinct<kT>& set, int first, int p,
-                                       u32x4 (&tp)[kT][kS][Planes<TQ_DT_F32, kW>::kOfX]) {
-    const int col = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4, ranks = a.parts * a.rank;
+// s_a t of kRows tokens from `first` on, part p's ranks, summed over the shares of K once for the block: lds[token][rank].
+template <int kRows, int kRow>
+__device__ __forceinline__ void sum_t(const AdaptArg& a, int first, int p, float (&lds)[kRows][kRow]) {
+    const int quads = a.rank / 4;
+    const int64_t ranks = a.parts * a.rank;
+    for (int i = threadIdx.x; i < kRows * quads; i += kBlock) {
+        const int row = i / quads, rank = 4 * (i - row * quads), tok = first + row;
+        const int who = tok < a.m ? a.index[tok] : -1;
+        f32x4 v{0, 0, 0, 0};
+        if (static_cast<uint32_t>(who) < static_cast<uint32_t>(a.count)) {
+            const float* src = a.t + tok * ranks + p * a.rank + rank;
+            const float scale = a.scales ? a.scales[who] : 1.f;
+            f32x4 x[kMaxSplits];  // all on their way at once; those past the last are the last again, and left out
 #pragma unroll
-    for (int s = 0; s < kT; ++s) {
-        const int tok = min(first + 16 * s + col, a.m - 1);
-        const float scale = set.mine[s] < 0 ? 0.f : a.scales ? a.scales[set.mine[s]] : 1.f;
+            for (int k = 0; k < kMaxSplits; ++k) x[k] = *reinterpret_cast<const f32x4*>(src + static_cast<int64_t>(min(k, a.splits - 1)) * a.m * ranks);
+#pragma unroll
+            for (int k = 0; k < kMaxSplits; ++k)
+                if (k < a.splits) v += x[k];
+            v *= scale;
+        }
+        *reinterpret_cast<f32x4*>(&lds[row][rank]) = v;
+    }
+}
+
+// Planes of it for the 16 kT tokens of a wave: the second operand of the second product, kept in registers.
+template <int kT, int kS, int kRow, int kN>
+__device__ __forceinline__ void planes_of_t(const AdaptArg& a, const float (&lds)[16 * kT][kRow], u32x4 (&tp)[kT][kS][kN]) {
+    const int col = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int s = 0; s < kT; ++s)
 #pragma unroll
         for (int h = 0; h < kS; ++h) {
             const int rank = 32 * h + 8 * quad;
-            f32x4 lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
-            if (rank < a.rank && set.mine[s] >= 0) {
-                const float* src = a.t + static_cast<int64_t>(tok) * ranks + p * a.rank + rank;
-                for (int i = 0; i < a.splits; ++i, src += static_cast<int64_t>(a.m) * ranks) {
-                    lo += *reinterpret_cast<const f32x4*>(src);
-                    hi += *reinterpret_cast<const f32x4*>(src + 4);
-                }
-            }
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = lo[i] * scale;
-                v[4 + i] = hi[i] * scale;
-            }
+            for (int i = 0; i < 8; ++i) v[i] = rank < a.rank ? lds[16 * s + col][rank + i] : 0.f;
             cut8(v, tp[s][h]);
         }
-    }
 }
 
-// What the wave's lanes wrote to LDS before is there for all of them (LDS serves a wave in order; the compiler has to
-// keep that order, too).
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Ranks of adapter `who` for output `row` of b: the first operand of the second product.
+// Ranks of adapter `who` for output `row` of b: the first operand of the second product.  Lanes behind the last rank
+// take other ranks of the row, which meet zeros of t.
 template <int kS>
 __device__ __forceinline__ void load_b(const AdaptArg& a, int who, int64_t row, u32x4 (&raw)[kS]) {
     const int quad = (threadIdx.x & 63) >> 4;
+    const uint16_t* from = a.b + (static_cast<int64_t>(who) * a.n + row) * a.rank;
 #pragma unroll
-    for (int h = 0; h < kS; ++h) {
-        raw[h] = u32x4{0, 0, 0, 0};
-        if (who >= 0 && 32 * h + 8 * quad < a.rank)
-            raw[h] = *reinterpret_cast<const u32x4*>(a.b + (static_cast<int64_t>(who) * a.n + row) * a.rank + 32 * h + 8 * quad);
-    }
+    for (int h = 0; h < kS; ++h) raw[h] = *reinterpret_cast<const u32x4*>(from + min(32 * h + 8 * quad, a.rank - 8));
 }
 
 template <int kW, int kS>
@@ -312,18 +350,20 @@ __device__ __forceinline__ f32x4 up_sums(const u32x4 (&raw)[kS], const u32x4 (&t
     return v;
 }
 
-// Few rows, and rows that no 16-byte access reaches.  Wave (token tile, part, range of outputs): outputs go by in tiles
-// of 16, 4 outputs of a token to a lane; up to kU distinct adapters' weights are loaded together, those of the
+// Few rows, and rows that no 16-byte access reaches.  Block (token tile, part, range of outputs), whose waves take tiles of 16
+// outputs in turn, 4 outputs of a token to a lane; up to kU distinct adapters' weights are loaded together, those of the
 // next tile before this one's sums.
 template <int kW, int kT, int kS, int kU, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    int id = blockIdx.x * kWaves + (threadIdx.x >> 6);
+    __shared__ float t[16 * kT][32 * kS + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    int id = blockIdx.x;
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int p = id % a.parts, range = id / a.parts;
-    if (range >= a.ranges) return;
-    const int first = tile * 16 * kT, np = a.n / a.parts, begin = range * a.per * 16, end = min(begin + a.per * 16, np);
+    const int first = tile * 16 * kT, np = a.n / a.parts;
+    const int begin = (range * a.per * kWaves + wave) * 16, end = min((range + 1) * a.per * kWaves * 16, np);
+    constexpr int kTurn = 16 * kWaves;
     Distinct<kT> set(a.index, a.count, first, a.m, lane);
     int64_t at[kT];
 #pragma unroll
@@ -347,13 +387,15 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
 #pragma unroll
         for (int i = 0; i < kU; ++i) {
             names[i] = set.next();
-            load_b(a, names[i], row_of_b(n0), raw[i]);
+            if (names[i] >= 0) load_b(a, names[i], row_of_b(n0), raw[i]);
         }
     };
-    load(begin);
+    load(begin < end ? begin : begin - 16 * wave);  // (a wave may have no tile: the block's first)
+    sum_t(a, first, p, t);
+    __syncthreads();
     u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
-    load_t<kW>(a, set, first, p, tp);
-    for (int n0 = begin; n0 < end; n0 += 16) {
+    planes_of_t(a, t, tp);
+    for (int n0 = begin; n0 < end; n0 += kTurn) {
         f32x4 d[kT];
 #pragma unroll
         for (int s = 0; s < kT; ++s) d[s] = f32x4{-0.f, -0.f, -0.f, -0.f};  // what leaves y as it is
@@ -375,11 +417,12 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
 #pragma unroll
             for (int i = 1; i < kU; ++i) names[i] = set.next();
 #pragma unroll
-            for (int i = 0; i < kU; ++i) load_b(a, names[i], row_of_b(n0), raw[i]);
+            for (int i = 0; i < kU; ++i)
+                if (names[i] >= 0) load_b(a, names[i], row_of_b(n0), raw[i]);
         }
 #pragma unroll
         for (int s = 0; s < kT; ++s) d[s] += y[s];
-        if (n0 + 16 < end) load(n0 + 16);
+        if (n0 + kTurn < end) load(n0 + kTurn);
 #pragma unroll
         for (int s = 0; s < kT; ++s) {
             if (first + 16 * s + col >= a.m) continue;
@@ -394,14 +437,14 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
     }
 }
 
-// Many rows.  Block (token tile, part, range of outputs), whose waves take 64 outputs each of 256 side by side: 16 kT tokens of a
-// wave.  The sums go through LDS (a wave's own part, no barrier) so that y is read and out written in runs of 256 bytes of a
-// row: the 64 bytes that a tile of the matrix instruction holds of one took 127 us where this takes 81 (4093 rows of 14336), with
-// stores that keep out of the caches (kStream: 106 us without), which then hold y and b.  y is on its way a step ahead.
+// Many rows.  Block (token tile, part, range of outputs): 16 kT tokens and 256 outputs a step, 64 for each wave.  The
+// sums go through LDS, so that y is read and out written in runs of 1 KB of a row: of 4093 rows of 14336 (rank 64), with y on
+// its way from HBM, 100 us; 106 in runs of 256 bytes, 127 in the 64 bytes that a tile of the matrix instruction holds of a row;
+// a copy of y takes 85.  kStream: loads and stores that are not kept in the caches, which b needs (109 us without).
 template <int kW, int kT, int kS, bool kStream>
 __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
-    constexpr int kRows = 16 * kT, kY = kRows / 4, kStep = kRowsOutputs * kWaves;
-    __shared__ float sums[kWaves][kRows][kRowsOutputs + 4];
+    constexpr int kRows = 16 * kT, kY = kRows / kWaves, kN = kStep / 16 / kWaves;
+    __shared__ float sums[kRows][kStep + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
     int id = blockIdx.x;
     const int range = id % a.ranges;
@@ -409,62 +452,57 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     const int p = id % a.parts, first = id / a.parts * kRows, np = a.n / a.parts;
     const int begin = range * a.per * kStep, end = min(begin + a.per * kStep, np);
     Distinct<kT> set(a.index, a.count, first, a.m, lane);
+    sum_t(a, first, p, sums);
+    __syncthreads();
     u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
-    load_t<kW>(a, set, first, p, tp);
+    planes_of_t(a, sums, tp);
+    __syncthreads();
     // rows without an adapter: nothing is ever added
 #pragma unroll
-    for (int i = 0; i < kY; ++i) *reinterpret_cast<f32x4*>(&sums[wave][4 * i + quad][4 * col]) = f32x4{-0.f, -0.f, -0.f, -0.f};
-    auto place = [&](int i, int n) { return static_cast<int64_t>(min(first + 4 * i + quad, a.m - 1)) * a.n + static_cast<int64_t>(p) * np + n; };
-    auto load_y = [&](int n0, f32x4 (&y)[kY]) {
-        const int n = min(n0 + wave * kRowsOutputs + 4 * col, np - 4);
+    for (int i = 0; i < kY; ++i) *reinterpret_cast<f32x4*>(&sums[kWaves * i + wave][4 * lane]) = f32x4{-0.f, -0.f, -0.f, -0.f};
+    __syncthreads();
+    const int64_t at = static_cast<int64_t>(first + wave) * a.n + static_cast<int64_t>(p) * np;
+    for (int n0 = begin; n0 < end; n0 += kStep) {
+        const int n = n0 + 4 * lane;
+        f32x4 y[kY];
+        u32x4 raw[kN][kS];
+        auto weights = [&](int who) {
 #pragma unroll
-        for (int i = 0; i < kY; ++i) y[i] = *reinterpret_cast<const f32x4*>(a.y + place(i, n));
-    };
-    constexpr int kN = kRowsOutputs / 16;
-    u32x4 raw[kN][kS];
-    auto weights = [&](int who, int n0) {
-#pragma unroll
-        for (int j = 0; j < kN; ++j)
-            load_b(a, who, static_cast<int64_t>(p) * np + min(n0 + wave * kRowsOutputs + 16 * j + col, np - 1), raw[j]);
-    };
-    auto multiply = [&](int who) {
-#pragma unroll
-        for (int s = 0; s < kT; ++s) {
-            const bool mine = set.mine[s] == who;
-            if (!__ballot(mine)) continue;
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const f32x4 v = up_sums<kW>(raw[j], tp[s]);
-                if (mine) *reinterpret_cast<f32x4*>(&sums[wave][16 * s + col][16 * j + 4 * quad]) = v;
-            }
-        }
-    };
-    auto step = [&](int n0, const f32x4 (&now)[kY], f32x4 (&next)[kY]) {
+            for (int j = 0; j < kN; ++j)
+                load_b(a, who, static_cast<int64_t>(p) * np + min(n0 + (wave * kN + j) * 16 + col, np - 1), raw[j]);
+        };
         set.restart();
         int who = set.next();
-        weights(who, n0);
-        load_y(n0 + kStep, next);
-        while (who >= 0) {
-            multiply(who);
-            if ((who = set.next()) >= 0) weights(who, n0);
-        }
-        wave_order();
-        const int n = n0 + wave * kRowsOutputs + 4 * col;
+        if (who >= 0) weights(who);  // before y: loads come back in order, and the sums wait for these alone
 #pragma unroll
         for (int i = 0; i < kY; ++i) {
-            const f32x4 v = now[i] + *reinterpret_cast<const f32x4*>(&sums[wave][4 * i + quad][4 * col]);
-            if (first + 4 * i + quad >= a.m || n >= end) continue;
-            f32x4* to = reinterpret_cast<f32x4*>(a.out + place(i, n));
+            const int64_t row = min(first + wave + kWaves * i, a.m - 1);
+            const f32x4* from = reinterpret_cast<const f32x4*>(a.y + row * a.n + static_cast<int64_t>(p) * np + min(n, np - 4));
+            y[i] = kStream ? __builtin_nontemporal_load(from) : *from;
+        }
+        while (who >= 0) {
+#pragma unroll
+            for (int s = 0; s < kT; ++s) {
+                const bool mine = set.mine[s] == who;
+                if (!__ballot(mine)) continue;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    const f32x4 v = up_sums<kW>(raw[j], tp[s]);
+                    if (mine) *reinterpret_cast<f32x4*>(&sums[16 * s + col][(wave * kN + j) * 16 + 4 * quad]) = v;
+                }
+            }
+            if ((who = set.next()) >= 0) weights(who);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kY; ++i) {
+            if (first + wave + kWaves * i >= a.m || n >= end) continue;
+            const f32x4 v = y[i] + *reinterpret_cast<const f32x4*>(&sums[kWaves * i + wave][4 * lane]);
+            f32x4* to = reinterpret_cast<f32x4*>(a.out + at + static_cast<int64_t>(kWaves) * i * a.n + n);
             if constexpr (kStream) __builtin_nontemporal_store(v, to);
             else *to = v;
         }
-        wave_order();
-    };
-    f32x4 y[2][kY];
-    load_y(begin, y[0]);
-    for (int n0 = begin; n0 < end; n0 += 2 * kStep) {
-        step(n0, y[0], y[1]);
-        if (n0 + kStep < end) step(n0 + kStep, y[1], y[0]);
+        __syncthreads();
     }
 }
 
@@ -487,8 +525,8 @@ Cut cut_of(const tq_adapters* a, int64_t m) {
     c.groups = static_cast<int>((rank_tiles + c.low_ranks - 1) / c.low_ranks);
     const int64_t units = (k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
     const int64_t blocks = (m + c.low_tokens - 1) / c.low_tokens * c.slots * c.groups;
-    // two blocks for each CU, four where there are many rows (4093 rows, rank 64: 38 us with one, 32 with two, 28 with four)
-    const int64_t splits = std::max<int64_t>(1, std::min(units, (c.few ? 2 : 4) * device_cu_count() / std::max<int64_t>(1, blocks)));
+    // four blocks for each CU (4093 rows, rank 64: 38 us with one, 32 with two, 28 with four), at most kMaxSplits
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({units, kMaxSplits, 4 * device_cu_count() / std::max<int64_t>(1, blocks)}));
     const int64_t per = (units + splits - 1) / splits;
     c.k_per = static_cast<int>(per * kKUnit * kWaves);
     c.splits = static_cast<int>((units + per - 1) / per);
@@ -531,19 +569,17 @@ void launch_low_tokens(const AdaptArg& a, const Cut& c, bool vec, int64_t blocks
     else launch_low_ranks<kX, kW, 2>(a, c.low_ranks, vec, blocks, st);
 }
 
-int64_t blocks_of(const AdaptArg& a, int waves) {
-    return (static_cast<int64_t>(a.tiles) * a.parts * a.ranges + waves - 1) / waves;
-}
+int64_t blocks_of(const AdaptArg& a) { return static_cast<int64_t>(a.tiles) * a.parts * a.ranges; }
 
-// Tiles of 16 kT tokens, a wave each, ranges so that there are about sixteen waves for each CU.
+// Blocks of 16 kT tokens, ranges so that there are about four blocks for each CU.
 template <int kW, int kT, int kS, int kU>
 int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
-    const int64_t n_tiles = (a.n / a.parts + 15) / 16;
+    const int64_t turns = (a.n / a.parts + 16 * kWaves - 1) / (16 * kWaves);
     a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
-    const int64_t all = a.tiles * a.parts * n_tiles;
-    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(32, all / (16 * device_cu_count()))));
-    a.ranges = static_cast<int>((n_tiles + a.per - 1) / a.per);
-    const int64_t blocks = blocks_of(a, kWaves);
+    const int64_t all = a.tiles * a.parts * turns;
+    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, all / (4 * device_cu_count()))));
+    a.ranges = static_cast<int>((turns + a.per - 1) / a.per);
+    const int64_t blocks = blocks_of(a);
     TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
     if (vec)
         k_adapt_up<kW, kT, kS, kU, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
@@ -552,24 +588,25 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
     return check_launch(what);
 }
 
-// Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps of 16 output tiles, and about 9 tiles'
-// time for a block's start (4093 rows of 14336, rank 64: 80, 81 and 86 us with one, two and four blocks for each CU).
+// Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps, and about one step's time for a block's
+// start; a block that is alone on its CU waits for its own loads (4093 rows of 14336, rank 64: 113, 100, 108, 125 and 130 us with
+// 1, 2, 4, 7 and 14 blocks for each CU).
 template <int kW, int kT, int kS>
 int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
-    const int64_t np = a.n / a.parts, steps = (np + kRowsOutputs * kWaves - 1) / (kRowsOutputs * kWaves);
+    const int64_t np = a.n / a.parts, steps = (np + kStep - 1) / kStep;
     a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
     const int64_t every = static_cast<int64_t>(a.tiles) * a.parts, cus = device_cu_count();
     int64_t best = 0;
     for (int64_t r = 1; r <= steps && r <= 64; ++r) {
         const int64_t per = (steps + r - 1) / r, blocks = every * ((steps + per - 1) / per);
-        const int64_t cost = (blocks + cus - 1) / cus * (16 * per + 9);
+        const int64_t on_one = (blocks + cus - 1) / cus, cost = on_one * (per + 1) * (on_one == 1 ? 6 : 5);
         if (best == 0 || cost < best) {
             best = cost;
             a.per = static_cast<int>(per);
         }
     }
     a.ranges = static_cast<int>((steps + a.per - 1) / a.per);
-    const int64_t blocks = blocks_of(a, 1);
+    const int64_t blocks = blocks_of(a);
     TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
     // outputs that the L2 caches (4 MB for each XCD) would not hold anyway
     if (static_cast<int64_t>(a.m) * a.n * 4 >= int64_t(32) << 20)
@@ -593,10 +630,10 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
         if (a.rank > 32) return launch_up_rows<kW, 2, 2>(a, st, what);
         return launch_up_rows<kW, 2, 1>(a, st, what);
     }
-    if (a.rank > 128) return launch_up<kW, 1, 8, 1>(a, vec_y, st, what);
-    if (a.rank > 64) return launch_up<kW, 1, 4, 2>(a, vec_y, st, what);
-    if (a.rank > 32) return launch_up<kW, 1, 2, 4>(a, vec_y, st, what);
-    return launch_up<kW, 1, 1, 4>(a, vec_y, st, what);
+    if (a.rank > 128) return launch_up<kW, 1, 8, 2>(a, vec_y, st, what);
+    if (a.rank > 64) return launch_up<kW, 1, 4, 4>(a, vec_y, st, what);
+    if (a.rank > 32) return launch_up<kW, 1, 2, 8>(a, vec_y, st, what);
+    return launch_up<kW, 1, 1, 8>(a, vec_y, st, what);
 }
 
 }  // namespace

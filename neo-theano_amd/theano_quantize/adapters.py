@@ -12,7 +12,7 @@ import torch
 
 from . import _abi
 from ._tensor import stream
-from .cache import _TYPES, _current_device, _device, _Fixed, _indices
+from .cache import _TYPES, _current_device, _dense, _device, _Fixed, _indices
 from .errors import InvalidArgument
 
 MAX_RANK = 256
@@ -78,22 +78,22 @@ class Adapters(_Fixed):
     def add(self, x, index, y, out=None):
         """y [rows, N] (f32) with each row's share added: x [rows, K] f32, bf16 or f16; index int32 [rows], the row's adapter,
         or a number outside 0 .. count - 1 for none.  out: where the sums go (y itself, or a new tensor)."""
-        code = _TYPES.get(_device(x, "Adapters.add: x").dtype)
-        m, k, n = index.shape[0], self.in_features, self.out_features
+        dev, m, k, n = self.device_index, index.shape[0], self.in_features, self.out_features
+        if dev != _current_device():
+            raise InvalidArgument("Adapters.add: the adapters and the current device differ")
+        code = _TYPES.get(x.dtype)
         if code is None or x.shape != (m, k):
             raise InvalidArgument(f"Adapters.add: x must be float32, bfloat16 or float16 [{m}, {k}], got {x.dtype} {tuple(x.shape)}")
-        _indices(index, torch.int32, 1, "Adapters.add: index")
-        if _device(y, "Adapters.add: y").dtype != torch.float32 or y.shape != (m, n) or not y.is_contiguous():
-            raise InvalidArgument(f"Adapters.add: y must be contiguous float32 [{m}, {n}], got {y.dtype} {tuple(y.shape)}")
-        if self.device_index != _current_device():
-            raise InvalidArgument("Adapters.add: the adapters and the current device differ")
-        if not x.is_contiguous():
-            x = x.contiguous()
+        if not _dense(x, x.dtype, 2, dev):
+            x = _device(x, "Adapters.add: x").contiguous()
+        _dense(index, torch.int32, 1, dev) or _indices(index, torch.int32, 1, "Adapters.add: index")
+        if not _dense(y, torch.float32, 2, dev) or y.shape != (m, n):
+            raise InvalidArgument(f"Adapters.add: y must be contiguous float32 [{m}, {n}] on the current GPU, got {y.dtype} "
+                                  f"{tuple(y.shape)}")
         if out is None:
             out = torch.empty_like(y)
-        elif out is not y and (_device(out, "Adapters.add: out").dtype != torch.float32 or out.shape != (m, n) or
-                               not out.is_contiguous()):
-            raise InvalidArgument(f"Adapters.add: out must be contiguous float32 [{m}, {n}]")
+        elif out is not y and (not _dense(out, torch.float32, 2, dev) or out.shape != (m, n)):
+            raise InvalidArgument(f"Adapters.add: out must be contiguous float32 [{m}, {n}] on the current GPU")
         nb = _abi.entry("tq_adapters_workspace_bytes")(self._desc, m)
         ws = y.new_empty(max(nb // 4, 1))
         _abi.call("tq_adapters_add", self._desc, x.data_ptr(), code, m, index.data_ptr(), y.data_ptr(), out.data_ptr(),

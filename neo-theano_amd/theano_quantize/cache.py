@@ -19,6 +19,7 @@ what it says is checked on the device, see ``KVBatch``.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -51,6 +52,12 @@ def _indices(t, dtype, dim, name):
     return t
 
 
+def _dense(t, dtype, dim, device):
+    """Whether `t` is a dense tensor of `dtype` with `dim` dimensions on `device`: what `_indices` asks for, found out faster (a
+    decoding step's calls are bound by the host)."""
+    return t.__class__ is torch.Tensor and t.dtype is dtype and t.dim() == dim and t.is_contiguous() and t.get_device() == device
+
+
 def _heads(t, name, dtype=None, tokens=None, heads=None, dim=None):
     """(tensor, descriptor, dtype code) of a [tokens, heads, head_dim] tensor."""
     _device(t, name)
@@ -79,6 +86,17 @@ class _Fixed:
             raise AttributeError(f"{type(self).__name__}.{name} is fixed: make another {type(self).__name__}")
 
 
+@functools.lru_cache(maxsize=64)
+def _packed_axes(axes):
+    """The axes of planes as tq_rotary_axes takes them, and how many there are."""
+    if any(x not in (0, 1, 2, 3) for x in axes):
+        raise InvalidArgument(f"Rotary: axes are numbers from 0 to 3, got {axes}")
+    words = [0, 0]
+    for i, x in enumerate(axes):
+        words[i // 32] |= int(x) << 2 * (i % 32)
+    return tuple(words), max(map(int, axes), default=0) + 1
+
+
 class Rotary(_Fixed):
     """Rotary positions: plane i of a head turns by position * frequencies[i].
 
@@ -93,14 +111,12 @@ class Rotary(_Fixed):
     def __init__(self, frequencies, interleaved=False, scale=1.0, axes=None):
         _indices(frequencies, torch.float64, 1, "Rotary: frequencies")
         r, interleaved, scale = 2 * frequencies.shape[0], bool(interleaved), float(scale)
-        planes, count = [0] * 2, 0
+        planes, count = (0, 0), 0
         if axes is not None:
             axes = tuple(axes)
-            if len(axes) != r // 2 or r > MAX_HEAD_DIM or any(x not in (0, 1, 2, 3) for x in axes):
+            if len(axes) != r // 2 or r > MAX_HEAD_DIM:
                 raise InvalidArgument(f"Rotary: axes are {r // 2} numbers from 0 to 3, one for each plane, got {axes}")
-            for i, x in enumerate(axes):
-                planes[i // 32] |= x << 2 * (i % 32)
-            count = max(axes, default=0) + 1
+            planes, count = _packed_axes(axes)
         self.__dict__.update(frequencies=frequencies, interleaved=interleaved, scale=scale, rotary_dim=r, axes=axes,
                              _planes=planes, _axes=count,
                              _desc=_abi.rotary_desc(frequencies.data_ptr(), r, interleaved, False, scale))
@@ -344,9 +360,9 @@ class KVCache(_Fixed):
         the place of its i-th new token, for i < kept[b] (int32 [batch, n], ascending, and [batch]).  Returns the
         lengths that the sequences then have (int32 [batch]).  A sequence whose path does not ascend inside its rows stays
         as it is.  Pages that sequences share are copied first (PagePool.fork does)."""
-        b = self._here(new)
-        _indices(path, torch.int32, 2, "KVCache.keep: path")
-        _indices(kept, torch.int32, 1, "KVCache.keep: kept")
+        b, dev = self._here(new), self.device_index
+        _dense(path, torch.int32, 2, dev) or _indices(path, torch.int32, 2, "KVCache.keep: path")
+        _dense(kept, torch.int32, 1, dev) or _indices(kept, torch.int32, 1, "KVCache.keep: kept")
         if path.shape[0] != new.batch or kept.shape[0] != new.batch:
             raise InvalidArgument(f"KVCache.keep: paths {tuple(path.shape)} and kept {tuple(kept.shape)} of {new.batch} sequences")
         lengths = torch.empty_like(kept)
@@ -357,9 +373,10 @@ class KVCache(_Fixed):
     def copy_pages(self, source, target):
         """Page target[j] becomes a copy of page source[j] (int32 [n] each, as PagePool.fork gives them; pairs with a page
         outside the cache are skipped).  A page is one pair's target and no pair's source."""
-        _indices(source, torch.int32, 1, "KVCache.copy_pages: source")
-        _indices(target, torch.int32, 1, "KVCache.copy_pages: target")
-        if source.shape != target.shape or self.device_index != source.get_device():
+        dev = self.device_index
+        _dense(source, torch.int32, 1, dev) or _indices(source, torch.int32, 1, "KVCache.copy_pages: source")
+        _dense(target, torch.int32, 1, dev) or _indices(target, torch.int32, 1, "KVCache.copy_pages: target")
+        if source.shape != target.shape or dev != _current_device():
             raise InvalidArgument(f"KVCache.copy_pages: {source.shape[0]} sources, {target.shape[0]} targets on the cache's device")
         _abi.call("tq_kv_copy_pages", self._ref, source.data_ptr(), target.data_ptr(), source.shape[0], stream())
 

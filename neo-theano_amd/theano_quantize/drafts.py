@@ -18,7 +18,7 @@ import torch
 
 from . import _abi
 from ._tensor import stream
-from .cache import _TYPES, _current_device, _device, _Fixed, _indices
+from .cache import _TYPES, _current_device, _dense, _device, _Fixed, _indices
 from .errors import InvalidArgument
 
 
@@ -43,11 +43,11 @@ def verify_drafts(tokens, target, new, accept, final, draft=None, parents=None):
 
     Returns (path, kept, token): int32 [batch, new.tokens] the accepted rows, root first, -1 behind them;
     int32 [batch] how many; int64 [batch] the token to go on with (-1: a sequence without rows)."""
-    n, batch = new.rows, new.batch
-    _indices(tokens, torch.int64, 1, "verify_drafts: tokens")
-    _indices(accept, torch.float32, 1, "verify_drafts: accept")
-    _indices(final, torch.float32, 1, "verify_drafts: final")
-    if new.device_index != _current_device():
+    n, batch, dev = new.rows, new.batch, _current_device()
+    _dense(tokens, torch.int64, 1, dev) or _indices(tokens, torch.int64, 1, "verify_drafts: tokens")
+    _dense(accept, torch.float32, 1, dev) or _indices(accept, torch.float32, 1, "verify_drafts: accept")
+    _dense(final, torch.float32, 1, dev) or _indices(final, torch.float32, 1, "verify_drafts: final")
+    if new.device_index != dev:
         raise InvalidArgument("verify_drafts: the batch and the current device differ")
     if tokens.shape[0] != n or accept.shape[0] != n or final.shape[0] != batch:
         raise InvalidArgument(f"verify_drafts: {tokens.shape[0]} tokens and {accept.shape[0]} numbers for {n} rows, "
@@ -58,16 +58,16 @@ def verify_drafts(tokens, target, new, accept, final, draft=None, parents=None):
         draft = _probabilities(draft, "verify_drafts: draft", n, target)
         dp, ds = draft.data_ptr(), draft.stride(0)
     if parents is not None:
-        _indices(parents, torch.int32, 1, "verify_drafts: parents")
+        _dense(parents, torch.int32, 1, dev) or _indices(parents, torch.int32, 1, "verify_drafts: parents")
         if parents.shape[0] != n:
             raise InvalidArgument(f"verify_drafts: {parents.shape[0]} parents for {n} rows")
         pp = parents.data_ptr()
-    vocab, dev = target.shape[1], tokens.device
-    path = torch.empty((batch, new.tokens), dtype=torch.int32, device=dev)
-    kept = torch.empty(batch, dtype=torch.int32, device=dev)
-    token = torch.empty(batch, dtype=torch.int64, device=dev)
+    vocab = target.shape[1]
+    path = new.lengths.new_empty((batch, new.tokens))
+    kept = new.lengths.new_empty(batch)
+    token = tokens.new_empty(batch)
     nb = _abi.entry("tq_verify_drafts_workspace_bytes")(new._desc, vocab)
-    ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+    ws = final.new_empty(max(nb // 4, 1))
     _abi.call("tq_verify_drafts", new._desc, tokens.data_ptr(), target.data_ptr(), target.stride(0), dp, ds,
               _TYPES[target.dtype], vocab, pp, accept.data_ptr(), final.data_ptr(), ws.data_ptr(), nb, path.data_ptr(),
               kept.data_ptr(), token.data_ptr(), stream())
@@ -93,8 +93,9 @@ class PagePool(_Fixed):
         return PagePool(torch.zeros(pages, dtype=torch.int32, device=torch.device("cuda", torch.cuda.current_device())), page)
 
     def _table(self, table, name):
-        _indices(table, torch.int32, 2, name)
-        if self.device_index != _current_device():
+        dev = self.device_index
+        _dense(table, torch.int32, 2, dev) or _indices(table, torch.int32, 2, name)
+        if dev != _current_device():
             raise InvalidArgument(f"{name}: the pool and the current device differ")
         return table.data_ptr(), table.stride(0), table.shape[1]
 
@@ -102,7 +103,7 @@ class PagePool(_Fixed):
         """Gives each sequence pages for `lengths` (int32 [batch]) tokens, behind those it has, in `table` itself: the
         lowest free ones, sequence by sequence."""
         where = self._table(table, "PagePool.grow: table")
-        _indices(lengths, torch.int32, 1, "PagePool.grow: lengths")
+        _dense(lengths, torch.int32, 1, self.device_index) or _indices(lengths, torch.int32, 1, "PagePool.grow: lengths")
         if lengths.shape[0] != table.shape[0]:
             raise InvalidArgument(f"PagePool.grow: {lengths.shape[0]} lengths for {table.shape[0]} sequences")
         _abi.call("tq_pages_grow", self._desc, *where, lengths.data_ptr(), table.shape[0], stream())
@@ -112,8 +113,9 @@ class PagePool(_Fixed):
         Whole pages are shared; a page that a sequence has begun is copied by
         ``KVCache.copy_pages(source, target)``, in each layer.  The parents stay until they are freed."""
         where = self._table(table, "PagePool.fork: table")
-        _indices(lengths, torch.int32, 1, "PagePool.fork: lengths")
-        _indices(parents, torch.int32, 1, "PagePool.fork: parents")
+        dev = self.device_index
+        _dense(lengths, torch.int32, 1, dev) or _indices(lengths, torch.int32, 1, "PagePool.fork: lengths")
+        _dense(parents, torch.int32, 1, dev) or _indices(parents, torch.int32, 1, "PagePool.fork: parents")
         if lengths.shape[0] != table.shape[0]:
             raise InvalidArgument(f"PagePool.fork: {lengths.shape[0]} lengths for {table.shape[0]} sequences")
         n = parents.shape[0]
