@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kBlock = 256, kWaves = 4;
 constexpr int kMaxRank = 256, kMaxParts = 16, kKUnit = 64;
-constexpr int kMaxSplits = 8;  // shares of K that the second product adds
+constexpr int kMaxShares = 8;  // shares of K that the second product adds
 constexpr int kStep = 256;  // outputs of a block's step where there are many rows
 constexpr int64_t kMaxRows = 1 << 30;
 
@@ -148,28 +148,47 @@ __device__ __forceinline__ f32x4 products(const u32x4 (&w)[kNW], const u32x4 (&x
 template <int kT>
 struct Distinct {
     int mine[kT];
-    uint32_t left[kT];
+    uint32_t firsts[kT], left[kT];  // bits of the tokens that are their adapter's first
     __device__ __forceinline__ Distinct(const int32_t* index, int count, int first, int m, int lane) {
+        const int col = lane & 15;
 #pragma unroll
         for (int s = 0; s < kT; ++s) {
-            const int tok = first + 16 * s + (lane & 15);
+            const int tok = first + 16 * s + col;
             const int a = tok < m ? index[tok] : -1;
             mine[s] = static_cast<uint32_t>(a) < static_cast<uint32_t>(count) ? a : -1;
+        }
+#pragma unroll
+        for (int s = 0; s < kT; ++s) {
+            bool again = mine[s] < 0;
+#pragma unroll
+            for (int t = 0; t <= s; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) again |= (t < s || i < col) && mine[s] == readlane(mine[t], i);
+            firsts[s] = static_cast<uint32_t>(__ballot(!again)) & 0xFFFFu;
         }
         restart();
     }
     __device__ __forceinline__ void restart() {
 #pragma unroll
-        for (int s = 0; s < kT; ++s) left[s] = static_cast<uint32_t>(__ballot(mine[s] >= 0)) & 0xFFFFu;
+        for (int s = 0; s < kT; ++s) left[s] = firsts[s];
+    }
+    __device__ __forceinline__ int all() const {
+        int n = 0;
+#pragma unroll
+        for (int s = 0; s < kT; ++s) n += __popc(firsts[s]);
+        return n;
     }
     __device__ __forceinline__ int next() {
         int who = -1;
+        bool done = false;
 #pragma unroll
-        for (int s = kT - 1; s >= 0; --s)
-            if (left[s]) who = __builtin_amdgcn_readlane(mine[s], __ffs(left[s]) - 1);
-        if (who >= 0) {
-#pragma unroll
-            for (int s = 0; s < kT; ++s) left[s] &= ~static_cast<uint32_t>(__ballot(mine[s] == who));
+        for (int s = 0; s < kT; ++s) {
+            const bool here = !done && left[s] != 0;
+            if (here) {
+                who = readlane(mine[s], __ffs(left[s]) - 1);
+                left[s] &= left[s] - 1;
+            }
+            done |= here;
         }
         return who;
     }
@@ -181,34 +200,39 @@ struct AdaptArg {
     const uint16_t* a;
     const uint16_t* b;
     const float* scales;
-    float* t;  // [splits, m, parts * rank]
+    int32_t* shares;  // of K, [low tiles]
+    float* t;         // [kMaxShares, m, parts * rank]
     const float* y;
     float* out;
-    int m, k, k_row, n, count, parts, rank;
-    int splits, k_per;        // K of a block of the first product
-    int slots, groups;        // first product: blocks for a tile's distinct adapters, and for its ranks
-    int ranges, per, tiles;   // second product: ranges of `per` turns of a block's waves, and token tiles
+    int m, k, k_row, n, np, count, parts, rank;  // np: outputs of a part
+    int low_shift, gang_shift, turns;            // first product: tiles of 1 << low_shift tokens, 1 << gang_shift blocks for each, k_row
+                                                 // in turns of a block's waves
+    int per;                                     // second product: turns (steps) of a block
 };
 
-// Block (token tile, rank group, slot, split): 16 kT tokens, 16 kR ranks, every slots-th distinct adapter.  The
-// waves take 64 of K in turn, a rank's 64 and a token's 64 or 128 bytes side by side in each load; the next 64 are on
-// their way while these are multiplied.
+// Grid (token tile and one of its gang, rank group): 16 kT tokens, 16 kR ranks.  The tile's distinct adapters, which only the
+// device knows, and as many shares of K as then keep the gang busy are its blocks' units of work.  The waves take
+// 64 of K in turn, a rank's 64 and a token's 64 or 128 bytes side by side in each load; the next 64 are on their way while these
+// are multiplied.
 template <int kX, int kW, int kT, int kR, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
     typedef Planes<kX, kW> P;
     __shared__ f32x4 part[kWaves][kT * kR][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int slot = id % a.slots;
-    id /= a.slots;
-    const int group = id % a.groups, first = id / a.groups * 16 * kT;
-    const int ranks = a.parts * a.rank, end = min((split + 1) * a.k_per, a.k_row);
+    // a gang's blocks are neighbours: they read neighbouring columns of the same rows
+    const int gang = 1 << a.gang_shift, tile = blockIdx.x >> a.gang_shift, mate = blockIdx.x & (gang - 1), group = blockIdx.y;
+    const int first = tile * 16 * kT, ranks = a.parts * a.rank;
     Distinct<kT> set(a.index, a.count, first, a.m, lane);
-    int u = 0;
-    for (int who; (who = set.next()) >= 0; ++u) {
-        if (u % a.slots != slot) continue;
+    const int adapters = set.all();
+    int bits = 0;  // the shares of K are a power of two
+    while (2 << bits <= min(kMaxShares, a.turns) && adapters << (bits + 1) <= gang) ++bits;
+    const int per = (a.turns + (1 << bits) - 1) >> bits;
+    if (mate == 0 && group == 0 && threadIdx.x == 0) a.shares[tile] = 1 << bits;
+    int who = -1, named = 0;  // the adapter that next() gave `named`-th
+    for (int unit = mate; unit < adapters << bits; unit += gang) {
+        const int share = unit & ((1 << bits) - 1), k_begin = min(share * per, a.turns) * kKUnit * kWaves,
+                  end = min(k_begin + per * kKUnit * kWaves, a.k_row);
+        for (; named <= unit >> bits; ++named) who = set.next();
         const char* xs[kT];
 #pragma unroll
         for (int s = 0; s < kT; ++s) {
@@ -260,7 +284,7 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
             }
         };
         constexpr int kAll = kKUnit * kWaves;
-        int k = split * a.k_per + kKUnit * wave;
+        int k = k_begin + kKUnit * wave;
         if (k < end) {
             Loads now = load(k);
             for (; k + kAll < end; k += kAll) {
@@ -280,7 +304,7 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
             const int s = j / kR, rank = (group * kR + j % kR) * 16;
             if (j % kWaves != wave || rank >= ranks || set.mine[s] != who) continue;
             const f32x4 v = (part[0][j][lane] + part[1][j][lane]) + (part[2][j][lane] + part[3][j][lane]);
-            const int64_t row = static_cast<int64_t>(split) * a.m + first + 16 * s + col;
+            const int64_t row = static_cast<int64_t>(share) * a.m + first + 16 * s + col;
             *reinterpret_cast<f32x4*>(a.t + row * ranks + rank + 4 * quad) = v;
         }
         __syncthreads();
@@ -288,23 +312,26 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
 }
 
 // s_a t of kRows tokens from `first` on, part p's ranks, summed over the shares of K once for the block: lds[token][rank].
-template <int kRows, int kRow>
+template <int kRows, int kS, int kRow>
 __device__ __forceinline__ void sum_t(const AdaptArg& a, int first, int p, float (&lds)[kRows][kRow]) {
-    const int quads = a.rank / 4;
     const int64_t ranks = a.parts * a.rank;
-    for (int i = threadIdx.x; i < kRows * quads; i += kBlock) {
-        const int row = i / quads, rank = 4 * (i - row * quads), tok = first + row;
+#pragma unroll
+    for (int i = threadIdx.x; i < kRows * 8 * kS; i += kBlock) {
+        const int row = i / (8 * kS), rank = 4 * (i % (8 * kS)), tok = first + row;
+        if (rank >= a.rank) continue;
         const int who = tok < a.m ? a.index[tok] : -1;
         f32x4 v{0, 0, 0, 0};
         if (static_cast<uint32_t>(who) < static_cast<uint32_t>(a.count)) {
             const float* src = a.t + tok * ranks + p * a.rank + rank;
             const float scale = a.scales ? a.scales[who] : 1.f;
-            f32x4 x[kMaxSplits];  // all on their way at once; those past the last are the last again, and left out
+            const int shares = a.shares[tok >> a.low_shift];
+            f32x4 x[kMaxShares];  // all on their way at once; those past the last are the first again, and left out
 #pragma unroll
-            for (int k = 0; k < kMaxSplits; ++k) x[k] = *reinterpret_cast<const f32x4*>(src + static_cast<int64_t>(min(k, a.splits - 1)) * a.m * ranks);
+            for (int k = 0; k < kMaxShares; ++k)
+                x[k] = *reinterpret_cast<const f32x4*>(src + (k < shares ? static_cast<int64_t>(k) * a.m * ranks : 0));
 #pragma unroll
-            for (int k = 0; k < kMaxSplits; ++k)
-                if (k < a.splits) v += x[k];
+            for (int k = 0; k < kMaxShares; ++k)
+                if (k < shares) v += x[k];
             v *= scale;
         }
         *reinterpret_cast<f32x4*>(&lds[row][rank]) = v;
@@ -350,18 +377,14 @@ __device__ __forceinline__ f32x4 up_sums(const u32x4 (&raw)[kS], const u32x4 (&t
     return v;
 }
 
-// Few rows, and rows that no 16-byte access reaches.  Block (token tile, part, range of outputs), whose waves take tiles of 16
+// Few rows, and rows that no 16-byte access reaches.  Grid (token tile, part, range of outputs): a block's waves take tiles of 16
 // outputs in turn, 4 outputs of a token to a lane; up to kU distinct adapters' weights are loaded together, those of the
 // next tile before this one's sums.
 template <int kW, int kT, int kS, int kU, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
     __shared__ float t[16 * kT][32 * kS + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    int id = blockIdx.x;
-    const int tile = id % a.tiles;
-    id /= a.tiles;
-    const int p = id % a.parts, range = id / a.parts;
-    const int first = tile * 16 * kT, np = a.n / a.parts;
+    const int p = blockIdx.y, range = blockIdx.z, first = blockIdx.x * 16 * kT, np = a.np;
     const int begin = (range * a.per * kWaves + wave) * 16, end = min((range + 1) * a.per * kWaves * 16, np);
     constexpr int kTurn = 16 * kWaves;
     Distinct<kT> set(a.index, a.count, first, a.m, lane);
@@ -391,7 +414,7 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
         }
     };
     load(begin < end ? begin : begin - 16 * wave);  // (a wave may have no tile: the block's first)
-    sum_t(a, first, p, t);
+    sum_t<16 * kT, kS>(a, first, p, t);
     __syncthreads();
     u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
     planes_of_t(a, t, tp);
@@ -437,7 +460,7 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
     }
 }
 
-// Many rows.  Block (token tile, part, range of outputs): 16 kT tokens and 256 outputs a step, 64 for each wave.  The
+// Many rows.  Grid (range of outputs, part, token tile): 16 kT tokens and 256 outputs a step, 64 for each wave.  The
 // sums go through LDS, so that y is read and out written in runs of 1 KB of a row: of 4093 rows of 14336 (rank 64), with y on
 // its way from HBM, 100 us; 106 in runs of 256 bytes, 127 in the 64 bytes that a tile of the matrix instruction holds of a row;
 // a copy of y takes 85.  kStream: loads and stores that are not kept in the caches, which b needs (109 us without).
@@ -446,13 +469,10 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     constexpr int kRows = 16 * kT, kY = kRows / kWaves, kN = kStep / 16 / kWaves;
     __shared__ float sums[kRows][kStep + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    int id = blockIdx.x;
-    const int range = id % a.ranges;
-    id /= a.ranges;
-    const int p = id % a.parts, first = id / a.parts * kRows, np = a.n / a.parts;
+    const int range = blockIdx.x, p = blockIdx.y, first = blockIdx.z * kRows, np = a.np;
     const int begin = range * a.per * kStep, end = min(begin + a.per * kStep, np);
     Distinct<kT> set(a.index, a.count, first, a.m, lane);
-    sum_t(a, first, p, sums);
+    sum_t<kRows, kS>(a, first, p, sums);
     __syncthreads();
     u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
     planes_of_t(a, sums, tp);
@@ -465,22 +485,12 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     for (int n0 = begin; n0 < end; n0 += kStep) {
         const int n = n0 + 4 * lane;
         f32x4 y[kY];
-        u32x4 raw[kN][kS];
-        auto weights = [&](int who) {
+        auto weights = [&](int who, u32x4 (&raw)[kN][kS]) {
 #pragma unroll
             for (int j = 0; j < kN; ++j)
                 load_b(a, who, static_cast<int64_t>(p) * np + min(n0 + (wave * kN + j) * 16 + col, np - 1), raw[j]);
         };
-        set.restart();
-        int who = set.next();
-        if (who >= 0) weights(who);  // before y: loads come back in order, and the sums wait for these alone
-#pragma unroll
-        for (int i = 0; i < kY; ++i) {
-            const int64_t row = min(first + wave + kWaves * i, a.m - 1);
-            const f32x4* from = reinterpret_cast<const f32x4*>(a.y + row * a.n + static_cast<int64_t>(p) * np + min(n, np - 4));
-            y[i] = kStream ? __builtin_nontemporal_load(from) : *from;
-        }
-        while (who >= 0) {
+        auto multiply = [&](int who, const u32x4 (&raw)[kN][kS]) {
 #pragma unroll
             for (int s = 0; s < kT; ++s) {
                 const bool mine = set.mine[s] == who;
@@ -491,7 +501,24 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
                     if (mine) *reinterpret_cast<f32x4*>(&sums[16 * s + col][(wave * kN + j) * 16 + 4 * quad]) = v;
                 }
             }
-            if ((who = set.next()) >= 0) weights(who);
+        };
+        set.restart();
+        u32x4 raw[2][kN][kS];
+        int who = set.next();
+        if (who >= 0) weights(who, raw[0]);  // before y: loads come back in order, and the sums wait for these alone
+#pragma unroll
+        for (int i = 0; i < kY; ++i) {
+            const int64_t row = min(first + wave + kWaves * i, a.m - 1);
+            const f32x4* from = reinterpret_cast<const f32x4*>(a.y + row * a.n + static_cast<int64_t>(p) * np + min(n, np - 4));
+            y[i] = kStream ? __builtin_nontemporal_load(from) : *from;
+        }
+        while (who >= 0) {  // the next adapter's weights are on their way while these are multiplied
+            const int then = set.next();
+            if (then >= 0) weights(then, raw[1]);
+            multiply(who, raw[0]);
+            if (then < 0) break;
+            if ((who = set.next()) >= 0) weights(who, raw[0]);
+            multiply(then, raw[1]);
         }
         __syncthreads();
 #pragma unroll
@@ -506,32 +533,37 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     }
 }
 
-// How a call is cut.
+// How the first product is cut.
 struct Cut {
     bool few;
-    int low_tokens, low_ranks, slots, groups, splits, k_per;
+    int tokens, ranks, gang_shift, groups;
+    int64_t tiles;
 };
 
-// Up to this many rows tiles are of 16 tokens and a tile's distinct adapters have blocks of their own.
-constexpr int kFewRows = 256;
+// Up to this many rows the first product's tiles are of 16 tokens, then of 32 (K 4096, rank 64, six adapters' runs of rows, both
+// products to 14336 outputs: 2048 rows 81 us with 16, 85 with 32; 4096 rows 144 and 140).
+constexpr int kFewRows = 2048;
 
 Cut cut_of(const tq_adapters* a, int64_t m) {
     Cut c;
-    const int64_t k_row = (a->k + kKUnit - 1) / kKUnit * kKUnit, rank_tiles = a->parts * a->rank / 16;
+    const int64_t turns = (a->k + kKUnit * kWaves - 1) / (kKUnit * kWaves), rank_tiles = a->parts * a->rank / 16;
     c.few = m <= kFewRows;
-    c.low_tokens = c.few ? 16 : 32;
-    c.low_ranks = rank_tiles == 1 ? 1 : rank_tiles == 2 ? 2 : 4;
-    c.slots = c.few ? static_cast<int>(std::min<int64_t>({16, m, a->count})) : 1;
-    c.groups = static_cast<int>((rank_tiles + c.low_ranks - 1) / c.low_ranks);
-    const int64_t units = (k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
-    const int64_t blocks = (m + c.low_tokens - 1) / c.low_tokens * c.slots * c.groups;
-    // four blocks for each CU (4093 rows, rank 64: 38 us with one, 32 with two, 28 with four), at most kMaxSplits
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({units, kMaxSplits, 4 * device_cu_count() / std::max<int64_t>(1, blocks)}));
-    const int64_t per = (units + splits - 1) / splits;
-    c.k_per = static_cast<int>(per * kKUnit * kWaves);
-    c.splits = static_cast<int>((units + per - 1) / per);
+    c.tokens = c.few ? 16 : 32;
+    c.ranks = rank_tiles == 1 ? 1 : rank_tiles == 2 ? 2 : 4;
+    c.groups = static_cast<int>((rank_tiles + c.ranks - 1) / c.ranks);
+    c.tiles = (m + c.tokens - 1) / c.tokens;
+    // about four blocks for each CU (4093 rows of one adapter each tile, rank 64: 38 us with one, 32 with two, 28 with four),
+    // no more than a tile can have adapters and shares
+    const int64_t blocks = c.tiles * c.groups;
+    const int64_t gang = std::min<int64_t>(4 * device_cu_count() / blocks,
+                                           std::min<int64_t>({c.tokens, m, a->count}) * std::min<int64_t>(turns, kMaxShares));
+    c.gang_shift = 0;
+    while (int64_t(2) << c.gang_shift <= gang) ++c.gang_shift;
     return c;
 }
+
+// Workspace: the shares of each tile, then t.
+int64_t shares_bytes(const Cut& c) { return (c.tiles * 4 + 15) / 16 * 16; }
 
 int check_adapters(const char* what, const tq_adapters* a, int64_t m) {
     TQ_REQUIRE(a, "%s: null adapters", what);
@@ -549,42 +581,38 @@ int check_adapters(const char* what, const tq_adapters* a, int64_t m) {
 }
 
 template <int kX, int kW, int kT, int kR>
-void launch_low(const AdaptArg& a, bool vec, int64_t blocks, hipStream_t st) {
+void launch_low(const AdaptArg& a, bool vec, dim3 grid, hipStream_t st) {
     if (vec)
-        k_adapt_low<kX, kW, kT, kR, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_low<kX, kW, kT, kR, true><<<grid, kBlock, 0, st>>>(a);
     else
-        k_adapt_low<kX, kW, kT, kR, false><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_low<kX, kW, kT, kR, false><<<grid, kBlock, 0, st>>>(a);
 }
 
 template <int kX, int kW, int kT>
-void launch_low_ranks(const AdaptArg& a, int ranks, bool vec, int64_t blocks, hipStream_t st) {
-    if (ranks == 1) launch_low<kX, kW, kT, 1>(a, vec, blocks, st);
-    else if (ranks == 2) launch_low<kX, kW, kT, 2>(a, vec, blocks, st);
-    else launch_low<kX, kW, kT, 4>(a, vec, blocks, st);
+void launch_low_ranks(const AdaptArg& a, int ranks, bool vec, dim3 grid, hipStream_t st) {
+    if (ranks == 1) launch_low<kX, kW, kT, 1>(a, vec, grid, st);
+    else if (ranks == 2) launch_low<kX, kW, kT, 2>(a, vec, grid, st);
+    else launch_low<kX, kW, kT, 4>(a, vec, grid, st);
 }
 
 template <int kX, int kW>
-void launch_low_tokens(const AdaptArg& a, const Cut& c, bool vec, int64_t blocks, hipStream_t st) {
-    if (c.few) launch_low_ranks<kX, kW, 1>(a, c.low_ranks, vec, blocks, st);
-    else launch_low_ranks<kX, kW, 2>(a, c.low_ranks, vec, blocks, st);
+void launch_low_tokens(const AdaptArg& a, const Cut& c, bool vec, dim3 grid, hipStream_t st) {
+    if (c.few) launch_low_ranks<kX, kW, 1>(a, c.ranks, vec, grid, st);
+    else launch_low_ranks<kX, kW, 2>(a, c.ranks, vec, grid, st);
 }
 
-int64_t blocks_of(const AdaptArg& a) { return static_cast<int64_t>(a.tiles) * a.parts * a.ranges; }
-
-// Blocks of 16 kT tokens, ranges so that there are about four blocks for each CU.
+// Tiles of 16 kT tokens, ranges so that there are about four blocks for each CU.
 template <int kW, int kT, int kS, int kU>
 int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
-    const int64_t turns = (a.n / a.parts + 16 * kWaves - 1) / (16 * kWaves);
-    a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
-    const int64_t all = a.tiles * a.parts * turns;
-    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, all / (4 * device_cu_count()))));
-    a.ranges = static_cast<int>((turns + a.per - 1) / a.per);
-    const int64_t blocks = blocks_of(a);
-    TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
+    const int64_t turns = (a.np + 16 * kWaves - 1) / (16 * kWaves), tiles = (a.m + 16 * kT - 1) / (16 * kT);
+    a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, tiles * a.parts * turns / (4 * device_cu_count()))));
+    const int64_t ranges = (turns + a.per - 1) / a.per;
+    TQ_REQUIRE(tiles <= kMaxBlocks && ranges <= 65535, "%s: %d tokens, %d outputs are more than a launch holds", what, a.m, a.n);
+    const dim3 blocks(static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.parts), static_cast<uint32_t>(ranges));
     if (vec)
-        k_adapt_up<kW, kT, kS, kU, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_up<kW, kT, kS, kU, true><<<blocks, kBlock, 0, st>>>(a);
     else
-        k_adapt_up<kW, kT, kS, kU, false><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_up<kW, kT, kS, kU, false><<<blocks, kBlock, 0, st>>>(a);
     return check_launch(what);
 }
 
@@ -593,38 +621,39 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
 // 1, 2, 4, 7 and 14 blocks for each CU).
 template <int kW, int kT, int kS>
 int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
-    const int64_t np = a.n / a.parts, steps = (np + kStep - 1) / kStep;
-    a.tiles = (a.m + 16 * kT - 1) / (16 * kT);
-    const int64_t every = static_cast<int64_t>(a.tiles) * a.parts, cus = device_cu_count();
+    const int64_t steps = (a.np + kStep - 1) / kStep, tiles = (a.m + 16 * kT - 1) / (16 * kT), cus = device_cu_count();
     int64_t best = 0;
     for (int64_t r = 1; r <= steps && r <= 64; ++r) {
-        const int64_t per = (steps + r - 1) / r, blocks = every * ((steps + per - 1) / per);
-        const int64_t on_one = (blocks + cus - 1) / cus, cost = on_one * (per + 1) * (on_one == 1 ? 6 : 5);
+        const int64_t per = (steps + r - 1) / r, on_one = (tiles * a.parts * ((steps + per - 1) / per) + cus - 1) / cus;
+        const int64_t cost = on_one * (per + 1) * (on_one == 1 ? 6 : 5);
         if (best == 0 || cost < best) {
             best = cost;
             a.per = static_cast<int>(per);
         }
     }
-    a.ranges = static_cast<int>((steps + a.per - 1) / a.per);
-    const int64_t blocks = blocks_of(a);
-    TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %d tokens are more than %lld blocks", what, a.m, (long long)kMaxBlocks);
+    TQ_REQUIRE(tiles <= 65535, "%s: %d tokens are more than a launch holds", what, a.m);
+    const dim3 blocks(static_cast<uint32_t>((steps + a.per - 1) / a.per), static_cast<uint32_t>(a.parts), static_cast<uint32_t>(tiles));
     // outputs that the L2 caches (4 MB for each XCD) would not hold anyway
     if (static_cast<int64_t>(a.m) * a.n * 4 >= int64_t(32) << 20)
-        k_adapt_up_rows<kW, kT, kS, true><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_up_rows<kW, kT, kS, true><<<blocks, kBlock, 0, st>>>(a);
     else
-        k_adapt_up_rows<kW, kT, kS, false><<<static_cast<int>(blocks), kBlock, 0, st>>>(a);
+        k_adapt_up_rows<kW, kT, kS, false><<<blocks, kBlock, 0, st>>>(a);
     return check_launch(what);
 }
 
 template <int kW>
-int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool vec_y, int64_t low, hipStream_t st, const char* what) {
+int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool vec_y, dim3 low, hipStream_t st, const char* what) {
     clear_error();
     if (dtype == TQ_DT_F32) launch_low_tokens<TQ_DT_F32, kW>(a, c, vec_x, low, st);
     else if (dtype == TQ_DT_BF16) launch_low_tokens<TQ_DT_BF16, kW>(a, c, vec_x, low, st);
     else launch_low_tokens<TQ_DT_F16, kW>(a, c, vec_x, low, st);
     const int rc = check_launch(what);
     if (rc != TQ_OK) return rc;
-    if (!c.few && vec_y) {
+    // the form of many rows from 2^23 outputs on (rank 16: 1024 x 4096 20.4 us against 21.8, 1024 x 14336 49.6 against 41.8), with more
+    // ranks from 2^20 on (rank 64: 64 x 14336 19.6 against 20.1, 128 x 14336 31.3 against 23.1, 512 x 4096 30.5 against 27.5) or 3 2^18
+    // (rank 128: 128 x 4096 15.5 against 17.8, 64 x 14336 22.7 against 18.3)
+    const int64_t many = a.rank > 64 ? 3 << 18 : a.rank > 32 ? 1 << 20 : 1 << 23;
+    if (vec_y && static_cast<int64_t>(a.m) * a.n >= many && a.m <= 16 * 65535) {
         if (a.rank > 128) return launch_up_rows<kW, 1, 8>(a, st, what);
         if (a.rank > 64) return launch_up_rows<kW, 1, 4>(a, st, what);
         if (a.rank > 32) return launch_up_rows<kW, 2, 2>(a, st, what);
@@ -644,7 +673,7 @@ extern "C" {
 int64_t tq_adapters_workspace_bytes(const tq_adapters* adapters, int64_t m) {
     using namespace tq;
     if (check_adapters("tq_adapters_add", adapters, m) != TQ_OK) return -1;
-    return m == 0 ? 0 : cut_of(adapters, m).splits * m * adapters->parts * adapters->rank * 4;
+    return m == 0 ? 0 : shares_bytes(cut_of(adapters, m)) + kMaxShares * m * adapters->parts * adapters->rank * 4;
 }
 
 int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64_t m, const int32_t* index, const float* y,
@@ -669,7 +698,8 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.a = static_cast<const uint16_t*>(adapters->a);
     a.b = static_cast<const uint16_t*>(adapters->b);
     a.scales = adapters->scales;
-    a.t = static_cast<float*>(workspace);
+    a.shares = static_cast<int32_t*>(workspace);
+    a.t = reinterpret_cast<float*>(static_cast<char*>(workspace) + shares_bytes(c));
     a.y = y;
     a.out = out;
     a.m = static_cast<int>(m);
@@ -679,14 +709,14 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.count = static_cast<int>(adapters->count);
     a.parts = static_cast<int>(adapters->parts);
     a.rank = static_cast<int>(adapters->rank);
-    a.splits = c.splits;
-    a.k_per = c.k_per;
-    a.slots = c.slots;
-    a.groups = c.groups;
-    const int64_t low = (m + c.low_tokens - 1) / c.low_tokens * c.slots * c.groups * c.splits;
-    TQ_REQUIRE(low <= kMaxBlocks, "%s: %lld tokens are more than %lld blocks", what, (long long)m, (long long)kMaxBlocks);
+    a.np = static_cast<int>(adapters->n / adapters->parts);
+    a.low_shift = c.tokens == 16 ? 4 : 5;
+    a.turns = (a.k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
+    a.gang_shift = c.gang_shift;
+    TQ_REQUIRE(c.tiles << c.gang_shift <= kMaxBlocks, "%s: %lld tokens are more than a launch holds", what, (long long)m);
+    const dim3 low(static_cast<uint32_t>(c.tiles << c.gang_shift), static_cast<uint32_t>(c.groups));
     const bool vec_x = aligned(x, 16) && adapters->k % 8 == 0;
-    const bool vec_y = aligned(y, 16) && aligned(out, 16) && adapters->n / adapters->parts % 4 == 0;
+    const bool vec_y = aligned(y, 16) && aligned(out, 16) && a.np % 4 == 0;
     return adapters->dtype == TQ_DT_F16 ? launch_typed<TQ_DT_F16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what)
                                         : launch_typed<TQ_DT_BF16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what);
 }

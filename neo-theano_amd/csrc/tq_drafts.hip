@@ -58,6 +58,7 @@ struct DraftArg {
     const int32_t* offsets;
     int batch, max_tokens, rows;
     int vocab, share, shares;  // share: probabilities of a block, shares * share >= vocab
+    FastDiv by_shares;
     int32_t* path;
     int32_t* kept;
     int64_t* next;
@@ -289,7 +290,7 @@ template <class T, bool kVec, bool kWalked>
 __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     __shared__ State shared;
     __shared__ uint32_t gone[kMaxShare / 32];
-    const int seq = blockIdx.x / a.shares, share = blockIdx.x - seq * a.shares, begin = share * a.share;
+    const int seq = static_cast<int>(a.by_shares.div(blockIdx.x)), share = blockIdx.x - seq * a.shares, begin = share * a.share;
     const Span s = span_of(a, seq);
     if (!a.draft)
         for (int i = threadIdx.x; i < a.share / 32; i += kBlock) gone[i] = 0;
@@ -581,6 +582,7 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
     a.vocab = static_cast<int>(vocab);
     a.share = share_of(vocab, batch->batch);
     a.shares = static_cast<int>(shares);
+    a.by_shares = FastDiv(static_cast<uint32_t>(shares));
     a.path = path;
     a.kept = kept;
     a.next = next;

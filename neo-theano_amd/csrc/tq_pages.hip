@@ -24,6 +24,7 @@ struct KeepArg {
     int64_t path_stride;
     const int32_t* kept;
     int path_width, heads, row;
+    FastDiv by_heads;  // 2 heads: keys and values
     int8_t* codes[2];  // k, v
     float* scales[2];
     int32_t* lengths_out;
@@ -35,7 +36,7 @@ struct KeepArg {
 __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
     const int lane = threadIdx.x & 63, u = blockIdx.x * (kBlock / 64) + threadIdx.x / 64;
     if (u >= units) return;
-    const int per_seq = 2 * a.heads, seq = u / per_seq, h = (u - seq * per_seq) >> 1, kv = u & 1;
+    const int seq = static_cast<int>(a.by_heads.div(static_cast<uint32_t>(u))), h = (u - seq * 2 * a.heads) >> 1, kv = u & 1;
     const int first = a.b.offsets ? a.b.offsets[seq] : seq * a.b.max_tokens;
     const int last = a.b.offsets ? a.b.offsets[seq + 1] : first + a.b.max_tokens;
     const int length = a.b.lengths[seq], kept = a.kept[seq], count = last - first;
@@ -48,29 +49,31 @@ __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
     }
     if (a.lengths_out && h == 0 && kv == 0 && lane == 0) a.lengths_out[seq] = fine ? length - count + kept : length;
     if (!fine) return;
+    auto at = [&](int r) -> int64_t {  // where new token r of the sequence lies, -1: nowhere
+        const int64_t pos = static_cast<int64_t>(length) - count + r;
+        if (pos < 0 || pos >= a.b.cap) return -1;
+        const int i = static_cast<int>(a.b.by_page.div(static_cast<uint32_t>(pos)));
+        const int page = a.b.table[seq * a.b.table_stride + i];
+        return page < 0 || page >= a.b.pages ? -1 : (static_cast<int64_t>(page) * a.heads + h) * a.b.page + (static_cast<int>(pos) - i * a.b.page);
+    };
     const int lanes = a.row / 16, rows = 64 / lanes, j = lane / lanes, c = lane - j * lanes;
     for (int i0 = 0; i0 < kept; i0 += rows) {
         const int i = i0 + j;
-        int64_t from = -1, to = -1;
+        int64_t from = -1, to = -1;  // rows of [pages, heads, page]
         if (j < rows && i < kept && path[i] != i) {
-            const KvPlace src = kv_place(a.b, first + path[i], seq), dst = kv_place(a.b, first + i, seq);
-            from = src.slot;
-            to = dst.slot;
+            from = at(path[i]);
+            to = at(i);
         }
         const bool moves = from >= 0 && to >= 0;
         u32x4 v{};
         float s = 0.f;
-        auto at = [&](int64_t slot) {  // [pages, heads, page]
-            const int64_t page = slot / a.b.page;
-            return (page * a.heads + h) * a.b.page + (slot - page * a.b.page);
-        };
         if (moves) {
-            v = *reinterpret_cast<const u32x4*>(a.codes[kv] + at(from) * a.row + 16 * c);
-            if (c == 0) s = a.scales[kv][at(from)];
+            v = *reinterpret_cast<const u32x4*>(a.codes[kv] + from * a.row + 16 * c);
+            if (c == 0) s = a.scales[kv][from];
         }
         if (moves) {
-            *reinterpret_cast<u32x4*>(a.codes[kv] + at(to) * a.row + 16 * c) = v;
-            if (c == 0) a.scales[kv][at(to)] = s;
+            *reinterpret_cast<u32x4*>(a.codes[kv] + to * a.row + 16 * c) = v;
+            if (c == 0) a.scales[kv][to] = s;
         }
     }
 }
@@ -83,13 +86,14 @@ struct CopyArg {
     u32x4* scales[2];
     int64_t code_units, scale_units;
     int chunks;  // blocks of a pair
+    FastDiv by_chunks;
     int pages;
 };
 
 constexpr int kCopyUnits = 4;  // in flight for each lane
 
 __global__ __launch_bounds__(kBlock) void k_copy_pages(CopyArg a) {
-    const int pair = blockIdx.x / a.chunks, chunk = blockIdx.x - pair * a.chunks;
+    const int pair = static_cast<int>(a.by_chunks.div(blockIdx.x)), chunk = blockIdx.x - pair * a.chunks;
     const int src = a.source[pair], dst = a.target[pair];
     if (src < 0 || src >= a.pages || dst < 0 || dst >= a.pages || src == dst) return;
     const int64_t all = 2 * (a.code_units + a.scale_units);
@@ -300,18 +304,18 @@ __global__ __launch_bounds__(kPoolBlock) void k_fork(ForkArg a) {
             if (a.target[c] < 0) a.source[c] = -1;
         return;
     }
-    const int64_t all = static_cast<int64_t>(a.children) * a.table_pages, step = static_cast<int64_t>(gridDim.x - 1) * kPoolBlock;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x - 1) * kPoolBlock + threadIdx.x; e < all; e += step) {
-        const int c = static_cast<int>(e / a.table_pages), i = static_cast<int>(e - static_cast<int64_t>(c) * a.table_pages);
+    for (int c = blockIdx.x - 1; c < a.children; c += gridDim.x - 1) {
         const int p = a.parents[c];
         const int whole = p < 0 || p >= a.batch ? 0 : min(max(a.lengths[p], 0) / a.pool.page, a.table_pages);
-        if (i == whole) continue;  // block 0's
-        int page = -1;
-        if (i < whole) {
-            page = a.table[p * a.stride + i];
-            if (page >= 0 && page < a.pool.pages) atomicAdd(a.pool.holders + page, 1);
+        for (int i = threadIdx.x; i < a.table_pages; i += kPoolBlock) {
+            if (i == whole) continue;  // block 0's
+            int page = -1;
+            if (i < whole) {
+                page = a.table[p * a.stride + i];
+                if (page >= 0 && page < a.pool.pages) atomicAdd(a.pool.holders + page, 1);
+            }
+            a.out[static_cast<int64_t>(c) * a.table_pages + i] = page;
         }
-        a.out[e] = page;
     }
 }
 
@@ -324,15 +328,15 @@ struct FreeArg {
 };
 
 __global__ __launch_bounds__(kBlock) void k_free(FreeArg a) {
-    const int64_t all = static_cast<int64_t>(a.batch) * a.table_pages, step = static_cast<int64_t>(gridDim.x) * kBlock;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; e < all; e += step) {
-        const int b = static_cast<int>(e / a.table_pages), i = static_cast<int>(e - static_cast<int64_t>(b) * a.table_pages);
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (a.which && !a.which[b]) continue;
-        int32_t* entry = a.table + b * a.stride + i;
-        const int page = *entry;
-        if (page >= 0 && page < a.pool.pages && atomicSub(a.pool.holders + page, 1) <= 0)
-            atomicAdd(a.pool.holders + page, 1);  // was free already: stays at 0
-        if (page >= 0) *entry = -1;
+        for (int i = threadIdx.x; i < a.table_pages; i += kBlock) {
+            int32_t* entry = a.table + b * a.stride + i;
+            const int page = *entry;
+            if (page >= 0 && page < a.pool.pages && atomicSub(a.pool.holders + page, 1) <= 0)
+                atomicAdd(a.pool.holders + page, 1);  // was free already: stays at 0
+            if (page >= 0) *entry = -1;
+        }
     }
 }
 
@@ -355,9 +359,8 @@ int check_table(const char* what, const int32_t* table, int64_t stride, int64_t 
     return TQ_OK;
 }
 
-int blocks_for(int64_t items, int block) {
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((items + block - 1) / block, 4 * device_cu_count())));
-}
+// Blocks for so many sequences, which they take in turn.
+int blocks_for(int64_t sequences) { return static_cast<int>(std::min<int64_t>(sequences, 8 * device_cu_count())); }
 
 }  // namespace
 }  // namespace tq
@@ -385,6 +388,7 @@ int tq_kv_keep(const tq_kv_cache* cache, const tq_kv_batch* batch, const int32_t
     a.path_width = static_cast<int>(path_width);
     a.kept = kept;
     a.heads = static_cast<int>(cache->heads);
+    a.by_heads = FastDiv(static_cast<uint32_t>(2 * cache->heads));
     a.row = static_cast<int>(kv_row(cache->head_dim));
     a.codes[0] = static_cast<int8_t*>(cache->k);
     a.codes[1] = static_cast<int8_t*>(cache->v);
@@ -420,6 +424,7 @@ int tq_kv_copy_pages(const tq_kv_cache* cache, const int32_t* source, const int3
     TQ_REQUIRE(chunks <= kMaxBlocks && n <= kMaxBlocks / chunks, "%s: %lld pages of %lld blocks are more than %lld blocks", what,
                (long long)n, (long long)chunks, (long long)kMaxBlocks);
     a.chunks = static_cast<int>(chunks);
+    a.by_chunks = FastDiv(static_cast<uint32_t>(chunks));
     clear_error();
     k_copy_pages<<<static_cast<int>(n * chunks), kBlock, 0, as_hip(stream)>>>(a);
     return check_launch(what);
@@ -472,7 +477,7 @@ int tq_pages_fork(const tq_page_pool* pool, const int32_t* table, int64_t table_
     a.source = source;
     a.target = target;
     clear_error();
-    k_fork<<<1 + blocks_for(children * table_pages, kPoolBlock), kPoolBlock, 0, as_hip(stream)>>>(a);
+    k_fork<<<1 + blocks_for(children), kPoolBlock, 0, as_hip(stream)>>>(a);
     return check_launch(what);
 }
 
@@ -491,7 +496,7 @@ int tq_pages_free(const tq_page_pool* pool, int32_t* table, int64_t table_stride
     a.batch = static_cast<int>(batch);
     a.which = sequences;
     clear_error();
-    k_free<<<blocks_for(batch * table_pages, kBlock), kBlock, 0, as_hip(stream)>>>(a);
+    k_free<<<blocks_for(batch), kBlock, 0, as_hip(stream)>>>(a);
     return check_launch(what);
 }
 
