@@ -661,8 +661,8 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
     }
     if (a.rank > 128) return launch_up<kW, 1, 8, 2>(a, vec_y, st, what);
     if (a.rank > 64) return launch_up<kW, 1, 4, 4>(a, vec_y, st, what);
-    if (a.rank > 32) return launch_up<kW, 1, 2, 8>(a, vec_y, st, what);
-    return launch_up<kW, 1, 1, 8>(a, vec_y, st, what);
+    if (a.rank > 32) return launch_up<kW, 1, 2, 4>(a, vec_y, st, what);
+    return launch_up<kW, 1, 1, 4>(a, vec_y, st, what);
 }
 
 }  // namespace

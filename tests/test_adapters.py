@@ -334,3 +334,57 @@ def test_what_python_refuses(tq):
         tq.Adapters.from_tensors([])
     with pytest.raises(tq.InvalidArgument):
         tq.Adapters.from_tensors([(a[0, 0], b[0]), (a[0, 0, :, :30], b[0])])
+
+
+@pytest.mark.gpu
+def test_outputs_and_inputs_past_32_bit_offsets(tq):
+    """9 GB of outputs, 5 GB of inputs: rows about each 2^31st element are those of a call of their own."""
+    import torch
+
+    for m, k, n, dtype in ((70000, 16, 32768, torch.float32), (300000, 8192, 16, torch.bfloat16)):
+        g = torch.Generator("cuda").manual_seed(3)
+        x = torch.empty(m, k, dtype=dtype, device="cuda").normal_(generator=g)
+        y = torch.empty(m, n, device="cuda").normal_(generator=g)
+        a = (torch.randn(3, 16, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+        ad = tq.Adapters(a, torch.randn(3, n, 16, generator=g, device="cuda").bfloat16())
+        index = torch.randint(-1, 3, (m,), generator=g, device="cuda", dtype=torch.int32)
+        width = max(k, n)
+        rows = sorted({0, m - 40, max((1 << 31) // width - 20, 0), max((1 << 32) // width - 20, 0)} & set(range(m - 39)))
+        before = [y[r:r + 40].clone() for r in rows]
+        ad.add(x, index, y, out=y)
+        for r, part in zip(rows, before):
+            ref, tol = reference(x[r:r + 40], part, ad.a[:, :, :, :k], ad.b, None, index[r:r + 40])
+            assert ((y[r:r + 40].double() - ref).abs() <= tol).all(), r
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(tq):
+    import torch
+
+    cases = [made(m, 5, 16, 1, 512, 1024, "float32", "bfloat16", m) for m in (7, 600)]
+    ads = [tq.Adapters(a, b, scales) for _, _, a, b, scales, _ in cases]
+    want = [ad.add(x, index, y) for ad, (x, y, _, _, _, index) in zip(ads, cases)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (ad, (x, y, _, _, _, index)) in enumerate(zip(ads, cases)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ad.add(x, index, y))
+    torch.cuda.synchronize()
+    for w, all_ in zip(want, got):
+        assert all(torch.equal(w, z) for z in all_)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,r", [(2049, 64, 16), (2048, 64, 16), (2100, 4100, 16), (513, 2048, 40), (600, 2000, 70), (400, 2100, 130), (1100, 1000, 200)])
+def test_sizes_on_both_sides_of_every_form(tq, m, n, r):
+    """Tiles of 16 and 32 tokens, the forms of few and many rows, each with one adapter, a few in runs and many mixed."""
+    import torch
+
+    for count, runs in ((1, True), (3, True), (50, False)):
+        x, y, a, b, scales, index = made(m, count, r, 1, 130, n, "float32", "bfloat16", m + count, runs)
+        ref, tol = reference(x, y, a, b, scales, index)
+        assert ((tq.Adapters(a, b, scales).add(x, index, y).double() - ref).abs() <= tol).all()
+    index.fill_(-1)
+    assert torch.equal(tq.Adapters(a, b, scales).add(x, index, y), y)

@@ -351,3 +351,77 @@ def test_what_python_refuses(tq):
     empty = tq.KVBatch(torch.zeros(0, 1, dtype=torch.int32).cuda(), torch.zeros(0, dtype=torch.int32).cuda(), 3)
     path, kept, token = tq.verify_drafts(args[0][:0], args[1][:0], empty, args[4][:0], args[5][:0])
     assert path.shape == (0, 3) and kept.shape == token.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tree,draft", [(False, True), (True, False), (True, True)])
+def test_padded_batches(tq, tree, draft):
+    """Rows behind the last sequence, sequences of fewer rows than max_tokens, sequences of none, a batch of none at all."""
+    import torch
+
+    counts = [3, 0, 5, 1]
+    tokens, p, q, parents, accept, final = make(counts, 500, tree, draft, torch.float32, 12)
+    pad = lambda x, v: None if x is None else torch.cat([x, torch.full((7, *x.shape[1:]), v, dtype=x.dtype)])  # noqa: E731
+    new = batch_of(tq, counts, most=9, extra=7)
+    check(tq, counts, pad(tokens, 1 << 50), pad(p, float("nan")), pad(q, float("nan")), pad(parents, 0), pad(accept, float("nan")), final, not tree, new)
+    none = tq.KVBatch(torch.zeros(2, 1, dtype=torch.int32).cuda(), torch.zeros(2, dtype=torch.int32).cuda(), 0)
+    e = lambda x: None if x is None else x[:0].cuda()  # noqa: E731
+    path, kept, token = tq.verify_drafts(e(tokens), e(p), none, e(accept), final[:2].cuda(), e(q), e(parents) if tree else None)
+    assert path.shape == (2, 0) and kept.tolist() == [0, 0] and token.tolist() == [-1, -1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("draft", [False, True])
+def test_probabilities_past_32_bit_offsets(tq, draft):
+    """5 GB of each model's: the last sequences are those of a call of their own."""
+    import torch
+
+    b, t, vocab = 2500, 8, 131072
+    g = torch.Generator("cuda").manual_seed(5)
+    p = torch.empty(b * t, vocab, dtype=torch.bfloat16, device="cuda").uniform_(generator=g).mul_(2.0 ** -16)
+    q = torch.empty_like(p).uniform_(generator=g).mul_(2.0 ** -16) if draft else None
+    tokens = torch.randint(0, vocab, (b * t,), generator=g, device="cuda")
+    accept, final = torch.rand(b * t, generator=g, device="cuda") * (1 if draft else 2.0 ** -17), torch.rand(b, generator=g, device="cuda")
+    full = lambda n: tq.KVBatch(torch.zeros(n, 1, dtype=torch.int32).cuda(), torch.full((n,), t, dtype=torch.int32).cuda(), t)  # noqa: E731
+    for parents in (None, torch.tensor([-1, 0, 0, 1, 1, 2, 3, 3], dtype=torch.int32).repeat(b).cuda()):
+        whole = tq.verify_drafts(tokens, p, full(b), accept, final, q, parents)
+        for first in (0, 2047, b - 3):  # (2^31 elements are 2048 sequences)
+            rows, seqs = slice(first * t, (first + 3) * t), slice(first, first + 3)
+            part = tq.verify_drafts(tokens[rows], p[rows], full(3), accept[rows], final[seqs], None if q is None else q[rows],
+                                    None if parents is None else parents[rows])
+            for a, c in zip(whole, part):
+                assert torch.equal(a[seqs], c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [262144, 262145, 300001, 1100000])
+def test_vocabularies_of_more_than_one_round_of_sums(tq, vocab):
+    """Against sums in 64 bits on the device: the first token whose running sum passes the goal."""
+    import torch
+
+    g = torch.Generator("cuda").manual_seed(vocab)
+    p = torch.softmax(torch.randn(6, vocab, generator=g, device="cuda"), 1)
+    q = torch.softmax(torch.randn(6, vocab, generator=g, device="cuda"), 1)
+    tokens = torch.zeros(6, dtype=torch.int64, device="cuda")
+    accept, final = torch.ones(6, device="cuda"), torch.tensor([0.0, 0.3, 0.999], device="cuda")
+    new = tq.KVBatch(torch.zeros(3, 1, dtype=torch.int32).cuda(), torch.full((3,), 2, dtype=torch.int32).cuda(), 2)
+    for draft in (None, q):
+        left = p[::2].double().clone()
+        yes = torch.zeros(3, dtype=torch.bool, device="cuda")
+        if draft is None:
+            left[:, 0] = 0
+        else:
+            yes = q[::2, 0] < p[::2, 0]  # token 0, by a number of 1: the leaf's own probabilities follow
+            left = torch.where(yes[:, None], p[1::2].double(), (left - q[::2].double()).clamp_min(0))
+        sums = left.cumsum(1)
+        goal = final.double()[:, None] * sums[:, -1:]
+        want = (sums <= goal).sum(1)
+        path, kept, token = tq.verify_drafts(tokens, p, new, accept, final, draft)
+        assert torch.equal(kept, 1 + yes.int()) and torch.equal(token, want)
+    # all of it beyond the first rounds
+    p.zero_()
+    p[:, vocab - 2] = 0.5
+    assert tq.verify_drafts(tokens, p, new, accept, final)[2].tolist() == [vocab - 2] * 3
+    # nothing left (q takes all): the target's own
+    path, kept, token = tq.verify_drafts(tokens, p, new, accept, final, p * 2)
+    assert token.tolist() == [vocab - 2] * 3

@@ -408,3 +408,80 @@ def test_drafts_from_positions_to_what_stays(tq, codes, most):
             assert torch.equal(a, c)
     pool.free(samples)
     assert (pool.holders == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+def test_caches_past_32_bit_offsets(tq, codes):
+    """5 GB of codes: pages and rows on both sides of 2^31 and 2^32 bytes."""
+    import torch
+
+    pages, page, heads, d = 80000, 64, 8, 128
+    cache = tq.KVCache.allocate(pages, page, heads, d, tq.QuantDType.Int8 if codes == "i8" else tq.QuantDType.FP8)
+    some = [0, 32767, 32768, 65535, 65536, pages - 1, pages - 2, 5]
+    g = torch.Generator("cuda").manual_seed(1)
+    for t in (cache.k, cache.v):
+        t[some] = torch.randint(0, 100, (len(some), heads, page, d), generator=g, device="cuda").to(t.dtype)
+    for t in (cache.k_scale, cache.v_scale):
+        t[some] = torch.rand(len(some), heads, page, generator=g, device="cuda")
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    names = ("k", "k_scale", "v", "v_scale")
+    cache.copy_pages(ints([65536, 32768, pages - 1]), ints([40000, 70000, 1]))
+    for n in names:
+        t = getattr(cache, n)
+        assert torch.equal(t[40000], t[65536]) and torch.equal(t[70000], t[32768]) and torch.equal(t[1], t[pages - 1]), n
+    before = {n: getattr(cache, n).clone()[[pages - 2, 32767]] for n in names}
+    new = tq.KVBatch(ints([[pages - 2, 32767]]), ints([120]), 100)  # positions 20 to 119
+    assert cache.keep(new, ints([[3, 50, 99]]), ints([3])).tolist() == [23]
+    for n in names:
+        t = getattr(cache, n)
+        for i, r in enumerate((3, 50, 99)):
+            src = 20 + r
+            assert torch.equal(t[pages - 2][:, 20 + i], before[n][src // page][:, src % page]), (n, i)
+
+
+@pytest.mark.gpu
+def test_keeping_and_pages_captured_and_replayed(tq):
+    """A step's keep, growth, fork, copy and end in a graph: each replay as the eager calls on the same state."""
+    import torch
+    from test_gpu_cache import Case
+
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+
+    def state():
+        case = Case(tq, [40, 33], [12, 12], 16, 2, 64, "i8", spare=20)
+        filled(tq, case, 3)
+        pool = tq.PagePool.allocate(case.cache.pages, 16)
+        pool.holders[case.table.flatten().long()] = 1
+        table = torch.cat([case.table, torch.full((2, 3), -1, dtype=torch.int32, device="cuda")], 1)
+        return case, pool, table, ints([[0, 2, 5, 9], [0, 1, 7, -1]]), ints([4, 3]), ints([1, 0, 1])
+
+    def step(case, pool, table, path, kept, parents):
+        lengths = case.cache.keep(case.batch, path, kept)
+        pool.grow(table, lengths + 20)
+        children, source, target = pool.fork(table, lengths, parents)
+        case.cache.copy_pages(source, target)
+        had = children.clone()
+        pool.free(children)
+        return lengths, had, source, target
+
+    eager, still = state(), state()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*state())
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*still)
+    for i in range(4):
+        for x in (eager, still):
+            x[0].batch.lengths.copy_(ints([40 + 3 * i, 33 + i]))
+        want = step(*eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+        assert torch.equal(eager[1].holders, still[1].holders) and torch.equal(eager[2], still[2])
+        for n in ("k", "k_scale", "v", "v_scale"):
+            assert torch.equal(getattr(eager[0].cache, n), getattr(still[0].cache, n)), (i, n)
