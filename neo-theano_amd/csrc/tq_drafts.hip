@@ -45,6 +45,7 @@ struct State {
     double a;     // share of q that is gone
     int node;     // last accepted row of the sequence; -1: the sequence has no rows
     int kept;
+    int summed;   // the sums are there already
 };
 
 struct DraftArg {
@@ -95,12 +96,12 @@ __device__ __forceinline__ double readlane_f64(double v, int l) {
 }
 
 // Walks the drafts of a sequence; whole waves, the result uniform.  path: where the accepted rows go, or null.
-// mass(node, a): the sum of what is left, called by all of the block's waves alike (only where q is there and a
-// node has another child after one that was turned down).
+// mass(node, a, w): makes w the sum of what is left, called by all of the block's waves alike (only where q is there and a
+// node has another child after one that was turned down); false: the walk stops there.
 template <class T, class Mass>
 __device__ __forceinline__ State walk(const DraftArg& a, Span s, int32_t* path, Mass mass) {
     const int lane = threadIdx.x & 63;
-    State st{0.0, s.count > 0 ? 0 : -1, s.count > 0 ? 1 : 0};
+    State st{0.0, s.count > 0 ? 0 : -1, s.count > 0 ? 1 : 0, 1};
     if (path && lane == 0 && s.count > 0) path[0] = 0;
     double w = 1.0;
     bool pending = false;  // a child was turned down and w is not yet that of what is left
@@ -137,7 +138,7 @@ __device__ __forceinline__ State walk(const DraftArg& a, Span s, int32_t* path, 
             const int tx = t0 + l;
             bool yes;
             if (a.draft) {
-                if (pending) w = mass(st.node, st.a);
+                if (pending && !mass(st.node, st.a, w)) return st;
                 pending = false;
                 yes = ux * qx * w < px - st.a * qx;
             } else {
@@ -209,49 +210,55 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
     return s;
 }
 
-// Elements i .. i + 3 of a row as f64, zeros from `end` on.
+template <class T>
+using Four = T __attribute__((ext_vector_type(4)));
+
+// Elements i .. i + 3 of a row, zeros from `end` on.
 template <class T, bool kVec>
-__device__ __forceinline__ void load4(const T* row, int i, int end, double (&v)[4]) {
+__device__ __forceinline__ Four<T> load4(const T* row, int i, int end) {
+    Four<T> x{};
     if constexpr (kVec) {  // rows 16-byte aligned (8 for 16-bit types), `end` a multiple of 4
-        typedef T V __attribute__((ext_vector_type(4)));
-        V x{};
-        if (i < end) x = *reinterpret_cast<const V*>(row + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = static_cast<double>(static_cast<float>(x[e]));
+        if (i < end) x = *reinterpret_cast<const Four<T>*>(row + i);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = i + e < end ? static_cast<double>(static_cast<float>(row[i + e])) : 0.0;
+        for (int e = 0; e < 4; ++e)
+            if (i + e < end) x[e] = row[i + e];
     }
+    return x;
 }
 
-// What is left of elements i .. i + 3.  gone: bits of the tokens tried, from the share's start on, or null.
+// What is left of four.  gone: bits of the tokens tried.
+template <class T>
+__device__ __forceinline__ void left4(Four<T> p, Four<T> q, double a, uint32_t gone, double (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        v[e] = gone >> e & 1 ? 0.0 : left_of(static_cast<double>(static_cast<float>(p[e])), static_cast<double>(static_cast<float>(q[e])), a);
+}
 template <class T, bool kVec>
 __device__ __forceinline__ void left4(const T* p, const T* q, double a, int i, int end, uint32_t gone, double (&v)[4]) {
-    double x[4], y[4] = {0, 0, 0, 0};
-    load4<T, kVec>(p, i, end, x);
-    if (q) load4<T, kVec>(q, i, end, y);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = gone >> e & 1 ? 0.0 : left_of(x[e], y[e], a);
+    const Four<T> x = load4<T, kVec>(p, i, end);
+    left4<T>(x, q ? load4<T, kVec>(q, i, end) : Four<T>{}, a, gone, v);
 }
 
-// Sum of what is left over the whole row, by one block; eight loads of a lane in flight (a block alone at work is bound
-// by their latency: 128256 f32 probabilities of two models took 12 us with two).
+// Sum of what is left over the whole row, by one block; kU loads of each model in flight for each lane (a block alone at work is
+// bound by their latency).
 template <class T, bool kVec, int kThreads>
 __device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int vocab, double* lds) {
     constexpr int kU = 4;
     double s = 0.0;
     for (int i0 = 4 * static_cast<int>(threadIdx.x); i0 < vocab; i0 += 4 * kThreads * kU) {
-        double x[kU][4], y[kU][4];
+        Four<T> x[kU], y[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            load4<T, kVec>(p, i0 + 4 * kThreads * u, vocab, x[u]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[u][e] = 0.0;
-            if (q) load4<T, kVec>(q, i0 + 4 * kThreads * u, vocab, y[u]);
+            x[u] = load4<T, kVec>(p, i0 + 4 * kThreads * u, vocab);
+            y[u] = q ? load4<T, kVec>(q, i0 + 4 * kThreads * u, vocab) : Four<T>{};
         }
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-            s += (left_of(x[u][0], y[u][0], a) + left_of(x[u][1], y[u][1], a)) + (left_of(x[u][2], y[u][2], a) + left_of(x[u][3], y[u][3], a));
+        for (int u = 0; u < kU; ++u) {
+            double v[4];
+            left4<T>(x[u], y[u], a, 0, v);
+            s += (v[0] + v[1]) + (v[2] + v[3]);
+        }
     }
     return block_sum<kThreads>(s, lds);
 }
@@ -261,17 +268,25 @@ __device__ __forceinline__ const T* row_of(const void* x, int64_t stride, int ro
     return x ? static_cast<const T*>(x) + row * stride : nullptr;
 }
 
-// Trees with draft probabilities: the walk needs sums of its own.  A block for each sequence.
+// Trees with draft probabilities, a block for each sequence: the walk needs sums on its way.  The first is there (k_left has
+// summed where the walk stops without it, over all CUs); others are rare, and this block's own (128256 f32 probabilities of two
+// models: 10 us, what one CU loads).
 template <class T, bool kVec>
 __global__ __launch_bounds__(kWalkBlock) void k_walk(DraftArg a) {
     __shared__ double lds[kWalkBlock / 64];
-    const int seq = blockIdx.x;
+    const int seq = blockIdx.x, segments = a.shares * (a.share / kSegment);
     const Span s = span_of(a, seq);
+    double first = 0.0;
+    for (int i = threadIdx.x; i < segments; i += kWalkBlock) first += a.sums[static_cast<int64_t>(seq) * segments + i];
     int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
-    const State st = walk<T>(a, s, threadIdx.x < 64 ? path : nullptr, [&](int node, double share) {
-        return row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node),
-                                             row_of<T>(a.draft, a.draft_stride, s.first + node), share, a.vocab, lds);
+    int calls = 0;
+    State st = walk<T>(a, s, threadIdx.x < 64 ? path : nullptr, [&](int node, double share, double& w) {
+        w = calls++ == 0 ? block_sum<kWalkBlock>(first, lds)
+                         : row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node),
+                                                         row_of<T>(a.draft, a.draft_stride, s.first + node), share, a.vocab, lds);
+        return true;
     });
+    st.summed = calls == 0;
     if (threadIdx.x == 0) a.state[seq] = st;
 }
 
@@ -284,9 +299,12 @@ __device__ __forceinline__ void mark_tried(const DraftArg& a, Span s, int node, 
     }
 }
 
-// Block (share, sequence): the sums of what is left of a share.  kWalked: k_walk was there; otherwise every block
-// walks (a few dependent loads) and the first share's block writes the path down.
-template <class T, bool kVec, bool kWalked>
+// When k_left runs: the only time; before k_walk, up to where the walk needs a sum; after it, where it went on.
+enum Stage { kOnly, kBefore, kAfter };
+
+// Block (share, sequence): the sums of what is left of a share, where the walk ends.  Every block walks by itself (a few
+// dependent loads); the first share's writes the path down.
+template <class T, bool kVec, Stage kStage>
 __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     __shared__ State shared;
     __shared__ uint32_t gone[kMaxShare / 32];
@@ -296,12 +314,14 @@ __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
         for (int i = threadIdx.x; i < a.share / 32; i += kBlock) gone[i] = 0;
     if (threadIdx.x < 64) {
         State st;
-        if constexpr (kWalked) {
+        if constexpr (kStage == kAfter) {
             st = a.state[seq];
+            if (st.summed) st.node = -1;  // nothing more to do
         } else {
-            st = walk<T>(a, s, share == 0 ? a.path + static_cast<int64_t>(seq) * a.max_tokens : nullptr,
-                         [](int, double) { return 0.0; });
-            if (share == 0 && threadIdx.x == 0) a.state[seq] = st;
+            const bool write = kStage == kOnly && share == 0;
+            st = walk<T>(a, s, write ? a.path + static_cast<int64_t>(seq) * a.max_tokens : nullptr,
+                         [](int, double, double&) { return false; });
+            if (write && threadIdx.x == 0) a.state[seq] = st;
         }
         if (threadIdx.x == 0) shared = st;
     }
@@ -508,12 +528,12 @@ int check_batch(const char* what, const tq_kv_batch* b, int64_t vocab) {
 
 template <class T, bool kVec>
 void launch_drafts(const DraftArg& a, hipStream_t st) {
-    const bool walk_first = a.draft && a.parents;
-    if (walk_first) {
+    if (a.draft && a.parents) {
+        k_left<T, kVec, kBefore><<<a.batch * a.shares, kBlock, 0, st>>>(a);
         k_walk<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
-        k_left<T, kVec, true><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+        k_left<T, kVec, kAfter><<<a.batch * a.shares, kBlock, 0, st>>>(a);
     } else {
-        k_left<T, kVec, false><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+        k_left<T, kVec, kOnly><<<a.batch * a.shares, kBlock, 0, st>>>(a);
     }
     k_pick<T, kVec><<<a.batch, kBlock, 0, st>>>(a);
 }
