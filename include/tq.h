@@ -594,15 +594,16 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
  * Low-rank adapters of many requests beside one projection: row i of the projection's output
  * gets adapter index[i]'s share (int32, device; outside 0 .. count - 1: none, out = y),
  *   out[i, n] = y[i, n] + scales[a] sum_r b[a, n, r] (sum_k a[a, p, r, k] x[i, k]),  p = n / (N / parts)
- * a: [count, parts, rank, K rounded up to 64], zeros past K; b: [count, N, rank]; both dtype
- * (TQ_DT_BF16 or TQ_DT_F16), dense, 16-byte aligned; rank a multiple of 16 up to 256 (smaller
- * ones padded with zeros); parts (1 to 16, dividing N): slices of the outputs of a fused
+ * a: [count, parts * rank / 16, K' / 32, 16, 32], K' = K rounded up to 64: tiles of 16 ranks (of
+ * part after part) x 32 columns, zeros past K; b: [count, N, rank]; both dtype (TQ_DT_BF16 or
+ * TQ_DT_F16), dense, 16-byte aligned; rank a multiple of 16 up to 256 (smaller ones padded
+ * with zeros); parts (1 to 16, dividing N): slices of the outputs of a fused
  * projection whose adapters read x by themselves; scales f32 [count] or NULL (1).
  * x: f32, bf16 or f16 [M, K]; y and out: f32 [M, N], dense; out may be y, and overlaps nothing
  * else.  Products are exact, sums f32 (the inner one is rounded to f32 and scaled before the
  * outer).  A row depends on its own adapter alone; one with infinities or NaN in x or in its
- * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes, 16-byte
- * aligned, contents need not be initialised. */
+ * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a
+ * few rows of low ranks), 16-byte aligned, contents need not be initialised. */
 typedef struct {
     const void* a;
     const void* b;

@@ -12,7 +12,8 @@
 //
 // The first product is bound by reading x (prompts) or A (a token for each adapter) once; K is split over the
 // waves of a block and over blocks, whose sums the second product adds as it loads t.  The second is bound by reading y
-// and writing out.
+// and writing out.  4093 rows of six adapters' runs, rank 64, 4096 to 14336: 23 + 106 us, the second 4.4 TB/s, where a large copy gets
+// 4.7; 64 rows of 48 adapters of rank 16: 5.7 + 10 us.
 #include <algorithm>
 
 #include "tq_internal.h"
@@ -20,7 +21,7 @@
 namespace tq {
 namespace {
 
-constexpr int kBlock = 256, kWaves = 4;
+constexpr int kBlock = 256, kWaves = 4, kOnceBlock = 512;
 constexpr int kMaxRank = 256, kMaxParts = 16, kKUnit = 64;
 constexpr int kMaxShares = 8;  // shares of K that the second product adds
 constexpr int kStep = 256;  // outputs of a block's step where there are many rows
@@ -210,13 +211,86 @@ struct AdaptArg {
     int per;                                     // second product: turns (steps) of a block
 };
 
+// Adds to acc the products of 16 kT tokens from `first` on with 16 kR ranks of adapter `who` from rank0 on (ranks past the last: the
+// last 16 again), over every step-th 64 columns from k to `end`.  A load takes a tile of 16 ranks x 32 columns, 1 KB in one run (of
+// rows 8 KB apart a block got 20 GB/s), and 64 or 128 bytes of a token.  kAtOnce 1: the next 64 columns are on their way while these are multiplied; more: so many are loaded together
+// (for a block with little to do beside it).
+template <int kX, int kW, int kT, int kR, bool kVec, int kAtOnce>
+__device__ __forceinline__ void low_products(const AdaptArg& a, const Distinct<kT>& set, int who, int first, int rank0, int k, int end, int step,
+                                             f32x4 (&acc)[kT][kR]) {
+    typedef Planes<kX, kW> P;
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, ranks = a.parts * a.rank;
+    const char* xs[kT];
+#pragma unroll
+    for (int s = 0; s < kT; ++s) {
+        // tokens of other adapters read a line that is read anyway
+        const uint64_t on = __ballot(set.mine[s] == who) & 0xFFFF;
+        const int tok = first + 16 * s + (set.mine[s] == who ? col : on ? __ffsll(static_cast<unsigned long long>(on)) - 1 : 0);
+        xs[s] = static_cast<const char*>(a.x) + static_cast<int64_t>(min(tok, a.m - 1)) * a.k * (kX == TQ_DT_F32 ? 4 : 2);
+    }
+    const uint16_t* ws[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int rank = min(rank0 + 16 * r, ranks - 16);
+        ws[r] = a.a + (static_cast<int64_t>(who) * ranks + rank) * a.k_row + 32 * col + 8 * quad;
+    }
+    struct Loads {
+        Raw8<kX> x[kT][2];
+        u32x4 w[kR][2];
+    };
+    auto load = [&](int k) {
+        Loads l;
+        k = min(k, a.k_row - kKUnit);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < kR; ++r) l.w[r][h] = *reinterpret_cast<const u32x4*>(ws[r] + 16 * k + 512 * h);
+#pragma unroll
+            for (int s = 0; s < kT; ++s) l.x[s][h] = fetch<kX, kVec>(xs[s], k + 32 * h + 8 * quad, a.k);
+        }
+        return l;
+    };
+    auto multiply = [&](int k, const Loads& l) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 xp[kT][P::kOfX];
+#pragma unroll
+            for (int s = 0; s < kT; ++s) planes_of<kX, kVec>(l.x[s][h], k + 32 * h + 8 * quad, a.k, xp[s]);
+#pragma unroll
+            for (int r = 0; r < kR; ++r) {
+                u32x4 wp[P::kOfW];
+                planes_of_16(l.w[r][h], wp);
+#pragma unroll
+                for (int s = 0; s < kT; ++s) acc[s][r] = products<P::kF16>(wp, xp[s], acc[s][r]);
+            }
+        }
+    };
+    if constexpr (kAtOnce > 1) {
+        for (; k < end; k += step * kAtOnce) {
+            Loads some[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) some[i] = load(k + i * step);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (k + i * step < end) multiply(k + i * step, some[i]);
+        }
+        return;
+    }
+    if (k >= end) return;
+    Loads now = load(k);
+    for (; k + step < end; k += step) {
+        const Loads next = load(k + step);
+        multiply(k, now);
+        now = next;
+    }
+    multiply(k, now);
+}
+
 // Grid (token tile and one of its gang, rank group): 16 kT tokens, 16 kR ranks.  The tile's distinct adapters, which only the
 // device knows, and as many shares of K as then keep the gang busy are its blocks' units of work.  The waves take
-// 64 of K in turn, a rank's 64 and a token's 64 or 128 bytes side by side in each load; the next 64 are on their way while these
-// are multiplied.
+// 64 of K in turn.
 template <int kX, int kW, int kT, int kR, bool kVec>
 __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
-    typedef Planes<kX, kW> P;
     __shared__ f32x4 part[kWaves][kT * kR][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
     // a gang's blocks are neighbours: they read neighbouring columns of the same rows
@@ -233,67 +307,8 @@ __global__ __launch_bounds__(kBlock) void k_adapt_low(AdaptArg a) {
         const int share = unit & ((1 << bits) - 1), k_begin = min(share * per, a.turns) * kKUnit * kWaves,
                   end = min(k_begin + per * kKUnit * kWaves, a.k_row);
         for (; named <= unit >> bits; ++named) who = set.next();
-        const char* xs[kT];
-#pragma unroll
-        for (int s = 0; s < kT; ++s) {
-            // tokens of other adapters read a line that is read anyway
-            const uint64_t on = __ballot(set.mine[s] == who) & 0xFFFF;
-            const int tok = first + 16 * s + (set.mine[s] == who ? col : on ? __ffsll(static_cast<unsigned long long>(on)) - 1 : 0);
-            xs[s] = static_cast<const char*>(a.x) + static_cast<int64_t>(min(tok, a.m - 1)) * a.k * (kX == TQ_DT_F32 ? 4 : 2);
-        }
-        const uint16_t* ws[kR];
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-            const int rank = min((group * kR + r) * 16, ranks - 16) + col;
-            ws[r] = a.a + (static_cast<int64_t>(who) * ranks + rank) * a.k_row + 8 * quad;
-        }
-        f32x4 acc[kT][kR];
-#pragma unroll
-        for (int s = 0; s < kT; ++s)
-#pragma unroll
-            for (int r = 0; r < kR; ++r) acc[s][r] = f32x4{0, 0, 0, 0};
-        struct Loads {
-            Raw8<kX> x[kT][2];
-            u32x4 w[kR][2];
-        };
-        auto load = [&](int k) {
-            Loads l;
-            k = min(k, a.k_row - kKUnit);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int r = 0; r < kR; ++r) l.w[r][h] = *reinterpret_cast<const u32x4*>(ws[r] + k + 32 * h);
-#pragma unroll
-                for (int s = 0; s < kT; ++s) l.x[s][h] = fetch<kX, kVec>(xs[s], k + 32 * h + 8 * quad, a.k);
-            }
-            return l;
-        };
-        auto multiply = [&](int k, const Loads& l) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4 xp[kT][P::kOfX];
-#pragma unroll
-                for (int s = 0; s < kT; ++s) planes_of<kX, kVec>(l.x[s][h], k + 32 * h + 8 * quad, a.k, xp[s]);
-#pragma unroll
-                for (int r = 0; r < kR; ++r) {
-                    u32x4 wp[P::kOfW];
-                    planes_of_16(l.w[r][h], wp);
-#pragma unroll
-                    for (int s = 0; s < kT; ++s) acc[s][r] = products<P::kF16>(wp, xp[s], acc[s][r]);
-                }
-            }
-        };
-        constexpr int kAll = kKUnit * kWaves;
-        int k = k_begin + kKUnit * wave;
-        if (k < end) {
-            Loads now = load(k);
-            for (; k + kAll < end; k += kAll) {
-                const Loads next = load(k + kAll);
-                multiply(k, now);
-                now = next;
-            }
-            multiply(k, now);
-        }
+        f32x4 acc[kT][kR] = {};
+        low_products<kX, kW, kT, kR, kVec, 1>(a, set, who, first, group * kR * 16, k_begin + kKUnit * wave, end, kKUnit * kWaves, acc);
 #pragma unroll
         for (int s = 0; s < kT; ++s)
 #pragma unroll
@@ -377,87 +392,116 @@ __device__ __forceinline__ f32x4 up_sums(const u32x4 (&raw)[kS], const u32x4 (&t
     return v;
 }
 
-// Few rows, and rows that no 16-byte access reaches.  Grid (token tile, part, range of outputs): a block's waves take tiles of 16
-// outputs in turn, 4 outputs of a token to a lane; up to kU distinct adapters' weights are loaded together, those of the
-// next tile before this one's sums.
-template <int kW, int kT, int kS, int kU, bool kVec>
-__global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
-    __shared__ float t[16 * kT][32 * kS + 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    const int p = blockIdx.y, range = blockIdx.z, first = blockIdx.x * 16 * kT, np = a.np;
-    const int begin = (range * a.per * kWaves + wave) * 16, end = min((range + 1) * a.per * kWaves * 16, np);
-    constexpr int kTurn = 16 * kWaves;
-    Distinct<kT> set(a.index, a.count, first, a.m, lane);
-    int64_t at[kT];
-#pragma unroll
-    for (int s = 0; s < kT; ++s)
-        at[s] = static_cast<int64_t>(min(first + 16 * s + col, a.m - 1)) * a.n + static_cast<int64_t>(p) * np + 4 * quad;
-    auto row_of_b = [&](int n0) { return static_cast<int64_t>(p) * np + min(n0 + col, np - 1); };
-    f32x4 y[kT];
+// Tiles of 16 outputs of part p for the 16 tokens from `first` on, 4 outputs of a token to a lane: up to kU distinct adapters'
+// weights are loaded together, those of the next tile before this one's sums.
+template <int kW, int kS, int kU, bool kVec>
+struct UpTiles {
+    const AdaptArg& a;
+    Distinct<1> set;
+    const int64_t at;  // y and out
+    const int first, p;
+    f32x4 y;
     u32x4 raw[kU][kS];
     int names[kU];
-    auto load = [&](int n0) {  // the tile's y, and its first kU adapters
-#pragma unroll
-        for (int s = 0; s < kT; ++s) {
-            if constexpr (kVec) {
-                y[s] = *reinterpret_cast<const f32x4*>(a.y + at[s] + min(n0, np - 4 - 4 * quad));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[s][i] = a.y[at[s] - 4 * quad + min(n0 + 4 * quad + i, np - 1)];
-            }
-        }
-        set.restart();
+
+    __device__ __forceinline__ UpTiles(const AdaptArg& arg, const Distinct<1>& tokens, int first_token, int part)
+        : a(arg), set(tokens), at(static_cast<int64_t>(min(first_token + col(), arg.m - 1)) * arg.n + static_cast<int64_t>(part) * arg.np + 4 * quad()),
+          first(first_token), p(part) {}
+    static __device__ __forceinline__ int col() { return threadIdx.x & 15; }
+    static __device__ __forceinline__ int quad() { return (threadIdx.x & 63) >> 4; }
+
+    __device__ __forceinline__ void weights(int n0) {  // of the next kU adapters
 #pragma unroll
         for (int i = 0; i < kU; ++i) {
             names[i] = set.next();
-            if (names[i] >= 0) load_b(a, names[i], row_of_b(n0), raw[i]);
+            if (names[i] >= 0) load_b(a, names[i], static_cast<int64_t>(p) * a.np + min(n0 + col(), a.np - 1), raw[i]);
         }
-    };
-    load(begin < end ? begin : begin - 16 * wave);  // (a wave may have no tile: the block's first)
-    sum_t<16 * kT, kS>(a, first, p, t);
-    __syncthreads();
-    u32x4 tp[kT][kS][Planes<TQ_DT_F32, kW>::kOfX];
-    planes_of_t(a, t, tp);
-    for (int n0 = begin; n0 < end; n0 += kTurn) {
-        f32x4 d[kT];
+    }
+    __device__ __forceinline__ void load(int n0) {
+        if constexpr (kVec) {
+            y = *reinterpret_cast<const f32x4*>(a.y + at + min(n0, a.np - 4 - 4 * quad()));
+        } else {
 #pragma unroll
-        for (int s = 0; s < kT; ++s) d[s] = f32x4{-0.f, -0.f, -0.f, -0.f};  // what leaves y as it is
-        while (true) {
+            for (int i = 0; i < 4; ++i) y[i] = a.y[at - 4 * quad() + min(n0 + 4 * quad() + i, a.np - 1)];
+        }
+        set.restart();
+        weights(n0);
+    }
+    // The tiles from `begin`, which load() has, to `end`, every turn-th output.
+    __device__ __forceinline__ void run(int begin, int end, int turn, const u32x4 (&tp)[kS][Planes<TQ_DT_F32, kW>::kOfX]) {
+        for (int n0 = begin; n0 < end; n0 += turn) {
+            f32x4 d{-0.f, -0.f, -0.f, -0.f};  // what leaves y as it is
+            while (names[0] >= 0) {
 #pragma unroll
-            for (int i = 0; i < kU; ++i) {
-                if (names[i] < 0) break;
+                for (int i = 0; i < kU; ++i) {
+                    if (names[i] < 0) break;
+                    const f32x4 v = up_sums<kW>(raw[i], tp);
 #pragma unroll
-                for (int s = 0; s < kT; ++s) {
-                    const bool mine = set.mine[s] == names[i];
-                    if (!__ballot(mine)) continue;
-                    const f32x4 v = up_sums<kW>(raw[i], tp[s]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[s][e] = mine ? v[e] : d[s][e];
+                    for (int e = 0; e < 4; ++e) d[e] = set.mine[0] == names[i] ? v[e] : d[e];
                 }
+                weights(n0);
             }
-            names[0] = set.next();
-            if (names[0] < 0) break;
-#pragma unroll
-            for (int i = 1; i < kU; ++i) names[i] = set.next();
-#pragma unroll
-            for (int i = 0; i < kU; ++i)
-                if (names[i] >= 0) load_b(a, names[i], row_of_b(n0), raw[i]);
-        }
-#pragma unroll
-        for (int s = 0; s < kT; ++s) d[s] += y[s];
-        if (n0 + kTurn < end) load(n0 + kTurn);
-#pragma unroll
-        for (int s = 0; s < kT; ++s) {
-            if (first + 16 * s + col >= a.m) continue;
+            d += y;
+            if (n0 + turn < end) load(n0 + turn);
+            if (first + col() >= a.m) continue;
             if constexpr (kVec) {
-                if (n0 + 4 * quad < np) *reinterpret_cast<f32x4*>(a.out + at[s] + n0) = d[s];
+                if (n0 + 4 * quad() < a.np) *reinterpret_cast<f32x4*>(a.out + at + n0) = d;
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (n0 + 4 * quad + i < np) a.out[at[s] + n0 + i] = d[s][i];
+                    if (n0 + 4 * quad() + i < a.np) a.out[at + n0 + i] = d[i];
             }
         }
     }
+};
+
+// Few rows, and rows that no 16-byte access reaches.  Grid (token tile, part, range of outputs): a block's waves take tiles of 16
+// outputs in turn.
+template <int kW, int kS, int kU, bool kVec>
+__global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
+    __shared__ float t[16][32 * kS + 4];
+    const int wave = threadIdx.x >> 6, p = blockIdx.y, first = blockIdx.x * 16, from = blockIdx.z * a.per * kWaves * 16;
+    const int begin = from + 16 * wave, end = min(from + a.per * kWaves * 16, a.np);
+    UpTiles<kW, kS, kU, kVec> tiles(a, Distinct<1>(a.index, a.count, first, a.m, threadIdx.x & 63), first, p);
+    tiles.load(begin < end ? begin : from);  // (a wave may have no tile: the block's first)
+    sum_t<16, kS>(a, first, p, t);
+    __syncthreads();
+    u32x4 tp[1][kS][Planes<TQ_DT_F32, kW>::kOfX];
+    planes_of_t(a, t, tp);
+    tiles.run(begin, end, 16 * kWaves, tp[0]);
+}
+
+// A token or a few and low ranks: both products in one launch, without a workspace.  Grid (range of outputs, part): every block
+// forms t of its part by itself, its waves 64 columns of K in turn, and then its outputs.  For the GPU that is no
+// less than two launches (a token in f32, rank 16, 4096 x 4096: 8.3 us against 8.1; another adapter is 5 us more), for the host a launch and a
+// buffer less (8.5 us a call against 11.7).
+template <int kX, int kW, int kR, bool kVecX, bool kVecY>
+__global__ __launch_bounds__(kOnceBlock) void k_adapt_once(AdaptArg a) {
+    constexpr int kOnceWaves = kOnceBlock / 64;
+    __shared__ f32x4 part[kOnceWaves][kR][64];
+    __shared__ float t[16][32 + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4, p = blockIdx.y;
+    const int from = blockIdx.x * kOnceWaves * 16, begin = from + 16 * wave, end = min(from + kOnceWaves * 16, a.np);
+    Distinct<1> set(a.index, a.count, 0, a.m, lane);
+    UpTiles<kW, 1, 4, kVecY> tiles(a, set, 0, p);
+    tiles.load(begin < end ? begin : from);
+    for (int who; (who = set.next()) >= 0;) {
+        f32x4 acc[1][kR] = {};
+        low_products<kX, kW, 1, kR, kVecX, kR == 1 ? 4 : 2>(a, set, who, 0, p * a.rank, kKUnit * wave, a.k_row, kKUnit * kOnceWaves, acc);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) part[wave][r][lane] = acc[0][r];
+        __syncthreads();
+        if (wave < kR && set.mine[0] == who) {
+            f32x4 v = part[0][wave][lane];
+#pragma unroll
+            for (int w = 1; w < kOnceWaves; ++w) v += part[w][wave][lane];
+            *reinterpret_cast<f32x4*>(&t[col][16 * wave + 4 * quad]) = v * (a.scales ? a.scales[who] : 1.f);
+        }
+        __syncthreads();
+    }
+    u32x4 tp[1][1][Planes<TQ_DT_F32, kW>::kOfX];
+    planes_of_t(a, t, tp);  // (of tokens without an adapter: anything, and left out)
+    tiles.run(begin, end, kOnceWaves * 16, tp[0]);
 }
 
 // Many rows.  Grid (range of outputs, part, token tile): 16 kT tokens and 256 outputs a step, 64 for each wave.  The
@@ -601,18 +645,18 @@ void launch_low_tokens(const AdaptArg& a, const Cut& c, bool vec, dim3 grid, hip
     else launch_low_ranks<kX, kW, 2>(a, c.ranks, vec, grid, st);
 }
 
-// Tiles of 16 kT tokens, ranges so that there are about four blocks for each CU.
-template <int kW, int kT, int kS, int kU>
+// Tiles of 16 tokens, ranges so that there are about four blocks for each CU.
+template <int kW, int kS, int kU>
 int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
-    const int64_t turns = (a.np + 16 * kWaves - 1) / (16 * kWaves), tiles = (a.m + 16 * kT - 1) / (16 * kT);
+    const int64_t turns = (a.np + 16 * kWaves - 1) / (16 * kWaves), tiles = (a.m + 15) / 16;
     a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, tiles * a.parts * turns / (4 * device_cu_count()))));
     const int64_t ranges = (turns + a.per - 1) / a.per;
     TQ_REQUIRE(tiles <= kMaxBlocks && ranges <= 65535, "%s: %d tokens, %d outputs are more than a launch holds", what, a.m, a.n);
     const dim3 blocks(static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.parts), static_cast<uint32_t>(ranges));
     if (vec)
-        k_adapt_up<kW, kT, kS, kU, true><<<blocks, kBlock, 0, st>>>(a);
+        k_adapt_up<kW, kS, kU, true><<<blocks, kBlock, 0, st>>>(a);
     else
-        k_adapt_up<kW, kT, kS, kU, false><<<blocks, kBlock, 0, st>>>(a);
+        k_adapt_up<kW, kS, kU, false><<<blocks, kBlock, 0, st>>>(a);
     return check_launch(what);
 }
 
@@ -641,6 +685,36 @@ int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
     return check_launch(what);
 }
 
+// Calls of one launch.
+constexpr int64_t kOnceWeights = 1 << 16;  // of t's that a block forms
+bool in_one_launch(const tq_adapters* a, int64_t m) {
+    return m <= 16 && a->rank <= 32 && m * a->rank * a->k <= kOnceWeights;
+}
+
+template <int kX, int kW, int kR>
+void launch_once_vec(const AdaptArg& a, bool vec_x, bool vec_y, dim3 blocks, hipStream_t st) {
+    if (vec_x && vec_y) k_adapt_once<kX, kW, kR, true, true><<<blocks, kOnceBlock, 0, st>>>(a);
+    else if (vec_x) k_adapt_once<kX, kW, kR, true, false><<<blocks, kOnceBlock, 0, st>>>(a);
+    else if (vec_y) k_adapt_once<kX, kW, kR, false, true><<<blocks, kOnceBlock, 0, st>>>(a);
+    else k_adapt_once<kX, kW, kR, false, false><<<blocks, kOnceBlock, 0, st>>>(a);
+}
+
+template <int kW>
+int launch_once(const AdaptArg& a, int dtype, bool vec_x, bool vec_y, hipStream_t st, const char* what) {
+    const dim3 blocks(static_cast<uint32_t>((a.np + kOnceBlock / 4 - 1) / (kOnceBlock / 4)), static_cast<uint32_t>(a.parts));
+    clear_error();
+    if (a.rank == 16) {
+        if (dtype == TQ_DT_F32) launch_once_vec<TQ_DT_F32, kW, 1>(a, vec_x, vec_y, blocks, st);
+        else if (dtype == TQ_DT_BF16) launch_once_vec<TQ_DT_BF16, kW, 1>(a, vec_x, vec_y, blocks, st);
+        else launch_once_vec<TQ_DT_F16, kW, 1>(a, vec_x, vec_y, blocks, st);
+    } else {
+        if (dtype == TQ_DT_F32) launch_once_vec<TQ_DT_F32, kW, 2>(a, vec_x, vec_y, blocks, st);
+        else if (dtype == TQ_DT_BF16) launch_once_vec<TQ_DT_BF16, kW, 2>(a, vec_x, vec_y, blocks, st);
+        else launch_once_vec<TQ_DT_F16, kW, 2>(a, vec_x, vec_y, blocks, st);
+    }
+    return check_launch(what);
+}
+
 template <int kW>
 int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool vec_y, dim3 low, hipStream_t st, const char* what) {
     clear_error();
@@ -659,10 +733,10 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
         if (a.rank > 32) return launch_up_rows<kW, 2, 2>(a, st, what);
         return launch_up_rows<kW, 2, 1>(a, st, what);
     }
-    if (a.rank > 128) return launch_up<kW, 1, 8, 2>(a, vec_y, st, what);
-    if (a.rank > 64) return launch_up<kW, 1, 4, 4>(a, vec_y, st, what);
-    if (a.rank > 32) return launch_up<kW, 1, 2, 4>(a, vec_y, st, what);
-    return launch_up<kW, 1, 1, 4>(a, vec_y, st, what);
+    if (a.rank > 128) return launch_up<kW, 8, 2>(a, vec_y, st, what);
+    if (a.rank > 64) return launch_up<kW, 4, 4>(a, vec_y, st, what);
+    if (a.rank > 32) return launch_up<kW, 2, 4>(a, vec_y, st, what);
+    return launch_up<kW, 1, 4>(a, vec_y, st, what);
 }
 
 }  // namespace
@@ -673,7 +747,7 @@ extern "C" {
 int64_t tq_adapters_workspace_bytes(const tq_adapters* adapters, int64_t m) {
     using namespace tq;
     if (check_adapters("tq_adapters_add", adapters, m) != TQ_OK) return -1;
-    return m == 0 ? 0 : shares_bytes(cut_of(adapters, m)) + kMaxShares * m * adapters->parts * adapters->rank * 4;
+    return m == 0 || in_one_launch(adapters, m) ? 0 : shares_bytes(cut_of(adapters, m)) + kMaxShares * m * adapters->parts * adapters->rank * 4;
 }
 
 int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64_t m, const int32_t* index, const float* y,
@@ -689,8 +763,8 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     TQ_REQUIRE(aligned(x, size) && aligned(index, 4) && aligned(y, 4) && aligned(out, 4), "%s: a pointer is not aligned to its elements",
                what);
     const int64_t need = tq_adapters_workspace_bytes(adapters, m);
-    TQ_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), "%s: workspace of %lld bytes, 16-byte aligned, needed",
-               what, (long long)need);
+    TQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
+               "%s: workspace of %lld bytes, 16-byte aligned, needed", what, (long long)need);
     const Cut c = cut_of(adapters, m);
     AdaptArg a{};
     a.x = x;
@@ -698,8 +772,6 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.a = static_cast<const uint16_t*>(adapters->a);
     a.b = static_cast<const uint16_t*>(adapters->b);
     a.scales = adapters->scales;
-    a.shares = static_cast<int32_t*>(workspace);
-    a.t = reinterpret_cast<float*>(static_cast<char*>(workspace) + shares_bytes(c));
     a.y = y;
     a.out = out;
     a.m = static_cast<int>(m);
@@ -710,13 +782,18 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.parts = static_cast<int>(adapters->parts);
     a.rank = static_cast<int>(adapters->rank);
     a.np = static_cast<int>(adapters->n / adapters->parts);
+    const bool vec_x = aligned(x, 16) && adapters->k % 8 == 0;
+    const bool vec_y = aligned(y, 16) && aligned(out, 16) && a.np % 4 == 0;
+    if (need == 0)
+        return adapters->dtype == TQ_DT_F16 ? launch_once<TQ_DT_F16>(a, dtype, vec_x, vec_y, as_hip(stream), what)
+                                            : launch_once<TQ_DT_BF16>(a, dtype, vec_x, vec_y, as_hip(stream), what);
+    a.shares = static_cast<int32_t*>(workspace);
+    a.t = reinterpret_cast<float*>(static_cast<char*>(workspace) + shares_bytes(c));
     a.low_shift = c.tokens == 16 ? 4 : 5;
     a.turns = (a.k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
     a.gang_shift = c.gang_shift;
     TQ_REQUIRE(c.tiles << c.gang_shift <= kMaxBlocks, "%s: %lld tokens are more than a launch holds", what, (long long)m);
     const dim3 low(static_cast<uint32_t>(c.tiles << c.gang_shift), static_cast<uint32_t>(c.groups));
-    const bool vec_x = aligned(x, 16) && adapters->k % 8 == 0;
-    const bool vec_y = aligned(y, 16) && aligned(out, 16) && a.np % 4 == 0;
     return adapters->dtype == TQ_DT_F16 ? launch_typed<TQ_DT_F16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what)
                                         : launch_typed<TQ_DT_BF16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what);
 }

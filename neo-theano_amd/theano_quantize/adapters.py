@@ -23,8 +23,8 @@ class Adapters(_Fixed):
 
     a: [count, rank, K], or [count, parts, rank, K] for a fused projection whose outputs are `parts`
     equal slices with adapters of their own (q, k and v); b: [count, N, rank]; bf16 or f16 device tensors,
-    rank up to 256.  scales: float32 [count] or None (1).  Where rank is no multiple of 16 or K none of 64, padded
-    copies are held in place of a and b."""
+    rank up to 256.  scales: float32 [count] or None (1).  Held are a in tiles of 16 ranks x 32 inputs (as the kernels load
+    it, padded with zeros) and b, padded to ranks of 16 where it has to be."""
 
     def __init__(self, a, b, scales=None):
         _device(a, "Adapters: a"), _device(b, "Adapters: b")
@@ -41,10 +41,11 @@ class Adapters(_Fixed):
                 raise InvalidArgument(f"Adapters: {scales.shape[0]} scales for {a.shape[0]} adapters")
         count, parts, rank, k = a.shape
         n, row, ranks = b.shape[1], (k + 63) // 64 * 64, (rank + 15) // 16 * 16
-        if ranks != rank or row != k or not a.is_contiguous() or a.data_ptr() % 16:
-            held = a.new_zeros(count, parts, ranks, row)
-            held[:, :, :rank, :k] = a
-            a = held
+        held = a.new_empty(count, parts * ranks // 16, row // 32, 16, 32)
+        if ranks != rank or row != k:
+            a = torch.nn.functional.pad(a, (0, row - k, 0, ranks - rank))
+        held.copy_(a.reshape(count, parts * ranks // 16, 16, row // 32, 32).transpose(2, 3))
+        a = held
         if ranks != rank or not b.is_contiguous() or b.data_ptr() % 16:
             held = b.new_zeros(count, n, ranks)
             held[..., :rank] = b
@@ -66,7 +67,7 @@ class Adapters(_Fixed):
         dev = torch.device("cuda", torch.cuda.current_device())
         rank = (max(b.shape[1] for _, b in pairs) + 15) // 16 * 16
         parts, _, k = pairs[0][0].shape
-        a = torch.zeros(len(pairs), parts, rank, (k + 63) // 64 * 64, dtype=dtype, device=dev)[..., :k]
+        a = torch.zeros(len(pairs), parts, rank, k, dtype=dtype, device=dev)
         b = torch.zeros(len(pairs), pairs[0][1].shape[0], rank, dtype=dtype, device=dev)
         for i, (x, y) in enumerate(pairs):
             a[i, :, :x.shape[1]] = x
@@ -95,7 +96,7 @@ class Adapters(_Fixed):
         elif out is not y and (not _dense(out, torch.float32, 2, dev) or out.shape != (m, n)):
             raise InvalidArgument(f"Adapters.add: out must be contiguous float32 [{m}, {n}] on the current GPU")
         nb = _abi.entry("tq_adapters_workspace_bytes")(self._desc, m)
-        ws = y.new_empty(max(nb // 4, 1))
+        ws = y.new_empty(nb // 4) if nb else None
         _abi.call("tq_adapters_add", self._desc, x.data_ptr(), code, m, index.data_ptr(), y.data_ptr(), out.data_ptr(),
-                  ws.data_ptr(), nb, stream())
+                  None if ws is None else ws.data_ptr(), nb, stream())
         return out

@@ -33,7 +33,7 @@ def test_the_packed_descriptor_is_the_structure(abi):
 
 
 def test_refusals(abi):
-    def no(d, x=256, dtype=2, m=3, index=256, y=256, out=256, ws=256, nb=1 << 40):
+    def no(d, x=256, dtype=2, m=30, index=256, y=256, out=256, ws=256, nb=1 << 40):
         refuse(abi, "tq_adapters_add", at(d), x, dtype, m, index, y, out, ws, nb, None)
 
     for kw in (dict(a=None), dict(a=264), dict(b=None), dict(b=264), dict(scales=258), dict(count=0), dict(count=(1 << 20) + 1), dict(parts=0),
@@ -46,8 +46,9 @@ def test_refusals(abi):
                dict(out=None), dict(out=258), dict(ws=None), dict(ws=264), dict(nb=100)):
         no(desc(), **kw)
     no(desc(parts=16, rank=256, n=1 << 24), m=1 << 30, nb=1 << 62)  # more blocks than a launch has
-    need = abi.entry("tq_adapters_workspace_bytes")(at(desc()), 3)
-    assert need >= 3 * 64 * 4 and need % 16 == 0
+    need = abi.entry("tq_adapters_workspace_bytes")(at(desc()), 30)
+    assert need >= 30 * 64 * 4 and need % 16 == 0
+    assert abi.entry("tq_adapters_workspace_bytes")(at(desc()), 3) == 0 < abi.entry("tq_adapters_workspace_bytes")(at(desc(k=1 << 10)), 3)
     no(desc(), nb=need - 1)
     abi.call("tq_adapters_add", at(desc()), None, 2, 0, None, None, None, None, 0, None)
     assert abi.entry("tq_adapters_workspace_bytes")(at(desc()), 0) == 0
@@ -346,14 +347,15 @@ def test_outputs_and_inputs_past_32_bit_offsets(tq):
         x = torch.empty(m, k, dtype=dtype, device="cuda").normal_(generator=g)
         y = torch.empty(m, n, device="cuda").normal_(generator=g)
         a = (torch.randn(3, 16, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
-        ad = tq.Adapters(a, torch.randn(3, n, 16, generator=g, device="cuda").bfloat16())
+        b = torch.randn(3, n, 16, generator=g, device="cuda").bfloat16()
+        ad = tq.Adapters(a, b)
         index = torch.randint(-1, 3, (m,), generator=g, device="cuda", dtype=torch.int32)
         width = max(k, n)
         rows = sorted({0, m - 40, max((1 << 31) // width - 20, 0), max((1 << 32) // width - 20, 0)} & set(range(m - 39)))
         before = [y[r:r + 40].clone() for r in rows]
         ad.add(x, index, y, out=y)
         for r, part in zip(rows, before):
-            ref, tol = reference(x[r:r + 40], part, ad.a[:, :, :, :k], ad.b, None, index[r:r + 40])
+            ref, tol = reference(x[r:r + 40], part, a[:, None], b, None, index[r:r + 40])
             assert ((y[r:r + 40].double() - ref).abs() <= tol).all(), r
 
 
