@@ -585,7 +585,7 @@ struct Cut {
 };
 
 // Up to this many rows the first product's tiles are of 16 tokens, then of 32 (K 4096, rank 64, six adapters' runs of rows, both
-// products to 14336 outputs: 2048 rows 81 us with 16, 85 with 32; 4096 rows 144 and 140).
+// products to 14336 outputs: 2048 rows 76 us with 16, 82 with 32; 4096 rows 138 and 134).
 constexpr int kFewRows = 2048;
 
 Cut cut_of(const tq_adapters* a, int64_t m) {
@@ -596,7 +596,8 @@ Cut cut_of(const tq_adapters* a, int64_t m) {
     c.ranks = rank_tiles == 1 ? 1 : rank_tiles == 2 ? 2 : 4;
     c.groups = static_cast<int>((rank_tiles + c.ranks - 1) / c.ranks);
     c.tiles = (m + c.tokens - 1) / c.tokens;
-    // about four blocks for each CU (4093 rows of one adapter each tile, rank 64: 38 us with one, 32 with two, 28 with four),
+    // about four blocks for each CU (the first product of 4093 rows, rank 64, before its weights lay in tiles: 38 us with one, 32 with two,
+    // 28 with four),
     // no more than a tile can have adapters and shares
     const int64_t blocks = c.tiles * c.groups;
     const int64_t gang = std::min<int64_t>(4 * device_cu_count() / blocks,
@@ -723,10 +724,10 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
     else launch_low_tokens<TQ_DT_F16, kW>(a, c, vec_x, low, st);
     const int rc = check_launch(what);
     if (rc != TQ_OK) return rc;
-    // the form of many rows from 2^23 outputs on (rank 16: 1024 x 4096 20.4 us against 21.8, 1024 x 14336 49.6 against 41.8), with more
-    // ranks from 2^20 on (rank 64: 64 x 14336 19.6 against 20.1, 128 x 14336 31.3 against 23.1, 512 x 4096 30.5 against 27.5) or 3 2^18
-    // (rank 128: 128 x 4096 15.5 against 17.8, 64 x 14336 22.7 against 18.3)
-    const int64_t many = a.rank > 64 ? 3 << 18 : a.rank > 32 ? 1 << 20 : 1 << 23;
+    // the form of many rows from 2^23 outputs on (rank 16, direct / rows: 512 x 14336 23.3 / 25.4 us, 1024 x 14336 45.4 / 40.6), with more
+    // ranks from 3 2^19 (rank 64: 256 x 4096 19.1 / 21.4, 128 x 14336 23.4 / 21.4) or 3 2^18 on (rank 128: 128 x 4096 19.4 / 21.6, 64 x
+    // 14336 25.0 / 21.2); six runs of rows, both products
+    const int64_t many = a.rank > 64 ? 3 << 18 : a.rank > 32 ? 3 << 19 : 1 << 23;
     if (vec_y && static_cast<int64_t>(a.m) * a.n >= many && a.m <= 16 * 65535) {
         if (a.rank > 128) return launch_up_rows<kW, 1, 8>(a, st, what);
         if (a.rank > 64) return launch_up_rows<kW, 1, 4>(a, st, what);
