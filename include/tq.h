@@ -600,8 +600,8 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
  * with zeros); parts (1 to 16, dividing N): slices of the outputs of a fused
  * projection whose adapters read x by themselves; scales f32 [count] or NULL (1).
  * x: f32, bf16 or f16 [M, K]; y and out: f32 [M, N], dense; out may be y, and overlaps nothing
- * else.  Products are exact, sums f32 (the inner one is rounded to f32 and scaled before the
- * outer).  A row depends on its own adapter alone; one with infinities or NaN in x or in its
+ * else.  Products are exact (of f32 and f16: to 2^-24), sums f32 (the inner one is rounded to f32
+ * and scaled before the outer).  A row depends on its own adapter alone; one with infinities or NaN in x or in its
  * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a
  * few rows of low ranks), 16-byte aligned, contents need not be initialised. */
 typedef struct {
@@ -611,6 +611,9 @@ typedef struct {
     int64_t count, parts, rank, k, n;
     int32_t dtype;
 } tq_adapters;
+/* 16-bit weights [groups, rank, K] (groups: count * parts, any rank up to 256) to such tiles:
+ * tiled [groups, rank rounded up to 16 / 16, K' / 32, 16, 32], 16-byte aligned. */
+int tq_repack_adapters_tiled(const void* a, int64_t groups, int64_t rank, int64_t k, void* tiled, tq_stream_t stream);
 int64_t tq_adapters_workspace_bytes(const tq_adapters* adapters, int64_t m);
 int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64_t m, const int32_t* index, const float* y,
                     float* out, void* workspace, int64_t workspace_bytes, tq_stream_t stream);

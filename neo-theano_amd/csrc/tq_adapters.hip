@@ -577,6 +577,23 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     }
 }
 
+// Eight elements of a tile a lane: a [groups, rank, K] to tiles of 16 x 32, zeros past rank and K.
+__global__ __launch_bounds__(kBlock) void k_tile(const uint16_t* a, int64_t units, int rank, int k, int rank_tiles, int k_tiles, u32x4* out) {
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; u < units; u += static_cast<int64_t>(gridDim.x) * kBlock) {
+        const int64_t tile = u / 64, row_tile = tile / k_tiles, group = row_tile / rank_tiles;
+        const int r = static_cast<int>(row_tile - group * rank_tiles) * 16 + (u % 64) / 4,
+                  k0 = static_cast<int>(tile - row_tile * k_tiles) * 32 + (u % 4) * 8;
+        u32x4 v{};
+        if (r < rank) {
+            const uint16_t* row = a + (group * rank + r) * k;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k0 + i < k) v[i / 2] |= static_cast<uint32_t>(row[k0 + i]) << (16 * (i & 1));
+        }
+        out[u] = v;
+    }
+}
+
 // How the first product is cut.
 struct Cut {
     bool few;
@@ -652,7 +669,7 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
     const int64_t turns = (a.np + 16 * kWaves - 1) / (16 * kWaves), tiles = (a.m + 15) / 16;
     a.per = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, tiles * a.parts * turns / (4 * device_cu_count()))));
     const int64_t ranges = (turns + a.per - 1) / a.per;
-    TQ_REQUIRE(tiles <= kMaxBlocks && ranges <= 65535, "%s: %d tokens, %d outputs are more than a launch holds", what, a.m, a.n);
+    // (N is at most 2^24: up to 32768 ranges)
     const dim3 blocks(static_cast<uint32_t>(tiles), static_cast<uint32_t>(a.parts), static_cast<uint32_t>(ranges));
     if (vec)
         k_adapt_up<kW, kS, kU, true><<<blocks, kBlock, 0, st>>>(a);
@@ -676,7 +693,6 @@ int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
             a.per = static_cast<int>(per);
         }
     }
-    TQ_REQUIRE(tiles <= 65535, "%s: %d tokens are more than a launch holds", what, a.m);
     const dim3 blocks(static_cast<uint32_t>((steps + a.per - 1) / a.per), static_cast<uint32_t>(a.parts), static_cast<uint32_t>(tiles));
     // outputs that the L2 caches (4 MB for each XCD) would not hold anyway
     if (static_cast<int64_t>(a.m) * a.n * 4 >= int64_t(32) << 20)
@@ -745,6 +761,21 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
 
 extern "C" {
 
+int tq_repack_adapters_tiled(const void* a, int64_t groups, int64_t rank, int64_t k, void* tiled, tq_stream_t stream) {
+    using namespace tq;
+    static const char* what = "tq_repack_adapters_tiled";
+    TQ_REQUIRE(groups >= 0 && groups <= int64_t(16) << 20 && rank >= 1 && rank <= kMaxRank && k >= 1 && k <= 1 << 24,
+               "%s: %lld groups, rank=%lld, K=%lld", what, (long long)groups, (long long)rank, (long long)k);
+    if (groups == 0) return TQ_OK;
+    TQ_REQUIRE(a && tiled && aligned(a, 2) && aligned(tiled, 16), "%s: null or unaligned pointer", what);
+    const int64_t rank_tiles = (rank + 15) / 16, k_tiles = (k + kKUnit - 1) / kKUnit * 2, units = groups * rank_tiles * k_tiles * 64;
+    clear_error();
+    k_tile<<<static_cast<int>(std::min<int64_t>((units + kBlock - 1) / kBlock, 16 * device_cu_count())), kBlock, 0, as_hip(stream)>>>(
+        static_cast<const uint16_t*>(a), units, static_cast<int>(rank), static_cast<int>(k), static_cast<int>(rank_tiles),
+        static_cast<int>(k_tiles), static_cast<u32x4*>(tiled));
+    return check_launch(what);
+}
+
 int64_t tq_adapters_workspace_bytes(const tq_adapters* adapters, int64_t m) {
     using namespace tq;
     if (check_adapters("tq_adapters_add", adapters, m) != TQ_OK) return -1;
@@ -793,7 +824,8 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     a.low_shift = c.tokens == 16 ? 4 : 5;
     a.turns = (a.k_row + kKUnit * kWaves - 1) / (kKUnit * kWaves);
     a.gang_shift = c.gang_shift;
-    TQ_REQUIRE(c.tiles << c.gang_shift <= kMaxBlocks, "%s: %lld tokens are more than a launch holds", what, (long long)m);
+    TQ_REQUIRE(c.tiles << c.gang_shift <= kMaxBlocks && (m + 15) / 16 <= kMaxBlocks, "%s: %lld tokens are more than a launch holds", what,
+               (long long)m);
     const dim3 low(static_cast<uint32_t>(c.tiles << c.gang_shift), static_cast<uint32_t>(c.groups));
     return adapters->dtype == TQ_DT_F16 ? launch_typed<TQ_DT_F16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what)
                                         : launch_typed<TQ_DT_BF16>(a, c, dtype, vec_x, vec_y, low, as_hip(stream), what);

@@ -525,6 +525,8 @@ int check_axes(const char* what, const tq_rotary_axes* x, const tq_rotary* r, Ax
     *out = AxesArg{{0, 0}, 0, 1};
     if (!x) return TQ_OK;
     TQ_REQUIRE(x->axes >= 1 && x->axes <= kMaxAxes, "%s: axes=%lld is not in 1..4", what, (long long)x->axes);
+    TQ_REQUIRE(r->rotary_dim <= kKvMaxHeadDim, "%s: axes are given for planes of up to 128 elements, not rotary_dim=%lld", what,
+               (long long)r->rotary_dim);
     TQ_REQUIRE(x->position_stride >= 0, "%s: position_stride=%lld", what, (long long)x->position_stride);
     *out = AxesArg{{x->planes[0], x->planes[1]}, x->position_stride, static_cast<int>(x->axes)};
     for (int64_t i = 0; i < r->rotary_dim / 2; ++i)

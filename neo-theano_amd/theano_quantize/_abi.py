@@ -117,6 +117,7 @@ SIGNATURES = {
     "tq_kv_read": [_p, _p, _int, _p, _p, _p],
     "tq_kv_attention_workspace_bytes": [_p, _p, _i64],
     "tq_kv_attention": [_p, _p, _p, _int, _p, _i64, ctypes.c_float, _p, _i64, _p, _p],
+    "tq_repack_adapters_tiled": [_p, _i64, _i64, _i64, _p, _p],
     "tq_adapters_workspace_bytes": [_p, _i64],
     "tq_adapters_add": [_p, _p, _int, _i64, _p, _p, _p, _p, _i64, _p],
     "tq_verify_drafts_workspace_bytes": [_p, _i64],

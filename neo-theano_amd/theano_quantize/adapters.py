@@ -23,11 +23,11 @@ class Adapters(_Fixed):
 
     a: [count, rank, K], or [count, parts, rank, K] for a fused projection whose outputs are `parts`
     equal slices with adapters of their own (q, k and v); b: [count, N, rank]; bf16 or f16 device tensors,
-    rank up to 256.  scales: float32 [count] or None (1).  Held are a in tiles of 16 ranks x 32 inputs (as the kernels load
-    it, padded with zeros) and b, padded to ranks of 16 where it has to be."""
+    rank up to 256.  scales: float32 [count] or None (1).  Held are a copy of a in tiles of 16 ranks x 32 inputs (as the
+    kernels load it, padded with zeros), and b, or a copy padded to ranks of 16 where it has to be."""
 
     def __init__(self, a, b, scales=None):
-        _device(a, "Adapters: a"), _device(b, "Adapters: b")
+        a, b = _device(a, "Adapters: a").detach(), _device(b, "Adapters: b").detach()
         if a.dim() == 3:
             a = a.unsqueeze(1)
         if a.dtype not in (torch.bfloat16, torch.float16) or b.dtype != a.dtype or a.dim() != 4 or b.dim() != 3 or \
@@ -42,9 +42,8 @@ class Adapters(_Fixed):
         count, parts, rank, k = a.shape
         n, row, ranks = b.shape[1], (k + 63) // 64 * 64, (rank + 15) // 16 * 16
         held = a.new_empty(count, parts * ranks // 16, row // 32, 16, 32)
-        if ranks != rank or row != k:
-            a = torch.nn.functional.pad(a, (0, row - k, 0, ranks - rank))
-        held.copy_(a.reshape(count, parts * ranks // 16, 16, row // 32, 32).transpose(2, 3))
+        a = a.contiguous()
+        _abi.call("tq_repack_adapters_tiled", a.data_ptr(), count * parts, rank, k, held.data_ptr(), stream())
         a = held
         if ranks != rank or not b.is_contiguous() or b.data_ptr() % 16:
             held = b.new_zeros(count, n, ranks)

@@ -390,3 +390,28 @@ def test_sizes_on_both_sides_of_every_form(tq, m, n, r):
         assert ((tq.Adapters(a, b, scales).add(x, index, y).double() - ref).abs() <= tol).all()
     index.fill_(-1)
     assert torch.equal(tq.Adapters(a, b, scales).add(x, index, y), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,parts,rank,k", [(1, 1, 1, 1), (3, 2, 16, 64), (2, 3, 17, 100), (5, 1, 256, 65), (1, 16, 8, 4097)])
+def test_the_tiles_of_a(tq, count, parts, rank, k):
+    import torch
+
+    a = torch.randn(count, parts, rank, k, device="cuda").bfloat16()
+    ranks, row = (rank + 15) // 16 * 16, (k + 63) // 64 * 64
+    full = torch.zeros(count, parts, ranks, row, dtype=a.dtype, device="cuda")
+    full[:, :, :rank, :k] = a
+    held = tq.Adapters(a, torch.zeros(count, parts, rank, dtype=a.dtype, device="cuda")).a
+    assert torch.equal(held, full.view(count, parts * ranks // 16, 16, row // 32, 32).transpose(2, 3))
+    back = torch.randn(count, rank, parts, k, device="cuda").half().transpose(1, 2)  # strided, f16
+    held = tq.Adapters(back, torch.zeros(count, parts, rank, dtype=torch.float16, device="cuda")).a
+    full = torch.zeros(count, parts, ranks, row, dtype=torch.float16, device="cuda")
+    full[:, :, :rank, :k] = back
+    assert torch.equal(held, full.view(count, parts * ranks // 16, 16, row // 32, 32).transpose(2, 3))
+
+
+def test_repacking_refusals(abi):
+    for args in ((None, 2, 16, 64, 256), (257, 2, 16, 64, 256), (256, 2, 16, 64, None), (256, 2, 16, 64, 264), (256, -1, 16, 64, 256),
+                 (256, 2, 0, 64, 256), (256, 2, 257, 64, 256), (256, 2, 16, 0, 256), (256, 2, 16, 1 << 25, 256), (256, 1 << 30, 16, 64, 256)):
+        refuse(abi, "tq_repack_adapters_tiled", *args, None)
+    abi.call("tq_repack_adapters_tiled", None, 0, 16, 64, None, None)

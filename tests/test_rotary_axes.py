@@ -39,6 +39,8 @@ def test_refusals(abi, bad):
     refuse(abi, "tq_rotary_apply_axes", at(r), at(good), None, 3, at(q), None, 2, 64, 256, None, None)
     refuse(abi, "tq_kv_write_rotary_axes", at(cache(abi)), at(batch(abi)), at(r), at(good), 260, at(q), at(q), at(q), 2, 256, None)
     refuse(abi, "tq_kv_write_rotary_axes", at(cache(abi)), at(batch(abi)), None, at(good), 256, at(q), at(q), at(q), 2, 256, None)
+    wide, big = rotary(abi, rotary_dim=4096), heads(abi, heads=0)  # more planes than the descriptor holds
+    refuse(abi, "tq_rotary_apply_axes", at(wide), at(good), 256, 3, at(big), None, 2, 4096, 256, None, None)
     # planes past rotary_dim are nobody's
     abi.call("tq_rotary_apply_axes", at(rotary(abi, rotary_dim=62)), at(Axes(2, 3, 3 << 62, 7)), 256, 0, at(q), None, 2, 64, 256, None, None)
 
