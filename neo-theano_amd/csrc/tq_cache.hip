@@ -344,9 +344,9 @@ __global__ __launch_bounds__(kRowBlock) void k_token_rows(RowsArg a) {
         if (place.behind) return;  // the whole block: left as it was
     }
     if constexpr (kTurn) {
-        if (tid < a.rot.half)
-            plane_angle(a.rot, tid, static_cast<double>(a.positions ? a.positions[a.axes.of(tid) * a.axes.stride + n] : place.pos), cs,
-                        sn);
+        int64_t pos = a.positions ? a.positions[n] : place.pos;  // (uniform, and the only one as a rule)
+        if (a.positions && a.axes.count > 1) pos = a.positions[a.axes.of(min(tid, a.rot.half - 1)) * a.axes.stride + n];
+        if (tid < a.rot.half) plane_angle(a.rot, tid, static_cast<double>(pos), cs, sn);
         __syncthreads();
     }
     if (h >= of) return;  // (whole groups)
