@@ -528,6 +528,7 @@ int check_axes(const char* what, const tq_rotary_axes* x, const tq_rotary* r, Ax
     TQ_REQUIRE(r->rotary_dim <= kKvMaxHeadDim, "%s: axes are given for planes of up to 128 elements, not rotary_dim=%lld", what,
                (long long)r->rotary_dim);
     TQ_REQUIRE(x->position_stride >= 0, "%s: position_stride=%lld", what, (long long)x->position_stride);
+    if (r->rotary_dim == 0) return TQ_OK;  // no plane: one axis, whose number the kernels need not look up
     *out = AxesArg{{x->planes[0], x->planes[1]}, x->position_stride, static_cast<int>(x->axes)};
     for (int64_t i = 0; i < r->rotary_dim / 2; ++i)
         TQ_REQUIRE(static_cast<int64_t>(x->planes[i / 32] >> (2 * (i % 32)) & 3) < x->axes, "%s: plane %lld is of none of the %lld axes",

@@ -45,6 +45,21 @@ def test_refusals(abi, bad):
     abi.call("tq_rotary_apply_axes", at(rotary(abi, rotary_dim=62)), at(Axes(2, 3, 3 << 62, 7)), 256, 0, at(q), None, 2, 64, 256, None, None)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 200])
+def test_heads_that_do_not_turn_read_no_axis(tq, n):
+    """rotary_dim 0, whatever the words of the planes hold: the numbers as they are."""
+    import torch
+    from theano_quantize import _abi
+
+    x, pos = torch.randn(n, 5, 64, device="cuda"), torch.arange(2 * n, device="cuda")
+    out = torch.full_like(x, 7.0)
+    _abi.call("tq_rotary_apply_axes", _abi.rotary_desc(0, 0, False, False, 1.0), _abi.rotary_axes_desc(2, n, 2 ** 64 - 1, 2 ** 64 - 1),
+              pos.data_ptr(), n, _abi.heads_desc(x.data_ptr(), 5, x.stride(0), x.stride(1)), None, 2, 64, out.data_ptr(), None, None)
+    torch.cuda.synchronize()
+    assert torch.equal(out, x)
+
+
 def axes_of(tq, order, half, count):
     if order == "turn":
         return tq.Rotary.axes_in_turn(half, count)
