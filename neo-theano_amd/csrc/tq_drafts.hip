@@ -77,15 +77,25 @@ __device__ __forceinline__ Span span_of(const DraftArg& a, int seq) {
     return Span{first, fits ? last - first : 0};
 }
 
+// A probability as it counts: NaN and negative ones are 0.
 template <class T>
-__device__ __forceinline__ double at(const void* x, int64_t stride, int row, int64_t token) {
-    return static_cast<double>(static_cast<float>(static_cast<const T*>(x)[row * stride + token]));
+__device__ __forceinline__ double counted(T x) {
+    const float v = static_cast<float>(x);
+    return static_cast<double>(v > 0.f ? v : 0.f);
 }
 
-// What is left of one token's probability (NaN: nothing).
-__device__ __forceinline__ double left_of(double p, double q, double a) {
-    const double v = p - a * q;
-    return v > 0.0 ? v : 0.0;
+template <class T>
+__device__ __forceinline__ double at(const void* x, int64_t stride, int row, int64_t token) {
+    return counted(static_cast<const T*>(x)[row * stride + token]);
+}
+
+// What is left of one token's probability, likewise: a q that is not above 0 takes nothing (the lesser of a number and NaN is
+// the number), and what is not above 0 is 0.  The sums of a tree are one CU's VALU work: cutting p and q off beforehand is 3 us more
+// for 128256 of them.
+template <class T>
+__device__ __forceinline__ double left_of(T p, T q, double a) {
+    const double x = static_cast<double>(static_cast<float>(p)), y = static_cast<double>(static_cast<float>(q));
+    return fmax(fmin(x - a * y, x), 0.0);
 }
 
 __device__ __forceinline__ double readlane_f64(double v, int l) {
@@ -232,7 +242,7 @@ template <class T>
 __device__ __forceinline__ void left4(Four<T> p, Four<T> q, double a, uint32_t gone, double (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        v[e] = gone >> e & 1 ? 0.0 : left_of(static_cast<double>(static_cast<float>(p[e])), static_cast<double>(static_cast<float>(q[e])), a);
+        v[e] = gone >> e & 1 ? 0.0 : left_of(p[e], q[e], a);
 }
 template <class T, bool kVec>
 __device__ __forceinline__ void left4(const T* p, const T* q, double a, int i, int end, uint32_t gone, double (&v)[4]) {
@@ -400,7 +410,7 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
             for (int e = 0; e < kPickEach; ++e) {
                 const int b0 = (c0 + tid * kPickEach + e) * kSegment, b1 = min(b0 + kSegment, a.vocab);
                 v[e] = 0.0;
-                for (int i = b0; i < b1; ++i) v[e] += left_of(static_cast<double>(static_cast<float>(p[i])), 0.0, 0.0);
+                for (int i = b0; i < b1; ++i) v[e] += counted(p[i]);
             }
         } else if (segments > kBlock * kPickEach) {
             load(c0);

@@ -57,6 +57,7 @@ def walk(tokens, p, q, parents, accept, final):
         return [], -1
     node, path, tried = 0, [0], []
     pos = lambda v: v if v > 0 else 0.0  # noqa: E731  (NaN: 0)
+    p, q = [[pos(v) for v in row] for row in p], None if q is None else [[pos(v) for v in row] for row in q]
     a, w = 0.0, 1.0
     for t in range(1, len(tokens)):
         if parents[t] != node:
@@ -213,6 +214,28 @@ def test_probabilities_that_are_none(tq, tree):
             else:
                 final.fill_(1.0 - 2.0 ** -24)
             check(tq, counts, tokens, p, q, parents, accept, final, not tree)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("tree,draft", [(False, True), (True, False), (True, True)])
+def test_single_probabilities_that_are_none_count_as_zeros(tq, tree, draft, dtype):
+    """Of the drafted tokens themselves and of others, in the target and in the draft: as if zeros stood there (the numbers
+    that accept are small: a child whose draft probability is none is accepted where the target's is above 0)."""
+    import torch
+
+    for seed, none in enumerate((float("nan"), -0.25, -float("inf"))):
+        counts = [12, 9, 16]
+        tokens, p, q, parents, accept, final = make(counts, 300, tree, draft, getattr(torch, dtype), 60 + seed, width=5)
+        accept *= 0.3
+        first = torch.tensor(sum(([sum(counts[:i])] * n for i, n in enumerate(counts)), []))
+        at_parent = first + parents.clamp(min=0)
+        p[at_parent[::3], tokens[::3]] = none
+        p[:, 7::11] = none
+        if draft:
+            q[at_parent[::2], tokens[::2]] = none
+            q[:, 5::9] = none
+        check(tq, counts, tokens, p, q, parents, accept, final, not tree)
 
 
 @pytest.mark.gpu
