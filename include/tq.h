@@ -601,7 +601,8 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
  * projection whose adapters read x by themselves; scales f32 [count] or NULL (1).
  * x: f32, bf16 or f16 [M, K]; y and out: f32 [M, N], dense; out may be y, and overlaps nothing
  * else.  Products are exact (of f32 and f16: to 2^-24), sums f32 (the inner one is rounded to f32
- * and scaled before the outer).  A row depends on its own adapter alone; one with infinities or NaN in x or in its
+ * and scaled before the outer).  A row depends on its own adapter alone (the order
+ * of its inner sum also on how many adapters its neighbours have); one with infinities or NaN in x or in its
  * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a
  * few rows of low ranks), 16-byte aligned, contents need not be initialised. */
 typedef struct {
@@ -652,7 +653,7 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
 /* What was verified stays: of a sequence's T new tokens, in the cache at its last T places,
  * rows path[0] < path[1] < .. < path[kept - 1] move to the first `kept` of these places, in
  * order and as they are coded.  path int32 [batch, path_width], rows path_stride apart; kept
- * int32 [batch].  lengths_out (or NULL; not the batch's lengths): length - T + kept.  A
+ * int32 [batch].  lengths_out (or NULL; neither the batch's lengths nor kept): length - T + kept.  A
  * sequence whose rows do not fit, whose kept is not in 0 .. min(T, path_width) or whose path does
  * not ascend within its rows stays as it is, its length too.  Rows with no place do not
  * move.  Pages that several sequences share are copied first: places are written. */

@@ -202,7 +202,7 @@ struct AdaptArg {
     const uint16_t* b;
     const float* scales;
     int32_t* shares;  // of K, [low tiles]
-    float* t;         // [kMaxShares, m, parts * rank]
+    float* t;         // [shares, m, parts * rank]
     const float* y;
     float* out;
     int m, k, k_row, n, np, count, parts, rank;  // np: outputs of a part
@@ -624,8 +624,14 @@ Cut cut_of(const tq_adapters* a, int64_t m) {
     return c;
 }
 
-// Workspace: the shares of each tile, then t.
+// Workspace: the shares of each tile, then t of as many shares of K as a gang can take.
 int64_t shares_bytes(const Cut& c) { return (c.tiles * 4 + 15) / 16 * 16; }
+int64_t most_shares(const Cut& c) { return std::min<int64_t>(kMaxShares, int64_t(1) << c.gang_shift); }
+
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
 
 int check_adapters(const char* what, const tq_adapters* a, int64_t m) {
     TQ_REQUIRE(a, "%s: null adapters", what);
@@ -779,7 +785,9 @@ int tq_repack_adapters_tiled(const void* a, int64_t groups, int64_t rank, int64_
 int64_t tq_adapters_workspace_bytes(const tq_adapters* adapters, int64_t m) {
     using namespace tq;
     if (check_adapters("tq_adapters_add", adapters, m) != TQ_OK) return -1;
-    return m == 0 || in_one_launch(adapters, m) ? 0 : shares_bytes(cut_of(adapters, m)) + kMaxShares * m * adapters->parts * adapters->rank * 4;
+    if (m == 0 || in_one_launch(adapters, m)) return 0;
+    const Cut c = cut_of(adapters, m);
+    return shares_bytes(c) + most_shares(c) * m * adapters->parts * adapters->rank * 4;
 }
 
 int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64_t m, const int32_t* index, const float* y,
@@ -794,6 +802,10 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     TQ_REQUIRE(x && index && y && out, "%s: null x, index, y or out", what);
     TQ_REQUIRE(aligned(x, size) && aligned(index, 4) && aligned(y, 4) && aligned(out, 4), "%s: a pointer is not aligned to its elements",
                what);
+    const int64_t y_bytes = m * adapters->n * 4;
+    TQ_REQUIRE(!overlap(out, y_bytes, x, m * adapters->k * size) && !overlap(out, y_bytes, index, m * 4) &&
+                   (out == y || !overlap(out, y_bytes, y, y_bytes)),
+               "%s: out overlaps x, index or a part of y", what);
     const int64_t need = tq_adapters_workspace_bytes(adapters, m);
     TQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
                "%s: workspace of %lld bytes, 16-byte aligned, needed", what, (long long)need);

@@ -379,7 +379,8 @@ int tq_kv_keep(const tq_kv_cache* cache, const tq_kv_batch* batch, const int32_t
     if (batch->batch == 0) return TQ_OK;
     TQ_REQUIRE((path || path_width == 0) && kept, "%s: null path or kept", what);
     TQ_REQUIRE(aligned(path, 4) && aligned(kept, 4) && aligned(lengths_out, 4), "%s: unaligned path, kept or lengths", what);
-    TQ_REQUIRE(lengths_out != batch->lengths, "%s: lengths_out is the batch's lengths, which the call reads", what);
+    TQ_REQUIRE(!lengths_out || (lengths_out != batch->lengths && lengths_out != kept),
+               "%s: lengths_out is the batch's lengths or kept, which the call reads", what);
     const int64_t units = 2 * batch->batch * cache->heads, blocks = (units + 3) / 4;
     TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %lld sequences of %lld heads are more than %lld blocks", what, (long long)batch->batch,
                (long long)cache->heads, (long long)kMaxBlocks);

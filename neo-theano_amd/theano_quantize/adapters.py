@@ -77,7 +77,8 @@ class Adapters(_Fixed):
 
     def add(self, x, index, y, out=None):
         """y [rows, N] (f32) with each row's share added: x [rows, K] f32, bf16 or f16; index int32 [rows], the row's adapter,
-        or a number outside 0 .. count - 1 for none.  out: where the sums go (y itself, or a new tensor)."""
+        or a number outside 0 .. count - 1 for none.  out: where the sums go (y itself, or a tensor that shares no memory with
+        x, index and y), a new tensor if None."""
         dev, m, k, n = self.device_index, index.shape[0], self.in_features, self.out_features
         if dev != _current_device():
             raise InvalidArgument("Adapters.add: the adapters and the current device differ")

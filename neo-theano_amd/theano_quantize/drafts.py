@@ -84,6 +84,8 @@ class PagePool(_Fixed):
 
     def __init__(self, holders, page):
         _indices(holders, torch.int32, 1, "PagePool: holders")
+        if holders.shape[0] < 1 or holders.data_ptr() % 16 or not 1 <= int(page) <= 65536:
+            raise InvalidArgument(f"PagePool: expected 16-byte aligned holders of pages of 1 to 65536 tokens, got {holders.shape[0]} of {page}")
         self.__dict__.update(holders=holders, page=int(page), pages=holders.shape[0], device_index=holders.get_device(),
                              _desc=_abi.page_pool_desc(holders.data_ptr(), holders.shape[0], int(page)))
 

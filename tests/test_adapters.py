@@ -33,7 +33,7 @@ def test_the_packed_descriptor_is_the_structure(abi):
 
 
 def test_refusals(abi):
-    def no(d, x=256, dtype=2, m=30, index=256, y=256, out=256, ws=256, nb=1 << 40):
+    def no(d, x=1 << 20, dtype=2, m=30, index=1 << 21, y=1 << 22, out=1 << 22, ws=256, nb=1 << 40):
         refuse(abi, "tq_adapters_add", at(d), x, dtype, m, index, y, out, ws, nb, None)
 
     for kw in (dict(a=None), dict(a=264), dict(b=None), dict(b=264), dict(scales=258), dict(count=0), dict(count=(1 << 20) + 1), dict(parts=0),
@@ -42,10 +42,14 @@ def test_refusals(abi):
         no(desc(**kw))
         assert abi.entry("tq_adapters_workspace_bytes")(at(desc(**kw)), 3) == -1
     no(None)
-    for kw in (dict(x=None), dict(x=258), dict(dtype=3), dict(m=-1), dict(m=1 << 31), dict(index=None), dict(index=258), dict(y=None), dict(y=258),
-               dict(out=None), dict(out=258), dict(ws=None), dict(ws=264), dict(nb=100)):
+    for kw in (dict(x=None), dict(x=(1 << 20) + 2), dict(dtype=3), dict(m=-1), dict(m=1 << 31), dict(index=None), dict(index=(1 << 21) + 2), dict(y=None), dict(y=(1 << 22) + 2, out=1 << 23),
+               dict(out=None), dict(out=(1 << 23) + 2),
+               dict(out=1 << 20), dict(out=(1 << 20) + 4 * 30 * 100 - 4), dict(out=(1 << 20) - 4 * 30 * 60 + 4), dict(out=1 << 21),
+               dict(out=(1 << 21) + 4 * 29), dict(out=(1 << 22) + 4), dict(out=(1 << 22) - 4), dict(out=(1 << 22) + 4 * 30 * 60 - 4), dict(ws=None), dict(ws=264), dict(nb=100)):
         no(desc(), **kw)
     no(desc(parts=16, rank=256, n=1 << 24), m=1 << 30, nb=1 << 62)  # more blocks than a launch has
+    # t of one share of K where the tiles of tokens are as many as the CUs take at once
+    assert abi.entry("tq_adapters_workspace_bytes")(at(desc(rank=256)), 1 << 20) == 4 * (1 << 15) + (1 << 20) * 512 * 4
     need = abi.entry("tq_adapters_workspace_bytes")(at(desc()), 30)
     assert need >= 30 * 64 * 4 and need % 16 == 0
     assert abi.entry("tq_adapters_workspace_bytes")(at(desc()), 3) == 0 < abi.entry("tq_adapters_workspace_bytes")(at(desc(k=1 << 10)), 3)
@@ -328,7 +332,7 @@ def test_what_python_refuses(tq):
         ad.a = a
     for args in ((x.double(), index, y), (x[:3], index, y), (x[:, :31], index, y), (x, index.long(), y), (x, index[:2], y), (x, index, y.half()),
                  (x, index, y[:, :19]), (x, index, y.t().contiguous().t()), (x.cpu(), index, y), (x, index.cpu(), y), (x, index, y.cpu()),
-                 (x, index, y, y.half()), (x, index, y, y[:2])):
+                 (x, index, y, y.half()), (x, index, y, y[:2]), (x, index, y, torch.as_strided(x, (4, 20), (20, 1)))):
         with pytest.raises(tq.InvalidArgument):
             ad.add(*args)
     with pytest.raises(tq.InvalidArgument):

@@ -45,7 +45,7 @@ def test_bad_moves(abi):
     c, b = cache(abi), batch(abi)
     for path, stride, width, kept, out in ((None, 1, 1, 256, 512), (256, 1, 1, None, 512), (258, 1, 1, 256, 512), (256, 1, 1, 258, 512),
                                            (256, 1, 1, 256, 514), (256, 0, 1, 256, 512), (256, 1, -1, 256, 512), (256, 1, 1 << 31, 256, 512),
-                                           (256, 1, 1, 512, 256)):  # (the batch's own lengths lie at 256)
+                                           (256, 1, 1, 512, 256), (256, 1, 1, 512, 512)):  # (the batch's own lengths lie at 256)
         refuse(abi, "tq_kv_keep", at(c), at(b), path, stride, width, kept, out, None)
     abi.call("tq_kv_keep", at(c), at(batch(abi, batch=0, tokens=0)), None, 0, 0, None, None, None)
     many = batch(abi, batch=1 << 26, tokens=1 << 26)
@@ -323,6 +323,16 @@ def test_as_many_sequences_as_a_call_takes_and_pages_that_run_out(tq):
     assert odd.tolist() == [[-1] * 3] and pool.holders.tolist() == [0] * 4
     pool.grow(odd[:, :0], torch.tensor([48], dtype=torch.int32).cuda())
     assert pool.fork(odd[:, :0], torch.tensor([48], dtype=torch.int32).cuda(), torch.zeros(2, dtype=torch.int32).cuda())[0].shape == (2, 0)
+
+
+@pytest.mark.gpu
+def test_pools_that_python_refuses(tq):
+    import torch
+
+    holders = torch.zeros(9, dtype=torch.int32).cuda()
+    for bad, page in ((holders[:0], 16), (holders, 0), (holders, -16), (holders, 65537), (holders[1:], 16), (holders.float(), 16)):
+        with pytest.raises(tq.InvalidArgument):
+            tq.PagePool(bad, page)
 
 
 @pytest.mark.gpu
