@@ -13,7 +13,7 @@
 // The first product is bound by reading x (prompts) or A (a token for each adapter) once; K is split over the
 // waves of a block and over blocks, whose sums the second product adds as it loads t.  The second is bound by reading y
 // and writing out.  4093 rows of six adapters' runs, rank 64, 4096 to 14336: 23 + 106 us, the second 4.4 TB/s, where a large copy gets
-// 4.7; 64 rows of 48 adapters of rank 16: 5.7 + 10 us.
+// 4.7; 64 rows of 48 adapters of rank 16: 5.7 + 10 us; a row alone, both in one launch: 7 us.
 #include <algorithm>
 
 #include "tq_internal.h"
@@ -472,9 +472,9 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
 }
 
 // A token or a few and low ranks: both products in one launch, without a workspace.  Grid (range of outputs, part): every block
-// forms t of its part by itself, its waves 64 columns of K in turn, and then its outputs.  For the GPU that is no
-// less than two launches (a token in f32, rank 16, 4096 x 4096: 8.3 us against 8.1; another adapter is 5 us more), for the host a launch and a
-// buffer less (8.5 us a call against 11.7).
+// forms t of its part by itself, its waves 64 columns of K in turn, and then its outputs.  For the GPU that is about
+// what two launches are (a token in bf16, rank 16, 4096 x 4096, replayed: 6.5 us against 7.2; in f32 8.3 and 8.1; another adapter is 5 us more),
+// for the host a launch and a buffer less (8.5 us a call against 12.5).
 template <int kX, int kW, int kR, bool kVecX, bool kVecY>
 __global__ __launch_bounds__(kOnceBlock) void k_adapt_once(AdaptArg a) {
     constexpr int kOnceWaves = kOnceBlock / 64;
@@ -709,7 +709,7 @@ int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
 }
 
 // Calls of one launch.
-constexpr int64_t kOnceWeights = 1 << 16;  // of t's that a block forms
+constexpr int64_t kOnceWeights = 1 << 16;  // of t's that a block forms: a row of rank 16 and 4096 inputs, or as much
 bool in_one_launch(const tq_adapters* a, int64_t m) {
     return m <= 16 && a->rank <= 32 && m * a->rank * a->k <= kOnceWeights;
 }
