@@ -354,6 +354,45 @@ __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     }
 }
 
+// One wave: the token inside segment `chosen`, before which the running sum is `before`.  tried: tokens of the node's children count
+// as nothing.
+template <class T, bool kVec>
+__device__ __forceinline__ void look_into(const DraftArg& a, int seq, Span s, int node, const T* p, const T* q, double share_of_q, bool tried, int chosen,
+                                          double before, double goal) {
+    const int lane = threadIdx.x & 63;
+    const int i = chosen * kSegment + 4 * lane, end = min(chosen * kSegment + kSegment, a.vocab);
+    uint32_t gone = 0;
+    if (tried) {
+        for (int t0 = node + 1; t0 < s.count; t0 += 64) {
+            const int t = t0 + lane;
+            const bool child = t < s.count && (a.parents ? a.parents[s.first + t] == node : t == node + 1);
+            const int64_t x = child ? a.tokens[s.first + t] - chosen * static_cast<int64_t>(kSegment) : -1;
+            const int inside = x >= 0 && x < kSegment ? static_cast<int>(x) : -1;
+            for (uint64_t those = __ballot(inside >= 0); those; those &= those - 1) {
+                const int gone_one = readlane(inside, __ffsll(static_cast<unsigned long long>(those)) - 1);
+                if (gone_one >> 2 == lane) gone |= 1u << (gone_one & 3);
+            }
+        }
+    }
+    double left[4];
+    left4<T, kVec>(p, q, share_of_q, i, end, gone, left);
+    const double mine = (left[0] + left[1]) + (left[2] + left[3]);
+    double run = before + (wave_running(mine) - mine);
+    int over = -1, some = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        run += left[e];
+        if (left[e] > 0.0) {
+            some = i + e;
+            if (over < 0 && run > goal) over = i + e;
+        }
+    }
+    const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+    const int l = overs ? __ffsll(static_cast<unsigned long long>(overs)) - 1 : somes ? 63 - __clzll(static_cast<long long>(somes)) : 0;
+    const int token = overs ? over : some;
+    if (lane == l) a.next[seq] = token;
+}
+
 constexpr int kPickEach = 4;  // sums of a lane: 1024, of 262144 probabilities, in one round
 
 // A block for each sequence: the segment where the running sum passes final * total, then the token in it.
@@ -478,37 +517,101 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
         if (lane == 0) a.next[seq] = -1;
         return;
     }
-    const int i = chosen * kSegment + 4 * lane, end = min(chosen * kSegment + kSegment, a.vocab);
-    uint32_t gone = 0;
-    if (tried) {
-        for (int t0 = st.node + 1; t0 < s.count; t0 += 64) {
-            const int t = t0 + lane;
-            const bool child = t < s.count && (a.parents ? a.parents[s.first + t] == st.node : t == st.node + 1);
-            const int64_t x = child ? a.tokens[s.first + t] - chosen * static_cast<int64_t>(kSegment) : -1;
-            const int inside = x >= 0 && x < kSegment ? static_cast<int>(x) : -1;
-            for (uint64_t those = __ballot(inside >= 0); those; those &= those - 1) {
-                const int gone_one = readlane(inside, __ffsll(static_cast<unsigned long long>(those)) - 1);
-                if (gone_one >> 2 == lane) gone |= 1u << (gone_one & 3);
+    look_into<T, kVec>(a, seq, s, st.node, p, q, share_of_q, tried, chosen, before_it, goal);
+}
+
+// Vocabularies that one block sums in about the time of a launch: all of it in one launch, a block for each sequence, without a
+// workspace.
+constexpr int kOnceVocab = 32768;
+
+template <class T, bool kVec>
+__global__ __launch_bounds__(kWalkBlock) void k_verify_once(DraftArg a) {
+    constexpr int kWaves = kWalkBlock / 64, kEach = kOnceVocab / kSegment / 64, kU = 4;
+    __shared__ double lds[kWaves], sums[kOnceVocab / kSegment];
+    __shared__ uint32_t gone[kOnceVocab / 32];
+    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Span s = span_of(a, seq);
+    if (!a.draft)
+        for (int i = tid; i < kOnceVocab / 32; i += kWalkBlock) gone[i] = 0;
+    for (int i = tid; i < kOnceVocab / kSegment; i += kWalkBlock) sums[i] = 0.0;
+    int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
+    const State st = walk<T>(a, s, wave == 0 ? path : nullptr, [&](int node, double share, double& w) {
+        w = row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node), row_of<T>(a.draft, a.draft_stride, s.first + node),
+                                          share, a.vocab, lds);
+        return true;
+    });
+    for (int i = st.kept + tid; i < a.max_tokens; i += kWalkBlock) path[i] = -1;
+    if (tid == 0) a.kept[seq] = st.kept;
+    if (st.node < 0) {
+        if (tid == 0) a.next[seq] = -1;
+        return;
+    }
+    __syncthreads();
+    if (!a.draft) {
+        mark_tried(a, s, st.node, 0, gone, kWalkBlock);
+        __syncthreads();
+    }
+    const T* p = row_of<T>(a.target, a.target_stride, s.first + st.node);
+    const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
+    double share_of_q = st.a, total, run;
+    bool tried = !a.draft;
+    for (bool own = false;; own = true) {  // a second time where nothing is left: the target's own probabilities
+        for (int i0 = wave * kSegment + 4 * lane; i0 < a.share; i0 += kWaves * kSegment * kU) {
+            Four<T> x[kU], y[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                x[u] = load4<T, kVec>(p, i0 + kWaves * kSegment * u, a.vocab);
+                y[u] = q ? load4<T, kVec>(q, i0 + kWaves * kSegment * u, a.vocab) : Four<T>{};
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int i = i0 + kWaves * kSegment * u;
+                if (i >= a.share) break;
+                double v[4];
+                left4<T>(x[u], y[u], share_of_q, tried ? gone[i / 32] >> (i & 31) : 0, v);
+                const double sum = wave_sum64((v[0] + v[1]) + (v[2] + v[3]));
+                if (lane == 0) sums[i / kSegment] = sum;
             }
         }
-    }
-    double left[4];
-    left4<T, kVec>(p, q, share_of_q, i, end, gone, left);
-    const double mine = (left[0] + left[1]) + (left[2] + left[3]);
-    double run = before_it + (wave_running(mine) - mine);
-    int over = -1, some = -1;
+        __syncthreads();
+        double mine = 0.0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        run += left[e];
-        if (left[e] > 0.0) {
-            some = i + e;
-            if (over < 0 && run > goal) over = i + e;
+        for (int e = 0; e < kEach; ++e) mine += sums[lane * kEach + e];
+        run = wave_running(mine);
+        total = readlane_f64(run, 63);
+        run -= mine;
+        if (total > 0.0 || own) break;
+        q = nullptr;
+        share_of_q = 0.0;
+        tried = false;
+        __syncthreads();
+    }
+    if (wave != 0) return;
+    if (!(total > 0.0)) {
+        if (lane == 0) a.next[seq] = -1;
+        return;
+    }
+    const double goal = static_cast<double>(a.final[seq]) * total;
+    // the first segment that passes the goal, or the last that has anything
+    int over = -1, some = -1;
+    double over_before = 0.0, some_before = 0.0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const double v = sums[lane * kEach + e];
+        if (v > 0.0) {
+            some = lane * kEach + e;
+            some_before = run;
+            if (over < 0 && run + v > goal) {
+                over = some;
+                over_before = run;
+            }
         }
+        run += v;
     }
     const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
-    const int l = overs ? __ffsll(static_cast<unsigned long long>(overs)) - 1 : somes ? 63 - __clzll(static_cast<long long>(somes)) : 0;
-    const int token = overs ? over : some;
-    if (lane == l) a.next[seq] = token;
+    const int l = overs ? __ffsll(static_cast<unsigned long long>(overs)) - 1 : 63 - __clzll(static_cast<long long>(somes));
+    look_into<T, kVec>(a, seq, s, st.node, p, q, share_of_q, tried, readlane(overs ? over : some, l),
+                       readlane_f64(overs ? over_before : some_before, l), goal);
 }
 
 // Probabilities of a share: so that all shares are about two blocks for each CU, at least 1024 (a load for each
@@ -538,6 +641,10 @@ int check_batch(const char* what, const tq_kv_batch* b, int64_t vocab) {
 
 template <class T, bool kVec>
 void launch_drafts(const DraftArg& a, hipStream_t st) {
+    if (a.vocab <= kOnceVocab) {
+        k_verify_once<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
+        return;
+    }
     if (a.draft && a.parents) {
         k_left<T, kVec, kBefore><<<a.batch * a.shares, kBlock, 0, st>>>(a);
         k_walk<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
@@ -568,6 +675,7 @@ extern "C" {
 int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab) {
     using namespace tq;
     if (check_batch("tq_verify_drafts", batch, vocab) != TQ_OK) return -1;
+    if (vocab <= kOnceVocab) return 0;
     return (batch->batch * static_cast<int64_t>(sizeof(State)) + batch->batch * shares_of(vocab, batch->batch) * (share_of(vocab, batch->batch) / kSegment) * 8 +
             15) / 16 * 16;
 }
@@ -594,7 +702,7 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
                "%s: %lld sequences with %lld shares of %lld tokens are more than %lld blocks", what, (long long)batch->batch,
                (long long)shares, (long long)vocab, (long long)kMaxBlocks);
     const int64_t need = tq_verify_drafts_workspace_bytes(batch, vocab);
-    TQ_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), "%s: workspace of %lld bytes, 16-byte aligned, needed",
+    TQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "%s: workspace of %lld bytes, 16-byte aligned, needed",
                what, (long long)need);
     DraftArg a{};
     a.tokens = tokens;
@@ -610,7 +718,7 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
     a.max_tokens = static_cast<int>(batch->max_tokens);
     a.rows = static_cast<int>(batch->tokens);
     a.vocab = static_cast<int>(vocab);
-    a.share = share_of(vocab, batch->batch);
+    a.share = vocab <= kOnceVocab ? static_cast<int>((vocab + kSegment - 1) / kSegment * kSegment) : share_of(vocab, batch->batch);
     a.shares = static_cast<int>(shares);
     a.by_shares = FastDiv(static_cast<uint32_t>(shares));
     a.path = path;

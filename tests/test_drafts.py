@@ -8,6 +8,7 @@ from test_cache_abi import batch, refuse
 
 
 HELD = []
+SMALL = 32768  # the largest vocabulary of one launch
 
 
 def at(x):
@@ -25,7 +26,7 @@ def abi():
 
 def test_refusals(abi):
     b = batch(abi)
-    good = [at(b), 256, 256, 100, 256, 100, 2, 100, 256, 256, 256, 256, 1 << 20, 256, 256, 256, None]
+    good = [at(b), 256, 256, 100000, 256, 100000, 2, 100000, 256, 256, 256, 256, 1 << 20, 256, 256, 256, None]
 
     def no(**kw):
         args = list(good)
@@ -42,7 +43,9 @@ def test_refusals(abi):
                  (9, None), (9, 258), (10, None), (10, 258), (11, None), (11, 264), (12, 8), (13, None), (13, 258), (14, None), (14, 258),
                  (15, None), (15, 260)):
         no(**{f"_{i}": v})
-    assert abi.entry("tq_verify_drafts_workspace_bytes")(at(b), 100) % 16 == 0
+    assert abi.entry("tq_verify_drafts_workspace_bytes")(at(b), 100000) % 16 == 0
+    assert abi.entry("tq_verify_drafts_workspace_bytes")(at(b), SMALL) == 0 < abi.entry("tq_verify_drafts_workspace_bytes")(at(b), SMALL + 1)
+    no(_7=SMALL, _2=None), no(_7=SMALL, _13=None)
     huge = batch(abi, batch=1 << 22, max_tokens=1, tokens=1 << 22)  # more blocks than a launch has
     no(_0=at(huge), _12=1 << 62)
     wide = batch(abi, batch=1 << 20, max_tokens=1, tokens=1 << 20)
@@ -130,6 +133,9 @@ def check(tq, counts, tokens, p, q, parents, accept, final, chain, new=None):
     import torch
 
     new = new or batch_of(tq, counts)
+    if p.shape[1] < SMALL:  # tokens that never come change nothing, and take the form of large vocabularies
+        wider = lambda x: None if x is None else torch.cat([x, x.new_zeros(len(x), SMALL + 9 - x.shape[1])], 1)  # noqa: E731
+        check(tq, counts, tokens, wider(p), wider(q), parents, accept, final, chain, new)
     cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
     path, kept, token = tq.verify_drafts(cuda(tokens), cuda(p), new, cuda(accept), cuda(final), cuda(q), None if chain else cuda(parents))
     assert path.dtype == kept.dtype == torch.int32 and token.dtype == torch.int64
@@ -150,7 +156,7 @@ def check(tq, counts, tokens, p, q, parents, accept, final, chain, new=None):
 @pytest.mark.parametrize("draft", [False, True])
 @pytest.mark.parametrize("tree", [False, True])
 @pytest.mark.parametrize("counts,vocab", [([1], 7), ([6], 1000), ([5, 1, 8, 3], 1025), ([2], 1), ([3, 0, 4], 33), ([9] * 5, 4100),
-                                          ([64, 65, 70], 40), ([150, 1, 40], 12), ([4, 7], 20004)])
+                                          ([64, 65, 70], 40), ([150, 1, 40], 12), ([4, 7], 20004), ([6, 2, 9], 32768), ([5, 8], 32769)])
 def test_decisions(tq, counts, vocab, tree, draft, dtype):
     import torch
 
@@ -239,25 +245,27 @@ def test_single_probabilities_that_are_none_count_as_zeros(tq, tree, draft, dtyp
 
 
 @pytest.mark.gpu
-def test_infinite_probabilities_end(tq):
+@pytest.mark.parametrize("vocab", [2000, 34000])
+def test_infinite_probabilities_end(tq, vocab):
     """What they give is unspecified, a token of the vocabulary or -1."""
     import torch
 
-    tokens, p, q, parents, accept, final = (None if x is None else x.cuda() for x in make([5, 5], 2000, False, True, torch.float32, 5))
+    tokens, p, q, parents, accept, final = (None if x is None else x.cuda() for x in make([5, 5], vocab, False, True, torch.float32, 5))
     p[:, 77] = float("inf")
     for draft in (None, q):
         path, kept, token = tq.verify_drafts(tokens, p, batch_of(tq, [5, 5]), accept, final, draft)
-        assert (token >= -1).all() and (token < 2000).all() and (kept >= 1).all()
+        assert (token >= -1).all() and (token < vocab).all() and (kept >= 1).all()
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("draft", [False, True])
-def test_rows_that_do_not_fit_and_rows_behind(tq, draft):
+@pytest.mark.parametrize("vocab", [64, 33000])
+def test_rows_that_do_not_fit_and_rows_behind(tq, draft, vocab):
     """Offsets that run out of the call or past max_tokens: kept 0, token -1; the other sequences as ever."""
     import torch
 
     counts = [5, 5, 5]
-    tokens, p, q, parents, accept, final = make(counts, 64, True, draft, torch.float32, 6)
+    tokens, p, q, parents, accept, final = make(counts, vocab, True, draft, torch.float32, 6)
     cuda = [None if x is None else x.cuda() for x in (tokens, p, q, parents, accept, final)]
     want = tq.verify_drafts(cuda[0], cuda[1], batch_of(tq, counts), cuda[4], cuda[5], cuda[2], cuda[3])
     table, lengths = torch.zeros(3, 1, dtype=torch.int32).cuda(), torch.zeros(3, dtype=torch.int32).cuda()
@@ -274,17 +282,18 @@ def test_rows_that_do_not_fit_and_rows_behind(tq, draft):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_strides_and_other_streams(tq, dtype):
+@pytest.mark.parametrize("vocab", [1024, 40000])
+def test_strides_and_other_streams(tq, dtype, vocab):
     import torch
 
     counts = [6, 4]
-    tokens, p, q, parents, accept, final = make(counts, 1024, True, True, getattr(torch, dtype), 8)
+    tokens, p, q, parents, accept, final = make(counts, vocab, True, True, getattr(torch, dtype), 8)
     args = [x.cuda() for x in (tokens, p, q, parents, accept, final)]
     new = batch_of(tq, counts)
     want = tq.verify_drafts(args[0], args[1], new, args[4], args[5], args[2], args[3])
-    for skip, wide in ((1, 1024 + 3), (0, 1031), (4, 2048)):
+    for skip, wide in ((1, vocab + 3), (0, vocab + 7), (4, 2 * vocab)):
         big = [torch.zeros(10 * wide + skip, dtype=p.dtype, device="cuda") for _ in range(2)]
-        view = [b[skip:].view(10, wide)[:, :1024] for b in big]
+        view = [b[skip:].view(10, wide)[:, :vocab] for b in big]
         view[0].copy_(args[1]), view[1].copy_(args[2])
         for a, b in zip(want, tq.verify_drafts(args[0], view[0], new, args[4], args[5], view[1], args[3])):
             assert torch.equal(a, b)
@@ -326,11 +335,12 @@ def test_what_comes_out_is_the_targets_distribution(tq, tree, draft):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tree,draft", [(False, True), (True, False), (True, True)])
-def test_captured_and_replayed(tq, tree, draft):
+@pytest.mark.parametrize("vocab", [3001, 33000])
+def test_captured_and_replayed(tq, tree, draft, vocab):
     import torch
 
     counts = [7, 3, 5]
-    sets = [make(counts, 3001, tree, draft, torch.float32, s) for s in range(4)]
+    sets = [make(counts, vocab, tree, draft, torch.float32, s) for s in range(4)]
     new, still = batch_of(tq, counts), [None if x is None else x.cuda() for x in sets[0]]
 
     def call():
@@ -395,11 +405,12 @@ def test_padded_batches(tq, tree, draft):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("draft", [False, True])
-def test_probabilities_past_32_bit_offsets(tq, draft):
+@pytest.mark.parametrize("b,vocab", [(2500, 131072), (10000, 32768)])
+def test_probabilities_past_32_bit_offsets(tq, draft, b, vocab):
     """5 GB of each model's: the last sequences are those of a call of their own."""
     import torch
 
-    b, t, vocab = 2500, 8, 131072
+    t = 8
     g = torch.Generator("cuda").manual_seed(5)
     p = torch.empty(b * t, vocab, dtype=torch.bfloat16, device="cuda").uniform_(generator=g).mul_(2.0 ** -16)
     q = torch.empty_like(p).uniform_(generator=g).mul_(2.0 ** -16) if draft else None
@@ -408,7 +419,7 @@ def test_probabilities_past_32_bit_offsets(tq, draft):
     full = lambda n: tq.KVBatch(torch.zeros(n, 1, dtype=torch.int32).cuda(), torch.full((n,), t, dtype=torch.int32).cuda(), t)  # noqa: E731
     for parents in (None, torch.tensor([-1, 0, 0, 1, 1, 2, 3, 3], dtype=torch.int32).repeat(b).cuda()):
         whole = tq.verify_drafts(tokens, p, full(b), accept, final, q, parents)
-        for first in (0, 2047, b - 3):  # (2^31 elements are 2048 sequences)
+        for first in (0, 2 ** 31 // (t * vocab) - 1, b - 3):  # (around 2^31 elements)
             rows, seqs = slice(first * t, (first + 3) * t), slice(first, first + 3)
             part = tq.verify_drafts(tokens[rows], p[rows], full(3), accept[rows], final[seqs], None if q is None else q[rows],
                                     None if parents is None else parents[rows])
