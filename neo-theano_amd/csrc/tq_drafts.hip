@@ -196,6 +196,26 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
 }
 
+// Sums over a wave of four values: in lanes 0 to 15 that of v[0], then of v[2], v[1] and v[3] (a fifth of the instructions of four
+// sums one by one: 32768 f32 probabilities of two models by one block 7.4 us with the rest of the call, 9.0 one by one; 32 rows
+// of 128256 by 512 blocks 13.9 and 15.3).
+__device__ __forceinline__ double wave_sums4(const double (&v)[4]) {
+    auto halves = [](double x, double y) {  // x's sum over both halves in the lower one, y's in the upper
+        const uint64_t a = __builtin_bit_cast(uint64_t, x), b = __builtin_bit_cast(uint64_t, y);
+        const auto lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(a), static_cast<uint32_t>(b), false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32), false, false);
+        return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+    };
+    const uint64_t a = __builtin_bit_cast(uint64_t, halves(v[0], v[1])), b = __builtin_bit_cast(uint64_t, halves(v[2], v[3]));
+    const auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(a), static_cast<uint32_t>(b), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32), false, false);
+    double s = __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+    s += dpp64<kDppXor1>(s);
+    s += dpp64<kDppXor2>(s);
+    s += dpp64<kDppHalfMirror>(s);
+    return s + dpp64<kDppMirror>(s);
+}
+
 // Running sums over a wave, the lane's own among them.
 __device__ __forceinline__ double wave_running(double v) {
     const int lane = threadIdx.x & 63;
@@ -222,37 +242,80 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 
 template <class T>
 using Four = T __attribute__((ext_vector_type(4)));
+template <class T>
+using FourAnywhere = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));  // (one load wherever the row lies)
 
 // Elements i .. i + 3 of a row, zeros from `end` on.
-template <class T, bool kVec>
+template <class T>
 __device__ __forceinline__ Four<T> load4(const T* row, int i, int end) {
     Four<T> x{};
-    if constexpr (kVec) {  // rows 16-byte aligned (8 for 16-bit types), `end` a multiple of 4
-        if (i < end) x = *reinterpret_cast<const Four<T>*>(row + i);
+    if (i + 4 <= end) {
+        x = *reinterpret_cast<const FourAnywhere<T>*>(row + i);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 3; ++e)
             if (i + e < end) x[e] = row[i + e];
     }
     return x;
 }
 
-// What is left of four.  gone: bits of the tokens tried.
+// What is left of four.  q: whether y is there; gone: bits of the tokens tried.
 template <class T>
-__device__ __forceinline__ void left4(Four<T> p, Four<T> q, double a, uint32_t gone, double (&v)[4]) {
+__device__ __forceinline__ void left4(Four<T> x, bool q, Four<T> y, double a, uint32_t gone, double (&v)[4]) {
+    if (q) {  // (uniform)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        v[e] = gone >> e & 1 ? 0.0 : left_of(p[e], q[e], a);
+        for (int e = 0; e < 4; ++e) v[e] = left_of(x[e], y[e], a);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = counted(x[e]);
+    }
+    if (gone & 15) {  // (few)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = gone >> e & 1 ? 0.0 : v[e];
+    }
 }
-template <class T, bool kVec>
-__device__ __forceinline__ void left4(const T* p, const T* q, double a, int i, int end, uint32_t gone, double (&v)[4]) {
-    const Four<T> x = load4<T, kVec>(p, i, end);
-    left4<T>(x, q ? load4<T, kVec>(q, i, end) : Four<T>{}, a, gone, v);
+
+// Sums of what is left of segments `first`, first + step, .. of those from `begin` on, by one wave: four at a time.  gone: the tokens tried,
+// or null.
+template <class T>
+__device__ __forceinline__ void segment_sums(const T* p, const T* q, double a, const uint32_t* gone, int begin, int end, int first, int step,
+                                             int segments, double* sums) {
+    const int lane = threadIdx.x & 63, row = lane >> 4;
+    int g = first;
+    for (; g + step < segments; g += 4 * step) {
+        Four<T> x[4], y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = begin + (g + u * step) * kSegment + 4 * lane;
+            x[u] = load4<T>(p, i, end);
+            y[u] = q ? load4<T>(q, i, end) : Four<T>{};
+        }
+        double sum[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            sum[u] = 0.0;
+            if (g + u * step >= segments) continue;  // (uniform)
+            const int at = (g + u * step) * kSegment + 4 * lane;
+            double v[4];
+            left4<T>(x[u], q != nullptr, y[u], a, gone ? gone[at / 32] >> (at & 31) : 0, v);
+            sum[u] = (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        const double mine = wave_sums4(sum);
+        const int seg = g + ((row & 1) * 2 + (row >> 1)) * step;
+        if ((lane & 15) == 0 && seg < segments) sums[seg] = mine;
+    }
+    if (g < segments) {  // one is left
+        const int at = g * kSegment + 4 * lane;
+        double v[4];
+        left4<T>(load4<T>(p, begin + at, end), q != nullptr, q ? load4<T>(q, begin + at, end) : Four<T>{}, a, gone ? gone[at / 32] >> (at & 31) : 0, v);
+        const double sum = wave_sum64((v[0] + v[1]) + (v[2] + v[3]));
+        if (lane == 0) sums[g] = sum;
+    }
 }
 
 // Sum of what is left over the whole row, by one block; kU loads of each model in flight for each lane (a block alone at work is
 // bound by their latency).
-template <class T, bool kVec, int kThreads>
+template <class T, int kThreads>
 __device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int vocab, double* lds) {
     constexpr int kU = 4;
     double s = 0.0;
@@ -260,13 +323,13 @@ __device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int
         Four<T> x[kU], y[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            x[u] = load4<T, kVec>(p, i0 + 4 * kThreads * u, vocab);
-            y[u] = q ? load4<T, kVec>(q, i0 + 4 * kThreads * u, vocab) : Four<T>{};
+            x[u] = load4<T>(p, i0 + 4 * kThreads * u, vocab);
+            y[u] = q ? load4<T>(q, i0 + 4 * kThreads * u, vocab) : Four<T>{};
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             double v[4];
-            left4<T>(x[u], y[u], a, 0, v);
+            left4<T>(x[u], true, y[u], a, 0, v);
             s += (v[0] + v[1]) + (v[2] + v[3]);
         }
     }
@@ -278,23 +341,43 @@ __device__ __forceinline__ const T* row_of(const void* x, int64_t stride, int ro
     return x ? static_cast<const T*>(x) + row * stride : nullptr;
 }
 
+// The same by a block's first wave (sixteen that walk side by side take each other's cycles); the others wait for the
+// node whose sum is asked for, or for the end.  sum: called by all of the block's waves.
+template <class T, class Sum>
+__device__ __forceinline__ State walk_by_one(const DraftArg& a, Span s, int32_t* path, State* shared, Sum sum) {
+    if (threadIdx.x < 64) {
+        State st = walk<T>(a, s, path, [&](int node, double share, double& w) {
+            if (threadIdx.x == 0) *shared = State{share, node, 0, 0};
+            __syncthreads();
+            w = sum(node, share);
+            return true;
+        });
+        if (threadIdx.x == 0) *shared = st;  // (summed: 1)
+    }
+    for (;;) {
+        __syncthreads();
+        const State st = *shared;
+        if (st.summed) return st;
+        sum(st.node, st.a);
+    }
+}
+
 // Trees with draft probabilities, a block for each sequence: the walk needs sums on its way.  The first is there (k_left has
 // summed where the walk stops without it, over all CUs); others are rare, and this block's own (128256 f32 probabilities of two
 // models: 10 us, what one CU loads).
-template <class T, bool kVec>
+template <class T>
 __global__ __launch_bounds__(kWalkBlock) void k_walk(DraftArg a) {
     __shared__ double lds[kWalkBlock / 64];
     const int seq = blockIdx.x, segments = a.shares * (a.share / kSegment);
     const Span s = span_of(a, seq);
     double first = 0.0;
     for (int i = threadIdx.x; i < segments; i += kWalkBlock) first += a.sums[static_cast<int64_t>(seq) * segments + i];
-    int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
     int calls = 0;
-    State st = walk<T>(a, s, threadIdx.x < 64 ? path : nullptr, [&](int node, double share, double& w) {
-        w = calls++ == 0 ? block_sum<kWalkBlock>(first, lds)
-                         : row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node),
-                                                         row_of<T>(a.draft, a.draft_stride, s.first + node), share, a.vocab, lds);
-        return true;
+    __shared__ State shared;
+    State st = walk_by_one<T>(a, s, a.path + static_cast<int64_t>(seq) * a.max_tokens, &shared, [&](int node, double share) {
+        return calls++ == 0 ? block_sum<kWalkBlock>(first, lds)
+                            : row_mass<T, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node),
+                                                      row_of<T>(a.draft, a.draft_stride, s.first + node), share, a.vocab, lds);
     });
     st.summed = calls == 0;
     if (threadIdx.x == 0) a.state[seq] = st;
@@ -314,7 +397,7 @@ enum Stage { kOnly, kBefore, kAfter };
 
 // Block (share, sequence): the sums of what is left of a share, where the walk ends.  Every block walks by itself (a few
 // dependent loads); the first share's writes the path down.
-template <class T, bool kVec, Stage kStage>
+template <class T, Stage kStage>
 __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     __shared__ State shared;
     __shared__ uint32_t gone[kMaxShare / 32];
@@ -346,17 +429,12 @@ __global__ __launch_bounds__(kBlock) void k_left(DraftArg a) {
     const T* q = st.a != 0.0 ? row_of<T>(a.draft, a.draft_stride, s.first + st.node) : nullptr;
     const int end = min(begin + a.share, a.vocab);
     double* sums = a.sums + (static_cast<int64_t>(seq) * a.shares + share) * (a.share / kSegment);
-    for (int i = begin + 4 * static_cast<int>(threadIdx.x); i < begin + a.share; i += 4 * kBlock) {
-        double v[4];
-        left4<T, kVec>(p, q, st.a, i, end, a.draft ? 0 : gone[(i - begin) / 32] >> ((i - begin) & 31), v);
-        const double sum = wave_sum64((v[0] + v[1]) + (v[2] + v[3]));
-        if ((threadIdx.x & 63) == 0) sums[(i - begin) / kSegment] = sum;
-    }
+    segment_sums<T>(p, q, st.a, a.draft ? nullptr : gone, begin, end, threadIdx.x >> 6, kBlock / 64, a.share / kSegment, sums);
 }
 
 // One wave: the token inside segment `chosen`, before which the running sum is `before`.  tried: tokens of the node's children count
 // as nothing.
-template <class T, bool kVec>
+template <class T>
 __device__ __forceinline__ void look_into(const DraftArg& a, int seq, Span s, int node, const T* p, const T* q, double share_of_q, bool tried, int chosen,
                                           double before, double goal) {
     const int lane = threadIdx.x & 63;
@@ -375,7 +453,7 @@ __device__ __forceinline__ void look_into(const DraftArg& a, int seq, Span s, in
         }
     }
     double left[4];
-    left4<T, kVec>(p, q, share_of_q, i, end, gone, left);
+    left4<T>(load4<T>(p, i, end), q != nullptr, q ? load4<T>(q, i, end) : Four<T>{}, share_of_q, gone, left);
     const double mine = (left[0] + left[1]) + (left[2] + left[3]);
     double run = before + (wave_running(mine) - mine);
     int over = -1, some = -1;
@@ -396,7 +474,7 @@ __device__ __forceinline__ void look_into(const DraftArg& a, int seq, Span s, in
 constexpr int kPickEach = 4;  // sums of a lane: 1024, of 262144 probabilities, in one round
 
 // A block for each sequence: the segment where the running sum passes final * total, then the token in it.
-template <class T, bool kVec>
+template <class T>
 __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
     __shared__ double lds[kBlock / 64];
     __shared__ double before_it;
@@ -434,7 +512,7 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
         q = nullptr;
         share_of_q = 0.0;
         tried = false;
-        total = row_mass<T, kVec, kBlock>(p, nullptr, 0.0, a.vocab, lds);
+        total = row_mass<T, kBlock>(p, nullptr, 0.0, a.vocab, lds);
         if (!(total > 0.0)) {
             if (tid == 0) a.next[seq] = -1;
             return;
@@ -517,28 +595,31 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
         if (lane == 0) a.next[seq] = -1;
         return;
     }
-    look_into<T, kVec>(a, seq, s, st.node, p, q, share_of_q, tried, chosen, before_it, goal);
+    look_into<T>(a, seq, s, st.node, p, q, share_of_q, tried, chosen, before_it, goal);
 }
 
 // Vocabularies that one block sums in about the time of a launch: all of it in one launch, a block for each sequence, without a
-// workspace.
+// workspace.  Against two launches (four for trees with draft probabilities), f32, replayed: a chain of 6 over 16000 tokens 6.2 us
+// (6.8), over 32768 7.4 (6.6), over 65536 13.9 (6.8), 32 chains over 32768 9.2 (9.9), 4 drawn trees of 24 over 32768 15.1 (17.4), over
+// 65536 23.5 (17.7).  A call from the host is 15.5 against 19.4 in all of these but the last: at 32768 the GPU's loss is less than
+// the host's gain.
 constexpr int kOnceVocab = 32768;
 
-template <class T, bool kVec>
+template <class T>
 __global__ __launch_bounds__(kWalkBlock) void k_verify_once(DraftArg a) {
-    constexpr int kWaves = kWalkBlock / 64, kEach = kOnceVocab / kSegment / 64, kU = 4;
+    constexpr int kWaves = kWalkBlock / 64, kEach = kOnceVocab / kSegment / 64;
     __shared__ double lds[kWaves], sums[kOnceVocab / kSegment];
     __shared__ uint32_t gone[kOnceVocab / 32];
+    __shared__ State shared;
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Span s = span_of(a, seq);
     if (!a.draft)
         for (int i = tid; i < kOnceVocab / 32; i += kWalkBlock) gone[i] = 0;
     for (int i = tid; i < kOnceVocab / kSegment; i += kWalkBlock) sums[i] = 0.0;
     int32_t* path = a.path + static_cast<int64_t>(seq) * a.max_tokens;
-    const State st = walk<T>(a, s, wave == 0 ? path : nullptr, [&](int node, double share, double& w) {
-        w = row_mass<T, kVec, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node), row_of<T>(a.draft, a.draft_stride, s.first + node),
-                                          share, a.vocab, lds);
-        return true;
+    const State st = walk_by_one<T>(a, s, path, &shared, [&](int node, double share) {
+        return row_mass<T, kWalkBlock>(row_of<T>(a.target, a.target_stride, s.first + node), row_of<T>(a.draft, a.draft_stride, s.first + node),
+                                       share, a.vocab, lds);
     });
     for (int i = st.kept + tid; i < a.max_tokens; i += kWalkBlock) path[i] = -1;
     if (tid == 0) a.kept[seq] = st.kept;
@@ -556,23 +637,7 @@ __global__ __launch_bounds__(kWalkBlock) void k_verify_once(DraftArg a) {
     double share_of_q = st.a, total, run;
     bool tried = !a.draft;
     for (bool own = false;; own = true) {  // a second time where nothing is left: the target's own probabilities
-        for (int i0 = wave * kSegment + 4 * lane; i0 < a.share; i0 += kWaves * kSegment * kU) {
-            Four<T> x[kU], y[kU];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                x[u] = load4<T, kVec>(p, i0 + kWaves * kSegment * u, a.vocab);
-                y[u] = q ? load4<T, kVec>(q, i0 + kWaves * kSegment * u, a.vocab) : Four<T>{};
-            }
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int i = i0 + kWaves * kSegment * u;
-                if (i >= a.share) break;
-                double v[4];
-                left4<T>(x[u], y[u], share_of_q, tried ? gone[i / 32] >> (i & 31) : 0, v);
-                const double sum = wave_sum64((v[0] + v[1]) + (v[2] + v[3]));
-                if (lane == 0) sums[i / kSegment] = sum;
-            }
-        }
+        segment_sums<T>(p, q, share_of_q, tried ? gone : nullptr, 0, a.vocab, wave, kWaves, a.share / kSegment, sums);
         __syncthreads();
         double mine = 0.0;
 #pragma unroll
@@ -610,7 +675,7 @@ __global__ __launch_bounds__(kWalkBlock) void k_verify_once(DraftArg a) {
     }
     const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
     const int l = overs ? __ffsll(static_cast<unsigned long long>(overs)) - 1 : 63 - __clzll(static_cast<long long>(somes));
-    look_into<T, kVec>(a, seq, s, st.node, p, q, share_of_q, tried, readlane(overs ? over : some, l),
+    look_into<T>(a, seq, s, st.node, p, q, share_of_q, tried, readlane(overs ? over : some, l),
                        readlane_f64(overs ? over_before : some_before, l), goal);
 }
 
@@ -639,31 +704,26 @@ int check_batch(const char* what, const tq_kv_batch* b, int64_t vocab) {
     return TQ_OK;
 }
 
-template <class T, bool kVec>
+template <class T>
 void launch_drafts(const DraftArg& a, hipStream_t st) {
     if (a.vocab <= kOnceVocab) {
-        k_verify_once<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
+        k_verify_once<T><<<a.batch, kWalkBlock, 0, st>>>(a);
         return;
     }
     if (a.draft && a.parents) {
-        k_left<T, kVec, kBefore><<<a.batch * a.shares, kBlock, 0, st>>>(a);
-        k_walk<T, kVec><<<a.batch, kWalkBlock, 0, st>>>(a);
-        k_left<T, kVec, kAfter><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+        k_left<T, kBefore><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+        k_walk<T><<<a.batch, kWalkBlock, 0, st>>>(a);
+        k_left<T, kAfter><<<a.batch * a.shares, kBlock, 0, st>>>(a);
     } else {
-        k_left<T, kVec, kOnly><<<a.batch * a.shares, kBlock, 0, st>>>(a);
+        k_left<T, kOnly><<<a.batch * a.shares, kBlock, 0, st>>>(a);
     }
-    k_pick<T, kVec><<<a.batch, kBlock, 0, st>>>(a);
+    k_pick<T><<<a.batch, kBlock, 0, st>>>(a);
 }
 
 template <class T>
 int launch_typed(const DraftArg& a, hipStream_t st, const char* what) {
-    const int size = sizeof(T), align = 4 * size;
-    auto fits = [&](const void* x, int64_t stride) { return !x || (aligned(x, align) && stride * size % align == 0); };
     clear_error();
-    if (a.vocab % 4 == 0 && fits(a.target, a.target_stride) && fits(a.draft, a.draft_stride))
-        launch_drafts<T, true>(a, st);
-    else
-        launch_drafts<T, false>(a, st);
+    launch_drafts<T>(a, st);
     return check_launch(what);
 }
 
