@@ -197,8 +197,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 }
 
 // Sums over a wave of four values: in lanes 0 to 15 that of v[0], then of v[2], v[1] and v[3] (a fifth of the instructions of four
-// sums one by one: 32768 f32 probabilities of two models by one block 7.4 us with the rest of the call, 9.0 one by one; 32 rows
-// of 128256 by 512 blocks 13.9 and 15.3).
+// sums one by one: a chain over 32768 f32 probabilities of two models by one block 7.4 us, 9.0 one by one; 32 rows of 128256 by 512
+// blocks 13.9 and 15.3).
 __device__ __forceinline__ double wave_sums4(const double (&v)[4]) {
     auto halves = [](double x, double y) {  // x's sum over both halves in the lower one, y's in the upper
         const uint64_t a = __builtin_bit_cast(uint64_t, x), b = __builtin_bit_cast(uint64_t, y);
@@ -245,12 +245,18 @@ using Four = T __attribute__((ext_vector_type(4)));
 template <class T>
 using FourAnywhere = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));  // (one load wherever the row lies)
 
-// Elements i .. i + 3 of a row, zeros from `end` on.
+// Elements i .. i + 3 of a row.
+template <class T>
+__device__ __forceinline__ Four<T> load4(const T* row, int i) {
+    return *reinterpret_cast<const FourAnywhere<T>*>(row + i);
+}
+
+// The same with zeros from `end` on.
 template <class T>
 __device__ __forceinline__ Four<T> load4(const T* row, int i, int end) {
     Four<T> x{};
     if (i + 4 <= end) {
-        x = *reinterpret_cast<const FourAnywhere<T>*>(row + i);
+        x = load4<T>(row, i);
     } else {
 #pragma unroll
         for (int e = 0; e < 3; ++e)
@@ -314,24 +320,36 @@ __device__ __forceinline__ void segment_sums(const T* p, const T* q, double a, c
 }
 
 // Sum of what is left over the whole row, by one block; kU loads of each model in flight for each lane (a block alone at work is
-// bound by their latency).
+// bound by their latency; without bounds to check where none is near: 8 % of 32 trees over 32768 tokens).
 template <class T, int kThreads>
 __device__ __forceinline__ double row_mass(const T* p, const T* q, double a, int vocab, double* lds) {
-    constexpr int kU = 4;
+    constexpr int kU = 4, kAll = 4 * kThreads * kU;
     double s = 0.0;
-    for (int i0 = 4 * static_cast<int>(threadIdx.x); i0 < vocab; i0 += 4 * kThreads * kU) {
-        Four<T> x[kU], y[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            x[u] = load4<T>(p, i0 + 4 * kThreads * u, vocab);
-            y[u] = q ? load4<T>(q, i0 + 4 * kThreads * u, vocab) : Four<T>{};
-        }
+    auto add = [&](const Four<T> (&x)[kU], const Four<T> (&y)[kU]) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             double v[4];
             left4<T>(x[u], true, y[u], a, 0, v);
             s += (v[0] + v[1]) + (v[2] + v[3]);
         }
+    };
+    Four<T> x[kU], y[kU];
+    int i = 4 * static_cast<int>(threadIdx.x), from = 0;
+    for (; q && from + kAll <= vocab; from += kAll, i += kAll) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            x[u] = load4<T>(p, i + 4 * kThreads * u);
+            y[u] = load4<T>(q, i + 4 * kThreads * u);
+        }
+        add(x, y);
+    }
+    for (; i < vocab; i += kAll) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            x[u] = load4<T>(p, i + 4 * kThreads * u, vocab);
+            y[u] = q ? load4<T>(q, i + 4 * kThreads * u, vocab) : Four<T>{};
+        }
+        add(x, y);
     }
     return block_sum<kThreads>(s, lds);
 }
@@ -599,10 +617,10 @@ __global__ __launch_bounds__(kBlock) void k_pick(DraftArg a) {
 }
 
 // Vocabularies that one block sums in about the time of a launch: all of it in one launch, a block for each sequence, without a
-// workspace.  Against two launches (four for trees with draft probabilities), f32, replayed: a chain of 6 over 16000 tokens 6.2 us
-// (6.8), over 32768 7.4 (6.6), over 65536 13.9 (6.8), 32 chains over 32768 9.2 (9.9), 4 drawn trees of 24 over 32768 15.1 (17.4), over
-// 65536 23.5 (17.7).  A call from the host is 15.5 against 19.4 in all of these but the last: at 32768 the GPU's loss is less than
-// the host's gain.
+// workspace.  Against two launches (four for trees with draft probabilities), f32, replayed: a chain of 6 over 16000 tokens 6.5 us
+// (6.9), over 32768 7.8 (6.6), over 65536 11.1 (6.7), 32 chains over 32768 9.5 (10.4), 4 drawn trees of 24 over 32768 14.0 (16.5), over
+// 65536 19.1 (17.3).  A call from the host is 15.5 against 19.4 where the GPU is no longer: up to 32768 its loss is less than the host's
+// gain.
 constexpr int kOnceVocab = 32768;
 
 template <class T>
