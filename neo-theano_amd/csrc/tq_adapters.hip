@@ -85,6 +85,10 @@ struct Raw8 {
     f32x4 v[kX == TQ_DT_F32 ? 2 : 1];
 };
 
+// Vectors wherever they lie.
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
 // Elements k .. k + 7 of a row of n > 0; what lies past it is any element of the row, see planes_of.
 template <int kX, bool kVec>
 __device__ __forceinline__ Raw8<kX> fetch(const void* row, int k, int n) {
@@ -95,6 +99,9 @@ __device__ __forceinline__ Raw8<kX> fetch(const void* row, int k, int n) {
             const int at = min(k, n - 8);
             r.v[0] = *reinterpret_cast<const f32x4*>(p + at);
             r.v[1] = *reinterpret_cast<const f32x4*>(p + at + 4);
+        } else if (k + 8 <= n) {
+            r.v[0] = *reinterpret_cast<const f32x4_a4*>(p + k);
+            r.v[1] = *reinterpret_cast<const f32x4_a4*>(p + k + 4);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) r.v[i / 4][i % 4] = p[min(k + i, n - 1)];
@@ -103,6 +110,8 @@ __device__ __forceinline__ Raw8<kX> fetch(const void* row, int k, int n) {
         const uint16_t* p = static_cast<const uint16_t*>(row);
         if constexpr (kVec) {
             r.v[0] = *reinterpret_cast<const f32x4*>(p + min(k, n - 8));
+        } else if (k + 8 <= n) {
+            r.v[0] = __builtin_bit_cast(f32x4, static_cast<u32x4>(*reinterpret_cast<const u32x4_a2*>(p + k)));
         } else {
             u32x4 raw;
 #pragma unroll
@@ -420,6 +429,8 @@ struct UpTiles {
     __device__ __forceinline__ void load(int n0) {
         if constexpr (kVec) {
             y = *reinterpret_cast<const f32x4*>(a.y + at + min(n0, a.np - 4 - 4 * quad()));
+        } else if (n0 + 4 * quad() + 4 <= a.np) {
+            y = *reinterpret_cast<const f32x4_a4*>(a.y + at + n0);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = a.y[at - 4 * quad() + min(n0 + 4 * quad() + i, a.np - 1)];
@@ -446,6 +457,8 @@ struct UpTiles {
             if (first + col() >= a.m) continue;
             if constexpr (kVec) {
                 if (n0 + 4 * quad() < a.np) *reinterpret_cast<f32x4*>(a.out + at + n0) = d;
+            } else if (n0 + 4 * quad() + 4 <= a.np) {
+                *reinterpret_cast<f32x4_a4*>(a.out + at + n0) = d;
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -601,14 +614,16 @@ struct Cut {
     int64_t tiles;
 };
 
-// Up to this many rows the first product's tiles are of 16 tokens, then of 32 (K 4096, rank 64, six adapters' runs of rows, both
-// products to 14336 outputs: 2048 rows 76 us with 16, 82 with 32; 4096 rows 138 and 134).
-constexpr int kFewRows = 2048;
+// The first product's tiles are of 16 tokens, or of 32 where it is long: from 3 2^28 products on (rows x ranks x K; f32, six
+// adapters' runs, 16 / 32: 4096 rows, rank 64, K 1408 20.1 / 28.3 us, rank 48, K 4096 29.0 / 28.9, rank 192, K 4096 86 / 69; 1024 rows,
+// rank 192, K 4096 31.8 / 29.4; 512 rows, rank 192, K 12288 41 / 44; 2048 rows, rank 256, K 12288 197 / 136), and more than 256 rows.
+constexpr int64_t kLong = int64_t(3) << 28;
+constexpr int kFewRows = 256;
 
 Cut cut_of(const tq_adapters* a, int64_t m) {
     Cut c;
     const int64_t turns = (a->k + kKUnit * kWaves - 1) / (kKUnit * kWaves), rank_tiles = a->parts * a->rank / 16;
-    c.few = m <= kFewRows;
+    c.few = m <= kFewRows || m < kLong / (a->parts * a->rank * a->k);
     c.tokens = c.few ? 16 : 32;
     c.ranks = rank_tiles == 1 ? 1 : rank_tiles == 2 ? 2 : 4;
     c.groups = static_cast<int>((rank_tiles + c.ranks - 1) / c.ranks);

@@ -397,6 +397,21 @@ def test_sizes_on_both_sides_of_every_form(tq, m, n, r):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,weights", [("float32", "bfloat16"), ("float32", "float16"), ("bfloat16", "bfloat16"), ("float16", "float16"),
+                                           ("float16", "bfloat16"), ("bfloat16", "float16")])
+@pytest.mark.parametrize("m,count,r,parts,k,n", [(20000, 7, 16, 1, 2601, 40), (10001, 3, 30, 1, 2600, 66), (5000, 60, 40, 1, 3500, 100),
+                                                 (1100, 4, 48, 16, 1000, 64), (300, 5, 256, 16, 701, 32)])
+def test_long_first_products(tq, m, count, r, parts, k, n, dtype, weights):
+    """Tiles of 32 tokens, of all ranks."""
+    ranks = parts * ((r + 15) // 16 * 16)
+    assert m * ranks * k >= 3 << 28
+    for runs in (False, True):
+        x, y, a, b, scales, index = made(m, count, r, parts, k, n, dtype, weights, m + runs, runs)
+        ref, tol = reference(x, y, a, b, scales, index)
+        assert ((tq.Adapters(a, b, scales).add(x, index, y).double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("count,parts,rank,k", [(1, 1, 1, 1), (3, 2, 16, 64), (2, 3, 17, 100), (5, 1, 256, 65), (1, 16, 8, 4097)])
 def test_the_tiles_of_a(tq, count, parts, rank, k):
     import torch
