@@ -701,15 +701,15 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
 
 // Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps, and about one step's time for a block's
 // start; a block that is alone on its CU waits for its own loads (4093 rows of 14336, rank 64: 113, 100, 108, 125 and 130 us with
-// 1, 2, 4, 7 and 14 blocks for each CU).
+// 1, 2, 4, 7 and 14 blocks for each CU; 512 rows, rank 64: 30 and 24 us with 1 and 2).  Of ranges that cost the same the shorter ones.
 template <int kW, int kT, int kS>
 int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
     const int64_t steps = (a.np + kStep - 1) / kStep, tiles = (a.m + 16 * kT - 1) / (16 * kT), cus = device_cu_count();
     int64_t best = 0;
     for (int64_t r = 1; r <= steps && r <= 64; ++r) {
         const int64_t per = (steps + r - 1) / r, on_one = (tiles * a.parts * ((steps + per - 1) / per) + cus - 1) / cus;
-        const int64_t cost = on_one * (per + 1) * (on_one == 1 ? 6 : 5);
-        if (best == 0 || cost < best) {
+        const int64_t cost = on_one * (per + 1) * (on_one == 1 ? 8 : 5);
+        if (best == 0 || cost <= best) {
             best = cost;
             a.per = static_cast<int>(per);
         }
@@ -761,10 +761,11 @@ int launch_typed(const AdaptArg& a, const Cut& c, int dtype, bool vec_x, bool ve
     else launch_low_tokens<TQ_DT_F16, kW>(a, c, vec_x, low, st);
     const int rc = check_launch(what);
     if (rc != TQ_OK) return rc;
-    // the form of many rows from 2^23 outputs on (rank 16, direct / rows: 512 x 14336 23.3 / 25.4 us, 1024 x 14336 45.4 / 40.6), with more
-    // ranks from 3 2^19 (rank 64: 256 x 4096 19.1 / 21.4, 128 x 14336 23.4 / 21.4) or 3 2^18 on (rank 128: 128 x 4096 19.4 / 21.6, 64 x
-    // 14336 25.0 / 21.2); six runs of rows, both products
-    const int64_t many = a.rank > 64 ? 3 << 18 : a.rank > 32 ? 3 << 19 : 1 << 23;
+    // the form of many rows where the outputs leave the caches (rank 16, direct / rows, us: 1536 x 6144 23.2 / 26.2, 2560 x 6144 45.1 / 34.3;
+    // rank 32: 1536 x 8192 27.7 / 26.9, 1024 x 14336 43.6 / 32.9), with more ranks from 3 2^19 outputs (rank 64: 256 x 4096 13.1 / 14.4,
+    // 128 x 14336 18.3 / 16.5, 512 x 8192 21.9 / 18.3) or 3 2^18 on (rank 128: 128 x 4096 13.6 / 15.3, 64 x 14336 21.2 / 17.4); six runs of
+    // rows, K 512, both products
+    const int64_t many = a.rank > 64 ? 3 << 18 : a.rank > 32 ? 3 << 19 : 12 << 20;
     if (vec_y && static_cast<int64_t>(a.m) * a.n >= many && a.m <= 16 * 65535) {
         if (a.rank > 128) return launch_up_rows<kW, 1, 8>(a, st, what);
         if (a.rank > 64) return launch_up_rows<kW, 1, 4>(a, st, what);

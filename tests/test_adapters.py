@@ -383,7 +383,7 @@ def test_two_streams_at_once(tq):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,r", [(2049, 64, 16), (2048, 64, 16), (2100, 4100, 16), (513, 2048, 40), (600, 2000, 70), (400, 2100, 130), (1100, 1000, 200)])
+@pytest.mark.parametrize("m,n,r", [(2049, 64, 16), (2048, 64, 16), (2100, 4100, 16), (3900, 4100, 16), (3100, 4100, 32), (513, 2048, 40), (600, 2000, 70), (400, 2100, 130), (1100, 1000, 200)])
 def test_sizes_on_both_sides_of_every_form(tq, m, n, r):
     """Tiles of 16 and 32 tokens, the forms of few and many rows, each with one adapter, a few in runs and many mixed."""
     import torch
