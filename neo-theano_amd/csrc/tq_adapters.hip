@@ -701,7 +701,8 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
 
 // Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps, and about one step's time for a block's
 // start; a block that is alone on its CU waits for its own loads (4093 rows of 14336, rank 64: 113, 100, 108, 125 and 130 us with
-// 1, 2, 4, 7 and 14 blocks for each CU; 512 rows, rank 64: 30 and 24 us with 1 and 2).  Of ranges that cost the same the shorter ones.
+// 1, 2, 4, 7 and 14 blocks for each CU; 512 rows, rank 64, both products: 30 and 24 us with 1 and 2).  Of ranges that cost the same the
+// shorter ones.
 template <int kW, int kT, int kS>
 int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
     const int64_t steps = (a.np + kStep - 1) / kStep, tiles = (a.m + 16 * kT - 1) / (16 * kT), cus = device_cu_count();
