@@ -642,8 +642,8 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
  * the vocabulary is turned down.  path [batch, max_tokens]: the accepted rows (counted
  * within the sequence, the root first), -1 behind them; kept [batch]: how many; next
  * [batch].  A sequence without rows, or whose rows do not fit (see tq_kv_batch), has kept 0
- * and next -1.  workspace: tq_verify_drafts_workspace_bytes(...) bytes, 16-byte aligned,
- * contents need not be initialised. */
+ * and next -1.  workspace: tq_verify_drafts_workspace_bytes(...) bytes (0 for up to 32768 tokens
+ * of the vocabulary), 16-byte aligned, contents need not be initialised. */
 int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab);
 int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void* target, int64_t target_stride,
                      const void* draft, int64_t draft_stride, int dtype, int64_t vocab, const int32_t* parents,
