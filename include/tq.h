@@ -600,7 +600,7 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
  * with zeros); parts (1 to 16, dividing N): slices of the outputs of a fused
  * projection whose adapters read x by themselves; scales f32 [count] or NULL (1).
  * x: f32, bf16 or f16 [M, K]; y and out: f32 [M, N], dense; out may be y, and overlaps nothing
- * else.  Products are exact (of f32 and f16: to 2^-24), sums f32 (the inner one is rounded to f32
+ * else.  Products are exact (but what an f32 value has below 2^-126), sums f32 (the inner one is rounded to f32
  * and scaled before the outer).  A row depends on its own adapter alone (the order
  * of its inner sum also on how many adapters its neighbours have); one with infinities or NaN in x or in its
  * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a

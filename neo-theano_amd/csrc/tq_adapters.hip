@@ -142,14 +142,15 @@ __device__ __forceinline__ void planes_of(const Raw8<kX>& r, int k, int n, u32x4
     }
 }
 
-// c + w x by all pairs of planes but those under 2^-24 of the product.
+// c + w x by all pairs of planes, which are the whole product (planes are cut, so a low one may be 2^-7 of what is above it, the
+// third 2^-15: of f16 weights and f32 values the lowest pair is up to 2^-22 of the product), the least first.
 template <bool kF16, int kNW, int kNX>
 __device__ __forceinline__ f32x4 products(const u32x4 (&w)[kNW], const u32x4 (&x)[kNX], f32x4 c) {
 #pragma unroll
     for (int p = kNW + kNX - 2; p >= 0; --p)
 #pragma unroll
         for (int i = 0; i < kNW; ++i)
-            if (p - i >= 0 && p - i < kNX && p <= 2) c = mfma<kF16>(w[i], x[p - i], c);
+            if (p - i >= 0 && p - i < kNX) c = mfma<kF16>(w[i], x[p - i], c);
     return c;
 }
 
