@@ -1,4 +1,5 @@
-"""Low-rank adapters beside a projection: every bit of both operands of both products, in every form."""
+"""Low-rank adapters beside a projection: every bit of both operands of both products, in every form, and what infinities
+and NaN do to the rows that use them."""
 import pytest
 
 # rows, rank, inputs, outputs: one launch; few rows in two; many rows in tiles of 16, and (rows x ranks x K from 3 2^28 on) of
@@ -63,3 +64,38 @@ def test_the_lowest_planes_meet(tq, m, k, n):
         got = tq.Adapters(a.half(), b.half()).add(x.float(), torch.zeros(m, dtype=torch.int32, device="cuda"), torch.zeros(m, n, device="cuda"))
         assert float((got.double() / (v * w) - 1).abs().max()) <= 2.0 ** -23, in_a
 
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [2, 20, 300, 1600])
+@pytest.mark.parametrize("k,n", [(80, 40), (79, 1000)])
+@pytest.mark.parametrize("dtype,weights", [("float32", "bfloat16"), ("bfloat16", "bfloat16"), ("float16", "float16"), ("float32", "float16"),
+                                           ("float16", "bfloat16"), ("bfloat16", "float16")])
+def test_rows_of_infinities_and_nan_are_not_finite(tq, m, k, n, dtype, weights):
+    """Each output of a row that has one in x (its last element too) or in its adapter's a; the outputs of those in b."""
+    import torch
+
+    g = torch.Generator("cuda").manual_seed(m + k)
+    f = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, y, index = f(m, k).to(getattr(torch, dtype)), f(m, n), torch.arange(m, dtype=torch.int32, device="cuda") % 6 - 1
+    a, b = f(5, 1, 40, k).to(getattr(torch, weights)), f(5, n, 40).to(getattr(torch, weights))
+    want = tq.Adapters(a, b).add(x, index, y)
+    assert torch.isfinite(want).all()
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for column in (0, 3, k - 1):
+            poisoned = x.clone()
+            poisoned[1::7, column] = bad
+            got = tq.Adapters(a, b).add(poisoned, index, y)
+            rows = torch.zeros(m, dtype=torch.bool, device="cuda")
+            rows[1::7] = True
+            rows &= index >= 0
+            assert not torch.isfinite(got[rows]).any() and torch.equal(got[~rows], want[~rows]), (bad, column)
+            a2 = a.clone()
+            a2[2, 0, 39, column] = bad
+            got, rows = tq.Adapters(a2, b).add(x, index, y), index == 2
+            assert not torch.isfinite(got[rows]).any() and torch.equal(got[~rows], want[~rows]), (bad, column)
+        b2 = b.clone()
+        b2[3, n - 1, 39], b2[0, 0, 0] = bad, bad
+        got = tq.Adapters(a, b2).add(x, index, y)
+        hit = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+        hit[index == 3, n - 1], hit[index == 0, 0] = True, True
+        assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want[~hit]), bad
