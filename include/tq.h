@@ -603,8 +603,8 @@ int tq_kv_attention(const tq_kv_cache* cache, const tq_kv_batch* batch, const tq
  * else.  Products are exact (but what an f32 value has below 2^-126), sums f32 (the inner one is rounded to f32
  * and scaled before the outer).  A row depends on its own adapter alone (the order
  * of its inner sum also on how many adapters its neighbours have); one with infinities or NaN in x or in its
- * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a
- * few rows of low ranks), 16-byte aligned, contents need not be initialised. */
+ * adapter gets infinities or NaN.  workspace: tq_adapters_workspace_bytes(...) bytes (0 for a few
+ * rows of few adapters and low ranks), 16-byte aligned, contents need not be initialised. */
 typedef struct {
     const void* a;
     const void* b;

@@ -485,10 +485,9 @@ __global__ __launch_bounds__(kBlock) void k_adapt_up(AdaptArg a) {
     tiles.run(begin, end, 16 * kWaves, tp[0]);
 }
 
-// A token or a few and low ranks: both products in one launch, without a workspace.  Grid (range of outputs, part): every block
-// forms t of its part by itself, its waves 64 columns of K in turn, and then its outputs.  For the GPU that is about
-// what two launches are (a token in bf16, rank 16, 4096 x 4096, replayed: 6.5 us against 7.2; in f32 8.3 and 8.1; another adapter is 5 us more),
-// for the host a launch and a buffer less (8.5 us a call against 12.5).
+// A token or a few, of few adapters and low ranks: both products in one launch, without a workspace.  Grid (range of outputs, part): every block
+// forms t of its part by itself, its waves 64 columns of K in turn, and then its outputs.  For the GPU that is about what
+// two launches are, for the host a launch and a buffer less; figures at in_one_launch.
 template <int kX, int kW, int kR, bool kVecX, bool kVecY>
 __global__ __launch_bounds__(kOnceBlock) void k_adapt_once(AdaptArg a) {
     constexpr int kOnceWaves = kOnceBlock / 64;
@@ -725,10 +724,20 @@ int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
     return check_launch(what);
 }
 
-// Calls of one launch.
-constexpr int64_t kOnceWeights = 1 << 16;  // of t's that a block forms: a row of rank 16 and 4096 inputs, or as much
+// Calls of one launch.  In it a block takes the adapters that its rows name one after the other, each with its own loads, sums over the
+// waves and barriers, so it is for few of them (the host knows how many there can be, not how many there are) and short products.
+// A call / replayed, us, rank 16, 4096 outputs, one launch against two:
+//   x bf16  1 row, K 4096 6.8 / 6.5, 9.6 / 7.2; K 5120 7.9 / 7.7, 9.7 / 7.4; 2 adapters, K 1024 7.5 / 7.3, 9.6 / 7.0;
+//           4, K 256 7.9 / 7.7, 9.6 / 7.2; 4, K 512 9.6 / 9.4, 9.6 / 7.2; 4, K 1024 11.1 / 11.0, 9.6 / 7.3;
+//           8, K 128 10.4 / 10.2, 9.6 / 8.0; 16, K 256 20.4 / 20.3, 10.0 / 9.7
+//   x f32   1 row, K 4096 8.2 / 8.0, 9.6 / 7.4; K 5120 9.8 / 9.6, 9.7 / 7.7; 2, K 1024 8.8 / 8.6, 9.6 / 7.2;
+//           2, K 2048 9.4 / 9.2, 9.8 / 7.3; 4, K 256 8.9 / 8.7, 9.5 / 7.5; 16, K 256 23.2 / 23.1, 10.2 / 9.9
+// (f32 rows of f16 weights, twice the matrix instructions: K 4096 10.2 / 10.0, 9.5 / 7.8.)
+constexpr int64_t kOnceWeights = 1 << 16;  // rows x ranks x K
+constexpr int64_t kOnceAdapters = 4;
 bool in_one_launch(const tq_adapters* a, int64_t m) {
-    return m <= 16 && a->rank <= 32 && m * a->rank * a->k <= kOnceWeights;
+    const int64_t named = std::min(m, a->count);
+    return m <= 16 && a->rank <= 32 && named <= kOnceAdapters && std::max(m, named * named) * a->rank * a->k <= kOnceWeights;
 }
 
 template <int kX, int kW, int kR>

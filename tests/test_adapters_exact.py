@@ -99,3 +99,15 @@ def test_rows_of_infinities_and_nan_are_not_finite(tq, m, k, n, dtype, weights):
         hit = torch.zeros(m, n, dtype=torch.bool, device="cuda")
         hit[index == 3, n - 1], hit[index == 0, 0] = True, True
         assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want[~hit]), bad
+
+
+def test_one_launch_is_for_rows_of_few_adapters():
+    """A block takes the adapters that rows may name one after the other: a workspace says that they are two launches'."""
+    from test_adapters import at, desc
+    from theano_quantize import _abi
+
+    need = lambda m, **kw: _abi.entry("tq_adapters_workspace_bytes")(at(desc(**dict(parts=1, rank=16, n=4096) | kw)), m)  # noqa: E731
+    for m, count, k in ((1, 48, 4096), (16, 1, 256), (2, 2, 1024), (4, 4, 256), (16, 4, 256), (3, 3, 455)):
+        assert need(m, count=count, k=k) == 0, (m, count, k)
+    for m, count, k in ((1, 48, 4097), (16, 1, 257), (2, 2, 1025), (4, 4, 257), (5, 5, 16), (16, 16, 16), (16, 48, 256), (17, 1, 16)):
+        assert need(m, count=count, k=k) > 0, (m, count, k)
