@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/tq.h"
 
@@ -38,6 +39,34 @@ int check_launch(const char* what);
 
 inline bool aligned(const void* p, uintptr_t a) {
     return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+
+// Memory that a call reads or writes: `rows` runs of `width` elements, `stride` elements apart.  A null or empty one is nowhere.
+struct Extent {
+    uintptr_t at;
+    uint64_t bytes;
+    Extent(const void* p, int64_t rows, int64_t stride, int64_t width, int64_t size) : at(reinterpret_cast<uintptr_t>(p)), bytes(0) {
+        if (!p || rows <= 0 || width <= 0) return;
+        const __int128 b = (static_cast<__int128>(rows - 1) * stride + width) * size;
+        bytes = b > INT64_MAX ? INT64_MAX : static_cast<uint64_t>(b);
+    }
+    Extent(const void* p, int64_t count, int64_t size) : Extent(p, 1, 0, count, size) {}
+};
+
+inline bool overlap(const Extent& a, const Extent& b) {
+    if (a.bytes == 0 || b.bytes == 0) return false;
+    return a.at < b.at ? b.at - a.at < a.bytes : a.at - b.at < b.bytes;
+}
+
+// Whether one that is written overlaps another one, or one that is read.
+inline bool overlap(std::initializer_list<Extent> written, std::initializer_list<Extent> read) {
+    for (const Extent* w = written.begin(); w != written.end(); ++w) {
+        for (const Extent* v = w + 1; v != written.end(); ++v)
+            if (overlap(*w, *v)) return true;
+        for (const Extent& r : read)
+            if (overlap(*w, r)) return true;
+    }
+    return false;
 }
 
 // Compute-unit count of the current device (cached per device, thread-safe).

@@ -379,8 +379,13 @@ int tq_kv_keep(const tq_kv_cache* cache, const tq_kv_batch* batch, const int32_t
     if (batch->batch == 0) return TQ_OK;
     TQ_REQUIRE((path || path_width == 0) && kept, "%s: null path or kept", what);
     TQ_REQUIRE(aligned(path, 4) && aligned(kept, 4) && aligned(lengths_out, 4), "%s: unaligned path, kept or lengths", what);
-    TQ_REQUIRE(!lengths_out || (lengths_out != batch->lengths && lengths_out != kept),
-               "%s: lengths_out is the batch's lengths or kept, which the call reads", what);
+    const int64_t held = cache->heads * cache->page, codes = held * kv_row(cache->head_dim);  // of a page
+    TQ_REQUIRE(!overlap({{lengths_out, batch->batch, 4}},
+                        {{batch->lengths, batch->batch, 4}, {kept, batch->batch, 4}, {path, batch->batch, path_stride, path_width, 4},
+                         {batch->table, batch->batch, batch->table_stride, batch->table_pages, 4}, {batch->offsets, batch->batch + 1, 4},
+                         {cache->k, cache->pages, codes, codes, 1}, {cache->v, cache->pages, codes, codes, 1},
+                         {cache->k_scale, cache->pages, held, held, 4}, {cache->v_scale, cache->pages, held, held, 4}}),
+               "%s: lengths_out overlaps the batch's lengths, table or offsets, path, kept or the cache", what);
     const int64_t units = 2 * batch->batch * cache->heads, blocks = (units + 3) / 4;
     TQ_REQUIRE(blocks <= kMaxBlocks, "%s: %lld sequences of %lld heads are more than %lld blocks", what, (long long)batch->batch,
                (long long)cache->heads, (long long)kMaxBlocks);
