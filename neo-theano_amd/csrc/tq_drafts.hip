@@ -782,6 +782,11 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
     const int64_t need = tq_verify_drafts_workspace_bytes(batch, vocab);
     TQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "%s: workspace of %lld bytes, 16-byte aligned, needed",
                what, (long long)need);
+    const int64_t rows = batch->tokens, sequences = batch->batch;
+    TQ_REQUIRE(!overlap({{path, sequences * batch->max_tokens, 4}, {kept, sequences, 4}, {next, sequences, 8}, {need == 0 ? nullptr : workspace, need, 1}},
+                        {{tokens, rows, 8}, {target, rows, target_stride, vocab, size}, {draft, rows, draft_stride, vocab, size}, {parents, rows, 4},
+                         {accept, rows, 4}, {final, sequences, 4}, {batch->offsets, sequences + 1, 4}}),
+               "%s: path, kept, next or the workspace overlaps another of them or an input", what);
     DraftArg a{};
     a.tokens = tokens;
     a.target = target;

@@ -36,3 +36,65 @@ def test_lengths_that_keep_writes(abi):
         for out in both_ends(first, size, 4 * n):
             refuse(abi, "tq_kv_keep", at(c), at(b), path, 11, 6, kept, out, None)
             message(abi, (first, out))
+
+
+def test_what_verification_writes(abi):
+    """path, kept, next and the workspace over each other and over every input, rows of probabilities with their strides."""
+    n, most, rows, vocab, stride = 3, 5, 11, 40000, 40008
+    b = batch(abi, table=None, table_pages=0, lengths=256, offsets=1 * M, batch=n, max_tokens=most, tokens=rows)
+    need = abi.entry("tq_verify_drafts_workspace_bytes")(at(b), vocab)
+    reads = {"offsets": (1 * M, 4 * (n + 1)), "tokens": (2 * M, 8 * rows), "target": (10 * M, 4 * ((rows - 1) * stride + vocab)),
+             "draft": (20 * M, 4 * ((rows - 1) * stride + vocab)), "parents": (3 * M, 4 * rows), "accept": (4 * M, 4 * rows), "final": (5 * M, 4 * n)}
+    writes = {"workspace": (30 * M, need), "path": (6 * M, 4 * n * most), "kept": (7 * M, 4 * n), "next": (8 * M, 8 * n)}
+
+    def no(draft, name, at_):
+        w = {k: v[0] for k, v in writes.items()} | {name: at_}
+        r = {k: v[0] for k, v in reads.items()} | ({} if draft else {"draft": None})
+        refuse(abi, "tq_verify_drafts", at(b), r["tokens"], r["target"], stride, r["draft"], stride, 2, vocab, r["parents"], r["accept"],
+               r["final"], w["workspace"], need, w["path"], w["kept"], w["next"], None)
+        message(abi, (name, at_))
+
+    for name, (_, length) in writes.items():
+        step = {"workspace": 16, "next": 8}.get(name, 4)
+        for other, (first, size) in (reads | writes).items():
+            if other == name:
+                continue
+            for draft in (True, False):
+                if not draft and other == "draft":
+                    continue
+                for place in (first, (first + size - 1) // step * step, (first - length) // step * step + step):
+                    no(draft, name, place)
+
+
+@pytest.mark.gpu
+def test_neighbours_are_not_refused(tq):
+    """Every input and output of a call one after the other in one buffer."""
+    import torch
+
+    abi, n, vocab, rows = tq._abi, 2, 50, 8
+    sizes = {"tokens": 8 * rows, "next": 8 * n, "target": 4 * rows * vocab, "path": 4 * rows, "draft": 4 * rows * vocab, "kept": 4 * n, "accept": 4 * rows,
+             "final": 4 * n, "parents": 4 * rows}
+    buffer, where, first = torch.zeros(sum(sizes.values()), dtype=torch.uint8, device="cuda"), {}, 0
+    for name, size in sizes.items():
+        where[name], first = buffer[first:first + size], first + size
+    as_ = lambda name, dtype: where[name].view(dtype)  # noqa: E731
+    p = torch.softmax(torch.randn(rows, vocab, device="cuda"), 1)
+    as_("target", torch.float32).copy_(p.flatten()), as_("draft", torch.float32).copy_(p.flatten().roll(1))
+    as_("accept", torch.float32).fill_(0.5), as_("final", torch.float32).fill_(0.5)
+    as_("parents", torch.int32).copy_(torch.tensor([-1, 0, 0, 1] * 2, dtype=torch.int32))
+    as_("tokens", torch.int64).copy_(torch.arange(rows))
+    new = tq.KVBatch(torch.zeros(n, 1, dtype=torch.int32).cuda(), torch.full((n,), 4, dtype=torch.int32).cuda(), 4)
+    ptr = {k: v.data_ptr() for k, v in where.items()}
+    abi.call("tq_verify_drafts", new._desc, ptr["tokens"], ptr["target"], vocab, ptr["draft"], vocab, 2, vocab, ptr["parents"], ptr["accept"],
+             ptr["final"], None, 0, ptr["path"], ptr["kept"], ptr["next"], torch.cuda.current_stream().cuda_stream)
+    want = tq.verify_drafts(torch.arange(rows, device="cuda"), p, new, torch.full((rows,), 0.5, device="cuda"), torch.full((n,), 0.5, device="cuda"),
+                            p.flatten().roll(1).view(rows, vocab), as_("parents", torch.int32).clone())
+    for name, w in zip(("path", "kept", "next"), want):
+        assert torch.equal(as_(name, w.dtype).view(w.shape), w), name
+    # keep's lengths between its paths and kept
+    cache = tq.KVCache.allocate(2, 16, 1, 32)
+    ints = torch.tensor([0, 2, 0, 3, -7, -7, 2, 2], dtype=torch.int32).cuda()
+    new = tq.KVBatch(torch.tensor([[0], [1]], dtype=torch.int32).cuda(), torch.tensor([9, 9], dtype=torch.int32).cuda(), 4)
+    abi.call("tq_kv_keep", cache._ref, new._desc, ints.data_ptr(), 2, 2, ints.data_ptr() + 24, ints.data_ptr() + 16,
+             torch.cuda.current_stream().cuda_stream)
+    assert ints.tolist() == [0, 2, 0, 3, 7, 7, 2, 2]
