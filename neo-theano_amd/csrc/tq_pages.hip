@@ -446,6 +446,8 @@ int tq_pages_grow(const tq_page_pool* pool, int32_t* table, int64_t table_stride
     if ((rc = check_table(what, table, table_stride, table_pages, batch, kPoolSequences)) != TQ_OK) return rc;
     if (batch == 0 || table_pages == 0) return TQ_OK;
     TQ_REQUIRE(lengths && aligned(lengths, 4), "%s: null or unaligned lengths", what);
+    TQ_REQUIRE(!overlap({{table, batch, table_stride, table_pages, 4}, {pool->holders, pool->pages, 4}}, {{lengths, batch, 4}}),
+               "%s: table, holders and lengths overlap", what);
     a.table = table;
     a.stride = table_stride;
     a.table_pages = static_cast<int>(table_pages);
@@ -472,6 +474,9 @@ int tq_pages_fork(const tq_page_pool* pool, const int32_t* table, int64_t table_
                "%s: null lengths, parents, source, target or children", what);
     TQ_REQUIRE(aligned(parents, 4) && aligned(source, 4) && aligned(target, 4) && aligned(lengths, 4) && aligned(children_table, 4),
                "%s: unaligned lengths, parents, source, target or children", what);
+    TQ_REQUIRE(!overlap({{children_table, children * table_pages, 4}, {source, children, 4}, {target, children, 4}, {pool->holders, pool->pages, 4}},
+                        {{table, batch, table_stride, table_pages, 4}, {lengths, batch, 4}, {parents, children, 4}}),
+               "%s: children, source, target or holders overlaps another of them or an input", what);
     a.table = table;
     a.stride = table_stride;
     a.table_pages = static_cast<int>(table_pages);
@@ -496,6 +501,8 @@ int tq_pages_free(const tq_page_pool* pool, int32_t* table, int64_t table_stride
     if (rc != TQ_OK) return rc;
     if ((rc = check_table(what, table, table_stride, table_pages, batch, kKvMaxRows)) != TQ_OK) return rc;
     if (batch == 0 || table_pages == 0) return TQ_OK;
+    TQ_REQUIRE(!overlap({{table, batch, table_stride, table_pages, 4}, {pool->holders, pool->pages, 4}}, {{sequences, batch, 1}}),
+               "%s: table, holders and sequences overlap", what);
     a.table = table;
     a.stride = table_stride;
     a.table_pages = static_cast<int>(table_pages);

@@ -66,6 +66,31 @@ def test_what_verification_writes(abi):
                     no(draft, name, place)
 
 
+def test_what_a_pool_writes(abi):
+    """Children, source and target over the table, lengths, parents, each other or the holders; the table over what calls read."""
+    pages, n, children, width, stride = 40, 3, 5, 4, 9
+    pool = at(Pool(1 * M, pages, 16))
+    reads = {"table": (2 * M, 4 * ((n - 1) * stride + width)), "lengths": (3 * M, 4 * n), "parents": (4 * M, 4 * children), "holders": (1 * M, 4 * pages)}
+    writes = {"out": (5 * M, 4 * children * width), "source": (6 * M, 4 * children), "target": (7 * M, 4 * children)}
+    for name, (_, length) in writes.items():
+        for other, (first, size) in (reads | writes).items():
+            for place in both_ends(first, size, length) if other != name else ():
+                w = {k: v[0] for k, v in writes.items()} | {name: place}
+                refuse(abi, "tq_pages_fork", pool, 2 * M, stride, width, 3 * M, n, 4 * M, children, w["out"], w["source"], w["target"], None)
+                message(abi, (name, place))
+    for place in both_ends(*reads["holders"], reads["table"][1]):
+        refuse(abi, "tq_pages_grow", pool, place, stride, width, 3 * M, n, None)
+        message(abi, place)
+        refuse(abi, "tq_pages_free", pool, place, stride, width, n, None, None)
+        message(abi, place)
+    for first, size in (reads["table"], reads["holders"]):
+        for place in both_ends(first, size, 4 * n):
+            refuse(abi, "tq_pages_grow", pool, 2 * M, stride, width, place, n, None)
+            message(abi, place)
+            refuse(abi, "tq_pages_free", pool, 2 * M, stride, width, n, max(place, first - n + 1), None)
+            message(abi, place)
+
+
 @pytest.mark.gpu
 def test_neighbours_are_not_refused(tq):
     """Every input and output of a call one after the other in one buffer."""
@@ -98,3 +123,15 @@ def test_neighbours_are_not_refused(tq):
     abi.call("tq_kv_keep", cache._ref, new._desc, ints.data_ptr(), 2, 2, ints.data_ptr() + 24, ints.data_ptr() + 16,
              torch.cuda.current_stream().cuda_stream)
     assert ints.tolist() == [0, 2, 0, 3, 7, 7, 2, 2]
+    # a pool's table behind its lengths, its holders behind both, and what a fork gives between parents and a strided table's rows
+    ints = torch.zeros(64, dtype=torch.int32, device="cuda")
+    ints[:2], ints[2:10], ints[12:24] = torch.tensor([17, 30]).cuda(), -1, 0
+    pool, table, s = abi.page_pool_desc(ints[12:].data_ptr(), 12, 16), ints[2:10], torch.cuda.current_stream().cuda_stream
+    abi.call("tq_pages_grow", pool, table.data_ptr(), 4, 4, ints.data_ptr(), 2, s)
+    assert ints[:24].tolist() == [17, 30, 0, 1, -1, -1, 2, 3, -1, -1, 0, 0] + [1] * 4 + [0] * 8
+    ints[24:26], ints[34:36] = torch.tensor([1, 0]).cuda(), 9
+    at_ = lambda i: ints.data_ptr() + 4 * i  # noqa: E731
+    abi.call("tq_pages_fork", pool, table.data_ptr(), 4, 4, ints.data_ptr(), 2, at_(24), 2, at_(26), at_(34), at_(36), s)
+    assert ints[26:38].tolist() == [2, 4, -1, -1, 0, 5, -1, -1, 3, 1, 4, 5]
+    abi.call("tq_pages_free", pool, at_(26), 4, 4, 2, None, s)
+    assert ints[12:24].tolist() == [1] * 4 + [0] * 8 and ints[26:34].tolist() == [-1] * 8
