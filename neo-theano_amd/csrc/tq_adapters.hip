@@ -643,11 +643,6 @@ Cut cut_of(const tq_adapters* a, int64_t m) {
 int64_t shares_bytes(const Cut& c) { return (c.tiles * 4 + 15) / 16 * 16; }
 int64_t most_shares(const Cut& c) { return std::min<int64_t>(kMaxShares, int64_t(1) << c.gang_shift); }
 
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
-}
-
 int check_adapters(const char* what, const tq_adapters* a, int64_t m) {
     TQ_REQUIRE(a, "%s: null adapters", what);
     TQ_REQUIRE(a->dtype == TQ_DT_F16 || a->dtype == TQ_DT_BF16, "%s: adapters are f16 or bf16, not dtype %d", what, a->dtype);
@@ -829,11 +824,13 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
     TQ_REQUIRE(x && index && y && out, "%s: null x, index, y or out", what);
     TQ_REQUIRE(aligned(x, size) && aligned(index, 4) && aligned(y, 4) && aligned(out, 4), "%s: a pointer is not aligned to its elements",
                what);
-    const int64_t y_bytes = m * adapters->n * 4;
-    TQ_REQUIRE(!overlap(out, y_bytes, x, m * adapters->k * size) && !overlap(out, y_bytes, index, m * 4) &&
-                   (out == y || !overlap(out, y_bytes, y, y_bytes)),
-               "%s: out overlaps x, index or a part of y", what);
-    const int64_t need = tq_adapters_workspace_bytes(adapters, m);
+    const int64_t need = tq_adapters_workspace_bytes(adapters, m), ranks = adapters->count * adapters->rank;
+    const Extent to{out, m * adapters->n, 4};
+    TQ_REQUIRE(out == y || !overlap(to, Extent{y, m * adapters->n, 4}), "%s: out overlaps a part of y", what);
+    TQ_REQUIRE(!overlap({to}, {{x, m * adapters->k, size}, {index, m, 4}, {adapters->scales, adapters->count, 4},
+                               {adapters->a, adapters->parts * ranks, (adapters->k + kKUnit - 1) / kKUnit * kKUnit * 2},
+                               {adapters->b, adapters->n * ranks, 2}, {need == 0 ? nullptr : workspace, need, 1}}),
+               "%s: out overlaps x, index, the adapters or the workspace", what);
     TQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
                "%s: workspace of %lld bytes, 16-byte aligned, needed", what, (long long)need);
     const Cut c = cut_of(adapters, m);

@@ -38,6 +38,21 @@ def test_lengths_that_keep_writes(abi):
             message(abi, (first, out))
 
 
+def test_what_adapters_write(abi):
+    """out over the adapters' weights and scales and over the workspace (x, index and parts of y: see test_adapters)."""
+    from test_adapters import desc
+
+    m, count, parts, rank, k, n = 30, 4, 2, 32, 100, 60
+    d = at(desc(a=40 * M, b=50 * M, scales=60 * M, count=count, parts=parts, rank=rank, k=k, n=n))
+    need = abi.entry("tq_adapters_workspace_bytes")(d, m)
+    assert need > 0
+    for first, size in ((40 * M, 2 * count * parts * rank * 128), (50 * M, 2 * count * n * rank), (60 * M, 4 * count), (70 * M, need)):
+        for out in both_ends(first, size, 4 * m * n):
+            for y in (out, 4 * M):
+                refuse(abi, "tq_adapters_add", d, 1 * M, 2, m, 2 * M, y, out, 70 * M, need, None)
+                message(abi, (first, out))
+
+
 def test_what_verification_writes(abi):
     """path, kept, next and the workspace over each other and over every input, rows of probabilities with their strides."""
     n, most, rows, vocab, stride = 3, 5, 11, 40000, 40008
