@@ -642,7 +642,7 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
  * the vocabulary is turned down.  path [batch, max_tokens]: the accepted rows (counted
  * within the sequence, the root first), -1 behind them; kept [batch]: how many; next
  * [batch].  A sequence without rows, or whose rows do not fit (see tq_kv_batch), has kept 0
- * and next -1.  workspace: tq_verify_drafts_workspace_bytes(...) bytes (0 for up to 32768 tokens
+ * and next -1.  path, kept, next and the workspace overlap nothing else.  workspace: tq_verify_drafts_workspace_bytes(...) bytes (0 for up to 32768 tokens
  * of the vocabulary), 16-byte aligned, contents need not be initialised. */
 int64_t tq_verify_drafts_workspace_bytes(const tq_kv_batch* batch, int64_t vocab);
 int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void* target, int64_t target_stride,
@@ -653,7 +653,7 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
 /* What was verified stays: of a sequence's T new tokens, in the cache at its last T places,
  * rows path[0] < path[1] < .. < path[kept - 1] move to the first `kept` of these places, in
  * order and as they are coded.  path int32 [batch, path_width], rows path_stride apart; kept
- * int32 [batch].  lengths_out (or NULL; neither the batch's lengths nor kept): length - T + kept.  A
+ * int32 [batch].  lengths_out (or NULL; nothing else that the call is given): length - T + kept.  A
  * sequence whose rows do not fit, whose kept is not in 0 .. min(T, path_width) or whose path does
  * not ascend within its rows stays as it is, its length too.  Rows with no place do not
  * move.  Pages that several sequences share are copied first: places are written. */
@@ -667,14 +667,20 @@ int tq_kv_copy_pages(const tq_kv_cache* cache, const int32_t* source, const int3
 /* Who holds a page: holders[p] (device, 16-byte aligned) counts the table entries that name
  * page p; 0 is a free page.  Tables are int32 [batch, table_pages], rows table_stride apart,
  * -1 where a sequence has no page, its pages first.  Pages that tables name are held;
- * entries outside the pool are not counted.  Calls on one pool are ordered by one stream.
+ * entries outside the pool are not counted.  Calls on one pool are ordered by one stream; what
+ * a call writes overlaps nothing else that it is given.
  * grow:  gives a sequence pages from behind its last one up to ceil(lengths / page) (or the
  *        table's end), the lowest free ones, sequence by sequence; entries for which none
- *        is left stay -1.  At most 4096 sequences.
+ *        is left stay -1.  At most 4096 sequences.  A page comes with what its last sequence left on
+ *        it: no token behind a sequence's last page may have been written for already.
+ * grow_stored: the same where tokens may have been: entries of the first stored[b] tokens that name no page
+ *        stay -1 (those tokens found no page and are nowhere).
+ * lacking: how many of the ceil(lengths / page) entries name no page of the pool or lie past the
+ *        table's end: what grow or fork found no page for.
  * fork:  child c becomes a copy of sequence parents[c] (outside 0 .. batch - 1: an empty one):
  *        its whole pages (length / page) are shared, a page that it has begun is to be copied: target[c], the
  *        lowest free one, from source[c] (-1, -1: nothing to copy, or no page left, then
- *        the entry is -1 too).  children_table is dense [children, table_pages], -1 behind.
+ *        the entry is -1 too, and what the child had on it is lost: see grow_stored).  children_table is dense [children, table_pages], -1 behind.
  *        At most 4096 children.
  * free:  the sequences (those whose byte is not 0; NULL: all) hold their pages no longer;
  *        their entries become -1. */
@@ -684,6 +690,10 @@ typedef struct {
 } tq_page_pool;
 int tq_pages_grow(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
                   int64_t batch, tq_stream_t stream);
+int tq_pages_grow_stored(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                         const int32_t* stored, int64_t batch, tq_stream_t stream);
+int tq_pages_lacking(const tq_page_pool* pool, const int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                     int64_t batch, int32_t* lacking, tq_stream_t stream);
 int tq_pages_fork(const tq_page_pool* pool, const int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
                   int64_t batch, const int32_t* parents, int64_t children, int32_t* children_table, int32_t* source,
                   int32_t* target, tq_stream_t stream);

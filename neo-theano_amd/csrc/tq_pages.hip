@@ -217,6 +217,7 @@ struct GrowArg {
     int64_t stride;
     int table_pages, batch;
     const int32_t* lengths;
+    const int32_t* stored;  // or null
 };
 
 // Pages that `length` tokens take, up to the table's end.
@@ -241,6 +242,8 @@ __global__ __launch_bounds__(kPoolBlock) void k_grow(GrowArg a) {
             }
             end = max(end - 64, 0);
         }
+        // a page that was missing when its tokens came: what lies on another one now is somebody else's
+        if (a.stored) end = max(end, min(pages_of(a.stored[b], a.pool.page, a.table_pages), need));
         if (lane == 0) {
             have[b] = end;
             want[b] = need - end;
@@ -252,6 +255,21 @@ __global__ __launch_bounds__(kPoolBlock) void k_grow(GrowArg a) {
         const int b = owner(want, a.batch, rank);
         a.table[b * a.stride + have[b] + (rank - want[b])] = page;
     });
+}
+
+// A wave for each sequence: the pages of its tokens that it does not have.
+__global__ __launch_bounds__(kBlock) void k_lacking(GrowArg a, int32_t* lacking) {
+    const int lane = threadIdx.x & 63;
+    for (int b = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6); b < a.batch; b += gridDim.x * (kBlock / 64)) {
+        const int need = pages_of(a.lengths[b], a.pool.page, INT32_MAX), here = min(need, a.table_pages);
+        int none = need - here;  // past the table
+        for (int i0 = 0; i0 < here; i0 += 64) {
+            const int i = i0 + lane;
+            const int page = i < here ? a.table[b * a.stride + i] : 0;
+            none += __popcll(__ballot(i < here && (page < 0 || page >= a.pool.pages)));
+        }
+        if (lane == 0) lacking[b] = none;
+    }
 }
 
 struct ForkArg {
@@ -362,6 +380,27 @@ int check_table(const char* what, const int32_t* table, int64_t stride, int64_t 
 // Blocks for so many sequences, which they take in turn.
 int blocks_for(int64_t sequences) { return static_cast<int>(std::min<int64_t>(sequences, 8 * device_cu_count())); }
 
+int grow(const char* what, const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+         const int32_t* stored, int64_t batch, tq_stream_t stream) {
+    GrowArg a{};
+    int rc = check_pool(what, pool, &a.pool);
+    if (rc != TQ_OK) return rc;
+    if ((rc = check_table(what, table, table_stride, table_pages, batch, kPoolSequences)) != TQ_OK) return rc;
+    if (batch == 0 || table_pages == 0) return TQ_OK;
+    TQ_REQUIRE(lengths && aligned(lengths, 4), "%s: null or unaligned lengths", what);
+    TQ_REQUIRE(!overlap({{table, batch, table_stride, table_pages, 4}, {pool->holders, pool->pages, 4}}, {{lengths, batch, 4}, {stored, batch, 4}}),
+               "%s: table or holders overlaps the other or lengths", what);
+    a.table = table;
+    a.stride = table_stride;
+    a.table_pages = static_cast<int>(table_pages);
+    a.batch = static_cast<int>(batch);
+    a.lengths = lengths;
+    a.stored = stored;
+    clear_error();
+    k_grow<<<1, kPoolBlock, 0, as_hip(stream)>>>(a);
+    return check_launch(what);
+}
+
 }  // namespace
 }  // namespace tq
 
@@ -438,23 +477,35 @@ int tq_kv_copy_pages(const tq_kv_cache* cache, const int32_t* source, const int3
 
 int tq_pages_grow(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
                   int64_t batch, tq_stream_t stream) {
+    return tq::grow("tq_pages_grow", pool, table, table_stride, table_pages, lengths, nullptr, batch, stream);
+}
+
+int tq_pages_grow_stored(const tq_page_pool* pool, int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                         const int32_t* stored, int64_t batch, tq_stream_t stream) {
+    static const char* what = "tq_pages_grow_stored";
+    TQ_REQUIRE(batch <= 0 || table_pages == 0 || (stored && tq::aligned(stored, 4)), "%s: null or unaligned stored lengths", what);
+    return tq::grow(what, pool, table, table_stride, table_pages, lengths, stored, batch, stream);
+}
+
+int tq_pages_lacking(const tq_page_pool* pool, const int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lengths,
+                     int64_t batch, int32_t* lacking, tq_stream_t stream) {
     using namespace tq;
-    static const char* what = "tq_pages_grow";
+    static const char* what = "tq_pages_lacking";
     GrowArg a{};
     int rc = check_pool(what, pool, &a.pool);
     if (rc != TQ_OK) return rc;
-    if ((rc = check_table(what, table, table_stride, table_pages, batch, kPoolSequences)) != TQ_OK) return rc;
-    if (batch == 0 || table_pages == 0) return TQ_OK;
-    TQ_REQUIRE(lengths && aligned(lengths, 4), "%s: null or unaligned lengths", what);
-    TQ_REQUIRE(!overlap({{table, batch, table_stride, table_pages, 4}, {pool->holders, pool->pages, 4}}, {{lengths, batch, 4}}),
-               "%s: table, holders and lengths overlap", what);
-    a.table = table;
+    if ((rc = check_table(what, table, table_stride, table_pages, batch, kKvMaxRows)) != TQ_OK) return rc;
+    if (batch == 0) return TQ_OK;
+    TQ_REQUIRE(lengths && aligned(lengths, 4) && lacking && aligned(lacking, 4), "%s: null or unaligned lengths or lacking", what);
+    TQ_REQUIRE(!overlap({{lacking, batch, 4}}, {{table, batch, table_stride, table_pages, 4}, {lengths, batch, 4}, {pool->holders, pool->pages, 4}}),
+               "%s: lacking overlaps the table, lengths or holders", what);
+    a.table = const_cast<int32_t*>(table);
     a.stride = table_stride;
     a.table_pages = static_cast<int>(table_pages);
     a.batch = static_cast<int>(batch);
     a.lengths = lengths;
     clear_error();
-    k_grow<<<1, kPoolBlock, 0, as_hip(stream)>>>(a);
+    k_lacking<<<blocks_for((batch + kBlock / 64 - 1) / (kBlock / 64)), kBlock, 0, as_hip(stream)>>>(a, lacking);
     return check_launch(what);
 }
 

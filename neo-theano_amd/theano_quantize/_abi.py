@@ -125,6 +125,8 @@ SIGNATURES = {
     "tq_kv_keep": [_p, _p, _p, _i64, _i64, _p, _p, _p],
     "tq_kv_copy_pages": [_p, _p, _p, _i64, _p],
     "tq_pages_grow": [_p, _p, _i64, _i64, _p, _i64, _p],
+    "tq_pages_grow_stored": [_p, _p, _i64, _i64, _p, _p, _i64, _p],
+    "tq_pages_lacking": [_p, _p, _i64, _i64, _p, _i64, _p, _p],
     "tq_pages_fork": [_p, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p],
     "tq_pages_free": [_p, _p, _i64, _i64, _i64, _p, _p],
 }

@@ -9,7 +9,8 @@ The reference has neither; both stand behind ``KVCache.attention``'s drafted tre
     pool = PagePool.allocate(pages=512, page=64)
     table, source, target = pool.fork(table, lengths, parents)   # samples of a prompt, beams
     cache.copy_pages(source, target)                             # in each layer's cache
-    pool.grow(table, lengths + 1)
+    pool.grow(table, lengths + 1, lengths)
+    ended |= pool.lacking(table, lengths + 1) > 0                # no page was left for them
     pool.free(table, ended)
 """
 from __future__ import annotations
@@ -80,7 +81,9 @@ class PagePool(_Fixed):
     holders: int32 [pages], how many table entries name each page (0: free); page: its tokens.  Tables
     are int32 [batch, n] as in KVBatch, -1 where a sequence has no page, its pages first.  Nothing is
     read on the host: where pages run out entries stay -1, rows of such places are not written and
-    seen by nobody.  Calls on one pool belong on one stream."""
+    seen by nobody, and `lacking` tells.  A page comes with what its last sequence left on it, so that the tokens of
+    a missing page are lost: the sequence ends, or goes on without them, and then `grow` is told which
+    of its tokens are stored, or it puts a page of somebody else's tokens in their place.  Calls on one pool belong on one stream."""
 
     def __init__(self, holders, page):
         _indices(holders, torch.int32, 1, "PagePool: holders")
@@ -101,19 +104,38 @@ class PagePool(_Fixed):
             raise InvalidArgument(f"{name}: the pool and the current device differ")
         return table.data_ptr(), table.stride(0), table.shape[1]
 
-    def grow(self, table, lengths):
-        """Gives each sequence pages for `lengths` (int32 [batch]) tokens, behind those it has, in `table` itself: the
-        lowest free ones, sequence by sequence."""
-        where = self._table(table, "PagePool.grow: table")
-        _dense(lengths, torch.int32, 1, self.device_index) or _indices(lengths, torch.int32, 1, "PagePool.grow: lengths")
+    def _lengths(self, lengths, table, name):
+        _dense(lengths, torch.int32, 1, self.device_index) or _indices(lengths, torch.int32, 1, name)
         if lengths.shape[0] != table.shape[0]:
-            raise InvalidArgument(f"PagePool.grow: {lengths.shape[0]} lengths for {table.shape[0]} sequences")
-        _abi.call("tq_pages_grow", self._desc, *where, lengths.data_ptr(), table.shape[0], stream())
+            raise InvalidArgument(f"{name}: {lengths.shape[0]} lengths for {table.shape[0]} sequences")
+        return lengths.data_ptr()
+
+    def grow(self, table, lengths, stored=None):
+        """Gives each sequence pages for `lengths` (int32 [batch]) tokens, behind those it has, in `table` itself: the
+        lowest free ones, sequence by sequence.  stored (int32 [batch]): how many of its tokens caches have been
+        written for; entries of theirs that have no page stay so, for their tokens are lost.  None: no token behind its
+        last page has been written yet."""
+        where = self._table(table, "PagePool.grow: table")
+        want = self._lengths(lengths, table, "PagePool.grow: lengths")
+        if stored is None:
+            _abi.call("tq_pages_grow", self._desc, *where, want, table.shape[0], stream())
+        else:
+            _abi.call("tq_pages_grow_stored", self._desc, *where, want, self._lengths(stored, table, "PagePool.grow: stored"), table.shape[0],
+                      stream())
+
+    def lacking(self, table, lengths):
+        """How many pages of its `lengths` (int32 [batch]) tokens each sequence does not have, int32 [batch]: those that `grow` or
+        `fork` found none for (past the table's end, too)."""
+        where = self._table(table, "PagePool.lacking: table")
+        want, out = self._lengths(lengths, table, "PagePool.lacking: lengths"), torch.empty_like(lengths)
+        _abi.call("tq_pages_lacking", self._desc, *where, want, table.shape[0], out.data_ptr(), stream())
+        return out
 
     def fork(self, table, lengths, parents):
         """(children, source, target): the table of copies of the sequences `parents` (int32 [n]) of `lengths` tokens.
         Whole pages are shared; a page that a sequence has begun is copied by
-        ``KVCache.copy_pages(source, target)``, in each layer.  The parents stay until they are freed."""
+        ``KVCache.copy_pages(source, target)``, in each layer.  Where no page is left for the copy the child has none there and its tokens on it are
+        lost (`lacking` of its lengths tells, and `grow` is told that they were stored).  The parents stay until they are freed."""
         where = self._table(table, "PagePool.fork: table")
         dev = self.device_index
         _dense(lengths, torch.int32, 1, dev) or _indices(lengths, torch.int32, 1, "PagePool.fork: lengths")
