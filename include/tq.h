@@ -656,7 +656,8 @@ int tq_verify_drafts(const tq_kv_batch* batch, const int64_t* tokens, const void
  * int32 [batch].  lengths_out (or NULL; nothing else that the call is given): length - T + kept.  A
  * sequence whose rows do not fit, whose kept is not in 0 .. min(T, path_width) or whose path does
  * not ascend within its rows stays as it is, its length too.  Rows with no place do not
- * move.  Pages that several sequences share are copied first: places are written. */
+ * move; where such a row's new place is one, which another row's codes are left on, the sequence ends
+ * before it (lengths_out: length - T + its number).  Pages that several sequences share are copied first: places are written. */
 int tq_kv_keep(const tq_kv_cache* cache, const tq_kv_batch* batch, const int32_t* path, int64_t path_stride, int64_t path_width,
                const int32_t* kept, int32_t* lengths_out, tq_stream_t stream);
 

@@ -47,8 +47,11 @@ __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
         const int v = i < kept ? path[i] : count, before = i > 0 && i < kept ? path[i - 1] : -1;
         fine = !__ballot(i < kept && (v <= before || v >= count));
     }
-    if (a.lengths_out && h == 0 && kv == 0 && lane == 0) a.lengths_out[seq] = fine ? length - count + kept : length;
-    if (!fine) return;
+    const bool tells = a.lengths_out && h == 0 && kv == 0;  // (uniform)
+    if (!fine) {
+        if (tells && lane == 0) a.lengths_out[seq] = length;
+        return;
+    }
     auto at = [&](int r) -> int64_t {  // where new token r of the sequence lies, -1: nowhere
         const int64_t pos = static_cast<int64_t>(length) - count + r;
         if (pos < 0 || pos >= a.b.cap) return -1;
@@ -57,6 +60,7 @@ __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
         return page < 0 || page >= a.b.pages ? -1 : (static_cast<int64_t>(page) * a.heads + h) * a.b.page + (static_cast<int>(pos) - i * a.b.page);
     };
     const int lanes = a.row / 16, rows = 64 / lanes, j = lane / lanes, c = lane - j * lanes;
+    int end = kept;  // the sequence ends before a kept row that lies nowhere, at whose place another row lies
     for (int i0 = 0; i0 < kept; i0 += rows) {
         const int i = i0 + j;
         int64_t from = -1, to = -1;  // rows of [pages, heads, page]
@@ -65,6 +69,10 @@ __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
             to = at(i);
         }
         const bool moves = from >= 0 && to >= 0;
+        if (tells) {
+            const uint64_t lost = __ballot(from < 0 && to >= 0);
+            if (lost) end = min(end, i0 + (__ffsll(static_cast<unsigned long long>(lost)) - 1) / lanes);
+        }
         u32x4 v{};
         float s = 0.f;
         if (moves) {
@@ -76,6 +84,7 @@ __global__ __launch_bounds__(kBlock) void k_keep(KeepArg a, int units) {
             if (c == 0) a.scales[kv][to] = s;
         }
     }
+    if (tells && lane == 0) a.lengths_out[seq] = length - count + end;
 }
 
 // A page's codes of k, of v, its scales of k, of v, as 16-byte units one after the other.

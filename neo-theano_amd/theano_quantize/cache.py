@@ -359,7 +359,7 @@ class KVCache(_Fixed):
         """What of the new tokens was verified (see `verify_drafts`) stays: row path[b, i] of sequence b moves to
         the place of its i-th new token, for i < kept[b] (int32 [batch, n], ascending, and [batch]).  Returns the
         lengths that the sequences then have (int32 [batch]).  A sequence whose path does not ascend inside its rows stays
-        as it is.  Pages that sequences share are copied first (PagePool.fork does)."""
+        as it is; one of whose kept rows lay nowhere (its page was missing) ends before the place that it would move to.  Pages that sequences share are copied first (PagePool.fork does)."""
         b, dev = self._here(new), self.device_index
         _dense(path, torch.int32, 2, dev) or _indices(path, torch.int32, 2, "KVCache.keep: path")
         _dense(kept, torch.int32, 1, dev) or _indices(kept, torch.int32, 1, "KVCache.keep: kept")

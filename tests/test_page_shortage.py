@@ -191,3 +191,28 @@ def test_captured_and_refused(tq):
         if bad is not None:
             with pytest.raises(tq.InvalidArgument):
                 pool.grow(table, lengths, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("codes", ["i8", "fp8"])
+def test_kept_rows_that_found_no_page_end_the_sequence(tq, codes):
+    """Drafts over a page that is missing, past the table or outside the cache: the rows of other branches that lie where such
+    a row would go are not the sequence's.  A row that stays where it is nowhere leaves a gap that nobody sees."""
+    import torch
+
+    made = tq.QuantDType.Int8 if codes == "i8" else tq.QuantDType.FP8
+    # 30 tokens of which the last 20 are new: places 10 to 29, rows 0 to 5 on the first page, 6 to 19 on the second
+    tables, paths, want = [], [], []
+    for table, path, n in (([0, -1], [0, 2, 7], 2), ([1, -1], [0, 7, 9], 1), ([2, 99], [6, 7], 0), ([3, 4], [0, 7, 19], 3), ([-1, 5], [0, 7, 8], 3),
+                           ([6, -1], [0, 1, 2, 3, 4, 5, 6, 7], 8), ([7, -1], [0, 1, 2, 3, 4, 6, 7], 5), ([-1, -1], [3, 9], 2), ([8, -1], [], 0)):
+        tables.append(table), paths.append(path + [-1] * (8 - len(path))), want.append(10 + n)
+    kept = ints([sum(r >= 0 for r in p) for p in paths])
+    for heads, d in ((1, 32), (3, 128), (5, 80)):
+        cache = tq.KVCache.allocate(10, 16, heads, d, made)
+        new = tq.KVBatch(ints(tables), ints([30] * 9), 20)
+        assert cache.keep(new, ints(paths), kept).tolist() == want, (heads, d)
+    # 100 tokens, all new: the first lost row past a wave's first step, and past the table
+    cache = tq.KVCache.allocate(10, 16, 2, 64, made)
+    new = tq.KVBatch(ints([[0, 1, 2, 3, -1]] * 2), ints([100, 100]), 100)
+    path = [list(range(1, 60)) + [70, 99], list(range(0, 80, 2)) + [-1] * 21]
+    assert cache.keep(new, ints(path), ints([61, 40])).tolist() == [59, 32]
