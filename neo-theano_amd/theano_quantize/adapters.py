@@ -75,6 +75,15 @@ class Adapters(_Fixed):
             scales = torch.as_tensor(scales, dtype=torch.float32).to(dev)
         return Adapters(a, b, scales)
 
+    def _fits(self, index, rows, in_features, out_features, name):
+        """These are adapters of such a projection, and `index` says those of so many rows, all on the current device."""
+        if not isinstance(index, torch.Tensor) or tuple(index.shape) != (rows,) or self.in_features != in_features or \
+                self.out_features != out_features:
+            raise InvalidArgument(f"{name}: adapters of [{out_features}, {in_features}] take an index of {rows} rows")
+        if self.device_index != _current_device():
+            raise InvalidArgument(f"{name}: the adapters and the current device differ")
+        _dense(index, torch.int32, 1, self.device_index) or _indices(index, torch.int32, 1, f"{name}: index")
+
     def add(self, x, index, y, out=None):
         """y [rows, N] (f32) with each row's share added: x [rows, K] f32, bf16 or f16; index int32 [rows], the row's adapter,
         or a number outside 0 .. count - 1 for none.  out: where the sums go (y itself, or a tensor that shares no memory with

@@ -183,9 +183,8 @@ class QuantizedLinear(Module):
                 f"QuantizedLinear.forward: shape mismatch, expected [*, {self.in_features}], "
                 f"got {tuple(x.shape)}")
         m = x.shape[0]
-        if adapters is not None and (adapters.in_features != k or adapters.out_features != n or
-                                     not isinstance(index, torch.Tensor) or tuple(index.shape) != (m,)):
-            raise InvalidArgument(f"QuantizedLinear.forward: adapters of [{n}, {k}] take an index of {m} rows")
+        if adapters is not None:
+            adapters._fits(index, m, k, n, "QuantizedLinear.forward")
         y, given = x.new_empty((m, n), dtype=torch.float32), x
         mode, st = self.mode, stream()
         if mode == "fp8_block":
@@ -413,6 +412,8 @@ class QuantizedMultiheadAttention(Module):
         if tuple(x.shape) != (new.rows, e) or cache.heads != h or cache.head_dim != d:
             raise InvalidArgument(f"QuantizedMultiheadAttention.forward_cached: x {tuple(x.shape)} for {new.rows} rows of {e}, "
                                   f"a cache of {cache.heads} heads of {cache.head_dim} for {h} of {d}")
+        if adapters[1] is not None:  # before the cache is written
+            adapters[1]._fits(index, new.rows, e, e, "QuantizedMultiheadAttention.forward_cached")
         qkv = self.qkv(self._act(x), adapters[0], index)
         q, k, v = (qkv[:, i * e:(i + 1) * e].view(new.rows, h, d) for i in range(3))
         if rotary is None:
