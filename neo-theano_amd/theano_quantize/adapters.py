@@ -88,24 +88,25 @@ class Adapters(_Fixed):
         """y [rows, N] (f32) with each row's share added: x [rows, K] f32, bf16 or f16; index int32 [rows], the row's adapter,
         or a number outside 0 .. count - 1 for none.  out: where the sums go (y itself, or a tensor that shares no memory with
         x, index and y), a new tensor if None."""
-        dev, m, k, n = self.device_index, index.shape[0], self.in_features, self.out_features
+        dev, k, n = self.device_index, self.in_features, self.out_features
         if dev != _current_device():
             raise InvalidArgument("Adapters.add: the adapters and the current device differ")
-        code = _TYPES.get(x.dtype)
+        _dense(index, torch.int32, 1, dev) or _indices(index, torch.int32, 1, "Adapters.add: index")
+        m = index.shape[0]
+        code = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
         if code is None or x.shape != (m, k):
-            raise InvalidArgument(f"Adapters.add: x must be float32, bfloat16 or float16 [{m}, {k}], got {x.dtype} {tuple(x.shape)}")
+            raise InvalidArgument(f"Adapters.add: x must be a float32, bfloat16 or float16 tensor [{m}, {k}]")
         if not _dense(x, x.dtype, 2, dev):
             x = _device(x, "Adapters.add: x").contiguous()
-        _dense(index, torch.int32, 1, dev) or _indices(index, torch.int32, 1, "Adapters.add: index")
-        if not _dense(y, torch.float32, 2, dev) or y.shape != (m, n):
-            raise InvalidArgument(f"Adapters.add: y must be contiguous float32 [{m}, {n}] on the current GPU, got {y.dtype} "
-                                  f"{tuple(y.shape)}")
+        if not (_dense(y, torch.float32, 2, dev) or _indices(y, torch.float32, 2, "Adapters.add: y").is_contiguous()) or y.shape != (m, n):
+            raise InvalidArgument(f"Adapters.add: y must be contiguous float32 [{m}, {n}] on the current GPU")
         if out is None:
             out = torch.empty_like(y)
-        elif out is not y and (not _dense(out, torch.float32, 2, dev) or out.shape != (m, n)):
+        elif out is not y and (not (_dense(out, torch.float32, 2, dev) or _indices(out, torch.float32, 2, "Adapters.add: out").is_contiguous()) or
+                               out.shape != (m, n)):
             raise InvalidArgument(f"Adapters.add: out must be contiguous float32 [{m}, {n}] on the current GPU")
         nb = _abi.entry("tq_adapters_workspace_bytes")(self._desc, m)
-        ws = y.new_empty(nb // 4) if nb else None
+        ws = y.new_empty(nb // 4) if nb > 0 else None
         _abi.call("tq_adapters_add", self._desc, x.data_ptr(), code, m, index.data_ptr(), y.data_ptr(), out.data_ptr(),
                   None if ws is None else ws.data_ptr(), nb, stream())
         return out

@@ -68,7 +68,7 @@ def verify_drafts(tokens, target, new, accept, final, draft=None, parents=None):
     kept = new.lengths.new_empty(batch)
     token = tokens.new_empty(batch)
     nb = _abi.entry("tq_verify_drafts_workspace_bytes")(new._desc, vocab)
-    ws = final.new_empty(nb // 4) if nb else None
+    ws = final.new_empty(nb // 4) if nb > 0 else None
     _abi.call("tq_verify_drafts", new._desc, tokens.data_ptr(), target.data_ptr(), target.stride(0), dp, ds,
               _TYPES[target.dtype], vocab, pp, accept.data_ptr(), final.data_ptr(), None if ws is None else ws.data_ptr(), nb, path.data_ptr(),
               kept.data_ptr(), token.data_ptr(), stream())

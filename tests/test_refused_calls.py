@@ -23,3 +23,36 @@ def test_a_layer_that_is_refused_has_not_written_its_cache(tq):
             assert torch.equal(getattr(case.cache, n), t), n
     layer.forward_cached(x, case.cache, case.batch, adapters=(None, out), index=index)
     assert not torch.equal(case.cache.k, before["k"])
+
+
+@pytest.mark.gpu
+def test_adapters_of_what_is_no_tensor(tq):
+    import torch
+
+    ad = tq.Adapters.from_tensors([(torch.randn(8, 32), torch.randn(20, 8))])
+    x, y, index = torch.randn(3, 32, device="cuda"), torch.randn(3, 20, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    for bad in (None, 5, [1.0, 2.0], torch.zeros((), dtype=torch.int32, device="cuda"), torch.zeros(()), x.cpu().numpy()):
+        for args in ((bad, index, y), (x, bad, y), (x, index, bad)) + (() if bad is None else ((x, index, y, bad),)):
+            with pytest.raises(tq.InvalidArgument):
+                ad.add(*args)
+    want = ad.add(x, index, y)  # parameters are tensors
+    p = lambda t: torch.nn.Parameter(t.clone(), requires_grad=False)  # noqa: E731
+    assert torch.equal(ad.add(p(x), p(index), p(y)), want)
+    out = p(torch.zeros_like(y))
+    assert ad.add(x, index, y, out=out) is out and torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_sizes_past_the_kernels(tq):
+    """More than 2^30 tokens of a vocabulary, or rows: no workspace, and an error that says so."""
+    import torch
+
+    new = tq.KVBatch(torch.zeros(1, 1, dtype=torch.int32).cuda(), torch.ones(1, dtype=torch.int32).cuda(), 1)
+    one, wide = torch.zeros(1, device="cuda"), torch.zeros(1, (1 << 30) + 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(tq.InvalidArgument):
+        tq.verify_drafts(torch.zeros(1, dtype=torch.int64, device="cuda"), wide, new, one, one)
+    m = (1 << 30) + 1
+    ad = tq.Adapters.from_tensors([(torch.randn(8, 1), torch.randn(1, 8))])
+    y = torch.zeros(m, 1, device="cuda")
+    with pytest.raises(tq.InvalidArgument):
+        ad.add(wide.view(m, 1), torch.zeros(m, dtype=torch.int32, device="cuda"), y, out=y)
