@@ -12,8 +12,8 @@
 //
 // The first product is bound by reading x (prompts) or A (a token for each adapter) once; K is split over the
 // waves of a block and over blocks, whose sums the second product adds as it loads t.  The second is bound by reading y
-// and writing out.  4093 rows of six adapters' runs, rank 64, 4096 to 14336: 23 + 106 us, the second 4.4 TB/s, where a large copy gets
-// 4.7; 64 rows of 48 adapters of rank 16: 5.7 + 10 us; a row alone, both in one launch: 7 us.
+// and writing out.  4093 rows of six adapters' runs, rank 64, 4096 to 14336: 24 + 107 us by a trace of the dispatches, the second 4.4 TB/s, where a
+// large copy gets 4.7; 64 rows of 48 adapters of rank 16: 5.6 + 10 us; a row alone, both in one launch: 7 us.
 #include <algorithm>
 
 #include "tq_internal.h"
@@ -518,9 +518,9 @@ __global__ __launch_bounds__(kOnceBlock) void k_adapt_once(AdaptArg a) {
 }
 
 // Many rows.  Grid (range of outputs, part, token tile): 16 kT tokens and 256 outputs a step, 64 for each wave.  The
-// sums go through LDS, so that y is read and out written in runs of 1 KB of a row: of 4093 rows of 14336 (rank 64), with y on
-// its way from HBM, 100 us; 106 in runs of 256 bytes, 127 in the 64 bytes that a tile of the matrix instruction holds of a row;
-// a copy of y takes 85.  kStream: loads and stores that are not kept in the caches, which b needs (109 us without).
+// sums go through LDS, so that y is read and out written in runs of 1 KB of a row: both products of 4093 rows, rank 64, 4096 to
+// 14336, replayed: 126 us, 190 with k_adapt_up, which touches 64 bytes of a row at a time.  kStream: loads and stores that are not kept in the
+// caches, which b needs (134 us without).
 template <int kW, int kT, int kS, bool kStream>
 __global__ __launch_bounds__(kBlock) void k_adapt_up_rows(AdaptArg a) {
     constexpr int kRows = 16 * kT, kY = kRows / kWaves, kN = kStep / 16 / kWaves;
@@ -695,9 +695,8 @@ int launch_up(AdaptArg a, bool vec, hipStream_t st, const char* what) {
 }
 
 // Blocks of 16 kT tokens; ranges by what the fullest CU gets: its blocks' steps, and about one step's time for a block's
-// start; a block that is alone on its CU waits for its own loads (4093 rows of 14336, rank 64: 113, 100, 108, 125 and 130 us with
-// 1, 2, 4, 7 and 14 blocks for each CU; 512 rows, rank 64, both products: 30 and 24 us with 1 and 2).  Of ranges that cost the same the
-// shorter ones.
+// start; a block that is alone on its CU waits for its own loads (both products, rank 64, replayed: 4093 rows, 4096 to 14336, 152, 126, 126, 139 and 131 us
+// with 1, 2, 4, 7 and 14 blocks for each CU; 512 rows 30 and 24 with 1 and 2).  Of ranges that cost the same the shorter ones.
 template <int kW, int kT, int kS>
 int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
     const int64_t steps = (a.np + kStep - 1) / kStep, tiles = (a.m + 16 * kT - 1) / (16 * kT), cus = device_cu_count();
@@ -727,7 +726,7 @@ int launch_up_rows(AdaptArg a, hipStream_t st, const char* what) {
 //           8, K 128 10.4 / 10.2, 9.6 / 8.0; 16, K 256 20.4 / 20.3, 10.0 / 9.7
 //   x f32   1 row, K 4096 8.2 / 8.0, 9.6 / 7.4; K 5120 9.8 / 9.6, 9.7 / 7.7; 2, K 1024 8.8 / 8.6, 9.6 / 7.2;
 //           2, K 2048 9.4 / 9.2, 9.8 / 7.3; 4, K 256 8.9 / 8.7, 9.5 / 7.5; 16, K 256 23.2 / 23.1, 10.2 / 9.9
-// (f32 rows of f16 weights, twice the matrix instructions: K 4096 10.2 / 10.0, 9.5 / 7.8.)
+// (x f16 and f16 weights 6.8 / 6.6, 9.5 / 7.3 at K 4096; f32 rows of f16 weights, twice the matrix instructions, 10.2 / 10.0, 9.5 / 7.8.)
 constexpr int64_t kOnceWeights = 1 << 16;  // rows x ranks x K
 constexpr int64_t kOnceAdapters = 4;
 bool in_one_launch(const tq_adapters* a, int64_t m) {

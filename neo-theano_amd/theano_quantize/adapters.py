@@ -24,7 +24,9 @@ class Adapters(_Fixed):
     a: [count, rank, K], or [count, parts, rank, K] for a fused projection whose outputs are `parts`
     equal slices with adapters of their own (q, k and v); b: [count, N, rank]; bf16 or f16 device tensors,
     rank up to 256.  scales: float32 [count] or None (1).  Held are a copy of a in tiles of 16 ranks x 32 inputs (as the
-    kernels load it, padded with zeros), and b, or a copy padded to ranks of 16 where it has to be."""
+    kernels load it, padded with zeros), scales themselves, and b itself, or a copy of it padded to ranks of 16 where it is not
+    dense, of another rank or off 16 bytes: what is written to a afterwards changes nothing, what is written to scales or such a b
+    changes the adapters."""
 
     def __init__(self, a, b, scales=None):
         a, b = _device(a, "Adapters: a").detach(), _device(b, "Adapters: b").detach()

@@ -163,7 +163,8 @@ class Rotary(_Fixed):
 
     @staticmethod
     def axes_in_turn(planes, axes):
-        """`axes` where plane i turns by axis i % axes."""
+        """`axes` where plane i turns by axis i % axes.  (Layouts that interleave sections of unequal sizes, whose last planes stay with
+        one axis, are such a tuple written by hand.)"""
         return tuple(i % axes for i in range(planes))
 
     def _positions(self, positions, n, name):

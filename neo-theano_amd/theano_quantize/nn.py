@@ -235,7 +235,8 @@ class QuantizedMLP(Module):
 
     The composition follows Linear (linear.rs:111-121), SiLU
     (crates/theano-nn/src/activation.rs:66-79) and Tensor::mul; the
-    SiLU(gate)*up intermediate is kept in f32."""
+    SiLU(gate)*up intermediate is kept in f32.  Its three products are one call and take no Adapters: a layer with
+    adapters on gate, up or down is three QuantizedLinear."""
 
     def __init__(self, d, f, gate, up, down, tiled=True):
         self.d, self.f = int(d), int(f)
