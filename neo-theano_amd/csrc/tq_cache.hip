@@ -357,13 +357,14 @@ __global__ __launch_bounds__(kRowBlock) void k_token_rows(RowsArg a) {
 
 // Many tokens: block (kTB adjacent tokens, share of the steps), a group of 16 lanes for each token and each of
 // 16 / kTB adjacent heads of a kind; a step is that many heads; two steps are in flight, four where nothing turns.  A lane keeps its token's
-// angles in registers.  kTB = 1 reads and writes a token's heads in one run.
-template <int kType, bool kVec, bool kTurn, int kTB, class Fmt>
+// angles in registers.  kTB = 1 reads and writes a token's heads in one run.  kAxes: positions of several axes, whose loads and lookup
+// cost one axis nothing (4093 tokens, 64 heads of 128, half of them turned, one axis, replayed: 23.9 us, 24.4 by the form of several).
+template <int kType, bool kVec, bool kTurn, int kTB, class Fmt, bool kAxes>
 __global__ __launch_bounds__(kRowBlock) void k_rows(RowsArg a, int per_share) {
     constexpr int kHalf = kKvMaxHeadDim / 2, kHS = kHeadsAtOnce / kTB, kU = kTurn ? 2 : 4;
     __shared__ float cs[kTB][kHalf], sn[kTB][kHalf];
     __shared__ int64_t slots[kTB];
-    __shared__ double at[kMaxAxes][kTB];
+    __shared__ double at[kAxes ? kMaxAxes : 1][kTB];
     const int tid = threadIdx.x, l = tid % kGroup, j = tid / kGroup, jt = j % kTB, jh = j / kTB, n0 = blockIdx.x * kTB;
     const int n = min(n0 + jt, a.n - 1);
     if (tid < 64) {
@@ -375,15 +376,16 @@ __global__ __launch_bounds__(kRowBlock) void k_rows(RowsArg a, int per_share) {
         }
         if (tid < kTB) {
             slots[tid] = n0 + tid >= a.n || p.behind ? -2 : p.slot;
-            for (int x = 0; x < a.axes.count; ++x)
-                at[x][tid] = static_cast<double>(a.positions ? a.positions[x * a.axes.stride + nn] : p.pos);
+            at[0][tid] = static_cast<double>(a.positions ? a.positions[nn] : p.pos);
+            if constexpr (kAxes)
+                for (int x = 1; x < a.axes.count; ++x) at[x][tid] = static_cast<double>(a.positions[x * a.axes.stride + nn]);
         }
     }
     __syncthreads();
     if constexpr (kTurn) {
         for (int i = tid; i < kTB * a.rot.half; i += kRowBlock) {
             const int t = i / a.rot.half, plane = i - t * a.rot.half;
-            plane_angle(a.rot, plane, at[a.axes.of(plane)][t], cs[t], sn[t]);
+            plane_angle(a.rot, plane, at[kAxes ? a.axes.of(plane) : 0][t], cs[t], sn[t]);
         }
         __syncthreads();
     }
@@ -540,14 +542,14 @@ RotaryArg rotary_arg(const tq_rotary* r) {
     return RotaryArg{r->frequencies, static_cast<int>(r->rotary_dim / 2), r->interleaved != 0, r->inverse != 0, r->scale};
 }
 
-template <int kType, bool kVec, bool kTurn, int kTB, class Fmt>
+template <int kType, bool kVec, bool kTurn, int kTB, class Fmt, bool kAxes = false>
 void launch_many(const RowsArg& a, hipStream_t st) {
     constexpr int kHS = kHeadsAtOnce / kTB;
     auto steps = [](int heads) { return (heads + kHS - 1) / kHS; };
     const int all = steps(a.q.heads) + steps(a.k.heads) + steps(a.v.heads), groups = (a.n + kTB - 1) / kTB;
     const int want = std::max(1, std::min((8 * device_cu_count() + groups - 1) / groups, (all + 1) / 2));
     const int per = (all + want - 1) / want;
-    k_rows<kType, kVec, kTurn, kTB, Fmt><<<dim3(groups, (all + per - 1) / per), kRowBlock, 0, st>>>(a, per);
+    k_rows<kType, kVec, kTurn, kTB, Fmt, kAxes><<<dim3(groups, (all + per - 1) / per), kRowBlock, 0, st>>>(a, per);
 }
 
 // Tokens to a block from 128 tokens on: 1 where heads only turn (4093 tokens, 64 heads of 128, bf16: 24 us, 26 with 4
@@ -561,8 +563,9 @@ template <int kType, bool kVec, bool kTurn, class Fmt>
 void launch_rows_vec(const RowsArg& a, hipStream_t st) {
     if (a.n >= kManyFrom) {
         if constexpr (!kTurn) return launch_many<kType, kVec, false, kCodeTokens, Fmt>(a, st);
-        if (a.k_codes) return launch_many<kType, kVec, true, kBothTokens, Fmt>(a, st);
-        return launch_many<kType, kVec, true, kTurnTokens, FmtI8>(a, st);
+        const bool axes = a.positions && a.axes.count > 1;  // (a row's place is the same on all)
+        if (a.k_codes) return axes ? launch_many<kType, kVec, true, kBothTokens, Fmt, true>(a, st) : launch_many<kType, kVec, true, kBothTokens, Fmt>(a, st);
+        return axes ? launch_many<kType, kVec, true, kTurnTokens, FmtI8, true>(a, st) : launch_many<kType, kVec, true, kTurnTokens, FmtI8>(a, st);
     }
     auto shares = [](int heads) { return (heads + kHeadsAtOnce - 1) / kHeadsAtOnce; };
     k_token_rows<kType, kVec, kTurn, Fmt>
