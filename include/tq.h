@@ -629,7 +629,8 @@ int tq_adapters_add(const tq_adapters* adapters, const void* x, int dtype, int64
  * row whose parent is not before it is nobody's child; NULL: t - 1, a chain).  target and
  * draft are probabilities [tokens, vocab] (dtype f32, bf16 or f16, rows target_stride and
  * draft_stride elements apart): of the token after each row, and those that its children
- * were drawn from (draft NULL: children are given, not drawn; each a point mass).
+ * were drawn from, each by itself, so that the same token may come twice (draft NULL: children are
+ * given, not drawn; each a point mass).
  * accept [tokens] and final [batch] are uniform numbers in [0, 1).
  *   From the root on, the children of the last accepted row c are tried in order.  After k
  *   were turned down, left_k = max(p_c - a_k q_c, 0), a_0 = 0, W_0 = 1, a_{k+1} = a_k + W_k,

@@ -37,8 +37,8 @@ def verify_drafts(tokens, target, new, accept, final, draft=None, parents=None):
 
     new: the KVBatch of the call; the first row of a sequence is its root (already sampled), the others
     are drafted.  tokens: int64 [rows].  target: probabilities [rows, vocab] (f32, bf16 or f16) of the
-    token after each row.  draft: likewise, those that a row's children were drawn from, or None where they
-    were not drawn (a draft model's likeliest).  parents: int32 [rows], the row (counted within the sequence)
+    token after each row.  draft: likewise, those that a row's children were drawn from, each by itself (siblings
+    drawn without replacement are not distributed so), or None where they were not drawn (a draft model's likeliest).  parents: int32 [rows], the row (counted within the sequence)
     that each drafted row follows, before it; None for a chain.  accept: float32 [rows] and final: float32
     [batch], uniform in [0, 1).
 
